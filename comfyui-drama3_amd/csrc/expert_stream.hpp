@@ -1,0 +1,252 @@
+// Expert products with few rows to an expert: a decode line's experts (gemv: a pass is one pair) and a short prompt's
+// groups in passes of up to 16 MT rows. HBM-bound: the experts' weights go by once, so what counts is how many bytes are
+// on their way. A wave streams its tiles of 16 weight rows from memory straight into the MFMA operands, DEPTH stages
+// ahead; nothing but the accumulators is shared along K, so there is no barrier in the loop. The pass's rows lie whole in
+// LDS (SEG stages at a time), read by all waves.
+#pragma once
+#include "ragged.hpp"
+
+namespace d3 {
+
+constexpr int ST_THREADS = 256;
+
+// LDS bytes of a row of the stages, and where its 16-byte piece j lies: pieces of 256 bytes swapped by the row, so that
+// 16 rows' pieces j are in 16 different groups of banks
+template <class F> constexpr int st_pitch() { return (F::SEG * F::ROW + 255) / 256 * 256; }
+D3_INLINE int st_piece(int r, int j) { return 16 * (j ^ (r & 15)); }
+
+// NT tiles of weight rows a wave; SWIGLU with NT 2: a gate tile and its up tile, with NT 1 (gemv): those of two
+// neighbouring waves
+template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH>
+__global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProduct a, int columns) {
+  constexpr int ROWS = GEMV ? 1 : 16 * MT, PITCH = st_pitch<F>(), SPITCH = 8 * F::SEG + 4, SEG = F::SEG;
+  __shared__ __attribute__((aligned(1024))) uint8_t xs[ROWS * PITCH];
+  __shared__ __attribute__((aligned(16))) uint8_t ss[F::SCALED ? ROWS * SPITCH : 16];
+  __shared__ f32x4 other[GEMV && SWIGLU ? ST_THREADS / 64 : 1][4];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q = lane >> 4, c = lane & 15;
+  const int column = blockIdx.x % columns, at = blockIdx.x / columns;
+  Pass pass;
+  int my_row;  // lane r: row r of the pass
+  if constexpr (GEMV) {
+    const int64_t id = a.ids[at];
+    const bool valid = id >= 0 && id < a.E;
+    pass = Pass{valid ? (int)id : -1, at, 1};
+    my_row = at / a.per_row;
+  } else {
+    pass = find_pass(a, ROWS, at);
+    if (pass.rows == 0) return;
+    my_row = row_at(a, pass.first + min(lane, pass.rows - 1));
+  }
+  // the wave's tiles of an expert's N / 16
+  const int tiles = a.N / 16, half = tiles / 2;
+  int tile[NT];
+  bool mine;  // the wave has a tile of its own (a column past the last one repeats it and stores nothing)
+  if constexpr (SWIGLU && NT == 1) {
+    const int unit = column * 2 + (w >> 1);
+    mine = unit < half;
+    tile[0] = min(unit, half - 1) + (w & 1) * half;
+  } else if constexpr (SWIGLU) {
+    const int unit = column * 4 + w;
+    mine = unit < half;
+    tile[0] = min(unit, half - 1);
+    tile[NT - 1] = tile[0] + half;
+  } else {
+    const int first = (column * 4 + w) * NT;
+    mine = first < tiles;
+#pragma unroll
+    for (int n = 0; n < NT; n++) tile[n] = min(first + n, tiles - 1);
+  }
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int m = 0; m < MT; m++) acc[n][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  if (!GEMV || pass.expert >= 0) {
+    const int S = a.stages;
+    const uint8_t* wp[NT];
+    const uint8_t* sp[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const size_t t = (size_t)pass.expert * tiles + tile[n];
+      wp[n] = a.w + F::a_base(t, S, lane);
+      sp[n] = F::SCALED ? a.w_scale + (t * 64 + lane) * mx_lane_scales(S) : nullptr;
+    }
+    const size_t row_bytes = (size_t)S * F::ROW;
+    for (int s0 = 0; s0 < S; s0 += SEG) {
+      const int n_st = min(SEG, S - s0);
+      i32x4 buf[DEPTH][NT][2];
+      uint32_t sa[NT][F::SCALED ? SEG / 2 : 1];
+      auto load = [&](int d, int st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int s = 0; s < 2; s++)
+            buf[d][n][s] = *(const i32x4*)(wp[n] + (size_t)(s0 + st) * F::A_STAGE + s * F::A_STEP);
+      };
+#pragma unroll
+      for (int d = 0; d < DEPTH; d++) load(d, min(d, n_st - 1));
+      if constexpr (F::SCALED) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int i = 0; i < SEG / 2; i++) sa[n][i] = ((const uint32_t*)(sp[n] + 2 * s0))[min(i, (n_st - 1) / 2)];
+      }
+      // the rows: wave w copies rows w, w + 4, .. to LDS, lane by lane into place
+      if (s0) __syncthreads();
+      for (int r = w; r < pass.rows; r += ST_THREADS / 64) {
+        const uint8_t* src = a.x + (size_t)__builtin_amdgcn_readlane(my_row, r) * row_bytes + (size_t)s0 * F::ROW;
+        for (int j = 0; j < n_st * F::ROW / 16; j += 64) {
+          const int slot = j + lane, piece = (slot & ~15) | ((slot ^ r) & 15);
+          if (16 * piece < n_st * F::ROW) dma16(lds_address(xs + r * PITCH + 16 * j), src, 16 * piece);
+        }
+      }
+      if constexpr (F::SCALED) {
+        for (int r = tid >> 4; r < pass.rows; r += ST_THREADS / 16) {
+          const int row = GEMV ? my_row : __shfl(my_row, r);
+          if ((tid & 15) < 2 * n_st)
+            *(uint32_t*)(ss + r * SPITCH + 4 * (tid & 15)) =
+                ((const uint32_t*)(a.x_scale + ((size_t)row * S + s0) * 8))[tid & 15];
+        }
+      }
+      dma_wait();
+      __syncthreads();
+      // lane's rows of the MT tiles (a row past the pass's repeats its last: its results are not stored)
+      int xr[MT];
+#pragma unroll
+      for (int m = 0; m < MT; m++) xr[m] = min(16 * m + c, pass.rows - 1);
+      auto products = [&]<int ODD>(int d, int st, uint32_t (&sw)[NT]) __attribute__((always_inline)) {
+        uint32_t sb[MT];
+        i32x4 b[MT][2][F::PIECES];
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+          sb[m] = F::SCALED ? *(const uint16_t*)(ss + xr[m] * SPITCH + 8 * st + 2 * q) : 0u;
+#pragma unroll
+          for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < F::PIECES; i++) {
+              const int j = st * (F::ROW / 16) + F::b_piece(s, q, i);
+              b[m][s][i] = *(const i32x4*)(xs + xr[m] * PITCH + 16 * (j & ~15) + st_piece(xr[m], j & 15));
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int m = 0; m < MT; m++) {
+            acc[n][m] = step_product<F, !OUT_BF16, 2 * ODD, 0>(buf[d][n][0], b[m][0], acc[n][m], sw[n], sb[m]);
+            acc[n][m] = step_product<F, !OUT_BF16, 2 * ODD + 1, 1>(buf[d][n][1], b[m][1], acc[n][m], sw[n], sb[m]);
+          }
+      };
+      auto run = [&](int d, int st) __attribute__((always_inline)) {
+        uint32_t sw[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) sw[n] = F::SCALED ? sa[n][st / 2] : 0u;
+        if (d & 1) products.template operator()<1>(d, st, sw);
+        else products.template operator()<0>(d, st, sw);
+      };
+      if constexpr (F::SCALED) {  // at most SEG / DEPTH turns, unrolled: the scale words stay in registers
+#pragma unroll
+        for (int base = 0; base < SEG; base += DEPTH) {
+          if (base + DEPTH < n_st) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++) {
+              run(d, base + d);
+              load(d, min(base + d + DEPTH, n_st - 1));
+            }
+          } else if (base < n_st) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++)
+              if (base + d < n_st) run(d, base + d);
+          }
+        }
+      } else {
+        int st = 0;
+        for (; st + DEPTH < n_st; st += DEPTH) {
+#pragma unroll
+          for (int d = 0; d < DEPTH; d++) {
+            run(d, st + d);
+            load(d, min(st + d + DEPTH, n_st - 1));
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++)
+          if (st + d < n_st) run(d, st + d);
+      }
+    }
+  }
+
+  // lane (q, c) holds weight rows 16 tile + 4 q .. + 3 of the pass's row 16 m + c
+  if constexpr (GEMV && SWIGLU) {
+    if (c == 0) other[w][q] = acc[0][0];
+    __syncthreads();
+    if (mine && !(w & 1) && c == 0) {
+      const f32x4 g = acc[0][0], u = other[w | 1][q];
+      *(i32x2*)((uint16_t*)a.out + (size_t)pass.first * (a.N / 2) + tile[0] * 16 + 4 * q) =
+          i32x2{(int)(swiglu_bf16(g[0], u[0]) | swiglu_bf16(g[1], u[1]) << 16),
+                (int)(swiglu_bf16(g[2], u[2]) | swiglu_bf16(g[3], u[3]) << 16)};
+    }
+  } else if (mine) {
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+      const int r = 16 * m + c;
+      if (r >= pass.rows) continue;
+      const size_t p = (size_t)(pass.first + r);
+      if constexpr (SWIGLU) {
+        const f32x4 g = acc[0][m], u = acc[NT - 1][m];
+        *(i32x2*)((uint16_t*)a.out + p * (a.N / 2) + tile[0] * 16 + 4 * q) =
+            i32x2{(int)(swiglu_bf16(g[0], u[0]) | swiglu_bf16(g[1], u[1]) << 16),
+                  (int)(swiglu_bf16(g[2], u[2]) | swiglu_bf16(g[3], u[3]) << 16)};
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          if ((column * 4 + w) * NT + n >= tiles) continue;
+          const f32x4 v = acc[n][m];
+          const size_t o = p * a.N + tile[n] * 16 + 4 * q;
+          if constexpr (OUT_BF16)
+            *(i32x2*)((uint16_t*)a.out + o) = i32x2{(int)(f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16),
+                                                    (int)(f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16)};
+          else
+            *(f32x4*)((float*)a.out + o) = v;
+        }
+      }
+    }
+  }
+}
+
+// workgroups to a pass
+template <bool GEMV, bool SWIGLU, int NT>
+int st_columns(int N) {
+  const int per = SWIGLU && NT == 1 ? 4 : SWIGLU ? 8 : 4 * NT;  // tiles of a workgroup
+  return (N / 16 + per - 1) / per;
+}
+
+template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH>
+void launch_stream_of(const ExpertProduct& a, int passes, hipStream_t s) {
+  const int columns = st_columns<GEMV, SWIGLU, NT>(a.N);
+  hipLaunchKernelGGL((expert_stream_kernel<F, GEMV, SWIGLU, OUT_BF16, NT, MT, DEPTH>), dim3((unsigned)(columns * passes)),
+                     dim3(ST_THREADS), 0, s, a, columns);
+}
+
+// passes of at most `most` rows that groups of `pairs` rows in all can have
+inline int most_passes(int pairs, int n_groups, int most) {
+  const int64_t n = (int64_t)pairs / most + n_groups;
+  return (int)(n < pairs ? n : pairs);
+}
+
+template <class F>
+void launch_gemv(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
+  if (swiglu) launch_stream_of<F, true, true, true, 1, 1, 8>(a, a.pairs, s);
+  else if (out_bf16) launch_stream_of<F, true, false, true, 1, 1, 8>(a, a.pairs, s);
+  else launch_stream_of<F, true, false, false, 1, 1, 8>(a, a.pairs, s);
+}
+
+template <class F, int MT>
+void launch_stream(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
+  const int passes = most_passes(a.pairs, a.n_groups, 16 * MT);
+  if (swiglu) launch_stream_of<F, false, true, true, 2, MT, 4>(a, passes, s);
+  else if (out_bf16) launch_stream_of<F, false, false, true, 2, MT, 4>(a, passes, s);
+  else launch_stream_of<F, false, false, false, 2, MT, 4>(a, passes, s);
+}
+
+}  // namespace d3

@@ -1,0 +1,173 @@
+// Rows to the microscaled formats and back (mx.hpp): per block of 32 columns the scale is the power of two
+// 2^(floor(log2 max|v|) - m), m = 2 for e2m1 and 8 for e4m3, so that the largest magnitude falls into the binade of the
+// format's largest element; the elements are v / scale to nearest, ties to even, saturated at +-6 or +-448. Dividing by
+// a power of two is exact, so the codes are those of the definition bit for bit. A block of zeros has scale code 0, a block with an
+// infinity or NaN has 255 (NaN: all its values read as NaN).
+//
+// HBM-bound. A lane takes 8 columns (one 16-byte load of bf16, two of float32), four lanes a block, whose maximum
+// goes round by DPP; consecutive lanes read and write consecutive bytes.
+#include "mx.hpp"
+#include "../../include/drama3_moe.h"
+
+#include <string>
+
+namespace d3 {
+int fail(const std::string& msg);
+int hip_fail(hipError_t err, const char* what);
+
+namespace {
+
+// columns 8 u .. 8 u + 7 of a row as float
+template <bool BF16>
+D3_INLINE void load8(const void* row, int u, float (&v)[8]) {
+  if constexpr (BF16) {
+    const i32x4 w = *((const i32x4*)row + u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v[2 * i] = __uint_as_float((uint32_t)w[i] << 16);
+      v[2 * i + 1] = __uint_as_float((uint32_t)w[i] & 0xFFFF0000u);
+    }
+  } else {
+    const f32x4 a = *((const f32x4*)row + 2 * u), b = *((const f32x4*)row + 2 * u + 1);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+  }
+}
+
+template <int BITS, bool BF16>
+__global__ void __launch_bounds__(256) mx_quantize_kernel(const uint8_t* x, int64_t stride, uint32_t units, int cols,
+                                                          int per, uint8_t* codes, uint8_t* scale) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= units) return;  // (whole blocks of lanes: a row's units are a multiple of 32)
+  const uint32_t r = i / (uint32_t)per;
+  const int u = (int)(i - r * (uint32_t)per);
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (8 * u < cols) load8<BF16>(x + (int64_t)r * stride, u, v);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+  top = max(top, (uint32_t)dpp_i32((int)top, 0xB1));
+  top = max(top, (uint32_t)dpp_i32((int)top, 0x4E));
+  const uint32_t e = top >> 23;
+  constexpr uint32_t M = BITS == 4 ? 2 : 8;
+  const uint32_t code = e == 255u ? 255u : e > M ? e - M : 0u;
+  const float inv = __uint_as_float((254u - min(code, 253u)) << 23);  // 2^(127 - code)
+  if constexpr (BITS == 4) {
+    uint32_t w = 0;
+#define D3_PAIR(b) w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2 * b] * inv, v[2 * b + 1] * inv, 1.0f, b)
+    D3_PAIR(0);
+    D3_PAIR(1);
+    D3_PAIR(2);
+    D3_PAIR(3);
+#undef D3_PAIR
+    ((uint32_t*)codes)[i] = w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = __builtin_amdgcn_fmed3f(v[j] * inv, -448.0f, 448.0f);
+    ((i32x2*)codes)[i] = i32x2{(int)f32x4_to_fp8x4(v[0], v[1], v[2], v[3]), (int)f32x4_to_fp8x4(v[4], v[5], v[6], v[7])};
+  }
+  if ((i & 3u) == 0u) scale[i >> 2] = (uint8_t)code;
+}
+
+template <int BITS, bool BF16>
+__global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* codes, const uint8_t* scale, uint32_t units,
+                                                            int cols, int per, uint8_t* out) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= units) return;
+  const uint32_t r = i / (uint32_t)(cols / 8);
+  const int u = (int)(i - r * (uint32_t)(cols / 8));
+  const int64_t at = (int64_t)r * per + u;  // the row's stored units reach to the next stage
+  const float s = mx_scale(scale[at >> 2]);
+  float v[8];
+  if constexpr (BITS == 4) {
+    const uint32_t w = ((const uint32_t*)codes)[at];
+#define D3_PAIR(b)                                                               \
+  {                                                                              \
+    const f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, b);        \
+    v[2 * b] = p.x * s, v[2 * b + 1] = p.y * s;                                  \
+  }
+    D3_PAIR(0);
+    D3_PAIR(1);
+    D3_PAIR(2);
+    D3_PAIR(3);
+#undef D3_PAIR
+  } else {
+    const i32x2 w = ((const i32x2*)codes)[at];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const f32x2 a = fp8x2_to_f32<false>((uint32_t)w[j]), b = fp8x2_to_f32<true>((uint32_t)w[j]);
+      v[4 * j] = a.x * s, v[4 * j + 1] = a.y * s, v[4 * j + 2] = b.x * s, v[4 * j + 3] = b.y * s;
+    }
+  }
+  if constexpr (BF16) {
+    i32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = (int)(f32_to_bf16(v[2 * j]) | f32_to_bf16(v[2 * j + 1]) << 16);
+    *((i32x4*)out + i) = o;
+  } else {
+    *((f32x4*)out + 2 * (int64_t)i) = f32x4{v[0], v[1], v[2], v[3]};
+    *((f32x4*)out + 2 * (int64_t)i + 1) = f32x4{v[4], v[5], v[6], v[7]};
+  }
+}
+
+bool misaligned(const void* p) { return (uintptr_t)p & 15u; }
+
+// the common checks of rows [rows, cols] in `bits`; the launch's units of 8 columns, `per` to a row
+int check_rows(const char* what, int32_t rows, int32_t cols, int32_t bits, int32_t type, int64_t per) {
+  if (bits != 4 && bits != 8) return fail(std::string(what) + ": bits must be 4 or 8");
+  if (type != 0 && type != 1) return fail(std::string(what) + ": type must be 0 (float32) or 1 (bfloat16)");
+  if (rows < 0 || cols < 1 || cols % MX_BLOCK) return fail(std::string(what) + ": cols must be a positive multiple of 32");
+  if ((int64_t)rows * per > INT32_MAX) return fail(std::string(what) + ": more than 2^31 units of 8 columns");
+  return 0;
+}
+
+}  // namespace
+}  // namespace d3
+
+using namespace d3;
+
+extern "C" int d3_mx_quantize(const void* x, int32_t type, int64_t stride, int32_t rows, int32_t cols, int32_t bits,
+                              void* codes, void* scale, void* stream) {
+  const int per = mx_stages(cols) * MX_STAGE / 8;
+  if (const int rc = check_rows("d3_mx_quantize", rows, cols, bits, type, per)) return rc;
+  const int64_t bytes = stride * (type ? 2 : 4);
+  if (stride < 0 || bytes % 16) return fail("d3_mx_quantize: the row stride must be a multiple of 16 bytes");
+  if (rows == 0) return 0;
+  if (!x || !codes || !scale) return fail("d3_mx_quantize: null pointer");
+  if (misaligned(x) || misaligned(codes)) return fail("d3_mx_quantize: x and codes must be 16-byte aligned");
+  const uint32_t units = (uint32_t)rows * (uint32_t)per;
+  const dim3 grid((units + 255u) / 256u), block(256);
+  const hipStream_t s = (hipStream_t)stream;
+#define D3_QUANTIZE(B, T)                                                                                           \
+  hipLaunchKernelGGL((mx_quantize_kernel<B, T>), grid, block, 0, s, (const uint8_t*)x, bytes, units, cols, per,      \
+                     (uint8_t*)codes, (uint8_t*)scale)
+  if (bits == 4 && type) D3_QUANTIZE(4, true);
+  else if (bits == 4) D3_QUANTIZE(4, false);
+  else if (type) D3_QUANTIZE(8, true);
+  else D3_QUANTIZE(8, false);
+#undef D3_QUANTIZE
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : hip_fail(e, "d3_mx_quantize launch");
+}
+
+extern "C" int d3_mx_dequantize(const void* codes, const void* scale, int32_t rows, int32_t cols, int32_t bits,
+                                int32_t type, void* out, void* stream) {
+  const int per = mx_stages(cols) * MX_STAGE / 8;
+  if (const int rc = check_rows("d3_mx_dequantize", rows, cols, bits, type, per)) return rc;
+  if (rows == 0) return 0;
+  if (!codes || !scale || !out) return fail("d3_mx_dequantize: null pointer");
+  if (misaligned(codes) || misaligned(out)) return fail("d3_mx_dequantize: codes and out must be 16-byte aligned");
+  const uint32_t units = (uint32_t)rows * (uint32_t)(cols / 8);
+  const dim3 grid((units + 255u) / 256u), block(256);
+  const hipStream_t s = (hipStream_t)stream;
+#define D3_DEQUANTIZE(B, T)                                                                                         \
+  hipLaunchKernelGGL((mx_dequantize_kernel<B, T>), grid, block, 0, s, (const uint8_t*)codes, (const uint8_t*)scale,  \
+                     units, cols, per, (uint8_t*)out)
+  if (bits == 4 && type) D3_DEQUANTIZE(4, true);
+  else if (bits == 4) D3_DEQUANTIZE(4, false);
+  else if (type) D3_DEQUANTIZE(8, true);
+  else D3_DEQUANTIZE(8, false);
+#undef D3_DEQUANTIZE
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : hip_fail(e, "d3_mx_dequantize launch");
+}

@@ -1,0 +1,147 @@
+// What the expert products on microscaled and bfloat16 banks share: their arguments, the operands' places (Format), and
+// the passes over ragged groups of rows.
+//
+// A product is out[p, n] = sum_k x[row(p), k] w[expert(p), n, k] for the pairs p of rows and experts, as
+// v_mfma tiles of 16 weight rows x 16 pairs. K goes by in stages of two MFMA steps; every kernel adds a pair's stages
+// and steps in the same order into one float32 accumulator, so a result depends on the pair's row and expert alone, not on
+// the kernel, the tile or the rows beside it.
+#pragma once
+#include "mx.hpp"
+#include "wide_tile.hpp"
+
+namespace d3 {
+
+struct ExpertProduct {
+  const uint8_t* x;        // rows [x_rows, row_bytes]
+  const uint8_t* x_scale;  // microscaled rows: [x_rows, 8 * stages]
+  int x_rows;
+  const int64_t* ids;      // gemv: [pairs]
+  int per_row;             // gemv: pairs to a row of x
+  const int32_t* groups;   // grouped: [n_groups, 5] (expert, ., ., first, rows)
+  int n_groups;
+  const int64_t* order;    // grouped: pair at each place, or null (the place's own row)
+  int k;                   // pairs to a row of x, with order
+  int pairs;
+  const uint8_t* w;
+  const uint8_t* w_scale;
+  int E, N, stages;        // N rows an expert; stages of K
+  void* out;               // [pairs, N] float32 or bf16; swiglu: [pairs, N / 2] bf16
+};
+
+// Where a format's operands lie. A (weights): a lane's 16 bytes of stage st, step s of tile t at
+// a_base(t, lane) + st * A_STAGE + s * A_STEP. B (rows): ROW bytes of a row to a stage; a lane's operand of step s is the
+// 16-byte pieces b_piece(s, q, 0 ..) of them.
+template <int BITS_>
+struct Mx {
+  static constexpr bool SCALED = true;
+  static constexpr int BITS = BITS_, ROW = 32 * BITS, PIECES = BITS / 4, SEG = 8;  // SEG: stages whose rows LDS holds
+  static constexpr int A_STAGE = 2048, A_STEP = 1024;
+  static D3_INLINE size_t a_base(size_t tile, int stages, int lane) { return tile * stages * 2048 + lane * 16; }
+  static D3_INLINE int b_piece(int s, int q, int i) {
+    return BITS == 4 ? 2 * q + s : 4 * (q >> 1) + 2 * s + (q & 1) + 8 * i;
+  }
+};
+// bfloat16: a stage is 64 columns (128 bytes of a row), step s multiplies the pieces 2 q + s of 8 columns; the weights lie
+// row by row
+struct Bf16 {
+  static constexpr bool SCALED = false;
+  static constexpr int BITS = 16, ROW = 128, PIECES = 1, SEG = 32;
+  static constexpr int A_STAGE = 128, A_STEP = 16;
+  static D3_INLINE size_t a_base(size_t tile, int stages, int lane) {
+    return (tile * 16 + (lane & 15)) * ((size_t)stages * 128) + 32 * (lane >> 4);
+  }
+  static D3_INLINE int b_piece(int s, int q, int) { return 2 * q + s; }
+};
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// A step's operand b of e4m3 rows in two parts, below 4 and from 4 on (zeros in between): b = low + high.
+//
+// Against e4m3, v_mfma_scale aligns a block's 32 products to the largest one's exponent and keeps 13 bits below it (measured:
+// of 256 - 256 + 2^-n it gives 2^-5 and nothing smaller; e2m1 against e2m1 loses nothing). e4m3 spans 18 binades, so
+// small elements beside a block's large ones are cut: 7e-6 of a result's norm on normally distributed rows with a
+// few large channels, where float32 sums give 2e-7. Of each part every product keeps all its bits: high is a
+// multiple of 1/2, low of 2^-9, e2m1 of 1/2, so products are multiples of 2^-2 with exponents up to 8 + 2 = 10, and of
+// 2^-10 with exponents up to 1 + 2 = 3.
+D3_INLINE void split_e4m3(i32x8 b, i32x8& low, i32x8& high) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint32_t v = (uint32_t)b[i];
+    const uint32_t from4 = (((v & 0x7F7F7F7Fu) + 0x38383838u) & 0x80808080u) >> 7;  // 4 is code 0x48; 1 in a byte from there on
+    const uint32_t mask = (from4 << 8) - from4;
+    high[i] = (int)(v & mask);
+    low[i] = (int)(v & ~mask);
+  }
+}
+
+// acc + a . b over a step. sa, sb: scale words, byte OA and OB of them. (The upper half of an e2m1 operand is not
+// read.) EXACT: e4m3 rows in two parts, for results that are kept in float32; those that are rounded to bf16 (2e-3
+// of their norm) take the instruction's own sums, at half the products.
+template <class F, bool EXACT, int OA, int OB>
+D3_INLINE f32x4 step_product(i32x4 a, const i32x4 (&b)[F::PIECES], f32x4 acc, uint32_t sa, uint32_t sb) {
+  if constexpr (F::SCALED) {
+    const i32x8 A = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
+    if constexpr (F::BITS == 4) {
+      const i32x8 B = __builtin_shufflevector(b[0], b[0], 0, 1, 2, 3, -1, -1, -1, -1);
+      return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc, 4, 4, OA, (int)sa, OB, (int)sb);
+    } else {
+      const i32x8 B = __builtin_shufflevector(b[0], b[F::PIECES - 1], 0, 1, 2, 3, 4, 5, 6, 7);
+      if constexpr (!EXACT) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc, 4, 0, OA, (int)sa, OB, (int)sb);
+      i32x8 low, high;
+      split_e4m3(B, low, high);
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, high, acc, 4, 0, OA, (int)sa, OB, (int)sb);
+      return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, low, acc, 4, 0, OA, (int)sa, OB, (int)sb);
+    }
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b[0]), acc,
+                                                   0, 0, 0);
+  }
+}
+
+// SiLU(gate) * up in float32 (float32 exp and division: within 2^-21 of the value), rounded to bf16 as the rows that
+// the next product reads
+D3_INLINE uint32_t swiglu_bf16(float gate, float up) { return f32_to_bf16(gate / (1.0f + __expf(-gate)) * up); }
+
+// Pass `at` of the groups' passes of at most `most` rows, in the groups' order: its expert, first place and rows (0: there
+// is no such pass). The whole wave calls; a group whose expert or rows lie outside the bank or the pairs has no pass.
+struct Pass {
+  int expert, first, rows;
+};
+D3_INLINE Pass find_pass(const ExpertProduct& a, int most, int at) {
+  const int lane = threadIdx.x & 63;
+  for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
+    const int g = g0 + lane;
+    int expert = 0, first = 0, rows = 0;
+    if (g < a.n_groups) {
+      const int32_t* p = a.groups + 5 * (size_t)g;
+      expert = p[0], first = p[3], rows = p[4];
+      if (expert < 0 || expert >= a.E || first < 0 || rows < 0 || first > a.pairs || rows > a.pairs - first) rows = 0;
+    }
+    const int np = (rows + most - 1) / most;
+    int incl = np;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(incl, d);
+      if (lane >= d) incl += u;
+    }
+    const uint64_t past = __ballot(incl > at);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      const int nth = at - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(np, l));
+      const int all = __builtin_amdgcn_readlane(rows, l);
+      return Pass{__builtin_amdgcn_readlane(expert, l), __builtin_amdgcn_readlane(first, l) + nth * most,
+                  min(most, all - nth * most)};
+    }
+    at -= __builtin_amdgcn_readlane(incl, 63);
+  }
+  return Pass{0, 0, 0};
+}
+
+// the row of x of the pair at place p
+D3_INLINE int row_at(const ExpertProduct& a, int p) {
+  if (!a.order) return min(p, a.x_rows - 1);
+  const int64_t pair = min<int64_t>(max<int64_t>(a.order[p], 0), INT32_MAX);
+  return min((int)((uint32_t)pair / (uint32_t)a.k), a.x_rows - 1);
+}
+
+}  // namespace d3

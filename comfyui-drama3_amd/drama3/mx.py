@@ -1,0 +1,193 @@
+"""Microscaled 4-bit expert banks (OCP MX): the quantizer, the banks' layout and the products that read them.
+
+A microscaled row holds elements of 4 bits (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) or 8 (e4m3) with one
+power-of-two scale (e8m0) per 32 columns. MI355X multiplies both operands as they are stored, scales included, so a bank
+of e2m1 weights costs 17/32 byte a weight and no decoding:
+
+    gate_up, down = mx.quantize_bank(w_gate_up), mx.quantize_bank(w_down)   # [E, 2I, H], [E, H, I] float -> MxBank
+    rows = mx.quantize(x, 8)                                                # [T, H] -> MxRows (e4m3; 4: e2m1)
+    h = mx.gemv(rows, ids, gate_up, swiglu=True)                            # decode lines: ids [T * k] int64
+    h = mx.grouped(rows, groups, gate_up, order=order, k=k, swiglu=True)    # a prompt (kernels.expert_groups)
+    out = mx.moe_layer(x, topk_idx, topk_weight, gate_up, down)             # the routed layer, rows of any number
+
+`rows_from` and `bank` take rows and weights that a checkpoint already holds in the format. The C entries are in
+include/drama3_moe.h (d3_mx_*); nothing waits on the host, and outputs are the only allocations, so a call can be captured
+in a graph. The reference has no counterpart.
+"""
+import dataclasses
+
+import torch
+
+from . import _lib, kernels
+
+BLOCK, STAGE = 32, 256
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _stages(cols):
+    return -(-cols // STAGE)
+
+
+@dataclasses.dataclass
+class MxRows:
+    """Rows of `cols` columns: codes [R, C * bits / 8] and scale [R, C / 32], uint8, C = cols rounded up to a multiple
+    of 256 (zeros there). e2m1 codes are two to a byte, column 2 j in the low half."""
+    codes: torch.Tensor
+    scale: torch.Tensor
+    bits: int
+    cols: int
+
+
+@dataclasses.dataclass
+class MxBank:
+    """E experts of `rows` e2m1 weight rows over `cols` columns, in the tiles that the products read (`bank` lays them
+    out): weight [E * rows, C / 2], scale [E * rows, 8 * stages], uint8, the stages of 256 columns rounded up to an
+    even number."""
+    weight: torch.Tensor
+    scale: torch.Tensor
+    experts: int
+    rows: int
+    cols: int
+
+    def to(self, device):
+        return dataclasses.replace(self, weight=self.weight.to(device), scale=self.scale.to(device))
+
+    def expert_bytes(self):
+        return (self.weight.numel() + self.scale.numel()) // self.experts
+
+
+def _check_cols(cols):
+    if cols < BLOCK or cols % BLOCK:
+        raise ValueError(f"microscaled rows have a positive multiple of {BLOCK} columns, not {cols}")
+
+
+def _check_rows(r):
+    C = _stages(r.cols) * STAGE
+    R = r.codes.shape[0]
+    if r.bits not in (4, 8):
+        raise ValueError(f"microscaled rows have 4 or 8 bits an element, not {r.bits}")
+    if r.codes.dtype != torch.uint8 or r.scale.dtype != torch.uint8:
+        raise TypeError("codes and scale must be uint8")
+    if r.codes.shape != (R, C * r.bits // 8) or r.scale.shape != (R, C // BLOCK):
+        raise ValueError(f"codes [R, {C * r.bits // 8}] and scale [R, {C // BLOCK}] expected for {r.cols} columns")
+    if not (r.codes.is_contiguous() and r.scale.is_contiguous()):
+        raise ValueError("codes and scale must be contiguous")
+    if r.scale.device != r.codes.device:
+        raise ValueError("codes and scale must be on one device")
+    return R
+
+
+def quantize(x, bits=4):
+    """Rows x [R, C] (float32 or bfloat16, any row stride) as MxRows: per 32 columns the scale is the power of two
+    2^(floor(log2 max|v|) - m), m = 2 for 4 bits and 8 for 8, the elements v / scale to nearest, ties to even, saturated
+    at +-6 or +-448. A block with an infinity or NaN reads as NaN."""
+    if x.dim() != 2 or x.dtype not in _TYPES:
+        raise TypeError("x [R, C] float32 or bfloat16 expected")
+    R, cols = x.shape
+    _check_cols(cols)
+    if bits not in (4, 8):
+        raise ValueError(f"4 or 8 bits an element, not {bits}")
+    if x.stride(1) != 1 or x.stride(0) < cols or x.stride(0) * x.element_size() % 16 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    C = _stages(cols) * STAGE
+    codes = torch.empty((R, C * bits // 8), dtype=torch.uint8, device=x.device)
+    scale = torch.empty((R, C // BLOCK), dtype=torch.uint8, device=x.device)
+    kernels.launch("d3_mx_quantize", x, x.data_ptr(), _TYPES[x.dtype], x.stride(0), R, cols, bits, codes.data_ptr(),
+                   scale.data_ptr())
+    return MxRows(codes, scale, bits, cols)
+
+
+def dequantize(rows, dtype=torch.float32):
+    """The values of MxRows: [R, cols] float32 or bfloat16."""
+    R = _check_rows(rows)
+    _check_cols(rows.cols)
+    if dtype not in _TYPES:
+        raise TypeError("float32 or bfloat16 expected")
+    out = torch.empty((R, rows.cols), dtype=dtype, device=rows.codes.device)
+    kernels.launch("d3_mx_dequantize", out, rows.codes.data_ptr(), rows.scale.data_ptr(), R, rows.cols, rows.bits,
+                   _TYPES[dtype], out.data_ptr())
+    return out
+
+
+def rows_from(codes, scale, bits):
+    """MxRows of codes [R, cols * bits / 8] and scale codes [R, cols / 32] (uint8), as a checkpoint holds them."""
+    R, cols = codes.shape[0], codes.shape[1] * 8 // bits
+    _check_cols(cols)
+    if codes.dtype != torch.uint8 or scale.dtype != torch.uint8 or scale.shape != (R, cols // BLOCK):
+        raise ValueError("codes [R, cols * bits / 8] and scale [R, cols / 32], uint8, expected")
+    more = -cols % STAGE
+    pad = torch.nn.functional.pad
+    return MxRows(pad(codes, (0, more * bits // 8)).contiguous(), pad(scale, (0, more // BLOCK)).contiguous(), bits, cols)
+
+
+def bank(rows, experts):
+    """MxRows of e2m1 weights (experts * N rows, N % 16 == 0) laid out for the products, once: tile t holds 16 rows, their
+    codes by stage of 256 columns, half s of the block pairs, pair q, row; their scales by pair, row, stage and s, where
+    block 2 q + s of a stage's eight is pair q's half s."""
+    R = _check_rows(rows)
+    if rows.bits != 4 or experts < 1 or R % experts or (R // experts) % 16:
+        raise ValueError("a bank holds experts of e2m1 rows, a multiple of 16 each")
+    tiles, stages = R // 16, _stages(rows.cols)
+    codes = rows.codes.view(tiles, 16, stages, 4, 2, 16).permute(0, 2, 4, 3, 1, 5).reshape(R, -1)
+    scale = rows.scale.view(tiles, 16, stages, 4, 2).permute(0, 3, 1, 2, 4)
+    scale = torch.nn.functional.pad(scale, (0, 0, 0, stages % 2)).reshape(R, -1)
+    return MxBank(codes.contiguous(), scale.contiguous(), experts, R // experts, rows.cols)
+
+
+def bank_rows(b):
+    """The MxRows of a bank: `bank`'s inverse."""
+    tiles, stages = b.weight.shape[0] // 16, _stages(b.cols)
+    codes = b.weight.view(tiles, stages, 2, 4, 16, 16).permute(0, 4, 1, 3, 2, 5).reshape(16 * tiles, -1)
+    scale = b.scale.view(tiles, 4, 16, -1, 2)[:, :, :, :stages].permute(0, 2, 3, 1, 4).reshape(16 * tiles, -1)
+    return MxRows(codes.contiguous(), scale.contiguous(), 4, b.cols)
+
+
+def quantize_bank(w):
+    """Float weights [E, N, K] as an MxBank (N a multiple of 16, K of 32)."""
+    E, n, k = w.shape
+    return bank(quantize(w.reshape(E * n, k), 4), E)
+
+
+def _check_bank(b, rows, swiglu):
+    stages = _stages(b.cols)
+    R = b.experts * b.rows
+    if rows.cols != b.cols:
+        raise ValueError(f"rows of {rows.cols} columns for a bank of {b.cols}")
+    if b.weight.dtype != torch.uint8 or b.scale.dtype != torch.uint8:
+        raise TypeError("a bank's weight and scale must be uint8")
+    if b.weight.shape != (R, stages * STAGE // 2) or b.scale.shape != (R, 8 * (stages + stages % 2)):
+        raise ValueError("the bank's tensors do not have its shape (mx.bank lays them out)")
+    if not (b.weight.is_contiguous() and b.scale.is_contiguous()):
+        raise ValueError("a bank's tensors must be contiguous")
+    if b.weight.device != rows.codes.device or b.scale.device != rows.codes.device:
+        raise ValueError("rows and bank must be on one device")
+
+
+def gemv(rows, ids, bank, swiglu=False, dtype=torch.float32, out=None):
+    """[P, N] of P pairs of rows and experts ids [P] (int64): pair p is row p // (P / R) of the R rows with expert
+    ids[p] of `bank`; float32 or bfloat16. With `swiglu` (gate rows, then up rows) [P, N / 2] bfloat16 = SiLU(gate) * up.
+    An id outside the bank gives zeros. For decode lines: every pair reads its expert by itself."""
+    R = _check_rows(rows)
+    _check_bank(bank, rows, swiglu)
+    out = kernels.product_out(rows.codes.device, ids.numel(), bank.rows, swiglu, dtype, out)
+    ids = kernels.pair_ids(ids, R, rows.codes.device)
+    kernels.launch("d3_mx_gemv", out, rows.codes.data_ptr(), rows.scale.data_ptr(), rows.bits, R, ids.data_ptr(),
+                   ids.numel(), bank.weight.data_ptr(), bank.scale.data_ptr(), bank.experts, bank.rows, bank.cols,
+                   int(swiglu), int(out.dtype == torch.bfloat16), out.data_ptr())
+    return out
+
+
+def grouped(rows, groups, bank, order=None, k=1, swiglu=False, dtype=torch.float32, out=None):
+    """[P, N] of pairs grouped by expert: groups [g, 5] int32 (expert, ., ., first place, rows) and order [P] int64 as
+    kernels.expert_groups makes them; place p multiplies row order[p] // k (its own row p without order) with its group's
+    expert. dtype and `swiglu` as for gemv. Places in no group are left as `out` had them (unset without it), as are groups
+    whose expert or places lie outside the bank or the pairs."""
+    R = _check_rows(rows)
+    _check_bank(bank, rows, swiglu)
+    device = rows.codes.device
+    P = kernels.check_groups(groups, order, k, R, device)
+    out = kernels.product_out(device, P, bank.rows, swiglu, dtype, out)
+    kernels.launch("d3_mx_grouped", out, rows.codes.data_ptr(), rows.scale.data_ptr(), rows.bits, R, _lib.ptr(order), k,
+                   P, groups.data_ptr(), groups.shape[0], bank.weight.data_ptr(), bank.scale.data_ptr(), bank.experts,
+                   bank.rows, bank.cols, int(swiglu), int(out.dtype == torch.bfloat16), out.data_ptr())
+    return out

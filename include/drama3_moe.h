@@ -394,6 +394,46 @@ int d3_resident_status(void* workspace, uint32_t* status);
 int d3_decode_codes(int32_t bits, const void* rows, const void* scales, const float* codebook, int32_t R, int32_t K,
                     void* out, void* stream);
 
+/* ---- Microscaled rows and banks (OCP MX; no counterpart in the reference) -------------------------------------------
+ * Elements of 4 bits (e2m1) or 8 (e4m3) in blocks of 32 columns with one e8m0 scale code c each: value = element *
+ * 2^(c - 127), 255 is NaN. Rows of `cols` columns (cols % 32 == 0), C = cols rounded up to a multiple of 256:
+ *   codes [rows, C * bits / 8]  e2m1: column 2 j in byte j's low half; e4m3: a byte a column; zeros past cols
+ *   scale [rows, C / 32]        zeros past cols
+ * d3_mx_quantize: x [rows, cols] float32 (type 0) or bf16 (type 1), rows `stride` elements apart (16-byte aligned, as is
+ * the stride). A block's scale is 2^(floor(log2 max|v|) - m), m = 2 (e2m1) or 8 (e4m3), its code clamped to 0..254;
+ * elements are v / scale to nearest, ties to even, saturated at +-6 or +-448: bit for bit the definition's. A block of
+ * zeros has code 0, one with an infinity or NaN code 255.
+ * d3_mx_dequantize: out [rows, cols] float32 or bf16 (every finite value with a scale code of 8 or more is exact in both). */
+int d3_mx_quantize(const void* x, int32_t type, int64_t stride, int32_t rows, int32_t cols, int32_t bits, void* codes,
+                   void* scale, void* stream);
+int d3_mx_dequantize(const void* codes, const void* scale, int32_t rows, int32_t cols, int32_t bits, int32_t type,
+                     void* out, void* stream);
+
+/* Products of experts on banks of e2m1 rows, out[p, n] = x[row of p] . w[expert of p, n], both operands as stored, on
+ * the scaled matrix instruction with float32 sums. w: E experts of N rows (N % 16 == 0; swiglu: % 32) of K columns
+ * (K % 32 == 0) in tiles of 16 rows: codes [E * N / 16][stage of 256 columns][s][q][row][16 bytes] and scales
+ * [E * N / 16][q][row][stage][s], block 2 q + s of the stage's eight; the scales' stages rounded up to an even number.
+ * x: rows as above, bits 4 or 8. out [pairs, N] float32 (out_bf16 0) or bf16; with swiglu (gate rows, then up rows)
+ * [pairs, N / 2] bf16 = SiLU(gate) * up of the float32 products. rows, weights and out 16-byte aligned. A pair's result depends on its
+ * row and expert alone, not on the other pairs of the call.
+ * gemv: pair p multiplies row p / (pairs / rows) with expert ids[p] (int64); an id outside [0, E) gives zeros.
+ * grouped: groups [n_groups, 5] int32 = (expert, ., ., first, rows) as d3_expert_groups makes them; place p of a group
+ * multiplies row order[p] / k (row p when order is NULL). Places in no group, and groups whose expert or rows lie
+ * outside the bank or the pairs, are left alone. */
+int d3_mx_gemv(const void* codes, const void* scale, int32_t bits, int32_t rows, const int64_t* ids, int32_t pairs,
+               const void* w, const void* w_scale, int32_t E, int32_t N, int32_t K, int32_t swiglu, int32_t out_bf16,
+               void* out, void* stream);
+int d3_mx_grouped(const void* codes, const void* scale, int32_t bits, int32_t rows, const int64_t* order, int32_t k,
+                  int32_t pairs, const int32_t* groups, int32_t n_groups, const void* w, const void* w_scale, int32_t E,
+                  int32_t N, int32_t K, int32_t swiglu, int32_t out_bf16, void* out, void* stream);
+
+/* The same on unquantized banks: x [rows, K] bf16, w [E * N, K] bf16 row by row, K % 64 == 0. */
+int d3_bf16_gemv(const void* x, int32_t rows, const int64_t* ids, int32_t pairs, const void* w, int32_t E, int32_t N,
+                 int32_t K, int32_t swiglu, int32_t out_bf16, void* out, void* stream);
+int d3_bf16_grouped(const void* x, int32_t rows, const int64_t* order, int32_t k, int32_t pairs, const int32_t* groups,
+                    int32_t n_groups, const void* w, int32_t E, int32_t N, int32_t K, int32_t swiglu, int32_t out_bf16,
+                    void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,361 @@
+"""The quantizer of microscaled rows bit for bit against its definition, and the expert products on microscaled and on
+bfloat16 banks against 64-bit sums of the values that their operands hold."""
+import numpy as np
+import pytest
+import torch
+
+from drama3 import kernels, mx
+from oracle import mx as omx
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).to(DEV)
+
+
+# ------------------------------------------------------------------------------------------------------- quantizer
+def _blocks():
+    """Rows of 32 columns that a quantizer can get wrong: zeros, powers of two, the borders between elements and around
+    saturation, subnormal maxima, the ends of float32's range, and blocks with an infinity or NaN."""
+    rng = np.random.default_rng(3)
+    rows = [np.zeros(32), -np.zeros(32), np.full(32, 1.0), np.full(32, -0.75)]
+    for g in (omx.E2M1, omx.E4M3):
+        mid = (g[1:] + g[:-1]) / 2
+        every = np.concatenate([g, mid, np.nextafter(mid.astype(np.float32), np.float32(0)).astype(np.float64),
+                                np.nextafter(mid.astype(np.float32), np.float32(1e9)).astype(np.float64)])
+        for part in np.array_split(every, -(-len(every) // 31)):
+            row = np.zeros(32)
+            row[:len(part)] = part * np.where(np.arange(len(part)) % 2, -1, 1)
+            row[31] = 1.875 * 2.0 ** np.floor(np.log2(g[-1]))  # in the largest element's binade: scale 1, and saturated
+            rows += [row, row * 2.0 ** 40, row * 2.0 ** -70]
+    for top in (2.0 ** -149, 2.0 ** -126, 2.0 ** -120, 3.4028234663852886e38):
+        row = rng.uniform(-1, 1, 32)
+        row[rng.integers(32)] = 1.0
+        rows += [row * top, row * top * 0.7]
+    for bad in (np.inf, -np.inf, np.nan):
+        row = rng.standard_normal(32)
+        row[7] = bad
+        rows.append(row)
+    return np.array(rows).astype(np.float32)
+
+
+def _check_quantized(x, got, bits):
+    """codes and scales equal the definition's (the sign of a zero and the elements of a NaN block aside)."""
+    want, scale = omx.quantize(x, bits)
+    cols = x.shape[1]
+    assert np.array_equal(got.scale.cpu().numpy()[:, :cols // 32], scale)
+    codes = omx.unpack(got.codes.cpu().numpy(), bits)
+    assert not codes[:, cols:].any() and not got.scale[:, cols // 32:].any()
+    fine = np.repeat(scale, 32, axis=1) != 255
+    a, b = (omx.values(c, np.full_like(scale, 127), bits)[fine] for c in (codes[:, :cols], want))
+    assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_quantize_edges(bits):
+    x = _blocks()
+    got = mx.quantize(dev(x), bits)
+    _check_quantized(x, got, bits)
+    # the same blocks side by side in one row, and in bfloat16
+    wide = x.reshape(1, -1)
+    _check_quantized(wide, mx.quantize(dev(wide), bits), bits)
+    half = dev(x).to(torch.bfloat16)
+    _check_quantized(half.float().cpu().numpy(), mx.quantize(half, bits), bits)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_quantize_every_bfloat16(bits):
+    """Every finite bfloat16 value in a block of each scale that it may meet: its own, and eight binades more."""
+    v = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(torch.bfloat16).float()
+    v = v[torch.isfinite(v)].numpy()
+    v = v[np.abs(v) < 2.0 ** 100]
+    for up in (0, 1, 4, 8):
+        x = np.zeros((len(v), 32), np.float32)
+        x[:, 3] = v
+        x[:, 20] = np.exp2(np.frexp(v)[1] - 1 + up)
+        h = dev(x).to(torch.bfloat16)
+        _check_quantized(x, mx.quantize(h, bits), bits)
+
+
+@pytest.mark.parametrize("R, cols", [(0, 64), (1, 32), (3, 96), (1, 2048), (37, 800), (1000, 768), (5, 4096)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_quantize_and_back(R, cols, dtype, bits):
+    gen = torch.Generator().manual_seed(R + cols)
+    x = (torch.randn((R, cols), generator=gen) * torch.randn((R, 1), generator=gen).exp2()).to(dtype)
+    got = mx.quantize(x.to(DEV), bits)
+    assert got.codes.shape == (R, -(-cols // 256) * 32 * bits) and got.scale.shape == (R, -(-cols // 256) * 8)
+    if R:
+        _check_quantized(x.float().numpy(), got, bits)
+    want = omx.values(*omx.quantize(x.float().numpy(), bits), bits) if R else np.zeros((0, cols))
+    assert np.array_equal(mx.dequantize(got).double().cpu().numpy(), want)
+    # an element has 2 or 4 significant bits: bfloat16 holds its value too
+    assert np.array_equal(mx.dequantize(got, torch.bfloat16).double().cpu().numpy(), want)
+
+
+def test_quantize_strided_rows():
+    """Rows further apart than their columns, a view at an offset that is not 16-byte aligned, transposed and expanded."""
+    x = torch.randn((40, 300), device=DEV)
+    for view in (x[:, :96], x[::2, 4:132], x[1:, 3:99], x[:32].t()[:64], x[:1, :64].expand(8, 64)):
+        a, b = mx.quantize(view, 8), mx.quantize(view.clone(memory_format=torch.contiguous_format), 8)
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scale, b.scale)
+
+
+def test_dequantize_every_scale_code():
+    """Every e2m1 and e4m3 code at every scale code: float32 exactly where it holds the value."""
+    for bits, n in ((4, 16), (8, 256)):
+        codes = np.zeros((256, 256), np.uint8)
+        codes[:, :n] = np.arange(n)
+        scale = np.repeat(np.arange(256)[:, None], 8, axis=1).astype(np.uint8)
+        rows = mx.rows_from(dev(omx.pack(codes, bits)), dev(scale), bits)
+        want = omx.values(codes, scale, bits)
+        with np.errstate(over="ignore"):
+            single = want.astype(np.float32)
+        assert np.array_equal(mx.dequantize(rows).cpu().numpy(), single, equal_nan=True)
+        got = mx.dequantize(rows, torch.bfloat16).float().cpu().numpy()
+        normal = np.isnan(want) | (want == 0) | ((np.abs(want) >= 2.0 ** -126) & (np.abs(want) < 3e38))
+        assert np.array_equal(got[normal], single[normal], equal_nan=True)
+
+
+# -------------------------------------------------------------------------------------------------------- products
+FORMATS = ["mx4", "mx8", "bf16"]
+
+
+class Case:
+    """A bank of E experts [n, K] and R rows in a format, their values in 64 bits, and the products on them."""
+
+    def __init__(self, fmt, E, n, K, R, seed=0, spread=0.0):
+        rng = np.random.default_rng(seed + 7919 * n + K)
+        self.fmt, self.E, self.n, self.K, self.R = fmt, E, n, K, R
+        x = rng.standard_normal((R, K)) * np.exp2(spread * rng.standard_normal((R, K // 32)).repeat(32, 1))
+        w = rng.standard_normal((E * n, K)) * 0.02 * np.exp2(spread * rng.standard_normal((E * n, K // 32)).repeat(32, 1))
+        if fmt == "bf16":
+            self.x, self.w = dev(x).to(torch.bfloat16), dev(w).to(torch.bfloat16)
+            self.xv, self.wv = self.x.double(), self.w.double().view(E, n, K)
+        else:
+            bits = int(fmt[2])
+            (xc, xs), (wc, ws) = omx.quantize(x, bits), omx.quantize(w, 4)
+            self.x = mx.rows_from(dev(omx.pack(xc, bits)), dev(xs), bits)
+            self.w = mx.bank(mx.rows_from(dev(omx.pack(wc, 4)), dev(ws), 4), E)
+            self.xv, self.wv = dev(omx.values(xc, xs, bits)), dev(omx.values(wc, ws, 4)).view(E, n, K)
+
+    def gemv(self, ids, **how):
+        if self.fmt == "bf16":
+            return kernels.gemv_bf16(self.x, ids, self.w, self.n, **how)
+        return mx.gemv(self.x, ids, self.w, **how)
+
+    def grouped(self, groups, **how):
+        if self.fmt == "bf16":
+            return kernels.grouped_bf16(self.x, groups, self.w, self.n, **how)
+        return mx.grouped(self.x, groups, self.w, **how)
+
+    def want(self, row, expert, swiglu, rounded):
+        """(values, allowed error before the output's own rounding) of pairs (row, expert), in 64 bits. Products are exact;
+        a step adds its 32 (bf16) or 128 of them to the sum with one rounding of what it aligns to 24 bits or more: at most
+        2 units of the last place of the largest partial sum, below sum |x w|, for each of the steps (two to a step of e4m3
+        rows). Results from e4m3 rows that are rounded to bf16: the instruction aligns a block's 32 products to the largest
+        one's exponent e and cuts what lies below 2^(e - 13). With 4 and 2 significant bits a product p's last place is at
+        least 2^-4 of its power of two, so only products below 2^(e - 8) are cut, each by less than 2^(e - 13) and |p|, and
+        2^e is at most the largest product."""
+        x, w = self.xv[row], self.wv[expert]
+        p = x[:, None] * w
+        out, size = p.sum(-1), p.abs().sum(-1)
+        off = (self.K // (32 if self.fmt == "bf16" else 64) + 3) * 2.0 ** -22 * size
+        if self.fmt == "mx8" and rounded:
+            p = p.abs().unflatten(-1, (-1, 32))
+            top = p.amax(-1, keepdim=True)
+            off += torch.where(p < top * 2.0 ** -8, torch.minimum(p, top * 2.0 ** -13), 0.0).sum((-2, -1))
+        if not swiglu:
+            return out, off
+        (g, u), (dg, du) = out.chunk(2, dim=1), off.chunk(2, dim=1)
+        silu = g * torch.sigmoid(g)
+        # |SiLU'| <= 1.1; SiLU in float32: exp within 2 ulp and of an argument rounded to |g| 2^-24, a sum, a division, a product
+        return silu * u, 1.1 * dg * u.abs() + silu.abs() * du + 1.1 * dg * du + \
+            (2.0 ** -21 + g.abs() * 2.0 ** -23) * (silu * u).abs()
+
+    def check(self, got, row, expert, swiglu=False):
+        for part in range(0, len(row), 32):
+            at = slice(part, part + 32)
+            want, off = self.want(row[at], expert[at], swiglu, got.dtype == torch.bfloat16)
+            eps = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24
+            err = (got[at].double() - want).abs()
+            allowed = off + eps * (want.abs() + off) + 1e-37
+            assert torch.all(err <= allowed), (self.fmt, float((err / allowed).max()))
+
+
+@pytest.mark.parametrize("n, K", [(16, 64), (32, 256), (48, 320), (96, 768), (160, 2048), (32, 2368), (64, 5120)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_gemv(fmt, n, K):
+    """Decode lines: one row for all its experts, a row per pair, repeated experts, ids outside the bank (zeros)."""
+    case = Case(fmt, 5, n, K, 3, spread=1.0)
+    ids = dev(np.array([4, 0, 2, 2, -1, 1, 5, 3, 0], np.int64))
+    row = torch.arange(9, device=DEV) // 3
+    ok = (ids >= 0) & (ids < 5)
+    for how in ({}, {"dtype": torch.bfloat16}, {"swiglu": True}):
+        if n % 32 and "swiglu" in how:
+            continue
+        got = case.gemv(ids, **how)
+        assert not got[~ok].any()
+        case.check(got[ok], row[ok], ids[ok], "swiglu" in how)
+    one = case.gemv(ids[:3])
+    assert torch.equal(one, case.gemv(ids)[[0]].new_tensor(one.tolist()))
+    assert case.gemv(ids[:0]).shape == (0, n)
+
+
+COUNTS = [0, 1, 15, 16, 17, 31, 33, 0, 64, 65, 130, 3]
+
+
+def _pairs(E, counts, seed=1):
+    """The pairs of `counts` rows an expert in random order, grouped: (ids, order, groups)."""
+    ids = torch.from_numpy(np.random.default_rng(seed).permutation(np.repeat(np.arange(E), counts))).to(DEV)
+    order, inverse, groups = kernels.expert_groups(ids.view(-1, 1), E)
+    return ids, order, inverse, groups
+
+
+@pytest.mark.parametrize("n, K", [(16, 64), (32, 256), (96, 320), (288, 768), (160, 2048), (32, 2368)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_grouped_ragged(fmt, n, K):
+    E, P = len(COUNTS), sum(COUNTS)
+    case = Case(fmt, E, n, K, P, spread=1.0)
+    ids, order, _, groups = _pairs(E, COUNTS)
+    for how in ({}, {"dtype": torch.bfloat16}, {"swiglu": True}):
+        if n % 32 and "swiglu" in how:
+            continue
+        case.check(case.grouped(groups, order=order, **how), order, ids[order], "swiglu" in how)
+    # without order: place p is row p
+    case.check(case.grouped(groups), torch.arange(P, device=DEV), ids[order])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_grouped_top_k(fmt):
+    """A prompt's pairs: row order[p] // k, several experts to a row."""
+    E, T, k = 12, 100, 3
+    case = Case(fmt, E, 64, 512, T)
+    ids = torch.from_numpy(np.argsort(np.random.default_rng(5).random((T, E)), axis=1)[:, :k].copy()).to(DEV)
+    order, inverse, groups = kernels.expert_groups(ids, E)
+    got = case.grouped(groups, order=order, k=k, swiglu=True)
+    case.check(got, order // k, ids.flatten()[order], True)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_results_do_not_depend_on_the_other_rows(fmt):
+    """A pair's result, bit for bit: as a decode line's, alone in its group, and among few and many other rows."""
+    E, n, K, R = 4, 320, 1024, 700
+    case = Case(fmt, E, n, K, R)
+    everything = torch.empty((R, n), device=DEV)
+    ids = torch.from_numpy(np.random.default_rng(2).integers(0, E, R)).to(DEV)
+    line = case.gemv(ids)
+    for counts in (R, 100, 17, 1):
+        rows = torch.arange(counts, device=DEV)
+        order, _, groups = kernels.expert_groups(ids[:counts].view(-1, 1), E)
+        for how in ({}, {"swiglu": True}):
+            got = case.grouped(groups, order=order, **how)
+            want = line if not how else case.gemv(ids, swiglu=True)
+            assert torch.equal(got, want[:counts][order])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_groups_outside_are_left_alone(fmt):
+    """Places in no group and groups whose expert or places lie outside keep what `out` held; order's values outside
+    the rows read the nearest row."""
+    case = Case(fmt, 3, 32, 256, 40)
+    groups = torch.tensor([[0, 0, 0, 5, 7], [3, 0, 0, 12, 4], [-1, 0, 0, 16, 4], [1, 0, 0, 38, 3], [2, 0, 0, -2, 3],
+                           [1, 0, 0, 20, 0], [2, 0, 0, 30, 2], [1, 0, 0, 25, -1], [2, 0, 0, 2 ** 31 - 1, 2],
+                           [0, 0, 0, 2, 2 ** 31 - 1]], dtype=torch.int32, device=DEV)
+    out = torch.full((40, 32), -7.0, device=DEV)
+    got = case.grouped(groups, out=out)
+    assert got is out
+    touched = torch.zeros(40, dtype=torch.bool, device=DEV)
+    touched[5:12] = touched[30:32] = True
+    assert torch.all(got[~touched] == -7)
+    rows = torch.arange(40, device=DEV)
+    case.check(got[5:12], rows[5:12], rows[5:12] * 0)
+    case.check(got[30:32], rows[30:32], rows[30:32] * 0 + 2)
+    order = torch.tensor([-5, 2 ** 40, 79, 0], device=DEV)
+    one = torch.tensor([[0, 0, 0, 0, 4]], dtype=torch.int32, device=DEV)
+    case.check(case.grouped(one, order=order, k=2), torch.tensor([0, 39, 39, 0], device=DEV), order * 0)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_what_is_not_finite_stays_in_its_row(fmt):
+    """A NaN row and an infinite weight reach their own results only, also within a tile."""
+    case = Case(fmt, 2, 64, 512, 20)
+    ids = torch.arange(20, device=DEV) % 2
+    order, _, groups = kernels.expert_groups(ids.view(-1, 1), 2)
+    before = case.grouped(groups, order=order)
+    if fmt == "bf16":
+        case.x[6, 100] = float("nan")
+        case.w[64 + 9, 3] = float("inf")
+    else:
+        case.x.scale[6, 3] = 255
+        rows = mx.bank_rows(case.w)
+        rows.scale[64 + 9, 0] = 255
+        case.w = mx.bank(rows, 2)
+    for got, pair in ((case.grouped(groups, order=order), order), (case.gemv(ids), torch.arange(20, device=DEV))):
+        before_here = before[torch.argsort(order)][pair]
+        bad = (pair == 6)[:, None] | ((ids[pair] == 1)[:, None] & (torch.arange(64, device=DEV) == 9))
+        assert not torch.isfinite(got[bad]).any()
+        assert torch.equal(got[~bad], before_here[~bad])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_capture_and_streams(fmt):
+    """Captured in a graph and replayed with other inputs in place and eager work between, and run on a side stream."""
+    case = Case(fmt, 6, 96, 768, 50)
+    other = Case(fmt, 6, 96, 768, 50, seed=1)
+    ids = torch.from_numpy(np.random.default_rng(3).integers(0, 6, 50)).to(DEV)
+    order, _, groups = kernels.expert_groups(ids.view(-1, 1), 6)
+
+    def run(c):
+        return c.grouped(groups, order=order, swiglu=True), c.gemv(ids)
+
+    want, want2 = run(case), run(other)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        assert all(torch.equal(a, b) for a, b in zip(run(case), want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = run(case)
+    torch.cuda.current_stream().wait_stream(stream)
+    tensors = [(case.x, other.x)] if fmt == "bf16" else [(case.x.codes, other.x.codes), (case.x.scale, other.x.scale)]
+    kept = [a.clone() for a, _ in tensors]
+    for turn in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        if turn % 2 == 0:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        else:
+            row = torch.arange(50, device=DEV)
+            mixed = Case.__new__(Case)
+            mixed.__dict__.update(case.__dict__, xv=other.xv)
+            mixed.check(got[1], row, ids)
+        for (a, b), k in zip(tensors, kept):
+            a.copy_(b if turn % 2 == 0 else k)
+        run(other)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("fmt", ["mx8", "bf16"])
+def test_banks_beyond_32_bit_offsets(fmt):
+    """The last experts of a bank of more than 4 GiB."""
+    n, K = 2048, 2048
+    E = 560 if fmt == "bf16" else 2100
+    small = Case(fmt, 2, n, K, 6)
+    if fmt == "bf16":
+        w = torch.zeros((E * n, K), dtype=torch.bfloat16, device=DEV)
+        w[-2 * n:] = small.w
+    else:
+        w = mx.MxBank(torch.zeros((E * n, K // 2), dtype=torch.uint8, device=DEV),
+                      torch.zeros((E * n, K // 32), dtype=torch.uint8, device=DEV), E, n, K)
+        w.weight[-2 * n:], w.scale[-2 * n:] = small.w.weight, small.w.scale
+    assert (w if fmt == "bf16" else w.weight).nbytes > 2 ** 32
+    ids = torch.tensor([E - 1, E - 2, E - 1, E - 2, E - 2, E - 1], device=DEV)
+    groups = torch.tensor([[E - 2, 0, 0, 0, 2], [E - 1, 0, 0, 2, 4]], dtype=torch.int32, device=DEV)
+    want = small.gemv(ids - (E - 2))
+    want_grouped = small.grouped(groups - torch.tensor([E - 2, 0, 0, 0, 0], dtype=torch.int32, device=DEV))
+    small.w, small.E = w, E
+    assert torch.equal(small.gemv(ids), want)
+    assert torch.equal(small.grouped(groups), want_grouped)
