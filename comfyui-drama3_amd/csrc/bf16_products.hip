@@ -1,6 +1,7 @@
 // Expert products on banks of bfloat16 weights, as a checkpoint holds them before conversion: [E * N, K] row by row,
 // bfloat16 rows, float32 sums on the matrix cores.
 #include "expert_stream.hpp"
+#include "expert_wide.hpp"
 #include "products_host.hpp"
 #include "../../include/drama3_moe.h"
 
@@ -28,7 +29,7 @@ extern "C" int d3_bf16_grouped(const void* x, int32_t rows, const int64_t* order
   a.w = (const uint8_t*)w, a.E = E, a.N = N, a.stages = K / 64, a.out = out;
   if (const int rc = check_product("d3_bf16_grouped", a, K, 64, false, swiglu, true)) return rc;
   if (pairs == 0) return 0;
-  launch_stream<Bf16, 1>(a, swiglu, out_bf16, (hipStream_t)stream);
+  launch_grouped<Bf16>(a, swiglu, out_bf16, (hipStream_t)stream);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : hip_fail(e, "d3_bf16_grouped launch");
 }

@@ -228,12 +228,6 @@ void launch_stream_of(const ExpertProduct& a, int passes, hipStream_t s) {
                      dim3(ST_THREADS), 0, s, a, columns);
 }
 
-// passes of at most `most` rows that groups of `pairs` rows in all can have
-inline int most_passes(int pairs, int n_groups, int most) {
-  const int64_t n = (int64_t)pairs / most + n_groups;
-  return (int)(n < pairs ? n : pairs);
-}
-
 template <class F>
 void launch_gemv(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
   if (swiglu) launch_stream_of<F, true, true, true, 1, 1, 8>(a, a.pairs, s);

@@ -1,6 +1,7 @@
 // Expert products on microscaled banks (mx.hpp): e2m1 weights against e4m3 or e2m1 rows on the scaled matrix
 // instruction, both operands as they are stored.
 #include "expert_stream.hpp"
+#include "expert_wide.hpp"
 #include "products_host.hpp"
 #include "../../include/drama3_moe.h"
 
@@ -40,8 +41,8 @@ extern "C" int d3_mx_grouped(const void* codes, const void* scale, int32_t bits,
   if (const int rc = check_product("d3_mx_grouped", a, K, MX_BLOCK, true, swiglu, true)) return rc;
   if (pairs == 0) return 0;
   a.stages = mx_stages(K);
-  if (bits == 4) launch_stream<Mx<4>, 1>(a, swiglu, out_bf16, (hipStream_t)stream);
-  else launch_stream<Mx<8>, 1>(a, swiglu, out_bf16, (hipStream_t)stream);
+  if (bits == 4) launch_grouped<Mx<4>>(a, swiglu, out_bf16, (hipStream_t)stream);
+  else launch_grouped<Mx<8>>(a, swiglu, out_bf16, (hipStream_t)stream);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : hip_fail(e, "d3_mx_grouped launch");
 }

@@ -102,37 +102,54 @@ D3_INLINE f32x4 step_product(i32x4 a, const i32x4 (&b)[F::PIECES], f32x4 acc, ui
 // the next product reads
 D3_INLINE uint32_t swiglu_bf16(float gate, float up) { return f32_to_bf16(gate / (1.0f + __expf(-gate)) * up); }
 
-// Pass `at` of the groups' passes of at most `most` rows, in the groups' order: its expert, first place and rows (0: there
-// is no such pass). The whole wave calls; a group whose expert or rows lie outside the bank or the pairs has no pass.
 struct Pass {
   int expert, first, rows;
 };
+
+// group g's expert, first place and rows; no rows past the last group, and where the expert or the places lie outside the
+// bank or the pairs
+D3_INLINE void read_group(const ExpertProduct& a, int g, int& expert, int& first, int& rows) {
+  expert = first = rows = 0;
+  if (g >= a.n_groups) return;
+  const int32_t* p = a.groups + 5 * (size_t)g;
+  expert = p[0], first = p[3], rows = p[4];
+  if (expert < 0 || expert >= a.E || first < 0 || rows < 0 || first > a.pairs || rows > a.pairs - first) rows = 0;
+}
+
+// The first lane with at < the sum of n over the lanes up to it, and in `before` the sum over those before it; -1 if
+// there is none, with the sum over all. The whole wave calls.
+D3_INLINE int find_lane(int n, int at, int& before) {
+  const int lane = threadIdx.x & 63;
+  int incl = n;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(incl, d);
+    if (lane >= d) incl += u;
+  }
+  const uint64_t past = __ballot(incl > at);
+  if (!past) {
+    before = __builtin_amdgcn_readlane(incl, 63);
+    return -1;
+  }
+  const int l = __ffsll((unsigned long long)past) - 1;
+  before = __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l);
+  return l;
+}
+
+// Pass `at` of the groups' passes of at most `most` rows, in the groups' order: its expert, first place and rows (0: there
+// is no such pass). The whole wave calls.
 D3_INLINE Pass find_pass(const ExpertProduct& a, int most, int at) {
   const int lane = threadIdx.x & 63;
   for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
-    const int g = g0 + lane;
-    int expert = 0, first = 0, rows = 0;
-    if (g < a.n_groups) {
-      const int32_t* p = a.groups + 5 * (size_t)g;
-      expert = p[0], first = p[3], rows = p[4];
-      if (expert < 0 || expert >= a.E || first < 0 || rows < 0 || first > a.pairs || rows > a.pairs - first) rows = 0;
+    int expert, first, rows, before;
+    read_group(a, g0 + lane, expert, first, rows);
+    const int l = find_lane((rows + most - 1) / most, at, before);
+    if (l >= 0) {
+      const int from = (at - before) * most;
+      return Pass{__builtin_amdgcn_readlane(expert, l), __builtin_amdgcn_readlane(first, l) + from,
+                  min(most, __builtin_amdgcn_readlane(rows, l) - from)};
     }
-    const int np = (rows + most - 1) / most;
-    int incl = np;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(incl, d);
-      if (lane >= d) incl += u;
-    }
-    const uint64_t past = __ballot(incl > at);
-    if (past) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      const int nth = at - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(np, l));
-      const int all = __builtin_amdgcn_readlane(rows, l);
-      return Pass{__builtin_amdgcn_readlane(expert, l), __builtin_amdgcn_readlane(first, l) + nth * most,
-                  min(most, all - nth * most)};
-    }
-    at -= __builtin_amdgcn_readlane(incl, 63);
+    at -= before;
   }
   return Pass{0, 0, 0};
 }
@@ -142,6 +159,12 @@ D3_INLINE int row_at(const ExpertProduct& a, int p) {
   if (!a.order) return min(p, a.x_rows - 1);
   const int64_t pair = min<int64_t>(max<int64_t>(a.order[p], 0), INT32_MAX);
   return min((int)((uint32_t)pair / (uint32_t)a.k), a.x_rows - 1);
+}
+
+// passes of at most `most` rows that groups of `pairs` rows in all can have
+inline int most_passes(int pairs, int n_groups, int most) {
+  const int64_t n = (int64_t)pairs / most + n_groups;
+  return (int)(n < pairs ? n : pairs);
 }
 
 }  // namespace d3

@@ -204,7 +204,9 @@ def test_gemv(fmt, n, K):
     assert case.gemv(ids[:0]).shape == (0, n)
 
 
+# rows of the experts: few on average, and many (around a pass's 128 and 256 rows)
 COUNTS = [0, 1, 15, 16, 17, 31, 33, 0, 64, 65, 130, 3]
+MANY = [0, 1, 127, 128, 129, 255, 256, 257, 0, 300, 513, 33, 16, 191]
 
 
 def _pairs(E, counts, seed=1):
@@ -214,12 +216,14 @@ def _pairs(E, counts, seed=1):
     return ids, order, inverse, groups
 
 
-@pytest.mark.parametrize("n, K", [(16, 64), (32, 256), (96, 320), (288, 768), (160, 2048), (32, 2368)])
+@pytest.mark.parametrize("counts, n, K", [
+    (COUNTS, 16, 64), (COUNTS, 32, 256), (COUNTS, 96, 320), (COUNTS, 288, 768), (COUNTS, 160, 2048), (COUNTS, 32, 2368),
+    (MANY, 16, 64), (MANY, 32, 192), (MANY, 288, 256), (MANY, 544, 320), (MANY, 160, 2048), (MANY, 256, 1344)])
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_grouped_ragged(fmt, n, K):
-    E, P = len(COUNTS), sum(COUNTS)
+def test_grouped_ragged(fmt, counts, n, K):
+    E, P = len(counts), sum(counts)
     case = Case(fmt, E, n, K, P, spread=1.0)
-    ids, order, _, groups = _pairs(E, COUNTS)
+    ids, order, _, groups = _pairs(E, counts)
     for how in ({}, {"dtype": torch.bfloat16}, {"swiglu": True}):
         if n % 32 and "swiglu" in how:
             continue
