@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProd
   } else {
     pass = find_pass(a, ROWS, at);
     if (pass.rows == 0) return;
-    my_row = row_at(a, pass.first + min(lane, pass.rows - 1));
+    my_row = pair_row(a, pair_at(a, pass.first + min(lane, pass.rows - 1)));
   }
   // the wave's tiles of an expert's N / 16
   const int tiles = a.N / 16, half = tiles / 2;
@@ -181,10 +181,8 @@ __global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProd
     if (c == 0) other[w][q] = acc[0][0];
     __syncthreads();
     if (mine && !(w & 1) && c == 0) {
-      const f32x4 g = acc[0][0], u = other[w | 1][q];
       *(i32x2*)((uint16_t*)a.out + (size_t)pass.first * (a.N / 2) + tile[0] * 16 + 4 * q) =
-          i32x2{(int)(swiglu_bf16(g[0], u[0]) | swiglu_bf16(g[1], u[1]) << 16),
-                (int)(swiglu_bf16(g[2], u[2]) | swiglu_bf16(g[3], u[3]) << 16)};
+          swiglu_4(acc[0][0], other[w | 1][q]);
     }
   } else if (mine) {
 #pragma unroll
@@ -193,21 +191,14 @@ __global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProd
       if (r >= pass.rows) continue;
       const size_t p = (size_t)(pass.first + r);
       if constexpr (SWIGLU) {
-        const f32x4 g = acc[0][m], u = acc[NT - 1][m];
-        *(i32x2*)((uint16_t*)a.out + p * (a.N / 2) + tile[0] * 16 + 4 * q) =
-            i32x2{(int)(swiglu_bf16(g[0], u[0]) | swiglu_bf16(g[1], u[1]) << 16),
-                  (int)(swiglu_bf16(g[2], u[2]) | swiglu_bf16(g[3], u[3]) << 16)};
+        *(i32x2*)((uint16_t*)a.out + p * (a.N / 2) + tile[0] * 16 + 4 * q) = swiglu_4(acc[0][m], acc[NT - 1][m]);
       } else {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           if ((column * 4 + w) * NT + n >= tiles) continue;
-          const f32x4 v = acc[n][m];
           const size_t o = p * a.N + tile[n] * 16 + 4 * q;
-          if constexpr (OUT_BF16)
-            *(i32x2*)((uint16_t*)a.out + o) = i32x2{(int)(f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16),
-                                                    (int)(f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16)};
-          else
-            *(f32x4*)((float*)a.out + o) = v;
+          if constexpr (OUT_BF16) *(i32x2*)((uint16_t*)a.out + o) = bf16_4(acc[n][m]);
+          else *(f32x4*)((float*)a.out + o) = acc[n][m];
         }
       }
     }

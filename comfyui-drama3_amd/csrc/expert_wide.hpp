@@ -1,32 +1,18 @@
-// Expert products with many rows to an expert: 256 weight rows against up to 256 rows (128 e4m3 rows, which are twice as
-// wide) a workgroup, both operands of a stage in LDS, copied there without passing through registers while the
+// Expert products with many rows to an expert: 256 weight rows against up to 320 rows (160 e4m3 rows, which are twice as
+// wide) at a time, both operands of a stage in LDS, copied there without passing through registers while the
 // stage before is multiplied. 8 waves, 4 over the weight rows (64 each) and 2 over the rows' 16-row tiles (in turn).
+//
+// One workgroup a CU, which walks its share of the (pass, column) items and fetches the next item's first stage during the
+// last of this.
 #pragma once
 #include "expert_stream.hpp"
+
+#include <algorithm>
 
 namespace d3 {
 
 constexpr int WX_N = 256, WX_THREADS = 512;
-template <class F> constexpr int wx_tiles() { return 2048 / F::ROW; }  // of 16 rows a pass
-
-// Pass `at` of the groups' passes in wx_tiles tiles or fewer, an expert's passes as long as each other but for the last
-template <class F>
-D3_INLINE Pass find_wide_pass(const ExpertProduct& a, int at) {
-  const int lane = threadIdx.x & 63;
-  for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
-    int expert, first, rows;
-    read_group(a, g0 + lane, expert, first, rows);
-    const int np = wt_passes(rows, wx_tiles<F>());
-    int before;
-    const int l = find_lane(np, at, before);
-    if (l >= 0) {
-      const int all = __builtin_amdgcn_readlane(rows, l), step = 16 * wt_tiles(all, wx_tiles<F>()), from = (at - before) * step;
-      return Pass{__builtin_amdgcn_readlane(expert, l), __builtin_amdgcn_readlane(first, l) + from, min(step, all - from)};
-    }
-    at -= before;
-  }
-  return Pass{0, 0, 0};
-}
+template <class F> constexpr int wx_tiles() { return 2560 / F::ROW; }  // of 16 rows a pass
 
 // 4 bytes per lane from base + off (the lane's own) into LDS at lds + 4 * lane: dma16's rules (wide_tile.hpp)
 D3_INLINE void dma4(uint32_t lds, const void* base, uint32_t off) {
@@ -40,136 +26,232 @@ D3_INLINE void dma4(uint32_t lds, const void* base, uint32_t off) {
                : "memory");
 }
 
-// the place in LDS of piece j (16 bytes) of row r of a stage, and where it comes from (the same swap)
+// the place in LDS of piece j (16 bytes) of row r of a stage: 16 lanes that read one (s, q) of 16 rows, and the mixed
+// groups of lanes that a 16-byte read takes together, meet 16 different groups of banks
 template <class F>
 D3_INLINE int wx_slot(int r, int j) {
-  return F::ROW == 128 ? wt_slot(r, j) : j ^ (r & 15);
+  return F::ROW == 128 ? ((j >> 1) | ((j & 1) << 2)) ^ ((r >> 1) & 7) : j ^ (r & 15);
+}
+// the piece in place t of row r
+template <class F>
+D3_INLINE int wx_piece(int r, int t) {
+  if constexpr (F::ROW != 128) return t ^ (r & 15);
+  const int p = t ^ ((r >> 1) & 7);
+  return ((p & 3) << 1) | (p >> 2);
+}
+
+// The passes of 64 items at once, one a lane: pass `at` (each lane's own) of the groups' passes in wx_tiles tiles or
+// fewer, an expert's passes as long as each other but for the last; no rows where there is no such pass.
+template <class F>
+D3_INLINE Pass wide_passes(const ExpertProduct& a, int at) {
+  const int lane = threadIdx.x & 63;
+  Pass mine{0, 0, 0};
+  bool found = false;
+  for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
+    int expert, first, rows;
+    read_group(a, g0 + lane, expert, first, rows);
+    const int np = wt_passes(rows, wx_tiles<F>());
+    int incl = np;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(incl, d);
+      if (lane >= d) incl += u;
+    }
+    const int all = __builtin_amdgcn_readlane(incl, 63);
+    int l = 0;  // the first lane whose sum is past `at`
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+      if (__shfl(incl, l + d - 1) <= at) l += d;
+    const int before = __shfl(incl - np, l), n = __shfl(rows, l), e = __shfl(expert, l), f = __shfl(first, l);
+    if (!found && at < all) {
+      const int step = 16 * wt_tiles(n, wx_tiles<F>()), from = (at - before) * step;
+      mine = Pass{e, f + from, min(step, n - from)};
+      found = true;
+    }
+    at -= all;
+  }
+  return mine;
 }
 
 template <class F, bool SWIGLU, bool OUT_BF16>
-__global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduct a, int columns) {
+__global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduct a, int columns, int items) {
   constexpr int TILES = wx_tiles<F>(), ROWS = 16 * TILES, A_BYTES = WX_N * 128, STAGE = A_BYTES + ROWS * F::ROW;
-  constexpr int PER = 1024 / F::ROW;            // rows of a 1 KB copy
-  constexpr int COPIES = ROWS / PER / 8;        // of the rows, per wave
+  constexpr int PER = 1024 / F::ROW, LANES = 64 / PER;  // rows of a 1 KB copy, lanes to a row of it
+  constexpr int COPIES = ROWS / PER / 8;                // of the rows, per wave
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
-  __shared__ __attribute__((aligned(16))) uint8_t xscale[2][F::SCALED ? 8 * ROWS : 16];
-  int at, column;
-  wt_place(blockIdx.x, columns, at, column);
-  const Pass pass = find_wide_pass<F>(a, at);
-  if (pass.rows == 0) return;
-  const int expert = __builtin_amdgcn_readfirstlane(pass.expert), first = __builtin_amdgcn_readfirstlane(pass.first),
-            rows = __builtin_amdgcn_readfirstlane(pass.rows), tiles = (rows + 15) / 16;
+  __shared__ __attribute__((aligned(256))) uint8_t xscale[2][F::SCALED ? 8 * ROWS : 256];
+  __shared__ __attribute__((aligned(256))) uint32_t wscale[2][F::SCALED ? 16 * 64 : 64];  // by stage pair: tile, lane
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, c = lane & 15, wn = w & 3, wm = w >> 2;
   const int S = a.stages, bank_tiles = a.N / 16, half = bank_tiles / 2;
   const uint32_t lds0 = lds_address(smem);
-  // the expert's tile in place `slot` of the workgroup's 16 (a place past the expert's last repeats that)
-  auto tile_of = [&](int slot) __attribute__((always_inline)) {
-    if constexpr (SWIGLU) return min(8 * column + 2 * (slot >> 2) + (slot & 1), half - 1) + ((slot >> 1) & 1) * half;
-    else return min(16 * column + slot, bank_tiles - 1);
-  };
-
-  // weights: wave w copies the places 2 w and 2 w + 1, two copies of 1 KB each
-  const uint8_t* src[2];
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-    src[i] = a.w + ((size_t)expert * bank_tiles + tile_of(2 * w + i)) * ((size_t)S * 2048);
-  uint32_t woff[2];  // from a stage's start, for the two copies
+  uint32_t woff[2];  // a lane's place in a stage of a tile, for the tile's two copies
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const int r = 8 * i + (lane >> 3);
-    woff[i] = F::SCALED ? 1024 * i + 16 * lane : (uint32_t)(r * S * 128 + 16 * wt_slot(r, lane & 7));
+    woff[i] = F::SCALED ? 1024 * i + 16 * lane : (uint32_t)(r * S * 128 + 16 * wx_piece<F>(r, lane & 7));
   }
-  // rows: wave w takes the copies w, w + 8, ..
-  uint32_t xoff[COPIES];
-#pragma unroll
-  for (int i = 0; i < COPIES; i++) {
-    const int r = PER * (w + 8 * i) + lane / (64 / PER);
-    xoff[i] = (uint32_t)row_at(a, first + min(r, rows - 1)) * (uint32_t)(S * F::ROW) +
-              16 * wx_slot<F>(r, lane % (64 / PER));
-  }
-  uint32_t soff = 0;  // scales: lane's word of the stage's 8 bytes a row
-  if constexpr (F::SCALED) soff = (uint32_t)row_at(a, first + min(tid >> 1, rows - 1)) * (uint32_t)(8 * S) + 4 * (tid & 1);
-  auto load = [&](int st, int buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-        dma16(lds0 + buf * STAGE + (2 * w + i) * 2048 + 1024 * j, src[i] + (size_t)st * F::A_STAGE, woff[j]);
-#pragma unroll
-    for (int i = 0; i < COPIES; i++)
-      if (PER * (w + 8 * i) < 16 * tiles)
-        dma16(lds0 + buf * STAGE + A_BYTES + (uint32_t)(w + 8 * i) * 1024, a.x + (size_t)st * F::ROW, xoff[i]);
-    if constexpr (F::SCALED)
-      if (w * 32 < 16 * tiles) dma4(lds_address(xscale[buf]) + 256 * w, a.x_scale + 8 * st, soff);
-  };
-  const uint32_t* wscale[4];  // a lane's scale words of its wave's tiles
-#pragma unroll
-  for (int n = 0; n < 4; n++)
-    wscale[n] = (const uint32_t*)(a.w_scale + (((size_t)expert * bank_tiles + tile_of(4 * wn + n)) * 64 + lane) *
-                                                  mx_lane_scales(S));
-  load(0, 0);
 
-  // A wave's tiles: rows 16 (wm + 2 j) .., j < NT (tiles past the pass's run on what lies there and store nothing)
+  // The workgroup's items: every gridDim.x-th of the list, 64 of them looked up at a time (lane i: item i)
+  Pass table;
+  int taken = 64, lin = (int)blockIdx.x - (int)gridDim.x;
+  struct Item {
+    int expert, first, rows, column;
+  };
+  auto next_item = [&](Item& t) __attribute__((always_inline)) {
+    t.rows = 0;
+    while (t.rows == 0) {
+      lin += gridDim.x;
+      if (lin >= items) return;
+      if (taken == 64) {
+        int at, column;
+        wt_place(lin + lane * gridDim.x, columns, at, column);
+        table = wide_passes<F>(a, at);
+        taken = 0;
+      }
+      int at;
+      wt_place(lin, columns, at, t.column);
+      t.expert = __builtin_amdgcn_readlane(table.expert, taken), t.first = __builtin_amdgcn_readlane(table.first, taken);
+      t.rows = __builtin_amdgcn_readlane(table.rows, taken);
+      taken++;
+    }
+  };
+  // where the item's operands lie
+  const uint8_t* src[2];  // wave w copies the weight tiles in places 2 w and 2 w + 1
+  const uint8_t* word[2];  // those tiles' scales
+  uint32_t xoff[COPIES], soff[2];  // the rows' copies w, w + 8, .. and their scale words w, w + 8 of 64
+  // the pairs whose rows those are: lane l that of copy l / PER, l % PER, and of scale words l / 32, l % 32
+  int64_t pair_x = 0, pair_s = 0;
+  auto find_pairs = [&](const Item& t) __attribute__((always_inline)) {
+    pair_x = pair_at(a, t.first + min(PER * (w + 8 * (lane / PER)) + lane % PER, t.rows - 1));
+    if constexpr (F::SCALED) pair_s = pair_at(a, t.first + min(32 * (w + 8 * (lane >> 5)) + (lane & 31), t.rows - 1));
+  };
+  auto find_places = [&](const Item& t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      // the expert's tile in the place of the 16 (a place past the expert's last tile repeats that)
+      const int slot = 2 * w + i;
+      const int tile = SWIGLU ? min(8 * t.column + 2 * (slot >> 2) + (slot & 1), half - 1) + ((slot >> 1) & 1) * half
+                              : min(16 * t.column + slot, bank_tiles - 1);
+      const size_t at = (size_t)t.expert * bank_tiles + tile;
+      src[i] = a.w + at * ((size_t)S * 2048);
+      word[i] = a.w_scale + at * (64 * (size_t)mx_lane_scales(S));
+    }
+    const int row_x = pair_row(a, pair_x), row_s = F::SCALED ? pair_row(a, pair_s) : 0;
+#pragma unroll
+    for (int i = 0; i < COPIES; i++) {
+      const int r = PER * (w + 8 * i) + lane / LANES;
+      xoff[i] = (uint32_t)__shfl(row_x, PER * i + lane / LANES) * (uint32_t)(S * F::ROW) + 16 * wx_piece<F>(r, lane % LANES);
+    }
+    if constexpr (F::SCALED) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) soff[i] = (uint32_t)__shfl(row_s, 32 * i + (lane >> 1)) * (uint32_t)(8 * S) + 4 * (lane & 1);
+    }
+  };
+  // copy k of a stage's weights and rows, and its scale words
+  auto load_weights = [&](int k, int st, int buf) __attribute__((always_inline)) {
+    dma16(lds0 + buf * STAGE + (2 * w + (k >> 1)) * 2048 + 1024 * (k & 1), src[k >> 1] + (size_t)st * F::A_STAGE, woff[k & 1]);
+  };
+  auto load_rows = [&](int k, int st, int buf) __attribute__((always_inline)) {
+    dma16(lds0 + buf * STAGE + A_BYTES + (uint32_t)(w + 8 * k) * 1024, a.x + (size_t)st * F::ROW, xoff[k]);
+  };
+  auto load_scales = [&](int st, int buf, int pair, int rows) __attribute__((always_inline)) {
+    if constexpr (F::SCALED) {
+#pragma unroll
+      for (int k = 0; k < (ROWS + 255) / 256; k++)
+        if (32 * (w + 8 * k) < rows) dma4(lds_address(xscale[buf]) + 256 * (w + 8 * k), a.x_scale + 8 * st, soff[k]);
+      if ((st & 1) == 0) {
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+          dma4(lds_address(wscale[pair]) + 256 * (2 * w + k), word[k] + 2 * st, lane * mx_lane_scales(S));
+      }
+    }
+  };
+
+  Item cur, nxt;
+  next_item(cur);
+  if (cur.rows == 0) return;
+  find_pairs(cur);
+  find_places(cur);
+  int buf = 0, pair = 1;  // the buffers of the stage and of the pair of stages (for its scale words)
+#pragma unroll
+  for (int k = 0; k < 4; k++) load_weights(k, 0, 0);
+#pragma unroll
+  for (int k = 0; k < COPIES; k++)
+    if (PER * (w + 8 * k) < cur.rows) load_rows(k, 0, 0);
+  load_scales(0, 0, 0, cur.rows);
+  next_item(nxt);
+
+  // An item's products. A wave's tiles: rows 16 (wm + 2 j) .., j < NT (tiles past the pass's run on what lies there and
+  // store nothing)
   auto run = [&]<int NT>() __attribute__((always_inline)) {
     f32x4 acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; j++)
 #pragma unroll
       for (int n = 0; n < 4; n++) acc[j][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t sw[4] = {0, 0, 0, 0}, sw_next[4] = {0, 0, 0, 0};
-    if constexpr (F::SCALED) {
-#pragma unroll
-      for (int n = 0; n < 4; n++) sw_next[n] = wscale[n][0];
-    }
     dma_wait();
     __syncthreads();
-    for (int st = 0; st < S; st++) {
-      const int buf = st & 1;
+    for (int st = 0; st < S; st++, buf ^= 1) {
+      if ((st & 1) == 0) pair ^= 1;
       const uint8_t* wbase = smem + buf * STAGE;
-      const uint8_t* xbase = wbase + A_BYTES;
-      i32x4 wa[4][2], b[2][2][F::PIECES];
-      uint32_t sb[2];
-      auto read_x = [&](int j) __attribute__((always_inline)) {
-        const int r = 16 * (wm + 2 * j) + c;
+      const uint8_t* xlane[2][F::PIECES];  // this lane's operands of the wave's first tile
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+      for (int s = 0; s < 2; s++)
 #pragma unroll
-          for (int i = 0; i < F::PIECES; i++)
-            b[j & 1][s][i] = *(const i32x4*)(xbase + r * F::ROW + 16 * wx_slot<F>(c, F::b_piece(s, q, i)));
-        sb[j & 1] = F::SCALED ? *(const uint16_t*)(xscale[buf] + 8 * r + 2 * q) : 0u;
+        for (int k = 0; k < F::PIECES; k++)
+          xlane[s][k] = wbase + A_BYTES + (16 * wm + c) * F::ROW + 16 * wx_slot<F>(c, F::b_piece(s, q, k));
+      const uint8_t* slane = xscale[buf] + 8 * (16 * wm + c) + 2 * q;
+      i32x4 wa[4], b[4][F::PIECES];
+      uint32_t sw[4] = {0, 0, 0, 0}, sb[4] = {0, 0, 0, 0};
+      auto read_w = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+          wa[n] = *(const i32x4*)(wbase + (4 * wn + n) * 2048 +
+                                     (F::SCALED ? 1024 * s + 16 * lane : c * 128 + 16 * wx_slot<F>(c, 2 * q + s)));
       };
+      auto read_x = [&](int i) __attribute__((always_inline)) {  // operand i: tile i % NT, step i / NT
 #pragma unroll
-      for (int n = 0; n < 4; n++)
-#pragma unroll
-        for (int s = 0; s < 2; s++)
-          wa[n][s] = *(const i32x4*)(wbase + (4 * wn + n) * 2048 +
-                                     (F::SCALED ? 1024 * s + 16 * lane : c * 128 + 16 * wt_slot(c, 2 * q + s)));
+        for (int k = 0; k < F::PIECES; k++) b[i & 3][k] = *(const i32x4*)(xlane[i / NT][k] + (i % NT) * 32 * F::ROW);
+        if constexpr (F::SCALED) sb[i & 3] = *(const uint16_t*)(slane + (i % NT) * 256);
+      };
+      read_w(0);
       read_x(0);
       if constexpr (F::SCALED) {
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-          if (st & 1) sw[n] >>= 16;
-          else sw[n] = sw_next[n];
-        }
+        for (int n = 0; n < 4; n++) sw[n] = wscale[pair][64 * (4 * wn + n) + lane] >> (16 * (st & 1));
       }
-      if (st + 1 < S) {
-        load(st + 1, buf ^ 1);
-        if constexpr (F::SCALED) {
-          if (st & 1) {
+      read_x(1);
+      // The next stage's copies, of this item or the next, go out between the products: those that this item's rows need
+      // without a branch (after the last item they copy what is there once more). Whatever branches stands before the
+      // products, which the compiler would move past it, with all their operands waiting in registers.
+      const bool last = st + 1 == S;
+      if (nxt.rows && (st + 2 == S || S == 1)) find_pairs(nxt);  // for the next stage
+      if (last && nxt.rows) find_places(nxt);
+      const int st_next = last ? 0 : st + 1;
+      load_scales(st_next, buf ^ 1, pair ^ 1, last ? nxt.rows : cur.rows);
+      constexpr int MINE = (32 * NT / PER + 7) / 8, SPREAD = (4 + MINE + NT - 1) / NT;  // copies; to a group of products
+      if (last) {
 #pragma unroll
-            for (int n = 0; n < 4; n++) sw_next[n] = wscale[n][(st + 1) / 2];
-          }
-        }
+        for (int k = MINE; k < COPIES; k++)
+          if (PER * (w + 8 * k) < nxt.rows) load_rows(k, 0, buf ^ 1);
       }
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        if (j + 1 < NT) read_x(j + 1);
+      for (int i = 0; i < 2 * NT; i++) {
+        if (i == NT) read_w(1);
+        if (i + 2 < 2 * NT) read_x(i + 2);
         __builtin_amdgcn_sched_barrier(0);  // the reads first
+        const int j = i % NT;
 #pragma unroll
-        for (int n = 0; n < 4; n++) acc[j][n] = step_product<F, !OUT_BF16, 0, 0>(wa[n][0], b[j & 1][0], acc[j][n], sw[n], sb[j & 1]);
+        for (int n = 0; n < 4; n++) {
+          if (i < NT) acc[j][n] = step_product<F, !OUT_BF16, 0, 0>(wa[n], b[i & 3], acc[j][n], sw[n], sb[i & 3]);
+          else acc[j][n] = step_product<F, !OUT_BF16, 1, 1>(wa[n], b[i & 3], acc[j][n], sw[n], sb[i & 3]);
+        }
 #pragma unroll
-        for (int n = 0; n < 4; n++) acc[j][n] = step_product<F, !OUT_BF16, 1, 1>(wa[n][1], b[j & 1][1], acc[j][n], sw[n], sb[j & 1]);
+        for (int k = SPREAD * i; k < SPREAD * (i + 1) && k < 4 + MINE; k++) {
+          if (k < 4) load_weights(k, st_next, buf ^ 1);
+          else load_rows(k - 4, st_next, buf ^ 1);
+        }
       }
       dma_wait();
       __syncthreads();
@@ -179,49 +261,65 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
 #pragma unroll
     for (int j = 0; j < NT; j++) {
       const int r = 16 * (wm + 2 * j) + c;
-      if (r >= rows) continue;
-      const size_t p = (size_t)(first + r);
+      if (r >= cur.rows) continue;
+      const size_t p = (size_t)(cur.first + r);
       if constexpr (SWIGLU) {
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-          const int unit = 8 * column + 2 * wn + n;
+          const int unit = 8 * cur.column + 2 * wn + n;
           if (unit >= half) continue;
-          const f32x4 g = acc[j][n], u = acc[j][n + 2];
-          *(i32x2*)((uint16_t*)a.out + p * (a.N / 2) + 16 * unit + 4 * q) =
-              i32x2{(int)(swiglu_bf16(g[0], u[0]) | swiglu_bf16(g[1], u[1]) << 16),
-                    (int)(swiglu_bf16(g[2], u[2]) | swiglu_bf16(g[3], u[3]) << 16)};
+          *(i32x2*)((uint16_t*)a.out + p * (a.N / 2) + 16 * unit + 4 * q) = swiglu_4(acc[j][n], acc[j][n + 2]);
         }
       } else {
 #pragma unroll
         for (int n = 0; n < 4; n++) {
-          const int tile = 16 * column + 4 * wn + n;
+          const int tile = 16 * cur.column + 4 * wn + n;
           if (tile >= bank_tiles) continue;
-          const f32x4 v = acc[j][n];
           const size_t o = p * a.N + 16 * tile + 4 * q;
-          if constexpr (OUT_BF16)
-            *(i32x2*)((uint16_t*)a.out + o) = i32x2{(int)(f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16),
-                                                    (int)(f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16)};
-          else
-            *(f32x4*)((float*)a.out + o) = v;
+          if constexpr (OUT_BF16) *(i32x2*)((uint16_t*)a.out + o) = bf16_4(acc[j][n]);
+          else *(f32x4*)((float*)a.out + o) = acc[j][n];
         }
       }
     }
   };
-  if constexpr (TILES > 8) {
-    if (tiles > 12) return run.template operator()<8>();
-    if (tiles > 8) return run.template operator()<6>();
+  while (true) {
+    const int mine = ((cur.rows + 15) / 16 + 1) / 2;  // tiles of a wave, at most
+    if constexpr (TILES > 10) {
+      if (mine > 9) run.template operator()<10>();
+      else if (mine > 8) run.template operator()<9>();
+      else if (mine > 7) run.template operator()<8>();
+      else if (mine > 6) run.template operator()<7>();
+      else if (mine > 5) run.template operator()<6>();
+    }
+    if (TILES <= 10 || mine <= 5) {
+      if (mine > 4) run.template operator()<5>();
+      else if (mine > 3) run.template operator()<4>();
+      else if (mine > 2) run.template operator()<3>();
+      else run.template operator()<2>();
+    }
+    if (nxt.rows == 0) return;
+    cur = nxt;
+    next_item(nxt);
   }
-  if (tiles > 4) run.template operator()<4>();
-  else run.template operator()<2>();
+}
+
+// compute units of the current device
+inline int device_cus() {
+  int device = 0, n = 0;
+  if (hipGetDevice(&device) != hipSuccess ||
+      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n < 1)
+    return 256;
+  return n;
 }
 
 template <class F>
 void launch_wide(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
   const int columns = (a.N + WX_N - 1) / WX_N, passes = most_passes(a.pairs, a.n_groups, 16 * wx_tiles<F>());
-  const dim3 grid((unsigned)(wt_places(passes) * columns)), block(WX_THREADS);
-  if (swiglu) hipLaunchKernelGGL((expert_wide_kernel<F, true, true>), grid, block, 0, s, a, columns);
-  else if (out_bf16) hipLaunchKernelGGL((expert_wide_kernel<F, false, true>), grid, block, 0, s, a, columns);
-  else hipLaunchKernelGGL((expert_wide_kernel<F, false, false>), grid, block, 0, s, a, columns);
+  const int items = wt_places(passes) * columns;
+  const dim3 grid((unsigned)std::min(items, device_cus())), block(WX_THREADS);
+  if (swiglu) hipLaunchKernelGGL((expert_wide_kernel<F, true, true>), grid, block, 0, s, a, columns, items);
+  else if (out_bf16) hipLaunchKernelGGL((expert_wide_kernel<F, false, true>), grid, block, 0, s, a, columns, items);
+  else hipLaunchKernelGGL((expert_wide_kernel<F, false, false>), grid, block, 0, s, a, columns, items);
 }
 
 // Whether a grouped product runs in wide passes: by the rows an expert has on average. (The copies to LDS take 32-bit

@@ -98,9 +98,19 @@ D3_INLINE f32x4 step_product(i32x4 a, const i32x4 (&b)[F::PIECES], f32x4 acc, ui
   }
 }
 
-// SiLU(gate) * up in float32 (float32 exp and division: within 2^-21 of the value), rounded to bf16 as the rows that
-// the next product reads
-D3_INLINE uint32_t swiglu_bf16(float gate, float up) { return f32_to_bf16(gate / (1.0f + __expf(-gate)) * up); }
+// four float32 sums rounded to bf16 (to nearest, ties to even, by the converter)
+D3_INLINE i32x2 bf16_4(f32x4 v) {
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(i32x2, __builtin_convertvector(v, bf16x4));
+}
+// SiLU(gate) * up in float32, then rounded to bf16 as the rows that the next product reads. exp and the reciprocal are the
+// hardware's, within 2 and 1 units of the last place: about 2^-21 of the value, which the rounding's 2^-9 hides.
+D3_INLINE i32x2 swiglu_4(f32x4 gate, f32x4 up) {
+  f32x4 h;
+#pragma unroll
+  for (int i = 0; i < 4; i++) h[i] = gate[i] * __builtin_amdgcn_rcpf(1.0f + __expf(-gate[i])) * up[i];
+  return bf16_4(h);
+}
 
 struct Pass {
   int expert, first, rows;
@@ -154,11 +164,11 @@ D3_INLINE Pass find_pass(const ExpertProduct& a, int most, int at) {
   return Pass{0, 0, 0};
 }
 
-// the row of x of the pair at place p
-D3_INLINE int row_at(const ExpertProduct& a, int p) {
-  if (!a.order) return min(p, a.x_rows - 1);
-  const int64_t pair = min<int64_t>(max<int64_t>(a.order[p], 0), INT32_MAX);
-  return min((int)((uint32_t)pair / (uint32_t)a.k), a.x_rows - 1);
+// the pair at place p, and the row of x of a pair
+D3_INLINE int64_t pair_at(const ExpertProduct& a, int p) { return a.order ? a.order[p] : p; }
+D3_INLINE int pair_row(const ExpertProduct& a, int64_t pair) {
+  const uint32_t at = (uint32_t)min<int64_t>(max<int64_t>(pair, 0), INT32_MAX);
+  return min((int)(a.order ? at / (uint32_t)a.k : at), a.x_rows - 1);
 }
 
 // passes of at most `most` rows that groups of `pairs` rows in all can have
