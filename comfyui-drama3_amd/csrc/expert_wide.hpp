@@ -2,8 +2,10 @@
 // wide) at a time, both operands of a stage in LDS, copied there without passing through registers while the
 // stage before is multiplied. 8 waves, 4 over the weight rows (64 each) and 2 over the rows' 16-row tiles (in turn).
 //
-// One workgroup a CU, which walks its share of the (pass, column) items and fetches the next item's first stage during the
-// last of this.
+// One workgroup a CU, which walks its share of the (pass, column) items as one stream of stages: the copies of the next
+// item begin during the last stages of this. The rows, which other columns' workgroups read too, are copied a stage ahead;
+// the weights come from HBM and are copied by halves of a stage (a step), three ahead, so that there are always some on
+// their way: with whole stages, one ahead, a stage of bf16 took 4200 clocks, of which the products take 2200.
 #pragma once
 #include "expert_stream.hpp"
 
@@ -26,19 +28,29 @@ D3_INLINE void dma4(uint32_t lds, const void* base, uint32_t off) {
                : "memory");
 }
 
+// all but the N last of this wave's loads have come
+template <int N>
+D3_INLINE void wait_loads() {
+  static_assert(N < 64);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // the place in LDS of piece j (16 bytes) of row r of a stage: 16 lanes that read one (s, q) of 16 rows, and the mixed
 // groups of lanes that a 16-byte read takes together, meet 16 different groups of banks
 template <class F>
 D3_INLINE int wx_slot(int r, int j) {
-  return F::ROW == 128 ? ((j >> 1) | ((j & 1) << 2)) ^ ((r >> 1) & 7) : j ^ (r & 15);
+  if constexpr (F::ROW != 128) return j ^ (r & 15);
+  return (F::SCALED ? (j >> 1) | ((j & 1) << 2) : j) ^ ((r >> 1) & 7);
 }
 // the piece in place t of row r
 template <class F>
 D3_INLINE int wx_piece(int r, int t) {
   if constexpr (F::ROW != 128) return t ^ (r & 15);
   const int p = t ^ ((r >> 1) & 7);
-  return ((p & 3) << 1) | (p >> 2);
+  return F::SCALED ? ((p & 3) << 1) | (p >> 2) : p;
 }
+// the same of bf16 weights by the step, 64 bytes a row: piece q of row r of 16
+D3_INLINE int wx_step_slot(int r, int q) { return q ^ ((4 - (r >> 2)) & 3); }
 
 // The passes of 64 items at once, one a lane: pass `at` (each lane's own) of the groups' passes in wx_tiles tiles or
 // fewer, an expert's passes as long as each other but for the last; no rows where there is no such pass.
@@ -75,22 +87,20 @@ D3_INLINE Pass wide_passes(const ExpertProduct& a, int at) {
 
 template <class F, bool SWIGLU, bool OUT_BF16>
 __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduct a, int columns, int items) {
-  constexpr int TILES = wx_tiles<F>(), ROWS = 16 * TILES, A_BYTES = WX_N * 128, STAGE = A_BYTES + ROWS * F::ROW;
+  constexpr int TILES = wx_tiles<F>(), ROWS = 16 * TILES, STEP = WX_N * 64, STAGE = ROWS * F::ROW;
   constexpr int PER = 1024 / F::ROW, LANES = 64 / PER;  // rows of a 1 KB copy, lanes to a row of it
   constexpr int COPIES = ROWS / PER / 8;                // of the rows, per wave
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
-  __shared__ __attribute__((aligned(256))) uint8_t xscale[2][F::SCALED ? 8 * ROWS : 256];
+  constexpr int SCOPIES = F::SCALED ? (ROWS + 255) / 256 : 0;  // of the rows' scale words, per wave
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * STEP + 2 * STAGE];  // four steps' weights, two stages' rows
+  __shared__ __attribute__((aligned(256))) uint8_t xscale[2][F::SCALED ? 2048 * SCOPIES : 16];
   __shared__ __attribute__((aligned(256))) uint32_t wscale[2][F::SCALED ? 16 * 64 : 64];  // by stage pair: tile, lane
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, c = lane & 15, wn = w & 3, wm = w >> 2;
   const int S = a.stages, bank_tiles = a.N / 16, half = bank_tiles / 2;
   const uint32_t lds0 = lds_address(smem);
-  uint32_t woff[2];  // a lane's place in a stage of a tile, for the tile's two copies
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int r = 8 * i + (lane >> 3);
-    woff[i] = F::SCALED ? 1024 * i + 16 * lane : (uint32_t)(r * S * 128 + 16 * wx_piece<F>(r, lane & 7));
-  }
+  // a lane's place in a step of a tile
+  const uint32_t woff = F::SCALED ? 16 * lane
+                                  : (uint32_t)((lane >> 2) * S * 128 + 16 * wx_step_slot(lane >> 2, lane & 3));
 
   // The workgroup's items: every gridDim.x-th of the list, 64 of them looked up at a time (lane i: item i)
   Pass table;
@@ -116,27 +126,31 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
       taken++;
     }
   };
-  // where the item's operands lie
-  const uint8_t* src[2];  // wave w copies the weight tiles in places 2 w and 2 w + 1
-  const uint8_t* word[2];  // those tiles' scales
-  uint32_t xoff[COPIES], soff[2];  // the rows' copies w, w + 8, .. and their scale words w, w + 8 of 64
-  // the pairs whose rows those are: lane l that of copy l / PER, l % PER, and of scale words l / 32, l % 32
-  int64_t pair_x = 0, pair_s = 0;
-  auto find_pairs = [&](const Item& t) __attribute__((always_inline)) {
-    pair_x = pair_at(a, t.first + min(PER * (w + 8 * (lane / PER)) + lane % PER, t.rows - 1));
-    if constexpr (F::SCALED) pair_s = pair_at(a, t.first + min(32 * (w + 8 * (lane >> 5)) + (lane & 31), t.rows - 1));
+  // where an item's weights lie: wave w copies the tiles in places 2 w and 2 w + 1, and their scales
+  struct Weights {
+    const uint8_t *src[2], *word[2];
   };
-  auto find_places = [&](const Item& t) __attribute__((always_inline)) {
+  auto find_weights = [&](const Item& t, Weights& at) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       // the expert's tile in the place of the 16 (a place past the expert's last tile repeats that)
       const int slot = 2 * w + i;
       const int tile = SWIGLU ? min(8 * t.column + 2 * (slot >> 2) + (slot & 1), half - 1) + ((slot >> 1) & 1) * half
                               : min(16 * t.column + slot, bank_tiles - 1);
-      const size_t at = (size_t)t.expert * bank_tiles + tile;
-      src[i] = a.w + at * ((size_t)S * 2048);
-      word[i] = a.w_scale + at * (64 * (size_t)mx_lane_scales(S));
+      const size_t n = (size_t)t.expert * bank_tiles + tile;
+      at.src[i] = a.w + n * ((size_t)S * 2048);
+      at.word[i] = a.w_scale + n * (64 * (size_t)mx_lane_scales(S));
     }
+  };
+  // and its rows
+  uint32_t xoff[COPIES], soff[2];  // the copies w, w + 8, .. and their scale words w, w + 8 of 64
+  // the pairs whose rows those are: lane l that of copy l / PER, l % PER, and of scale words l / 32, l % 32
+  int64_t pair_x = 0, pair_s = 0;
+  auto find_pairs = [&](const Item& t) __attribute__((always_inline)) {
+    pair_x = pair_at(a, t.first + min(PER * (w + 8 * (lane / PER)) + lane % PER, t.rows - 1));
+    if constexpr (F::SCALED) pair_s = pair_at(a, t.first + min(32 * (w + 8 * (lane >> 5)) + (lane & 31), t.rows - 1));
+  };
+  auto find_rows = [&]() __attribute__((always_inline)) {
     const int row_x = pair_row(a, pair_x), row_s = F::SCALED ? pair_row(a, pair_s) : 0;
 #pragma unroll
     for (int i = 0; i < COPIES; i++) {
@@ -148,39 +162,47 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
       for (int i = 0; i < 2; i++) soff[i] = (uint32_t)__shfl(row_s, 32 * i + (lane >> 1)) * (uint32_t)(8 * S) + 4 * (lane & 1);
     }
   };
-  // copy k of a stage's weights and rows, and its scale words
-  auto load_weights = [&](int k, int st, int buf) __attribute__((always_inline)) {
-    dma16(lds0 + buf * STAGE + (2 * w + (k >> 1)) * 2048 + 1024 * (k & 1), src[k >> 1] + (size_t)st * F::A_STAGE, woff[k & 1]);
+  Item cur, nxt;
+  Weights at, at_next;
+  // the copies of step s of stage st (from the next item where this one ends) to step buffer `to`
+  auto load_weights = [&](int st, int s, int to) __attribute__((always_inline)) {
+    const bool here = st < S || nxt.rows == 0;
+    st = st < S ? st : nxt.rows ? st - S : S - 1;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      dma16(lds0 + to * STEP + (2 * w + i) * 1024, (here ? at.src[i] : at_next.src[i]) + (size_t)st * F::A_STAGE + s * F::A_STEP,
+            woff);
   };
   auto load_rows = [&](int k, int st, int buf) __attribute__((always_inline)) {
-    dma16(lds0 + buf * STAGE + A_BYTES + (uint32_t)(w + 8 * k) * 1024, a.x + (size_t)st * F::ROW, xoff[k]);
+    dma16(lds0 + 4 * STEP + buf * STAGE + (uint32_t)(w + 8 * k) * 1024, a.x + (size_t)st * F::ROW, xoff[k]);
   };
-  auto load_scales = [&](int st, int buf, int pair, int rows) __attribute__((always_inline)) {
+  // (all waves as many copies, so that each knows how many of its loads are on their way: past the rows, the last one again)
+  auto load_scales = [&](int st, int buf, int pair, const Weights& of) __attribute__((always_inline)) {
     if constexpr (F::SCALED) {
 #pragma unroll
-      for (int k = 0; k < (ROWS + 255) / 256; k++)
-        if (32 * (w + 8 * k) < rows) dma4(lds_address(xscale[buf]) + 256 * (w + 8 * k), a.x_scale + 8 * st, soff[k]);
-      if ((st & 1) == 0) {
+      for (int k = 0; k < SCOPIES; k++) dma4(lds_address(xscale[buf]) + 256 * (w + 8 * k), a.x_scale + 8 * st, soff[k]);
 #pragma unroll
-        for (int k = 0; k < 2; k++)
-          dma4(lds_address(wscale[pair]) + 256 * (2 * w + k), word[k] + 2 * st, lane * mx_lane_scales(S));
-      }
+      for (int k = 0; k < 2; k++)
+        dma4(lds_address(wscale[pair]) + 256 * (2 * w + k), of.word[k] + 4 * (st >> 1), lane * mx_lane_scales(S));
     }
   };
 
-  Item cur, nxt;
   next_item(cur);
   if (cur.rows == 0) return;
   find_pairs(cur);
-  find_places(cur);
+  find_weights(cur, at);
+  nxt.rows = 0;
   int buf = 0, pair = 1;  // the buffers of the stage and of the pair of stages (for its scale words)
-#pragma unroll
-  for (int k = 0; k < 4; k++) load_weights(k, 0, 0);
+  load_weights(0, 0, 0);
+  load_weights(0, 1, 1);
+  load_weights(1, 0, 2);
+  find_rows();
 #pragma unroll
   for (int k = 0; k < COPIES; k++)
     if (PER * (w + 8 * k) < cur.rows) load_rows(k, 0, 0);
-  load_scales(0, 0, 0, cur.rows);
+  load_scales(0, 0, 0, at);
   next_item(nxt);
+  if (nxt.rows) find_weights(nxt, at_next);
 
   // An item's products. A wave's tiles: rows 16 (wm + 2 j) .., j < NT (tiles past the pass's run on what lies there and
   // store nothing)
@@ -190,25 +212,23 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
     for (int j = 0; j < NT; j++)
 #pragma unroll
       for (int n = 0; n < 4; n++) acc[j][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    dma_wait();
-    __syncthreads();
+    // (the copies of the first stage: the start's, or the last stage's before, which waited for them)
     for (int st = 0; st < S; st++, buf ^= 1) {
       if ((st & 1) == 0) pair ^= 1;
-      const uint8_t* wbase = smem + buf * STAGE;
       const uint8_t* xlane[2][F::PIECES];  // this lane's operands of the wave's first tile
 #pragma unroll
       for (int s = 0; s < 2; s++)
 #pragma unroll
         for (int k = 0; k < F::PIECES; k++)
-          xlane[s][k] = wbase + A_BYTES + (16 * wm + c) * F::ROW + 16 * wx_slot<F>(c, F::b_piece(s, q, k));
+          xlane[s][k] = smem + 4 * STEP + buf * STAGE + (16 * wm + c) * F::ROW + 16 * wx_slot<F>(c, F::b_piece(s, q, k));
       const uint8_t* slane = xscale[buf] + 8 * (16 * wm + c) + 2 * q;
       i32x4 wa[4], b[4][F::PIECES];
       uint32_t sw[4] = {0, 0, 0, 0}, sb[4] = {0, 0, 0, 0};
       auto read_w = [&](int s) __attribute__((always_inline)) {
+        const uint8_t* from = smem + (2 * buf + s) * STEP + 4 * wn * 1024 +
+                              (F::SCALED ? 16 * lane : c * 64 + 16 * wx_step_slot(c, q));
 #pragma unroll
-        for (int n = 0; n < 4; n++)
-          wa[n] = *(const i32x4*)(wbase + (4 * wn + n) * 2048 +
-                                     (F::SCALED ? 1024 * s + 16 * lane : c * 128 + 16 * wx_slot<F>(c, 2 * q + s)));
+        for (int n = 0; n < 4; n++) wa[n] = *(const i32x4*)(from + 1024 * n);
       };
       auto read_x = [&](int i) __attribute__((always_inline)) {  // operand i: tile i % NT, step i / NT
 #pragma unroll
@@ -222,38 +242,44 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
         for (int n = 0; n < 4; n++) sw[n] = wscale[pair][64 * (4 * wn + n) + lane] >> (16 * (st & 1));
       }
       read_x(1);
-      // The next stage's copies, of this item or the next, go out between the products: those that this item's rows need
+      // The next stage's rows, of this item or the next, go out between the products: those that this item's rows need
       // without a branch (after the last item they copy what is there once more). Whatever branches stands before the
       // products, which the compiler would move past it, with all their operands waiting in registers.
       const bool last = st + 1 == S;
-      if (nxt.rows && (st + 2 == S || S == 1)) find_pairs(nxt);  // for the next stage
-      if (last && nxt.rows) find_places(nxt);
+      if (nxt.rows && st + 2 == S) find_pairs(nxt);  // for the next stage
+      if (last && nxt.rows) find_rows();
       const int st_next = last ? 0 : st + 1;
-      load_scales(st_next, buf ^ 1, pair ^ 1, last ? nxt.rows : cur.rows);
-      constexpr int MINE = (32 * NT / PER + 7) / 8, SPREAD = (4 + MINE + NT - 1) / NT;  // copies; to a group of products
+      constexpr int MINE = (32 * NT / PER + 7) / 8;
       if (last) {
 #pragma unroll
         for (int k = MINE; k < COPIES; k++)
           if (PER * (w + 8 * k) < nxt.rows) load_rows(k, 0, buf ^ 1);
       }
+      load_scales(st_next, buf ^ 1, st_next & 1 ? pair : pair ^ 1, last && nxt.rows ? at_next : at);
+      auto products = [&]<int s>() __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 2 * NT; i++) {
-        if (i == NT) read_w(1);
-        if (i + 2 < 2 * NT) read_x(i + 2);
-        __builtin_amdgcn_sched_barrier(0);  // the reads first
-        const int j = i % NT;
+        for (int j = 0; j < NT; j++) {
+          if (s * NT + j + 2 < 2 * NT) read_x(s * NT + j + 2);
+          __builtin_amdgcn_sched_barrier(0);  // the reads first
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-          if (i < NT) acc[j][n] = step_product<F, !OUT_BF16, 0, 0>(wa[n], b[i & 3], acc[j][n], sw[n], sb[i & 3]);
-          else acc[j][n] = step_product<F, !OUT_BF16, 1, 1>(wa[n], b[i & 3], acc[j][n], sw[n], sb[i & 3]);
+          for (int n = 0; n < 4; n++)
+            acc[j][n] = step_product<F, !OUT_BF16, s, s>(wa[n], b[(s * NT + j) & 3], acc[j][n], sw[n], sb[(s * NT + j) & 3]);
+          if (s == 0) {
+            constexpr int SPREAD = (MINE + NT - 1) / NT;
+#pragma unroll
+            for (int k = SPREAD * j; k < SPREAD * (j + 1) && k < MINE; k++) load_rows(k, st_next, buf ^ 1);
+          }
         }
-#pragma unroll
-        for (int k = SPREAD * i; k < SPREAD * (i + 1) && k < 4 + MINE; k++) {
-          if (k < 4) load_weights(k, st_next, buf ^ 1);
-          else load_rows(k - 4, st_next, buf ^ 1);
-        }
-      }
-      dma_wait();
+      };
+      products.template operator()<0>();
+      load_weights(st + 1, 1, 2 * (buf ^ 1) + 1);
+      // the second step's weights: all but the step after them and this step's copies
+      wait_loads<2 + SCOPIES + (F::SCALED ? 2 : 0) + MINE + 2>();
+      __syncthreads();
+      read_w(1);
+      load_weights(st + 2, 0, 2 * buf);
+      products.template operator()<1>();
+      wait_loads<4>();  // the next stage: all but the last two steps' weights
       __syncthreads();
     }
 
@@ -282,6 +308,8 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
       }
     }
   };
+  wait_loads<0>();
+  __syncthreads();
   while (true) {
     const int mine = ((cur.rows + 15) / 16 + 1) / 2;  // tiles of a wave, at most
     if constexpr (TILES > 10) {
@@ -297,10 +325,13 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
       else if (mine > 2) run.template operator()<3>();
       else run.template operator()<2>();
     }
-    if (nxt.rows == 0) return;
+    if (nxt.rows == 0) break;
     cur = nxt;
+    at = at_next;
     next_item(nxt);
+    if (nxt.rows) find_weights(nxt, at_next);
   }
+  wait_loads<0>();  // no copy is on its way to an LDS that is another workgroup's
 }
 
 // compute units of the current device
@@ -326,7 +357,7 @@ void launch_wide(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t
 // offsets.)
 template <class F>
 bool wide_fits(const ExpertProduct& a) {
-  return (int64_t)a.pairs >= (int64_t)32 * a.n_groups && (int64_t)a.x_rows * a.stages * F::ROW <= UINT32_MAX;
+  return (int64_t)a.pairs >= (int64_t)32 * a.n_groups && a.stages >= 2 && (int64_t)a.x_rows * a.stages * F::ROW <= UINT32_MAX;
 }
 
 template <class F>

@@ -41,16 +41,16 @@ struct Mx {
     return BITS == 4 ? 2 * q + s : 4 * (q >> 1) + 2 * s + (q & 1) + 8 * i;
   }
 };
-// bfloat16: a stage is 64 columns (128 bytes of a row), step s multiplies the pieces 2 q + s of 8 columns; the weights lie
+// bfloat16: a stage is 64 columns (128 bytes of a row), step s multiplies the pieces 4 s + q of 8 columns; the weights lie
 // row by row
 struct Bf16 {
   static constexpr bool SCALED = false;
   static constexpr int BITS = 16, ROW = 128, PIECES = 1, SEG = 32;
-  static constexpr int A_STAGE = 128, A_STEP = 16;
+  static constexpr int A_STAGE = 128, A_STEP = 64;
   static D3_INLINE size_t a_base(size_t tile, int stages, int lane) {
-    return (tile * 16 + (lane & 15)) * ((size_t)stages * 128) + 32 * (lane >> 4);
+    return (tile * 16 + (lane & 15)) * ((size_t)stages * 128) + 16 * (lane >> 4);
   }
-  static D3_INLINE int b_piece(int s, int q, int) { return 2 * q + s; }
+  static D3_INLINE int b_piece(int s, int q, int) { return 4 * s + q; }
 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
