@@ -539,40 +539,49 @@ def fp8_linear(x, weight, scale):
 
 
 # ------------------------------------------------------------- products of unquantized and of microscaled (mx.py) banks
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def launch(name, t, *args):
-    """C entry `name` with `args` and torch's current stream of t's device, that device the current one."""
-    device = t.device
-    if device.type != "cuda":
-        raise ValueError(f"{name}: the kernels run on a GPU, not on {device}")
-    if device.index == torch.cuda.current_device():
-        return _call(name, *args, _lib.stream_of(device))
-    with torch.cuda.device(device):
-        return _call(name, *args, _lib.stream_of(device))
+    """C entry `name` with `args` and torch's current stream of t's device, that device the current one. (The stream's
+    handle as torch's own generated code asks for it: a Stream object costs 2 us, as much as the launch.)"""
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{name}: the kernels run on a GPU, not on {t.device}")
+    fn = getattr(_lib.lib(), name)
+    if index == _current():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def product_out(device, pairs, n, swiglu, dtype, out):
     """The tensor a product of `pairs` rows with experts of n weight rows writes: `out` checked, or a new one."""
-    if swiglu and n % 32:
-        raise ValueError(f"gate and up rows are multiples of 16 each, not {n} in all")
-    if n % 16:
-        raise ValueError(f"experts have a multiple of 16 weight rows, not {n}")
-    if dtype not in (torch.float32, torch.bfloat16):
+    if n % (32 if swiglu else 16):
+        raise ValueError(f"gate and up rows are multiples of 16 each, not {n} in all" if swiglu else
+                         f"experts have a multiple of 16 weight rows, not {n}")
+    if swiglu:
+        n, dtype = n // 2, torch.bfloat16
+    elif dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise TypeError("products are float32 or bfloat16")
-    shape, dtype = (pairs, n // 2 if swiglu else n), torch.bfloat16 if swiglu else dtype
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
-        raise ValueError(f"out {list(shape)} {dtype}, contiguous, on {device}, expected")
+        return torch.empty((pairs, n), dtype=dtype, device=device)
+    if out.shape != (pairs, n) or out.dtype != dtype or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out [{pairs}, {n}] {dtype}, contiguous, on {device}, expected")
     return out
 
 
 def pair_ids(ids, rows, device):
-    """A gemv's expert ids [P] int64, contiguous: a multiple of the rows."""
-    if ids.dtype != torch.int64 or ids.dim() != 1 or ids.device != device:
+    """A gemv's expert ids [P] int64, contiguous, and P: a multiple of the rows."""
+    if ids.dtype is not torch.int64 or ids.dim() != 1 or ids.device != device:
         raise ValueError(f"ids [P] int64 on {device} expected")
-    if rows == 0 and ids.numel() or rows and ids.numel() % rows:
-        raise ValueError(f"{ids.numel()} ids for {rows} rows: a multiple of the rows is expected")
-    return ids.contiguous()
+    P = ids.numel()
+    if P % rows if rows else P:
+        raise ValueError(f"{P} ids for {rows} rows: a multiple of the rows is expected")
+    return ids.contiguous(), P
 
 
 def check_groups(groups, order, k, rows, device):
@@ -592,17 +601,17 @@ def check_groups(groups, order, k, rows, device):
 
 
 def _bf16_operands(x, weight, n):
-    """(x [R, K], K, experts) of a product on a bank of bfloat16 weights [E * n, K]."""
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+    """(x, R, K, experts, device) of a product of rows x [R, K] with a bank of bfloat16 weights [E * n, K]."""
+    if x.dim() != 2 or x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16:
         raise TypeError("x [R, K] and weight [E * n, K] bfloat16 expected")
-    K = x.shape[1]
+    (R, K), device = x.shape, x.device
     if K < 64 or K % 64:
         raise ValueError(f"K is a positive multiple of 64, not {K}")
-    if n < 1 or weight.dim() != 2 or weight.shape[1] != K or weight.shape[0] % n or not weight.is_contiguous() \
-            or weight.device != x.device:
-        raise ValueError(f"weight [E * {n}, {K}], contiguous, on {x.device}, expected")
+    if n < 1 or weight.dim() != 2 or weight.size(1) != K or weight.size(0) % n or not weight.is_contiguous() \
+            or weight.device != device:
+        raise ValueError(f"weight [E * {n}, {K}], contiguous, on {device}, expected")
     x = x.contiguous()
-    return (x if x.data_ptr() % 16 == 0 else x.clone()), K, weight.shape[0] // n
+    return (x if x.data_ptr() % 16 == 0 else x.clone()), R, K, weight.size(0) // n, device
 
 
 def gemv_bf16(x, ids, weight, n, swiglu=False, dtype=torch.float32, out=None):
@@ -610,11 +619,11 @@ def gemv_bf16(x, ids, weight, n, swiglu=False, dtype=torch.float32, out=None):
     x [R, K] and experts ids [P] (int64): [P, n] float32 or bfloat16, pair p row p // (P / R) of x with expert ids[p],
     float32 sums. With `swiglu` (gate rows, then up rows) [P, n / 2] bfloat16 = SiLU(gate) * up. An id outside the bank
     gives zeros."""
-    x, K, E = _bf16_operands(x, weight, n)
-    out = product_out(x.device, ids.numel(), n, swiglu, dtype, out)
-    ids = pair_ids(ids, x.shape[0], x.device)
-    launch("d3_bf16_gemv", out, _p(x), x.shape[0], _p(ids), ids.numel(), _p(weight), E, n, K, int(swiglu),
-           int(out.dtype == torch.bfloat16), _p(out))
+    x, R, K, E, device = _bf16_operands(x, weight, n)
+    ids, P = pair_ids(ids, R, device)
+    out = product_out(device, P, n, swiglu, dtype, out)
+    launch("d3_bf16_gemv", out, x.data_ptr(), R, ids.data_ptr(), P, weight.data_ptr(), E, n, K, swiglu,
+           out.dtype is torch.bfloat16, out.data_ptr())
     return out
 
 
@@ -623,11 +632,11 @@ def grouped_bf16(x, groups, weight, n, order=None, k=1, swiglu=False, dtype=torc
     place p row order[p] // k of the bfloat16 rows x [R, K] (its own row p without order), order and groups as
     expert_groups makes them. dtype and `swiglu` as for gemv_bf16. Places in no group are left as `out` had them (unset
     without it), as are groups whose expert or places lie outside the bank or the pairs."""
-    x, K, E = _bf16_operands(x, weight, n)
-    P = check_groups(groups, order, k, x.shape[0], x.device)
-    out = product_out(x.device, P, n, swiglu, dtype, out)
-    launch("d3_bf16_grouped", out, _p(x), x.shape[0], _p(order), k, P, _p(groups), groups.shape[0], _p(weight), E, n, K,
-           int(swiglu), int(out.dtype == torch.bfloat16), _p(out))
+    x, R, K, E, device = _bf16_operands(x, weight, n)
+    P = check_groups(groups, order, k, R, device)
+    out = product_out(device, P, n, swiglu, dtype, out)
+    launch("d3_bf16_grouped", out, x.data_ptr(), R, _p(order), k, P, groups.data_ptr(), groups.shape[0],
+           weight.data_ptr(), E, n, K, swiglu, out.dtype is torch.bfloat16, out.data_ptr())
     return out
 
 

@@ -62,19 +62,20 @@ def _check_cols(cols):
 
 
 def _check_rows(r):
-    C = _stages(r.cols) * STAGE
-    R = r.codes.shape[0]
-    if r.bits not in (4, 8):
-        raise ValueError(f"microscaled rows have 4 or 8 bits an element, not {r.bits}")
-    if r.codes.dtype != torch.uint8 or r.scale.dtype != torch.uint8:
+    """(codes, scale, R, device) of MxRows, checked."""
+    codes, scale, bits = r.codes, r.scale, r.bits
+    if bits != 4 and bits != 8:
+        raise ValueError(f"microscaled rows have 4 or 8 bits an element, not {bits}")
+    if codes.dtype is not torch.uint8 or scale.dtype is not torch.uint8:
         raise TypeError("codes and scale must be uint8")
-    if r.codes.shape != (R, C * r.bits // 8) or r.scale.shape != (R, C // BLOCK):
-        raise ValueError(f"codes [R, {C * r.bits // 8}] and scale [R, {C // BLOCK}] expected for {r.cols} columns")
-    if not (r.codes.is_contiguous() and r.scale.is_contiguous()):
+    R, C, device = codes.size(0), -(-r.cols // STAGE) * STAGE, codes.device
+    if codes.shape != (R, C * bits // 8) or scale.shape != (R, C // BLOCK):
+        raise ValueError(f"codes [R, {C * bits // 8}] and scale [R, {C // BLOCK}] expected for {r.cols} columns")
+    if not (codes.is_contiguous() and scale.is_contiguous()):
         raise ValueError("codes and scale must be contiguous")
-    if r.scale.device != r.codes.device:
+    if scale.device != device:
         raise ValueError("codes and scale must be on one device")
-    return R
+    return codes, scale, R, device
 
 
 def quantize(x, bits=4):
@@ -99,13 +100,13 @@ def quantize(x, bits=4):
 
 def dequantize(rows, dtype=torch.float32):
     """The values of MxRows: [R, cols] float32 or bfloat16."""
-    R = _check_rows(rows)
+    codes, scale, R, device = _check_rows(rows)
     _check_cols(rows.cols)
     if dtype not in _TYPES:
         raise TypeError("float32 or bfloat16 expected")
-    out = torch.empty((R, rows.cols), dtype=dtype, device=rows.codes.device)
-    kernels.launch("d3_mx_dequantize", out, rows.codes.data_ptr(), rows.scale.data_ptr(), R, rows.cols, rows.bits,
-                   _TYPES[dtype], out.data_ptr())
+    out = torch.empty((R, rows.cols), dtype=dtype, device=device)
+    kernels.launch("d3_mx_dequantize", out, codes.data_ptr(), scale.data_ptr(), R, rows.cols, rows.bits, _TYPES[dtype],
+                   out.data_ptr())
     return out
 
 
@@ -124,7 +125,7 @@ def bank(rows, experts):
     """MxRows of e2m1 weights (experts * N rows, N % 16 == 0) laid out for the products, once: tile t holds 16 rows, their
     codes by stage of 256 columns, half s of the block pairs, pair q, row; their scales by pair, row, stage and s, where
     block 2 q + s of a stage's eight is pair q's half s."""
-    R = _check_rows(rows)
+    R = _check_rows(rows)[2]
     if rows.bits != 4 or experts < 1 or R % experts or (R // experts) % 16:
         raise ValueError("a bank holds experts of e2m1 rows, a multiple of 16 each")
     tiles, stages = R // 16, _stages(rows.cols)
@@ -148,32 +149,34 @@ def quantize_bank(w):
     return bank(quantize(w.reshape(E * n, k), 4), E)
 
 
-def _check_bank(b, rows, swiglu):
-    stages = _stages(b.cols)
-    R = b.experts * b.rows
-    if rows.cols != b.cols:
-        raise ValueError(f"rows of {rows.cols} columns for a bank of {b.cols}")
-    if b.weight.dtype != torch.uint8 or b.scale.dtype != torch.uint8:
+def _check_bank(b, cols, device):
+    """(weight, scale) of a bank that rows of `cols` columns on `device` go through, checked."""
+    weight, scale = b.weight, b.scale
+    if cols != b.cols:
+        raise ValueError(f"rows of {cols} columns for a bank of {b.cols}")
+    if weight.dtype is not torch.uint8 or scale.dtype is not torch.uint8:
         raise TypeError("a bank's weight and scale must be uint8")
-    if b.weight.shape != (R, stages * STAGE // 2) or b.scale.shape != (R, 8 * (stages + stages % 2)):
+    stages, R = -(-cols // STAGE), b.experts * b.rows
+    if weight.shape != (R, stages * STAGE // 2) or scale.shape != (R, 8 * (stages + stages % 2)):
         raise ValueError("the bank's tensors do not have its shape (mx.bank lays them out)")
-    if not (b.weight.is_contiguous() and b.scale.is_contiguous()):
+    if not (weight.is_contiguous() and scale.is_contiguous()):
         raise ValueError("a bank's tensors must be contiguous")
-    if b.weight.device != rows.codes.device or b.scale.device != rows.codes.device:
+    if weight.device != device or scale.device != device:
         raise ValueError("rows and bank must be on one device")
+    return weight, scale
 
 
 def gemv(rows, ids, bank, swiglu=False, dtype=torch.float32, out=None):
     """[P, N] of P pairs of rows and experts ids [P] (int64): pair p is row p // (P / R) of the R rows with expert
     ids[p] of `bank`; float32 or bfloat16. With `swiglu` (gate rows, then up rows) [P, N / 2] bfloat16 = SiLU(gate) * up.
     An id outside the bank gives zeros. For decode lines: every pair reads its expert by itself."""
-    R = _check_rows(rows)
-    _check_bank(bank, rows, swiglu)
-    out = kernels.product_out(rows.codes.device, ids.numel(), bank.rows, swiglu, dtype, out)
-    ids = kernels.pair_ids(ids, R, rows.codes.device)
-    kernels.launch("d3_mx_gemv", out, rows.codes.data_ptr(), rows.scale.data_ptr(), rows.bits, R, ids.data_ptr(),
-                   ids.numel(), bank.weight.data_ptr(), bank.scale.data_ptr(), bank.experts, bank.rows, bank.cols,
-                   int(swiglu), int(out.dtype == torch.bfloat16), out.data_ptr())
+    codes, scale, R, device = _check_rows(rows)
+    weight, wscale = _check_bank(bank, rows.cols, device)
+    ids, P = kernels.pair_ids(ids, R, device)
+    out = kernels.product_out(device, P, bank.rows, swiglu, dtype, out)
+    kernels.launch("d3_mx_gemv", out, codes.data_ptr(), scale.data_ptr(), rows.bits, R, ids.data_ptr(), P,
+                   weight.data_ptr(), wscale.data_ptr(), bank.experts, bank.rows, bank.cols, swiglu,
+                   out.dtype is torch.bfloat16, out.data_ptr())
     return out
 
 
@@ -182,12 +185,11 @@ def grouped(rows, groups, bank, order=None, k=1, swiglu=False, dtype=torch.float
     kernels.expert_groups makes them; place p multiplies row order[p] // k (its own row p without order) with its group's
     expert. dtype and `swiglu` as for gemv. Places in no group are left as `out` had them (unset without it), as are groups
     whose expert or places lie outside the bank or the pairs."""
-    R = _check_rows(rows)
-    _check_bank(bank, rows, swiglu)
-    device = rows.codes.device
+    codes, scale, R, device = _check_rows(rows)
+    weight, wscale = _check_bank(bank, rows.cols, device)
     P = kernels.check_groups(groups, order, k, R, device)
     out = kernels.product_out(device, P, bank.rows, swiglu, dtype, out)
-    kernels.launch("d3_mx_grouped", out, rows.codes.data_ptr(), rows.scale.data_ptr(), rows.bits, R, _lib.ptr(order), k,
-                   P, groups.data_ptr(), groups.shape[0], bank.weight.data_ptr(), bank.scale.data_ptr(), bank.experts,
-                   bank.rows, bank.cols, int(swiglu), int(out.dtype == torch.bfloat16), out.data_ptr())
+    kernels.launch("d3_mx_grouped", out, codes.data_ptr(), scale.data_ptr(), rows.bits, R, _lib.ptr(order), k, P,
+                   groups.data_ptr(), groups.size(0), weight.data_ptr(), wscale.data_ptr(), bank.experts, bank.rows,
+                   bank.cols, swiglu, out.dtype is torch.bfloat16, out.data_ptr())
     return out
