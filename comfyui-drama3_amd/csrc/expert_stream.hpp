@@ -12,20 +12,20 @@ constexpr int ST_THREADS = 256;
 
 // LDS bytes of a row of the stages, and where its 16-byte piece j lies: pieces of 256 bytes swapped by the row, so that
 // 16 rows' pieces j are in 16 different groups of banks
-template <class F> constexpr int st_pitch() { return (F::SEG * F::ROW + 255) / 256 * 256; }
+template <class F, int SEG> constexpr int st_pitch() { return (SEG * F::ROW + 255) / 256 * 256; }
 D3_INLINE int st_piece(int r, int j) { return 16 * (j ^ (r & 15)); }
 
 // NT tiles of weight rows a wave; SWIGLU with NT 2: a gate tile and its up tile, with NT 1 (gemv): those of two
 // neighbouring waves
-template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH>
-__global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProduct a, int columns) {
-  constexpr int ROWS = GEMV ? 1 : 16 * MT, PITCH = st_pitch<F>(), SPITCH = 8 * F::SEG + 4, SEG = F::SEG;
+template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH, int SEG>
+__global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProduct a, int columns, int per) {
+  constexpr int ROWS = GEMV ? 1 : 16 * MT, PITCH = st_pitch<F, SEG>(), SPITCH = 8 * SEG + 4;
   __shared__ __attribute__((aligned(1024))) uint8_t xs[ROWS * PITCH];
   __shared__ __attribute__((aligned(16))) uint8_t ss[F::SCALED ? ROWS * SPITCH : 16];
-  __shared__ f32x4 other[GEMV && SWIGLU ? ST_THREADS / 64 : 1][4];
+  __shared__ f32x4 other[2][GEMV && SWIGLU ? ST_THREADS / 64 : 1][4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, c = lane & 15;
-  const int column = blockIdx.x % columns, at = blockIdx.x / columns;
+  const int strips = (columns + per - 1) / per, at = blockIdx.x / strips, column0 = (blockIdx.x % strips) * per;
   Pass pass;
   int my_row;  // lane r: row r of the pass
   if constexpr (GEMV) {
@@ -38,8 +38,9 @@ __global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProd
     if (pass.rows == 0) return;
     my_row = pair_row(a, pair_at(a, pass.first + min(lane, pass.rows - 1)));
   }
-  // the wave's tiles of an expert's N / 16
   const int tiles = a.N / 16, half = tiles / 2;
+  for (int column = column0; column < (GEMV ? column0 + 1 : min(column0 + per, columns)); column++) {
+  // the wave's tiles of an expert's N / 16
   int tile[NT];
   bool mine;  // the wave has a tile of its own (a column past the last one repeats it and stores nothing)
   if constexpr (SWIGLU && NT == 1) {
@@ -93,8 +94,9 @@ __global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProd
 #pragma unroll
           for (int i = 0; i < SEG / 2; i++) sa[n][i] = ((const uint32_t*)(sp[n] + 2 * s0))[min(i, (n_st - 1) / 2)];
       }
-      // the rows: wave w copies rows w, w + 4, .. to LDS, lane by lane into place
-      if (s0) __syncthreads();
+      // the rows: wave w copies rows w, w + 4, .. to LDS, lane by lane into place (once for all columns if they fit)
+      if (S > SEG || column == column0) {
+      if (s0 || column != column0) __syncthreads();
       for (int r = w; r < pass.rows; r += ST_THREADS / 64) {
         const uint8_t* src = a.x + (size_t)__builtin_amdgcn_readlane(my_row, r) * row_bytes + (size_t)s0 * F::ROW;
         for (int j = 0; j < n_st * F::ROW / 16; j += 64) {
@@ -112,6 +114,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProd
       }
       dma_wait();
       __syncthreads();
+      }
       // lane's rows of the MT tiles (a row past the pass's repeats its last: its results are not stored)
       int xr[MT];
 #pragma unroll
@@ -178,11 +181,11 @@ __global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProd
 
   // lane (q, c) holds weight rows 16 tile + 4 q .. + 3 of the pass's row 16 m + c
   if constexpr (GEMV && SWIGLU) {
-    if (c == 0) other[w][q] = acc[0][0];
+    if (c == 0) other[column & 1][w][q] = acc[0][0];
     __syncthreads();
     if (mine && !(w & 1) && c == 0) {
       *(i32x2*)((uint16_t*)a.out + (size_t)pass.first * (a.N / 2) + tile[0] * 16 + 4 * q) =
-          swiglu_4(acc[0][0], other[w | 1][q]);
+          swiglu_4(acc[0][0], other[column & 1][w | 1][q]);
     }
   } else if (mine) {
 #pragma unroll
@@ -203,6 +206,7 @@ __global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProd
       }
     }
   }
+  }
 }
 
 // workgroups to a pass
@@ -212,26 +216,31 @@ int st_columns(int N) {
   return (N / 16 + per - 1) / per;
 }
 
-template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH>
-void launch_stream_of(const ExpertProduct& a, int passes, hipStream_t s) {
+template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH, int SEG>
+void launch_stream_of(const ExpertProduct& a, int passes, int per, hipStream_t s) {
   const int columns = st_columns<GEMV, SWIGLU, NT>(a.N);
-  hipLaunchKernelGGL((expert_stream_kernel<F, GEMV, SWIGLU, OUT_BF16, NT, MT, DEPTH>), dim3((unsigned)(columns * passes)),
-                     dim3(ST_THREADS), 0, s, a, columns);
+  per = per < columns ? per : columns;
+  hipLaunchKernelGGL((expert_stream_kernel<F, GEMV, SWIGLU, OUT_BF16, NT, MT, DEPTH, SEG>),
+                     dim3((unsigned)((columns + per - 1) / per * passes)), dim3(ST_THREADS), 0, s, a, columns, per);
 }
 
 template <class F>
 void launch_gemv(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
-  if (swiglu) launch_stream_of<F, true, true, true, 1, 1, 8>(a, a.pairs, s);
-  else if (out_bf16) launch_stream_of<F, true, false, true, 1, 1, 8>(a, a.pairs, s);
-  else launch_stream_of<F, true, false, false, 1, 1, 8>(a, a.pairs, s);
+  if (swiglu) launch_stream_of<F, true, true, true, 1, 1, 8, F::SEG>(a, a.pairs, 1, s);
+  else if (out_bf16) launch_stream_of<F, true, false, true, 1, 1, 8, F::SEG>(a, a.pairs, 1, s);
+  else launch_stream_of<F, true, false, false, 1, 1, 8, F::SEG>(a, a.pairs, 1, s);
 }
 
-template <class F, int MT>
+template <class F, int MT, int SEG>
 void launch_stream(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
   const int passes = most_passes(a.pairs, a.n_groups, 16 * MT);
-  if (swiglu) launch_stream_of<F, false, true, true, 2, MT, 4>(a, passes, s);
-  else if (out_bf16) launch_stream_of<F, false, false, true, 2, MT, 4>(a, passes, s);
-  else launch_stream_of<F, false, false, false, 2, MT, 4>(a, passes, s);
+  // A workgroup finds its pass and copies the rows before it streams anything: with few stages to a column it takes some
+  // columns in turn. Second bank of 128 experts (2048 x 768, e4m3), 256 rows: 32 us with two, 38 with one; first bank
+  // (8 stages): 51 with one, 53 with two.
+  const int per = F::SCALED && a.stages < 6 ? 6 / a.stages : 1;
+  if (swiglu) launch_stream_of<F, false, true, true, 2, MT, 4, SEG>(a, passes, per, s);
+  else if (out_bf16) launch_stream_of<F, false, false, true, 2, MT, 4, SEG>(a, passes, per, s);
+  else launch_stream_of<F, false, false, false, 2, MT, 4, SEG>(a, passes, per, s);
 }
 
 }  // namespace d3

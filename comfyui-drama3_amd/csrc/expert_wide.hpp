@@ -360,10 +360,20 @@ bool wide_fits(const ExpertProduct& a) {
   return (int64_t)a.pairs >= (int64_t)32 * a.n_groups && a.stages >= 2 && (int64_t)a.x_rows * a.stages * F::ROW <= UINT32_MAX;
 }
 
+// Wide passes, or streamed ones of 32 rows, or of 16, by the rows an expert has on average. Top-8 of 128 experts (FFN 768),
+// us with 16 / 32 / wide: first bank, e4m3 rows, 256 rows (16 to an expert) 51 / 46 / 52, 400 rows 67 / 50 / 53, 700 rows
+// 73 wide and 74 streamed (256 experts, Zipf); second bank 16 to an expert 31 / 36 / 43 (few stages: a 32-row pass has
+// less to stream than it takes to set up), 25 to an expert 40 / 41 / 42, 44 to an expert 60 streamed, 47 wide; bf16 first
+// bank 16 to an expert 182 / 187 / 190, 25: 238 / 185 / 192; second bank 16: 100 / 91 / 102.
 template <class F>
 void launch_grouped(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
-  if (wide_fits<F>(a)) launch_wide<F>(a, swiglu, out_bf16, s);
-  else launch_stream<F, 1>(a, swiglu, out_bf16, s);
+  if (wide_fits<F>(a)) return launch_wide<F>(a, swiglu, out_bf16, s);
+  const bool small = a.stages <= F::SEG / 2;  // half the LDS holds the rows
+  const bool two = (int64_t)a.pairs >= (int64_t)(F::SCALED && small ? 24 : 12) * a.n_groups;
+  if (two && small) launch_stream<F, 2, F::SEG / 2>(a, swiglu, out_bf16, s);
+  else if (two) launch_stream<F, 2, F::SEG>(a, swiglu, out_bf16, s);
+  else if (small) launch_stream<F, 1, F::SEG / 2>(a, swiglu, out_bf16, s);
+  else launch_stream<F, 1, F::SEG>(a, swiglu, out_bf16, s);
 }
 
 }  // namespace d3

@@ -207,6 +207,7 @@ def test_gemv(fmt, n, K):
 # rows of the experts: few on average, and many (around a pass's 128 and 256 rows)
 COUNTS = [0, 1, 15, 16, 17, 31, 33, 0, 64, 65, 130, 3]
 MANY = [0, 1, 127, 128, 129, 255, 256, 257, 0, 300, 513, 33, 16, 191]
+FEW = [0, 1, 3, 16, 17, 0, 2, 5, 33, 1]
 
 
 def _pairs(E, counts, seed=1):
@@ -218,7 +219,7 @@ def _pairs(E, counts, seed=1):
 
 @pytest.mark.parametrize("counts, n, K", [
     (COUNTS, 16, 64), (COUNTS, 32, 256), (COUNTS, 96, 320), (COUNTS, 288, 768), (COUNTS, 160, 2048), (COUNTS, 32, 2368),
-    (MANY, 16, 64), (MANY, 32, 192), (MANY, 288, 256), (MANY, 544, 320), (MANY, 160, 2048), (MANY, 256, 1344)])
+    (FEW, 32, 64), (FEW, 288, 512), (FEW, 160, 2368), (MANY, 16, 64), (MANY, 32, 192), (MANY, 288, 256), (MANY, 544, 320), (MANY, 160, 2048), (MANY, 256, 1344)])
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_grouped_ragged(fmt, counts, n, K):
     E, P = len(counts), sum(counts)
