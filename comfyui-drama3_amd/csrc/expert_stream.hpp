@@ -13,12 +13,15 @@ constexpr int ST_THREADS = 256;
 // LDS bytes of a row of the stages, and where its 16-byte piece j lies: pieces of 256 bytes swapped by the row, so that
 // 16 rows' pieces j are in 16 different groups of banks
 template <class F, int SEG> constexpr int st_pitch() { return (SEG * F::ROW + 255) / 256 * 256; }
+// waves of a SIMD that LDS has room for, up to two
+template <class F, int SEG, int MT> constexpr int st_waves() { return 16 * MT * st_pitch<F, SEG>() > 80000 ? 1 : 2; }
 D3_INLINE int st_piece(int r, int j) { return 16 * (j ^ (r & 15)); }
 
 // NT tiles of weight rows a wave; SWIGLU with NT 2: a gate tile and its up tile, with NT 1 (gemv): those of two
 // neighbouring waves
 template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH, int SEG>
-__global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProduct a, int columns, int per) {
+__global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
+    expert_stream_kernel(ExpertProduct a, int columns, int per) {
   constexpr int ROWS = GEMV ? 1 : 16 * MT, PITCH = st_pitch<F, SEG>(), SPITCH = 8 * SEG + 4;
   __shared__ __attribute__((aligned(1024))) uint8_t xs[ROWS * PITCH];
   __shared__ __attribute__((aligned(16))) uint8_t ss[F::SCALED ? ROWS * SPITCH : 16];
@@ -105,9 +108,10 @@ __global__ void __launch_bounds__(ST_THREADS, 2) expert_stream_kernel(ExpertProd
         }
       }
       if constexpr (F::SCALED) {
-        for (int r = tid >> 4; r < pass.rows; r += ST_THREADS / 16) {
-          const int row = GEMV ? my_row : __shfl(my_row, r);
-          if ((tid & 15) < 2 * n_st)
+#pragma unroll
+        for (int r0 = 0; r0 < ROWS; r0 += ST_THREADS / 16) {
+          const int r = r0 + (tid >> 4), row = GEMV ? my_row : __shfl(my_row, r);  // (all lanes: each may be read)
+          if (r < pass.rows && (tid & 15) < 2 * n_st)
             *(uint32_t*)(ss + r * SPITCH + 4 * (tid & 15)) =
                 ((const uint32_t*)(a.x_scale + ((size_t)row * S + s0) * 8))[tid & 15];
         }
