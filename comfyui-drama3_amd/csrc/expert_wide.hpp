@@ -59,30 +59,47 @@ D3_INLINE Pass wide_passes(const ExpertProduct& a, int at) {
   const int lane = threadIdx.x & 63;
   Pass mine{0, 0, 0};
   bool found = false;
-  for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
-    int expert, first, rows;
-    read_group(a, g0 + lane, expert, first, rows);
-    const int np = wt_passes(rows, wx_tiles<F>());
-    int incl = np;
+  constexpr int AT_ONCE = 4;  // times 64 groups on their way together
+  for (int g0 = 0; g0 < a.n_groups; g0 += 64 * AT_ONCE) {
+    int expert[AT_ONCE], first[AT_ONCE], rows[AT_ONCE];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(incl, d);
-      if (lane >= d) incl += u;
-    }
-    const int all = __builtin_amdgcn_readlane(incl, 63);
-    int l = 0;  // the first lane whose sum is past `at`
+    for (int i = 0; i < AT_ONCE; i++) read_group(a, g0 + 64 * i + lane, expert[i], first[i], rows[i]);
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1)
-      if (__shfl(incl, l + d - 1) <= at) l += d;
-    const int before = __shfl(incl - np, l), n = __shfl(rows, l), e = __shfl(expert, l), f = __shfl(first, l);
-    if (!found && at < all) {
-      const int step = 16 * wt_tiles(n, wx_tiles<F>()), from = (at - before) * step;
-      mine = Pass{e, f + from, min(step, n - from)};
-      found = true;
+    for (int i = 0; i < AT_ONCE; i++) {
+      if (g0 + 64 * i >= a.n_groups) break;
+      const int np = wt_passes(rows[i], wx_tiles<F>());
+      int incl = np;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(incl, d);
+        if (lane >= d) incl += u;
+      }
+      const int all = __builtin_amdgcn_readlane(incl, 63);
+      int l = 0;  // the first lane whose sum is past `at`
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1)
+        if (__shfl(incl, l + d - 1) <= at) l += d;
+      const int before = __shfl(incl - np, l), n = __shfl(rows[i], l), e = __shfl(expert[i], l), f = __shfl(first[i], l);
+      if (!found && at < all) {
+        const int step = 16 * wt_tiles(n, wx_tiles<F>()), from = (at - before) * step;
+        mine = Pass{e, f + from, min(step, n - from)};
+        found = true;
+      }
+      at -= all;
     }
-    at -= all;
   }
   return mine;
+}
+
+// A row's 16 results of two neighbouring tiles (of `tiles` that there are), lane (q, c) holding 4 of each, as two 16-byte
+// stores a row and tile instead of four of 8: the odd q's of the first tile change places with the even ones of the second,
+// so that a lane holds 8 in a row of one tile. The whole wave calls, also for rows that are not stored.
+D3_INLINE void store_pair(uint16_t* row, i32x2 v0, i32x2 v1, bool stored, int tiles) {
+  const int q = (threadIdx.x & 63) >> 4;
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v0[0], (uint32_t)v1[0], false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)v0[1], (uint32_t)v1[1], false, false);
+  if (stored && (q & 1) < tiles)
+    *(i32x4*)(row + 16 * (q & 1) + 8 * (q >> 1)) = i32x4{(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
 }
 
 template <class F, bool SWIGLU, bool OUT_BF16>
@@ -287,23 +304,23 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
 #pragma unroll
     for (int j = 0; j < NT; j++) {
       const int r = 16 * (wm + 2 * j) + c;
-      if (r >= cur.rows) continue;
       const size_t p = (size_t)(cur.first + r);
       if constexpr (SWIGLU) {
+        const int unit = 8 * cur.column + 2 * wn;  // the wave's two
+        store_pair((uint16_t*)a.out + p * (a.N / 2) + 16 * unit, swiglu_4(acc[j][0], acc[j][2]),
+                   swiglu_4(acc[j][1], acc[j][3]), r < cur.rows, half - unit);
+      } else if constexpr (OUT_BF16) {
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-          const int unit = 8 * cur.column + 2 * wn + n;
-          if (unit >= half) continue;
-          *(i32x2*)((uint16_t*)a.out + p * (a.N / 2) + 16 * unit + 4 * q) = swiglu_4(acc[j][n], acc[j][n + 2]);
+        for (int n = 0; n < 4; n += 2) {
+          const int tile = 16 * cur.column + 4 * wn + n;
+          store_pair((uint16_t*)a.out + p * a.N + 16 * tile, bf16_4(acc[j][n]), bf16_4(acc[j][n + 1]), r < cur.rows,
+                     bank_tiles - tile);
         }
       } else {
 #pragma unroll
         for (int n = 0; n < 4; n++) {
           const int tile = 16 * cur.column + 4 * wn + n;
-          if (tile >= bank_tiles) continue;
-          const size_t o = p * a.N + 16 * tile + 4 * q;
-          if constexpr (OUT_BF16) *(i32x2*)((uint16_t*)a.out + o) = bf16_4(acc[j][n]);
-          else *(f32x4*)((float*)a.out + o) = acc[j][n];
+          if (r < cur.rows && tile < bank_tiles) *(f32x4*)((float*)a.out + p * a.N + 16 * tile + 4 * q) = acc[j][n];
         }
       }
     }
