@@ -69,6 +69,13 @@ __global__ void __launch_bounds__(1024) prompt_scatter_kernel(PromptGroups g) {
     else g.perm[at] = p;
     if (g.inverse) g.inverse[p] = valid ? at : -1;
   }
+  if (b == 0 && g.groups && tid < E) {
+    int* of = g.groups + 5 * tid;
+    of[0] = of[1] = tid;
+    of[2] = 0;
+    of[3] = first;
+    of[4] = v;
+  }
   if (b == 0) {  // bucket k: passes of tiles - k tiles
     const int np = wt_passes(v, g.tiles), tiles = wt_tiles(v, g.tiles);
     if (np) atomicAdd(&pcount[g.tiles - tiles], np);

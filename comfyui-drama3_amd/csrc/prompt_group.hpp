@@ -23,6 +23,7 @@ struct PromptGroups {
   int4* passes;                // [cap] (expert, first place, rows, 0), the passes with most tiles first
   int cap, tiles;              // at most `tiles` 16-row tiles a pass
   int* hist;                   // [PG_BLOCKS, E]
+  int* groups = nullptr;       // [E, 5] (expert, expert, 0, first place, pairs), or null
 };
 
 // pairs per block: whole workgroups' worth, at most PG_BLOCKS of them

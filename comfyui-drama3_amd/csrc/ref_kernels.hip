@@ -2219,6 +2219,17 @@ int d3_prompt_groups(const int64_t* ids, int32_t P, int32_t E, int64_t* order, i
   return done("d3_prompt_groups");
 }
 
+int d3_prompt_expert_groups(const int64_t* ids, int32_t P, int32_t E, int64_t* order, int32_t* inverse, int32_t* groups,
+                            int32_t* scratch, int64_t scratch_ints, void* stream) {
+  if (!groups) return fail("d3_prompt_expert_groups: null pointer");
+  PromptGroups g;
+  if (const int e = prompt_groups_of("d3_prompt_expert_groups", ids, P, E, order, inverse, scratch, scratch_ints, g)) return e;
+  g.groups = groups;
+  launch_prompt_hist(g, (hipStream_t)stream);
+  launch_prompt_scatter(g, (hipStream_t)stream);
+  return done("d3_prompt_expert_groups");
+}
+
 int d3_grouped_fp8(const void* planes, int32_t n_planes, int64_t plane, const int64_t* order, int32_t k,
                    int32_t rows, const int32_t* groups, int32_t n_groups, const int32_t* work, int64_t work_ints,
                    int32_t fills_first, void* slot_w, void* slot_s, const void* host_w, const void* host_s,

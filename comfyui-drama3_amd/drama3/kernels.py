@@ -332,6 +332,22 @@ def prompt_groups(topk_idx, num_experts):
     return order, inverse, passes
 
 
+def prompt_expert_groups(topk_idx, num_experts):
+    """expert_groups (without a plan) over many workgroups: (order, inverse, groups) of a long prompt's pairs."""
+    ids = topk_idx.reshape(-1).contiguous()
+    if ids.dtype != torch.int64:
+        ids = ids.long()
+    P, device = ids.shape[0], ids.device
+    order = torch.empty(P, dtype=torch.int64, device=device)
+    inverse = torch.empty(P, dtype=torch.int32, device=device)
+    groups = torch.empty((num_experts, 5), dtype=torch.int32, device=device)
+    ints = _lib.lib().d3_prompt_pass_ints(num_experts, P)
+    scratch = torch.empty(ints, dtype=torch.int32, device=device)
+    launch("d3_prompt_expert_groups", ids, ids.data_ptr(), P, num_experts, order.data_ptr(), inverse.data_ptr(),
+           groups.data_ptr(), scratch.data_ptr(), ints)
+    return order, inverse, groups
+
+
 def prompt_prep_i8(topk_idx, num_experts, x, rotate):
     """expert_groups_prep_i8 for prompt_i8: (order, inverse, passes, planes, scales), passes the wide products' plan."""
     ids = topk_idx.reshape(-1).contiguous()
@@ -638,6 +654,53 @@ def grouped_bf16(x, groups, weight, n, order=None, k=1, swiglu=False, dtype=torc
     launch("d3_bf16_grouped", out, x.data_ptr(), R, _p(order), k, P, groups.data_ptr(), groups.shape[0],
            weight.data_ptr(), E, n, K, swiglu, out.dtype is torch.bfloat16, out.data_ptr())
     return out
+
+
+# Rows up to which a layer's pairs read their experts one by one (gemv): a grouping launch and its reads cost more there
+# than the experts that several rows share.
+LINE_ROWS = 4
+# Pairs from which the grouping runs over many workgroups: one takes 1 ns a pair, the two launches of many about 8 us.
+GROUPING_PAIRS = 8192
+
+
+def direct_layer(x, topk_idx, topk_weight, num_experts, gemv, grouped):
+    """The routed experts of rows x [T, H], topk_idx [T, k] and topk_weight [T, k] on banks whose products read them as they
+    are stored: gemv(i, rows, ids) and grouped(i, rows, groups, order, k) run bank i (0 gate_up with SiLU(gate) * up, on
+    x; 1 down, on the hidden rows) for pairs of rows and experts. [T, H] in x's dtype: each pair's product weighted and
+    summed over k in float32. A row's result does not depend on the other rows. Nothing waits on the host."""
+    T, k = topk_idx.shape
+    if topk_weight.shape != (T, k) or x.dim() != 2 or x.shape[0] != T:
+        raise ValueError("x [T, H], topk_idx [T, k] and topk_weight [T, k] expected")
+    if not 1 <= num_experts <= 1024:
+        raise ValueError("1 to 1024 experts")
+    if T == 0 or k == 0:
+        return torch.zeros_like(x)
+    if x.get_device() < 0:
+        raise ValueError(f"the kernels run on a GPU, not on {x.device}")
+    with torch.cuda.device(x.device):
+        if T <= LINE_ROWS:
+            ids = topk_idx.reshape(-1).to(torch.int64)
+            parts = gemv(1, gemv(0, x, ids), ids)
+            inverse = torch.arange(T * k, dtype=torch.int32, device=x.device)
+        else:
+            group = prompt_expert_groups if T * k >= GROUPING_PAIRS else expert_groups
+            order, inverse, groups = group(topk_idx, num_experts)
+            parts = grouped(1, grouped(0, x, groups, order, k), groups, None, 1)
+        return combine_rows(parts, inverse, topk_weight, x.dtype)
+
+
+def bf16_layer(x, topk_idx, topk_weight, gate_up, down, num_experts):
+    """The routed layer on banks of bfloat16 weights [E * 2I, H] and [E * H, I]: bfloat16 rows x [T, H] -> [T, H]."""
+    banks = (gate_up, down)
+    if gate_up.shape[0] % num_experts or down.shape[0] % num_experts:
+        raise ValueError(f"banks of {num_experts} experts expected")
+    n = [b.shape[0] // num_experts for b in banks]
+    if n[1] != x.shape[-1] or n[0] != 2 * down.shape[1]:
+        raise ValueError("gate_up [E * 2I, H] and down [E * H, I] expected")
+    return direct_layer(
+        x, topk_idx, topk_weight, num_experts,
+        lambda i, rows, ids: gemv_bf16(rows, ids, banks[i], n[i], swiglu=i == 0),
+        lambda i, rows, groups, order, k: grouped_bf16(rows, groups, banks[i], n[i], order, k, swiglu=i == 0))
 
 
 def decode_codes(qdata, scale, codebook, bits, table=False):

@@ -193,3 +193,16 @@ def grouped(rows, groups, bank, order=None, k=1, swiglu=False, dtype=torch.float
                    groups.data_ptr(), groups.size(0), weight.data_ptr(), wscale.data_ptr(), bank.experts, bank.rows,
                    bank.cols, swiglu, out.dtype is torch.bfloat16, out.data_ptr())
     return out
+
+
+def moe_layer(x, topk_idx, topk_weight, gate_up, down, bits=8):
+    """The routed layer on MxBanks (gate_up [E, 2I, H], down [E, H, I]): rows x [T, H] bfloat16 or float32, topk_idx [T, k],
+    topk_weight [T, k] -> [T, H] in x's dtype. The rows, and the hidden rows SiLU(gate) * up in bfloat16, are quantized to
+    `bits` (8: e4m3, 4: e2m1). A row's result does not depend on the other rows."""
+    banks = (gate_up, down)
+    if down.experts != gate_up.experts or down.rows != x.shape[-1] or gate_up.rows != 2 * down.cols:
+        raise ValueError("gate_up [E, 2I, H] and down [E, H, I] expected")
+    return kernels.direct_layer(
+        x, topk_idx, topk_weight, gate_up.experts,
+        lambda i, rows, ids: gemv(quantize(rows, bits), ids, banks[i], swiglu=i == 0),
+        lambda i, rows, groups, order, k: grouped(quantize(rows, bits), groups, banks[i], order, k, swiglu=i == 0))

@@ -21,6 +21,9 @@ Banks are field dicts of flat tensors, as the kernels read them (offload.py:72-9
   fp8    {"weight": uint8 e4m3 [E * N, K], "scale": float32 [E * N / 128, K / 128]}
   w4/w6  {"_qdata": uint8 [E * N, K * bits / 8], "scale": uint8 e4m3 [E * N, K / 16], "s_channel": float32 [E * N]},
          plus a float32 [16] codebook per bank at 4 bits                       ConvRot basis
+The resident kernels and ExpertTable also take two kinds that the reference has not, as they are (no rotation):
+  bf16   {"weight": bfloat16 [E * N, K]}                                       a checkpoint before conversion
+  mx4    {"weight", "scale"}: the tensors of an mx.MxBank (mx.py), rows quantized to e4m3
 
 ComfyUI (comfy.quant_ops, comfy.model_management) is used when it is importable; without it a quantized weight is any
 object with QuantizedTensor's `_qdata`, `_params` and `_layout_cls`, and the memory budget comes from torch.
@@ -36,7 +39,7 @@ import time
 import torch
 import torch.nn as nn
 
-from . import kernels
+from . import kernels, mx
 
 # The reference's policy constants (offload.py:30-51), with its names and values.
 RESERVE_BASE = 512 * 1024 ** 2           # device memory a generation needs besides the model and the cache
@@ -221,7 +224,21 @@ def _constants(device):
 
 
 def _rows(kind, fields, num_experts):
-    return fields["weight" if kind == "fp8" else "_qdata"].shape[0] // num_experts
+    return fields["weight" if "weight" in fields else "_qdata"].shape[0] // num_experts
+
+
+DIRECT_KINDS = ("bf16", "mx4")  # banks that the products read as they are stored, without rotation or planes
+
+
+def _direct(x, topk_idx, topk_weight, banks, rows, kind):
+    """The routed layer on banks of a direct kind, for rows of any number."""
+    weights = [b["weight"] for b in banks]
+    experts = weights[0].shape[0] // rows[0]
+    if kind == "bf16":
+        return kernels.bf16_layer(x, topk_idx, topk_weight, *weights, experts)
+    cols = (x.shape[-1], rows[0] // 2)
+    gate_up, down = (mx.MxBank(w, b["scale"], experts, n, k) for w, b, n, k in zip(weights, banks, rows, cols))
+    return mx.moe_layer(x, topk_idx, topk_weight, gate_up, down)
 
 
 # Launches of the resident decode where the layer's shape allows: 2 (kernels.resident_decode / resident_decode_routed)
@@ -238,6 +255,8 @@ def resident_decode(x, ids, weights, banks, rows, kind, codebooks):
     expert) (offload.py:108-123): bf16 [1, H]. One launch (kernels.resident_decode_fused) or two (gate_up with x
     rotated in its prologue; down with SwiGLU, the rotation and the weighted sum) where the shapes allow, else the
     reference's five. Nothing waits on the host."""
+    if kind in DIRECT_KINDS:
+        return _direct(x, ids.view(1, -1), weights.view(1, -1), banks, rows, kind)
     gate_up_rows, down_rows = rows
     H, I = down_rows, gate_up_rows // 2
     if H in (1024, 2048) and I in (512, 768, 1024) and ids.shape[0] <= 8 and x.dtype == torch.bfloat16:
@@ -258,7 +277,7 @@ def routed_decode(x, logits, k, banks, rows, kind, codebooks):
         raise ValueError(f"{logits.numel()} logits for banks of {experts} experts: a routed id past the banks would be "
                          f"read out of bounds")
     if (H in (1024, 2048) and I in (512, 768, 1024) and k <= 8 and k <= logits.numel() <= 256
-            and x.dtype == torch.bfloat16 and logits.dtype == torch.bfloat16):
+            and x.dtype == torch.bfloat16 and logits.dtype == torch.bfloat16 and kind not in DIRECT_KINDS):
         if RESIDENT_LAUNCHES == 1 and kernels.resident_fused_fits(kind, H, I, k):
             return kernels.resident_decode_fused(x, banks, kind, codebooks, H, I, logits=logits, k=k)
         return kernels.resident_decode_routed(x, logits, k, banks, kind, codebooks, H, I)
@@ -405,6 +424,8 @@ def _wide_pairs(x, topk_idx, banks, rows, kind, codebooks, num_experts):
 def resident_prefill(x, topk_idx, topk_weight, banks, rows, kind, codebooks, num_experts):
     """Many rows x [T, H] through banks held whole on the GPU (offload.py:138-149): one grouped kernel per bank over
     the pairs grouped by expert on the device, each product weighted and summed over k; x's dtype."""
+    if kind in DIRECT_KINDS:
+        return _direct(x, topk_idx, topk_weight, banks, rows, kind)
     top_k = topk_idx.shape[1]
     planes = None
     if topk_idx.is_cuda and kernels.prompt_wide_fits(kind, banks, rows, topk_idx.numel(), num_experts, x.shape[1]):

@@ -394,6 +394,11 @@ int d3_resident_status(void* workspace, uint32_t* status);
 int d3_decode_codes(int32_t bits, const void* rows, const void* scales, const float* codebook, int32_t R, int32_t K,
                     void* out, void* stream);
 
+/* d3_expert_groups over many workgroups, for long prompts (no counterpart in the reference, whose grouping is torch's sort
+ * and bincount): the same order, inverse and groups; scratch int32 [>= d3_prompt_pass_ints(E, P)], needs no clearing; P >= 1. */
+int d3_prompt_expert_groups(const int64_t* ids, int32_t P, int32_t E, int64_t* order, int32_t* inverse, int32_t* groups,
+                            int32_t* scratch, int64_t scratch_ints, void* stream);
+
 /* ---- Microscaled rows and banks (OCP MX; no counterpart in the reference) -------------------------------------------
  * Elements of 4 bits (e2m1) or 8 (e4m3) in blocks of 32 columns with one e8m0 scale code c each: value = element *
  * 2^(c - 127), 255 is NaN. Rows of `cols` columns (cols % 32 == 0), C = cols rounded up to a multiple of 256:
