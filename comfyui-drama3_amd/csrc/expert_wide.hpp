@@ -4,8 +4,8 @@
 //
 // One workgroup a CU, which walks its share of the (pass, column) items as one stream of stages: the copies of the next
 // item begin during the last stages of this. The rows, which other columns' workgroups read too, are copied a stage ahead;
-// the weights come from HBM and are copied by halves of a stage (a step), three ahead, so that there are always some on
-// their way: with whole stages, one ahead, a stage of bf16 took 4200 clocks, of which the products take 2200.
+// the weights come from HBM and are copied by halves of a stage (a step), three (bf16: four) ahead, so that there are always
+// some on their way: with whole stages, one ahead, a stage of bf16 took 4200 clocks, of which the products take 2200.
 #pragma once
 #include "expert_stream.hpp"
 
@@ -102,15 +102,30 @@ D3_INLINE void store_pair(uint16_t* row, i32x2 v0, i32x2 v1, bool stored, int ti
     *(i32x4*)(row + 16 * (q & 1) + 8 * (q >> 1)) = i32x4{(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
 }
 
+// how many passes there are
+template <class F>
+D3_INLINE int count_passes(const ExpertProduct& a) {
+  int n = 0;
+#pragma unroll 4
+  for (int g0 = 0; g0 < a.n_groups; g0 += 64) {
+    int expert, first, rows;
+    read_group(a, g0 + (threadIdx.x & 63), expert, first, rows);
+    n += wt_passes(rows, wx_tiles<F>());
+  }
+  return wave_sum_i32(n);
+}
+
 template <class F, bool SWIGLU, bool OUT_BF16>
-__global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduct a, int columns, int items) {
+__global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduct a, int columns) {
   constexpr int TILES = wx_tiles<F>(), ROWS = 16 * TILES, STEP = WX_N * 64, STAGE = ROWS * F::ROW;
   constexpr int PER = 1024 / F::ROW, LANES = 64 / PER;  // rows of a 1 KB copy, lanes to a row of it
   constexpr int COPIES = ROWS / PER / 8;                // of the rows, per wave
   constexpr int SCOPIES = F::SCALED ? (ROWS + 255) / 256 : 0;  // of the rows' scale words, per wave
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * STEP + 2 * STAGE];  // four steps' weights, two stages' rows
-  __shared__ __attribute__((aligned(256))) uint8_t xscale[2][F::SCALED ? 2048 * SCOPIES : 16];
-  __shared__ __attribute__((aligned(256))) uint32_t wscale[2][F::SCALED ? 16 * 64 : 64];  // by stage pair: tile, lane
+  // LDS: RING steps' weights, two stages' rows, and of microscaled ones the rows' scales of two stages and the weights' scale
+  // words of two pairs of stages (tile, lane); all of a CU's 160 KB for bf16 and e2m1
+  constexpr int RING = F::SCALED ? 4 : 5, XSCALE = 2048 * SCOPIES, WSCALE = F::SCALED ? 16 * 256 : 0;
+  constexpr int AT_ROWS = RING * STEP, AT_XSCALE = AT_ROWS + 2 * STAGE, AT_WSCALE = AT_XSCALE + 2 * XSCALE;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[AT_WSCALE + 2 * WSCALE];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, c = lane & 15, wn = w & 3, wm = w >> 2;
   const int S = a.stages, bank_tiles = a.N / 16, half = bank_tiles / 2;
@@ -119,29 +134,47 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
   const uint32_t woff = F::SCALED ? 16 * lane
                                   : (uint32_t)((lane >> 2) * S * 128 + 16 * wx_step_slot(lane >> 2, lane & 3));
 
-  // The workgroup's items: every gridDim.x-th of the list, 64 of them looked up at a time (lane i: item i)
-  Pass table;
-  int taken = 64, lin = (int)blockIdx.x - (int)gridDim.x;
+  // The workgroup's items. Two passes that follow each other (mostly one expert's) go to one XCD with all columns of each, so
+  // that their weights and rows are read once into its L2; its items are dealt to its workgroups in turn. Those that are left
+  // for the last turn, if they are at most half as many as the workgroups, are shared by two each: such an item has every
+  // other tile twice in LDS and stores one (its products cost as much as before, its weights from HBM half).
+  const int xcd = blockIdx.x & 7, turn0 = blockIdx.x >> 3, per_turn = gridDim.x >> 3;
+  const int passes = count_passes<F>(a), mine = passes / 16 * 2 + min(max(passes % 16 - 2 * xcd, 0), 2);
+  const int items = mine * columns, turns = items / per_turn, rest = items % per_turn;
+  const bool shared = 2 * rest <= per_turn;
   struct Item {
-    int expert, first, rows, column;
+    int expert, first, rows, column, part;  // part: 0 or 1 of a shared item, -1 of a whole one
   };
+  // item k of this workgroup, an index into the XCD's items (-1: none), with its part; the pass and column of an item
+  auto item_at = [&](int k, int& part) __attribute__((always_inline)) {
+    part = k == turns && shared ? turn0 & 1 : -1;
+    if (k < turns) return turn0 + k * per_turn;
+    const int at = shared ? turn0 >> 1 : turn0;
+    return k == turns && at < rest ? turns * per_turn + at : -1;
+  };
+  auto place = [&](int i, int& at, int& column) __attribute__((always_inline)) {
+    const int chunk = i / (2 * columns), in = i % (2 * columns), size = min(2, mine - 2 * chunk);
+    at = 16 * chunk + 2 * xcd + in % size;
+    column = in / size;
+  };
+  Pass table;  // of 64 items: lane l that of item 64 n + l
+  int taken = 0;
   auto next_item = [&](Item& t) __attribute__((always_inline)) {
     t.rows = 0;
-    while (t.rows == 0) {
-      lin += gridDim.x;
-      if (lin >= items) return;
-      if (taken == 64) {
-        int at, column;
-        wt_place(lin + lane * gridDim.x, columns, at, column);
-        table = wide_passes<F>(a, at);
-        taken = 0;
-      }
-      int at;
-      wt_place(lin, columns, at, t.column);
-      t.expert = __builtin_amdgcn_readlane(table.expert, taken), t.first = __builtin_amdgcn_readlane(table.first, taken);
-      t.rows = __builtin_amdgcn_readlane(table.rows, taken);
-      taken++;
+    const int i = item_at(taken, t.part);
+    if (i < 0) return;
+    int at, column;
+    if ((taken & 63) == 0) {
+      int part;
+      const int own = item_at(taken + lane, part);
+      place(max(own, 0), at, column);
+      table = wide_passes<F>(a, at);
     }
+    place(i, at, t.column);
+    const int l = taken & 63;
+    t.expert = __builtin_amdgcn_readlane(table.expert, l), t.first = __builtin_amdgcn_readlane(table.first, l);
+    t.rows = __builtin_amdgcn_readlane(table.rows, l);
+    taken++;
   };
   // where an item's weights lie: wave w copies the tiles in places 2 w and 2 w + 1, and their scales
   struct Weights {
@@ -151,9 +184,10 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       // the expert's tile in the place of the 16 (a place past the expert's last tile repeats that)
-      const int slot = 2 * w + i;
-      const int tile = SWIGLU ? min(8 * t.column + 2 * (slot >> 2) + (slot & 1), half - 1) + ((slot >> 1) & 1) * half
-                              : min(16 * t.column + slot, bank_tiles - 1);
+      const int slot = 2 * w + i, part = max(t.part, 0);
+      const int unit = t.part < 0 ? 2 * (slot >> 2) + (slot & 1) : 4 * part + (slot >> 2);
+      const int tile = SWIGLU ? min(8 * t.column + unit, half - 1) + ((slot >> 1) & 1) * half
+                              : min(16 * t.column + (t.part < 0 ? slot : 8 * part + (slot >> 1)), bank_tiles - 1);
       const size_t n = (size_t)t.expert * bank_tiles + tile;
       at.src[i] = a.w + n * ((size_t)S * 2048);
       at.word[i] = a.w_scale + n * (64 * (size_t)mx_lane_scales(S));
@@ -191,16 +225,16 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
             woff);
   };
   auto load_rows = [&](int k, int st, int buf) __attribute__((always_inline)) {
-    dma16(lds0 + 4 * STEP + buf * STAGE + (uint32_t)(w + 8 * k) * 1024, a.x + (size_t)st * F::ROW, xoff[k]);
+    dma16(lds0 + AT_ROWS + buf * STAGE + (uint32_t)(w + 8 * k) * 1024, a.x + (size_t)st * F::ROW, xoff[k]);
   };
   // (all waves as many copies, so that each knows how many of its loads are on their way: past the rows, the last one again)
   auto load_scales = [&](int st, int buf, int pair, const Weights& of) __attribute__((always_inline)) {
     if constexpr (F::SCALED) {
 #pragma unroll
-      for (int k = 0; k < SCOPIES; k++) dma4(lds_address(xscale[buf]) + 256 * (w + 8 * k), a.x_scale + 8 * st, soff[k]);
+      for (int k = 0; k < SCOPIES; k++) dma4(lds0 + AT_XSCALE + buf * XSCALE + 256 * (w + 8 * k), a.x_scale + 8 * st, soff[k]);
 #pragma unroll
       for (int k = 0; k < 2; k++)
-        dma4(lds_address(wscale[pair]) + 256 * (2 * w + k), of.word[k] + 4 * (st >> 1), lane * mx_lane_scales(S));
+        dma4(lds0 + AT_WSCALE + pair * WSCALE + 256 * (2 * w + k), of.word[k] + 4 * (st >> 1), lane * mx_lane_scales(S));
     }
   };
 
@@ -209,10 +243,10 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
   find_pairs(cur);
   find_weights(cur, at);
   nxt.rows = 0;
-  int buf = 0, pair = 1;  // the buffers of the stage and of the pair of stages (for its scale words)
-  load_weights(0, 0, 0);
-  load_weights(0, 1, 1);
-  load_weights(1, 0, 2);
+  // the buffers of the step's weights, of the stage's rows and of the pair of stages' scale words
+  int ring = 0, buf = 0, pair = 1;
+#pragma unroll
+  for (int h = 0; h < RING - 1; h++) load_weights(h >> 1, h & 1, h);
   find_rows();
 #pragma unroll
   for (int k = 0; k < COPIES; k++)
@@ -237,12 +271,12 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
       for (int s = 0; s < 2; s++)
 #pragma unroll
         for (int k = 0; k < F::PIECES; k++)
-          xlane[s][k] = smem + 4 * STEP + buf * STAGE + (16 * wm + c) * F::ROW + 16 * wx_slot<F>(c, F::b_piece(s, q, k));
-      const uint8_t* slane = xscale[buf] + 8 * (16 * wm + c) + 2 * q;
+          xlane[s][k] = smem + AT_ROWS + buf * STAGE + (16 * wm + c) * F::ROW + 16 * wx_slot<F>(c, F::b_piece(s, q, k));
+      const uint8_t* slane = smem + AT_XSCALE + buf * XSCALE + 8 * (16 * wm + c) + 2 * q;
       i32x4 wa[4], b[4][F::PIECES];
       uint32_t sw[4] = {0, 0, 0, 0}, sb[4] = {0, 0, 0, 0};
       auto read_w = [&](int s) __attribute__((always_inline)) {
-        const uint8_t* from = smem + (2 * buf + s) * STEP + 4 * wn * 1024 +
+        const uint8_t* from = smem + ring * STEP + 4 * wn * 1024 +
                               (F::SCALED ? 16 * lane : c * 64 + 16 * wx_step_slot(c, q));
 #pragma unroll
         for (int n = 0; n < 4; n++) wa[n] = *(const i32x4*)(from + 1024 * n);
@@ -256,7 +290,7 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
       read_x(0);
       if constexpr (F::SCALED) {
 #pragma unroll
-        for (int n = 0; n < 4; n++) sw[n] = wscale[pair][64 * (4 * wn + n) + lane] >> (16 * (st & 1));
+        for (int n = 0; n < 4; n++) sw[n] = *(const uint32_t*)(smem + AT_WSCALE + pair * WSCALE + 256 * (4 * wn + n) + 4 * lane) >> (16 * (st & 1));
       }
       read_x(1);
       // The next stage's rows, of this item or the next, go out between the products: those that this item's rows need
@@ -288,16 +322,23 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
           }
         }
       };
+      // A step's weights go to the buffer of the step before. They come in the order in which they were asked for: with the
+      // next stage's rows, those of its steps that went out before have come too.
+      auto next_step = [&](int s) __attribute__((always_inline)) {  // RING - 1 steps on
+        load_weights(st + (s + RING - 1) / 2, (s + RING - 1) & 1, ring ? ring - 1 : RING - 1);
+      };
+      auto turn = [&]() __attribute__((always_inline)) { ring = ring + 1 < RING ? ring + 1 : 0; };
       products.template operator()<0>();
-      load_weights(st + 1, 1, 2 * (buf ^ 1) + 1);
-      // the second step's weights: all but the step after them and this step's copies
-      wait_loads<2 + SCOPIES + (F::SCALED ? 2 : 0) + MINE + 2>();
+      next_step(0);
+      if constexpr (RING == 4) wait_loads<2 + SCOPIES + 2 + MINE + 2>();  // all but the step after the next and this step's copies
       __syncthreads();
+      turn();
       read_w(1);
-      load_weights(st + 2, 0, 2 * buf);
+      next_step(1);
       products.template operator()<1>();
-      wait_loads<4>();  // the next stage: all but the last two steps' weights
+      wait_loads<4>();  // all but this stage's two steps of weights
       __syncthreads();
+      turn();
     }
 
     // lane l holds weight rows 4 q .. + 3 of its tiles of the pass's row 16 (wm + 2 j) + c
@@ -305,22 +346,27 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
     for (int j = 0; j < NT; j++) {
       const int r = 16 * (wm + 2 * j) + c;
       const size_t p = (size_t)(cur.first + r);
+      const bool whole = cur.part < 0, stored = r < cur.rows;
       if constexpr (SWIGLU) {
-        const int unit = 8 * cur.column + 2 * wn;  // the wave's two
+        const int unit = 8 * cur.column + (whole ? 2 * wn : 4 * cur.part + wn);  // the wave's two, or one
         store_pair((uint16_t*)a.out + p * (a.N / 2) + 16 * unit, swiglu_4(acc[j][0], acc[j][2]),
-                   swiglu_4(acc[j][1], acc[j][3]), r < cur.rows, half - unit);
-      } else if constexpr (OUT_BF16) {
-#pragma unroll
-        for (int n = 0; n < 4; n += 2) {
-          const int tile = 16 * cur.column + 4 * wn + n;
-          store_pair((uint16_t*)a.out + p * a.N + 16 * tile, bf16_4(acc[j][n]), bf16_4(acc[j][n + 1]), r < cur.rows,
-                     bank_tiles - tile);
-        }
+                   swiglu_4(acc[j][1], acc[j][3]), stored, min(half - unit, whole ? 2 : 1));
       } else {
+        const int tile0 = 16 * cur.column + (whole ? 4 * wn : 8 * cur.part + 2 * wn);
+        if constexpr (OUT_BF16) {
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-          const int tile = 16 * cur.column + 4 * wn + n;
-          if (r < cur.rows && tile < bank_tiles) *(f32x4*)((float*)a.out + p * a.N + 16 * tile + 4 * q) = acc[j][n];
+          for (int n = 0; n < 4; n += 2) {
+            const int tile = tile0 + (whole ? n : n >> 1);
+            store_pair((uint16_t*)a.out + p * a.N + 16 * tile, bf16_4(acc[j][n]), bf16_4(acc[j][n + 1]), stored,
+                       min(bank_tiles - tile, whole ? 2 : 1));
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < 4; n++) {
+            const int tile = tile0 + (whole ? n : n >> 1);
+            if (stored && tile < bank_tiles && (whole || !(n & 1)))
+              *(f32x4*)((float*)a.out + p * a.N + 16 * tile + 4 * q) = acc[j][n];
+          }
         }
       }
     }
@@ -328,18 +374,18 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
   wait_loads<0>();
   __syncthreads();
   while (true) {
-    const int mine = ((cur.rows + 15) / 16 + 1) / 2;  // tiles of a wave, at most
+    const int most = ((cur.rows + 15) / 16 + 1) / 2;  // tiles of a wave
     if constexpr (TILES > 10) {
-      if (mine > 9) run.template operator()<10>();
-      else if (mine > 8) run.template operator()<9>();
-      else if (mine > 7) run.template operator()<8>();
-      else if (mine > 6) run.template operator()<7>();
-      else if (mine > 5) run.template operator()<6>();
+      if (most > 9) run.template operator()<10>();
+      else if (most > 8) run.template operator()<9>();
+      else if (most > 7) run.template operator()<8>();
+      else if (most > 6) run.template operator()<7>();
+      else if (most > 5) run.template operator()<6>();
     }
-    if (TILES <= 10 || mine <= 5) {
-      if (mine > 4) run.template operator()<5>();
-      else if (mine > 3) run.template operator()<4>();
-      else if (mine > 2) run.template operator()<3>();
+    if (TILES <= 10 || most <= 5) {
+      if (most > 4) run.template operator()<5>();
+      else if (most > 3) run.template operator()<4>();
+      else if (most > 2) run.template operator()<3>();
       else run.template operator()<2>();
     }
     if (nxt.rows == 0) break;
@@ -363,11 +409,12 @@ inline int device_cus() {
 template <class F>
 void launch_wide(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
   const int columns = (a.N + WX_N - 1) / WX_N, passes = most_passes(a.pairs, a.n_groups, 16 * wx_tiles<F>());
-  const int items = wt_places(passes) * columns;
-  const dim3 grid((unsigned)std::min(items, device_cus())), block(WX_THREADS);
-  if (swiglu) hipLaunchKernelGGL((expert_wide_kernel<F, true, true>), grid, block, 0, s, a, columns, items);
-  else if (out_bf16) hipLaunchKernelGGL((expert_wide_kernel<F, false, true>), grid, block, 0, s, a, columns, items);
-  else hipLaunchKernelGGL((expert_wide_kernel<F, false, false>), grid, block, 0, s, a, columns, items);
+  const int64_t items = (int64_t)2 * passes * columns;  // shared ones twice
+  const int cus = std::max(device_cus() & ~7, 8);       // as many for each XCD
+  const dim3 grid((unsigned)std::min<int64_t>((items + 7) & ~7, cus)), block(WX_THREADS);
+  if (swiglu) hipLaunchKernelGGL((expert_wide_kernel<F, true, true>), grid, block, 0, s, a, columns);
+  else if (out_bf16) hipLaunchKernelGGL((expert_wide_kernel<F, false, true>), grid, block, 0, s, a, columns);
+  else hipLaunchKernelGGL((expert_wide_kernel<F, false, false>), grid, block, 0, s, a, columns);
 }
 
 // Whether a grouped product runs in wide passes: by the rows an expert has on average. (The copies to LDS take 32-bit
