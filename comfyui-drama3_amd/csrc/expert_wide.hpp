@@ -52,54 +52,48 @@ D3_INLINE int wx_piece(int r, int t) {
 // the same of bf16 weights by the step, 64 bytes a row: piece q of row r of 16
 D3_INLINE int wx_step_slot(int r, int q) { return q ^ ((4 - (r >> 2)) & 3); }
 
+// The passes go by what they cost: those of most tiles first (three classes of them), so that the items of a turn take
+// about as long as each other. How many passes of class `k` an expert's rows have.
+constexpr int WX_CLASSES = 3;
+template <class F>
+D3_INLINE int class_passes(int rows, int k) {
+  const int tiles = 20 * wt_tiles(rows, wx_tiles<F>()) / wx_tiles<F>();
+  return k == (tiles > 14 ? 0 : tiles > 7 ? 1 : 2) ? wt_passes(rows, wx_tiles<F>()) : 0;
+}
+
 // The passes of 64 items at once, one a lane: pass `at` (each lane's own) of the groups' passes in wx_tiles tiles or
-// fewer, an expert's passes as long as each other but for the last; no rows where there is no such pass.
+// fewer, an expert's passes as long as each other but for the last.
 template <class F>
 D3_INLINE Pass wide_passes(const ExpertProduct& a, int at) {
   const int lane = threadIdx.x & 63;
   Pass mine{0, 0, 0};
-  bool found = false;
   constexpr int AT_ONCE = 4;  // times 64 groups on their way together
-  for (int g0 = 0; g0 < a.n_groups; g0 += 64 * AT_ONCE) {
-    int expert[AT_ONCE], first[AT_ONCE], rows[AT_ONCE];
+  for (int k = 0; k < WX_CLASSES; k++) {
+    for (int g0 = 0; g0 < a.n_groups; g0 += 64 * AT_ONCE) {
+      int expert[AT_ONCE], first[AT_ONCE], rows[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < AT_ONCE; i++) read_group(a, g0 + 64 * i + lane, expert[i], first[i], rows[i]);
+      for (int i = 0; i < AT_ONCE; i++) read_group(a, g0 + 64 * i + lane, expert[i], first[i], rows[i]);
 #pragma unroll
-    for (int i = 0; i < AT_ONCE; i++) {
-      if (g0 + 64 * i >= a.n_groups) break;
-      const int np = wt_passes(rows[i], wx_tiles<F>());
-      int incl = np;
+      for (int i = 0; i < AT_ONCE; i++) {
+        if (g0 + 64 * i >= a.n_groups) break;
+        const int np = class_passes<F>(rows[i], k), incl = wave_scan_i32(np), all = __builtin_amdgcn_readlane(incl, 63);
+        if (__ballot(at >= 0 && at < all)) {
+          int l = 0;  // the first lane whose sum is past `at`
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(incl, d);
-        if (lane >= d) incl += u;
+          for (int d = 32; d > 0; d >>= 1)
+            if (__shfl(incl, l + d - 1) <= at) l += d;
+          l = min(l, 63);
+          const int before = __shfl(incl - np, l), n = __shfl(rows[i], l), e = __shfl(expert[i], l), f = __shfl(first[i], l);
+          if (at >= 0 && at < all) {
+            const int step = 16 * wt_tiles(n, wx_tiles<F>()), from = (at - before) * step;
+            mine = Pass{e, f + from, min(step, n - from)};
+          }
+        }
+        at -= all;  // (below zero once found)
       }
-      const int all = __builtin_amdgcn_readlane(incl, 63);
-      int l = 0;  // the first lane whose sum is past `at`
-#pragma unroll
-      for (int d = 32; d > 0; d >>= 1)
-        if (__shfl(incl, l + d - 1) <= at) l += d;
-      const int before = __shfl(incl - np, l), n = __shfl(rows[i], l), e = __shfl(expert[i], l), f = __shfl(first[i], l);
-      if (!found && at < all) {
-        const int step = 16 * wt_tiles(n, wx_tiles<F>()), from = (at - before) * step;
-        mine = Pass{e, f + from, min(step, n - from)};
-        found = true;
-      }
-      at -= all;
     }
   }
   return mine;
-}
-
-// A row's 16 results of two neighbouring tiles (of `tiles` that there are), lane (q, c) holding 4 of each, as two 16-byte
-// stores a row and tile instead of four of 8: the odd q's of the first tile change places with the even ones of the second,
-// so that a lane holds 8 in a row of one tile. The whole wave calls, also for rows that are not stored.
-D3_INLINE void store_pair(uint16_t* row, i32x2 v0, i32x2 v1, bool stored, int tiles) {
-  const int q = (threadIdx.x & 63) >> 4;
-  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v0[0], (uint32_t)v1[0], false, false);
-  const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)v0[1], (uint32_t)v1[1], false, false);
-  if (stored && (q & 1) < tiles)
-    *(i32x4*)(row + 16 * (q & 1) + 8 * (q >> 1)) = i32x4{(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
 }
 
 // how many passes there are
@@ -113,6 +107,17 @@ D3_INLINE int count_passes(const ExpertProduct& a) {
     n += wt_passes(rows, wx_tiles<F>());
   }
   return wave_sum_i32(n);
+}
+
+// A row's 16 results of two neighbouring tiles (of `tiles` that there are), lane (q, c) holding 4 of each, as two 16-byte
+// stores a row and tile instead of four of 8: the odd q's of the first tile change places with the even ones of the second,
+// so that a lane holds 8 in a row of one tile. The whole wave calls, also for rows that are not stored.
+D3_INLINE void store_pair(uint16_t* row, i32x2 v0, i32x2 v1, bool stored, int tiles) {
+  const int q = (threadIdx.x & 63) >> 4;
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v0[0], (uint32_t)v1[0], false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)v0[1], (uint32_t)v1[1], false, false);
+  if (stored && (q & 1) < tiles)
+    *(i32x4*)(row + 16 * (q & 1) + 8 * (q >> 1)) = i32x4{(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
 }
 
 template <class F, bool SWIGLU, bool OUT_BF16>

@@ -125,16 +125,21 @@ D3_INLINE void read_group(const ExpertProduct& a, int g, int& expert, int& first
   if (expert < 0 || expert >= a.E || first < 0 || rows < 0 || first > a.pairs || rows > a.pairs - first) rows = 0;
 }
 
+// the sum of n over the lanes up to this one
+D3_INLINE int wave_scan_i32(int n) {
+  n += __builtin_amdgcn_update_dpp(0, n, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8: within rows of 16 lanes
+  n += __builtin_amdgcn_update_dpp(0, n, 0x112, 0xF, 0xF, true);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x114, 0xF, 0xF, true);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x118, 0xF, 0xF, true);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x142, 0xA, 0xF, false);  // row_bcast 15: the first row's sum to the second, ..
+  n += __builtin_amdgcn_update_dpp(0, n, 0x143, 0xC, 0xF, false);  // row_bcast 31: the first half's to the second
+  return n;
+}
+
 // The first lane with at < the sum of n over the lanes up to it, and in `before` the sum over those before it; -1 if
 // there is none, with the sum over all. The whole wave calls.
 D3_INLINE int find_lane(int n, int at, int& before) {
-  const int lane = threadIdx.x & 63;
-  int incl = n;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int u = __shfl_up(incl, d);
-    if (lane >= d) incl += u;
-  }
+  const int incl = wave_scan_i32(n);
   const uint64_t past = __ballot(incl > at);
   if (!past) {
     before = __builtin_amdgcn_readlane(incl, 63);
