@@ -26,6 +26,8 @@ inline int check_product(const std::string& what, const ExpertProduct& a, int K,
   if (grouped) {
     if (!a.groups || a.n_groups < 1) return fail(what + ": pairs without groups");
     if (a.k < 1) return fail(what + ": k must be positive");
+    // (groups may overlap: what the passes are counted in)
+    if (((int64_t)a.pairs / 16 + 1) * a.n_groups > INT32_MAX) return fail(what + ": too many pairs and groups for one launch");
     if (!a.order && a.x_rows < a.pairs) return fail(what + ": fewer rows than pairs, and no order");
   } else {
     if (!a.ids) return fail(what + ": null pointer");

@@ -261,11 +261,29 @@ def test_results_do_not_depend_on_the_other_rows(fmt):
             assert torch.equal(got, want[:counts][order])
 
 
+@pytest.mark.parametrize("E, rows, n", [(10, 300, 800), (70, 33, 800), (100, 34, 800), (300, 34, 96)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_more_items_than_workgroups(fmt, E, rows, n):
+    """Wide passes where a workgroup walks several of them, with a last turn that is shared and one that is not, more
+    than 256 groups, and a last column that is not full: bit for bit the single pairs' results, some of them checked."""
+    K = 128 if fmt == "bf16" else 512
+    counts = np.random.default_rng(E).integers(rows - 1, rows + 2, E)
+    counts[3], counts[5] = 0, 7 * rows
+    P = int(counts.sum())
+    case = Case(fmt, E, n, K, P)
+    ids, order, _, groups = _pairs(E, counts)
+    for how in ({}, {"swiglu": True}, {"dtype": torch.bfloat16}):
+        got = case.grouped(groups, order=order, **how)
+        assert torch.equal(got, case.gemv(ids, **how)[order])
+        at = torch.arange(0, P, 499, device=DEV)
+        case.check(got[at], order[at], ids[order[at]], "swiglu" in how)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_groups_outside_are_left_alone(fmt):
     """Places in no group and groups whose expert or places lie outside keep what `out` held; order's values outside
     the rows read the nearest row."""
-    case = Case(fmt, 3, 32, 256, 40)
+    case = Case(fmt, 3, 32, 512, 40)
     groups = torch.tensor([[0, 0, 0, 5, 7], [3, 0, 0, 12, 4], [-1, 0, 0, 16, 4], [1, 0, 0, 38, 3], [2, 0, 0, -2, 3],
                            [1, 0, 0, 20, 0], [2, 0, 0, 30, 2], [1, 0, 0, 25, -1], [2, 0, 0, 2 ** 31 - 1, 2],
                            [0, 0, 0, 2, 2 ** 31 - 1]], dtype=torch.int32, device=DEV)
@@ -278,6 +296,14 @@ def test_groups_outside_are_left_alone(fmt):
     rows = torch.arange(40, device=DEV)
     case.check(got[5:12], rows[5:12], rows[5:12] * 0)
     case.check(got[30:32], rows[30:32], rows[30:32] * 0 + 2)
+    # the same groups in wide passes (40 places an entry)
+    wide, far = torch.full((400, 32), -7.0, device=DEV), torch.arange(400, device=DEV) % 40
+    case.grouped(groups, order=far, out=wide)
+    touched = torch.zeros(400, dtype=torch.bool, device=DEV)
+    for first, n, e in ((5, 7, 0), (30, 2, 2), (38, 3, 1)):
+        touched[first:first + n] = True
+        case.check(wide[first:first + n], far[first:first + n], far[first:first + n] * 0 + e)
+    assert torch.all(wide[~touched] == -7)
     order = torch.tensor([-5, 2 ** 40, 79, 0], device=DEV)
     one = torch.tensor([[0, 0, 0, 0, 4]], dtype=torch.int32, device=DEV)
     case.check(case.grouped(one, order=order, k=2), torch.tensor([0, 39, 39, 0], device=DEV), order * 0)
