@@ -343,8 +343,8 @@ def prompt_expert_groups(topk_idx, num_experts):
     groups = torch.empty((num_experts, 5), dtype=torch.int32, device=device)
     ints = _lib.lib().d3_prompt_pass_ints(num_experts, P)
     scratch = torch.empty(ints, dtype=torch.int32, device=device)
-    launch("d3_prompt_expert_groups", ids, ids.data_ptr(), P, num_experts, order.data_ptr(), inverse.data_ptr(),
-           groups.data_ptr(), scratch.data_ptr(), ints)
+    launch("d3_prompt_expert_groups", ids.get_device(), ids.data_ptr(), P, num_experts, order.data_ptr(),
+           inverse.data_ptr(), groups.data_ptr(), scratch.data_ptr(), ints)
     return order, inverse, groups
 
 
@@ -558,12 +558,11 @@ def fp8_linear(x, weight, scale):
 _raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def launch(name, t, *args):
-    """C entry `name` with `args` and torch's current stream of t's device, that device the current one. (The stream's
+def launch(name, index, *args):
+    """C entry `name` with `args` and torch's current stream of device `index`, that device the current one. (The stream's
     handle as torch's own generated code asks for it: a Stream object costs 2 us, as much as the launch.)"""
-    index = t.get_device()
     if index < 0:
-        raise ValueError(f"{name}: the kernels run on a GPU, not on {t.device}")
+        raise ValueError(f"{name}: the kernels run on a GPU, not on the CPU")
     fn = getattr(_lib.lib(), name)
     if index == _current():
         rc = fn(*args, _raw_stream(index))
@@ -574,8 +573,9 @@ def launch(name, t, *args):
         _lib.check(rc, name)
 
 
-def product_out(device, pairs, n, swiglu, dtype, out):
-    """The tensor a product of `pairs` rows with experts of n weight rows writes: `out` checked, or a new one."""
+def product_out(like, pairs, n, swiglu, dtype, out):
+    """The tensor a product of `pairs` rows with experts of n weight rows writes, on `like`'s device: `out` checked, or a
+    new one."""
     if n % (32 if swiglu else 16):
         raise ValueError(f"gate and up rows are multiples of 16 each, not {n} in all" if swiglu else
                          f"experts have a multiple of 16 weight rows, not {n}")
@@ -584,50 +584,50 @@ def product_out(device, pairs, n, swiglu, dtype, out):
     elif dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise TypeError("products are float32 or bfloat16")
     if out is None:
-        return torch.empty((pairs, n), dtype=dtype, device=device)
-    if out.shape != (pairs, n) or out.dtype != dtype or out.device != device or not out.is_contiguous():
-        raise ValueError(f"out [{pairs}, {n}] {dtype}, contiguous, on {device}, expected")
+        return like.new_empty((pairs, n), dtype=dtype)
+    if out.shape != (pairs, n) or out.dtype is not dtype or out.device != like.device or not out.is_contiguous():
+        raise ValueError(f"out [{pairs}, {n}] {dtype}, contiguous, on {like.device}, expected")
     return out
 
 
-def pair_ids(ids, rows, device):
+def pair_ids(ids, rows, index):
     """A gemv's expert ids [P] int64, contiguous, and P: a multiple of the rows."""
-    if ids.dtype is not torch.int64 or ids.dim() != 1 or ids.device != device:
-        raise ValueError(f"ids [P] int64 on {device} expected")
+    if ids.dtype is not torch.int64 or ids.dim() != 1 or ids.get_device() != index:
+        raise ValueError("ids [P] int64 on the rows' device expected")
     P = ids.numel()
     if P % rows if rows else P:
         raise ValueError(f"{P} ids for {rows} rows: a multiple of the rows is expected")
     return ids.contiguous(), P
 
 
-def check_groups(groups, order, k, rows, device):
+def check_groups(groups, order, k, rows, index):
     """The pairs of a grouped product: order's places, or the rows themselves without it."""
-    if groups.dtype != torch.int32 or groups.dim() != 2 or groups.shape[1] != 5 or not groups.is_contiguous() \
-            or groups.device != device:
-        raise ValueError(f"groups [g, 5] int32, contiguous, on {device}, expected")
+    if groups.dtype is not torch.int32 or groups.dim() != 2 or groups.size(1) != 5 or not groups.is_contiguous() \
+            or groups.get_device() != index:
+        raise ValueError("groups [g, 5] int32, contiguous, on the rows' device, expected")
     if k < 1:
         raise ValueError(f"k is positive, not {k}")
     if order is None:
         if k != 1:
             raise ValueError("k goes with order")
         return rows
-    if order.dtype != torch.int64 or order.dim() != 1 or not order.is_contiguous() or order.device != device:
-        raise ValueError(f"order [P] int64, contiguous, on {device}, expected")
-    return order.shape[0]
+    if order.dtype is not torch.int64 or order.dim() != 1 or not order.is_contiguous() or order.get_device() != index:
+        raise ValueError("order [P] int64, contiguous, on the rows' device, expected")
+    return order.size(0)
 
 
 def _bf16_operands(x, weight, n):
-    """(x, R, K, experts, device) of a product of rows x [R, K] with a bank of bfloat16 weights [E * n, K]."""
+    """(x, R, K, experts, device index) of a product of rows x [R, K] with a bank of bfloat16 weights [E * n, K]."""
     if x.dim() != 2 or x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16:
         raise TypeError("x [R, K] and weight [E * n, K] bfloat16 expected")
-    (R, K), device = x.shape, x.device
+    (R, K), index = x.shape, x.get_device()
     if K < 64 or K % 64:
         raise ValueError(f"K is a positive multiple of 64, not {K}")
     if n < 1 or weight.dim() != 2 or weight.size(1) != K or weight.size(0) % n or not weight.is_contiguous() \
-            or weight.device != device:
-        raise ValueError(f"weight [E * {n}, {K}], contiguous, on {device}, expected")
+            or weight.get_device() != index:
+        raise ValueError(f"weight [E * {n}, {K}], contiguous, on the rows' device, expected")
     x = x.contiguous()
-    return (x if x.data_ptr() % 16 == 0 else x.clone()), R, K, weight.size(0) // n, device
+    return (x if x.data_ptr() % 16 == 0 else x.clone()), R, K, weight.size(0) // n, index
 
 
 def gemv_bf16(x, ids, weight, n, swiglu=False, dtype=torch.float32, out=None):
@@ -635,10 +635,10 @@ def gemv_bf16(x, ids, weight, n, swiglu=False, dtype=torch.float32, out=None):
     x [R, K] and experts ids [P] (int64): [P, n] float32 or bfloat16, pair p row p // (P / R) of x with expert ids[p],
     float32 sums. With `swiglu` (gate rows, then up rows) [P, n / 2] bfloat16 = SiLU(gate) * up. An id outside the bank
     gives zeros."""
-    x, R, K, E, device = _bf16_operands(x, weight, n)
-    ids, P = pair_ids(ids, R, device)
-    out = product_out(device, P, n, swiglu, dtype, out)
-    launch("d3_bf16_gemv", out, x.data_ptr(), R, ids.data_ptr(), P, weight.data_ptr(), E, n, K, swiglu,
+    x, R, K, E, index = _bf16_operands(x, weight, n)
+    ids, P = pair_ids(ids, R, index)
+    out = product_out(x, P, n, swiglu, dtype, out)
+    launch("d3_bf16_gemv", index, x.data_ptr(), R, ids.data_ptr(), P, weight.data_ptr(), E, n, K, swiglu,
            out.dtype is torch.bfloat16, out.data_ptr())
     return out
 
@@ -648,10 +648,10 @@ def grouped_bf16(x, groups, weight, n, order=None, k=1, swiglu=False, dtype=torc
     place p row order[p] // k of the bfloat16 rows x [R, K] (its own row p without order), order and groups as
     expert_groups makes them. dtype and `swiglu` as for gemv_bf16. Places in no group are left as `out` had them (unset
     without it), as are groups whose expert or places lie outside the bank or the pairs."""
-    x, R, K, E, device = _bf16_operands(x, weight, n)
-    P = check_groups(groups, order, k, R, device)
-    out = product_out(device, P, n, swiglu, dtype, out)
-    launch("d3_bf16_grouped", out, x.data_ptr(), R, _p(order), k, P, groups.data_ptr(), groups.shape[0],
+    x, R, K, E, index = _bf16_operands(x, weight, n)
+    P = check_groups(groups, order, k, R, index)
+    out = product_out(x, P, n, swiglu, dtype, out)
+    launch("d3_bf16_grouped", index, x.data_ptr(), R, _p(order), k, P, groups.data_ptr(), groups.shape[0],
            weight.data_ptr(), E, n, K, swiglu, out.dtype is torch.bfloat16, out.data_ptr())
     return out
 

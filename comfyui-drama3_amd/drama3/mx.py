@@ -62,20 +62,20 @@ def _check_cols(cols):
 
 
 def _check_rows(r):
-    """(codes, scale, R, device) of MxRows, checked."""
+    """(codes, scale, R, device index) of MxRows, checked."""
     codes, scale, bits = r.codes, r.scale, r.bits
-    if bits != 4 and bits != 8:
+    if bits != 8 and bits != 4:
         raise ValueError(f"microscaled rows have 4 or 8 bits an element, not {bits}")
     if codes.dtype is not torch.uint8 or scale.dtype is not torch.uint8:
         raise TypeError("codes and scale must be uint8")
-    R, C, device = codes.size(0), -(-r.cols // STAGE) * STAGE, codes.device
+    R, C, index = codes.size(0), -(-r.cols // STAGE) * STAGE, codes.get_device()
     if codes.shape != (R, C * bits // 8) or scale.shape != (R, C // BLOCK):
         raise ValueError(f"codes [R, {C * bits // 8}] and scale [R, {C // BLOCK}] expected for {r.cols} columns")
     if not (codes.is_contiguous() and scale.is_contiguous()):
         raise ValueError("codes and scale must be contiguous")
-    if scale.device != device:
+    if scale.get_device() != index:
         raise ValueError("codes and scale must be on one device")
-    return codes, scale, R, device
+    return codes, scale, R, index
 
 
 def quantize(x, bits=4):
@@ -91,21 +91,21 @@ def quantize(x, bits=4):
     if x.stride(1) != 1 or x.stride(0) < cols or x.stride(0) * x.element_size() % 16 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     C = _stages(cols) * STAGE
-    codes = torch.empty((R, C * bits // 8), dtype=torch.uint8, device=x.device)
-    scale = torch.empty((R, C // BLOCK), dtype=torch.uint8, device=x.device)
-    kernels.launch("d3_mx_quantize", x, x.data_ptr(), _TYPES[x.dtype], x.stride(0), R, cols, bits, codes.data_ptr(),
-                   scale.data_ptr())
+    codes = x.new_empty((R, C * bits // 8), dtype=torch.uint8)
+    scale = x.new_empty((R, C // BLOCK), dtype=torch.uint8)
+    kernels.launch("d3_mx_quantize", x.get_device(), x.data_ptr(), _TYPES[x.dtype], x.stride(0), R, cols, bits,
+                   codes.data_ptr(), scale.data_ptr())
     return MxRows(codes, scale, bits, cols)
 
 
 def dequantize(rows, dtype=torch.float32):
     """The values of MxRows: [R, cols] float32 or bfloat16."""
-    codes, scale, R, device = _check_rows(rows)
+    codes, scale, R, index = _check_rows(rows)
     _check_cols(rows.cols)
     if dtype not in _TYPES:
         raise TypeError("float32 or bfloat16 expected")
-    out = torch.empty((R, rows.cols), dtype=dtype, device=device)
-    kernels.launch("d3_mx_dequantize", out, codes.data_ptr(), scale.data_ptr(), R, rows.cols, rows.bits, _TYPES[dtype],
+    out = codes.new_empty((R, rows.cols), dtype=dtype)
+    kernels.launch("d3_mx_dequantize", index, codes.data_ptr(), scale.data_ptr(), R, rows.cols, rows.bits, _TYPES[dtype],
                    out.data_ptr())
     return out
 
@@ -149,8 +149,8 @@ def quantize_bank(w):
     return bank(quantize(w.reshape(E * n, k), 4), E)
 
 
-def _check_bank(b, cols, device):
-    """(weight, scale) of a bank that rows of `cols` columns on `device` go through, checked."""
+def _check_bank(b, cols, index):
+    """(weight, scale) of a bank that rows of `cols` columns on device `index` go through, checked."""
     weight, scale = b.weight, b.scale
     if cols != b.cols:
         raise ValueError(f"rows of {cols} columns for a bank of {b.cols}")
@@ -161,7 +161,7 @@ def _check_bank(b, cols, device):
         raise ValueError("the bank's tensors do not have its shape (mx.bank lays them out)")
     if not (weight.is_contiguous() and scale.is_contiguous()):
         raise ValueError("a bank's tensors must be contiguous")
-    if weight.device != device or scale.device != device:
+    if weight.get_device() != index or scale.get_device() != index:
         raise ValueError("rows and bank must be on one device")
     return weight, scale
 
@@ -170,11 +170,11 @@ def gemv(rows, ids, bank, swiglu=False, dtype=torch.float32, out=None):
     """[P, N] of P pairs of rows and experts ids [P] (int64): pair p is row p // (P / R) of the R rows with expert
     ids[p] of `bank`; float32 or bfloat16. With `swiglu` (gate rows, then up rows) [P, N / 2] bfloat16 = SiLU(gate) * up.
     An id outside the bank gives zeros. For decode lines: every pair reads its expert by itself."""
-    codes, scale, R, device = _check_rows(rows)
-    weight, wscale = _check_bank(bank, rows.cols, device)
-    ids, P = kernels.pair_ids(ids, R, device)
-    out = kernels.product_out(device, P, bank.rows, swiglu, dtype, out)
-    kernels.launch("d3_mx_gemv", out, codes.data_ptr(), scale.data_ptr(), rows.bits, R, ids.data_ptr(), P,
+    codes, scale, R, index = _check_rows(rows)
+    weight, wscale = _check_bank(bank, rows.cols, index)
+    ids, P = kernels.pair_ids(ids, R, index)
+    out = kernels.product_out(codes, P, bank.rows, swiglu, dtype, out)
+    kernels.launch("d3_mx_gemv", index, codes.data_ptr(), scale.data_ptr(), rows.bits, R, ids.data_ptr(), P,
                    weight.data_ptr(), wscale.data_ptr(), bank.experts, bank.rows, bank.cols, swiglu,
                    out.dtype is torch.bfloat16, out.data_ptr())
     return out
@@ -185,11 +185,11 @@ def grouped(rows, groups, bank, order=None, k=1, swiglu=False, dtype=torch.float
     kernels.expert_groups makes them; place p multiplies row order[p] // k (its own row p without order) with its group's
     expert. dtype and `swiglu` as for gemv. Places in no group are left as `out` had them (unset without it), as are groups
     whose expert or places lie outside the bank or the pairs."""
-    codes, scale, R, device = _check_rows(rows)
-    weight, wscale = _check_bank(bank, rows.cols, device)
-    P = kernels.check_groups(groups, order, k, R, device)
-    out = kernels.product_out(device, P, bank.rows, swiglu, dtype, out)
-    kernels.launch("d3_mx_grouped", out, codes.data_ptr(), scale.data_ptr(), rows.bits, R, _lib.ptr(order), k, P,
+    codes, scale, R, index = _check_rows(rows)
+    weight, wscale = _check_bank(bank, rows.cols, index)
+    P = kernels.check_groups(groups, order, k, R, index)
+    out = kernels.product_out(codes, P, bank.rows, swiglu, dtype, out)
+    kernels.launch("d3_mx_grouped", index, codes.data_ptr(), scale.data_ptr(), rows.bits, R, _lib.ptr(order), k, P,
                    groups.data_ptr(), groups.size(0), weight.data_ptr(), wscale.data_ptr(), bank.experts, bank.rows,
                    bank.cols, swiglu, out.dtype is torch.bfloat16, out.data_ptr())
     return out
