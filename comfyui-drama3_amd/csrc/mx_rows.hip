@@ -112,11 +112,15 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* codes
 
 bool misaligned(const void* p) { return (uintptr_t)p & 15u; }
 
-// the common checks of rows [rows, cols] in `bits`; the launch's units of 8 columns, `per` to a row
+// a row's units of 8 columns, those of its last stage whole (in 64 bits: of any int32)
+int64_t row_units(int32_t cols) { return ((int64_t)cols + MX_STAGE - 1) / MX_STAGE * (MX_STAGE / 8); }
+
+// the common checks of rows [rows, cols] in `bits`, `per` units to a row
 int check_rows(const char* what, int32_t rows, int32_t cols, int32_t bits, int32_t type, int64_t per) {
   if (bits != 4 && bits != 8) return fail(std::string(what) + ": bits must be 4 or 8");
   if (type != 0 && type != 1) return fail(std::string(what) + ": type must be 0 (float32) or 1 (bfloat16)");
   if (rows < 0 || cols < 1 || cols % MX_BLOCK) return fail(std::string(what) + ": cols must be a positive multiple of 32");
+  if (8 * per > INT32_MAX) return fail(std::string(what) + ": cols must be below 2^31 - 255");
   if ((int64_t)rows * per > INT32_MAX) return fail(std::string(what) + ": more than 2^31 units of 8 columns");
   return 0;
 }
@@ -128,7 +132,7 @@ using namespace d3;
 
 extern "C" int d3_mx_quantize(const void* x, int32_t type, int64_t stride, int32_t rows, int32_t cols, int32_t bits,
                               void* codes, void* scale, void* stream) {
-  const int per = mx_stages(cols) * MX_STAGE / 8;
+  const int64_t per = row_units(cols);
   if (const int rc = check_rows("d3_mx_quantize", rows, cols, bits, type, per)) return rc;
   const int64_t bytes = stride * (type ? 2 : 4);
   if (stride < 0 || bytes % 16) return fail("d3_mx_quantize: the row stride must be a multiple of 16 bytes");
@@ -139,7 +143,7 @@ extern "C" int d3_mx_quantize(const void* x, int32_t type, int64_t stride, int32
   const dim3 grid((units + 255u) / 256u), block(256);
   const hipStream_t s = (hipStream_t)stream;
 #define D3_QUANTIZE(B, T)                                                                                           \
-  hipLaunchKernelGGL((mx_quantize_kernel<B, T>), grid, block, 0, s, (const uint8_t*)x, bytes, units, cols, per,      \
+  hipLaunchKernelGGL((mx_quantize_kernel<B, T>), grid, block, 0, s, (const uint8_t*)x, bytes, units, cols, (int)per, \
                      (uint8_t*)codes, (uint8_t*)scale)
   if (bits == 4 && type) D3_QUANTIZE(4, true);
   else if (bits == 4) D3_QUANTIZE(4, false);
@@ -152,7 +156,7 @@ extern "C" int d3_mx_quantize(const void* x, int32_t type, int64_t stride, int32
 
 extern "C" int d3_mx_dequantize(const void* codes, const void* scale, int32_t rows, int32_t cols, int32_t bits,
                                 int32_t type, void* out, void* stream) {
-  const int per = mx_stages(cols) * MX_STAGE / 8;
+  const int64_t per = row_units(cols);
   if (const int rc = check_rows("d3_mx_dequantize", rows, cols, bits, type, per)) return rc;
   if (rows == 0) return 0;
   if (!codes || !scale || !out) return fail("d3_mx_dequantize: null pointer");
@@ -162,7 +166,7 @@ extern "C" int d3_mx_dequantize(const void* codes, const void* scale, int32_t ro
   const hipStream_t s = (hipStream_t)stream;
 #define D3_DEQUANTIZE(B, T)                                                                                         \
   hipLaunchKernelGGL((mx_dequantize_kernel<B, T>), grid, block, 0, s, (const uint8_t*)codes, (const uint8_t*)scale,  \
-                     units, cols, per, (uint8_t*)out)
+                     units, cols, (int)per, (uint8_t*)out)
   if (bits == 4 && type) D3_DEQUANTIZE(4, true);
   else if (bits == 4) D3_DEQUANTIZE(4, false);
   else if (type) D3_DEQUANTIZE(8, true);

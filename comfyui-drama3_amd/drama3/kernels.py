@@ -555,6 +555,7 @@ def fp8_linear(x, weight, scale):
 
 
 # ------------------------------------------------------------- products of unquantized and of microscaled (mx.py) banks
+_INT_MAX = 2 ** 31 - 1  # of the C entries' sizes, which ctypes would cut to their low bits
 _raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
@@ -595,8 +596,8 @@ def pair_ids(ids, rows, index):
     if ids.dtype is not torch.int64 or ids.dim() != 1 or ids.get_device() != index:
         raise ValueError("ids [P] int64 on the rows' device expected")
     P = ids.numel()
-    if P % rows if rows else P:
-        raise ValueError(f"{P} ids for {rows} rows: a multiple of the rows is expected")
+    if (P % rows if rows else P) or P > _INT_MAX:
+        raise ValueError(f"{P} ids for {rows} rows: a multiple of the rows, below 2^31, is expected")
     return ids.contiguous(), P
 
 
@@ -605,14 +606,16 @@ def check_groups(groups, order, k, rows, index):
     if groups.dtype is not torch.int32 or groups.dim() != 2 or groups.size(1) != 5 or not groups.is_contiguous() \
             or groups.get_device() != index:
         raise ValueError("groups [g, 5] int32, contiguous, on the rows' device, expected")
-    if k < 1:
-        raise ValueError(f"k is positive, not {k}")
+    if not 1 <= k <= _INT_MAX or groups.size(0) > _INT_MAX:
+        raise ValueError(f"k is positive, not {k}, and below 2^31, as are the groups")
     if order is None:
         if k != 1:
             raise ValueError("k goes with order")
         return rows
     if order.dtype is not torch.int64 or order.dim() != 1 or not order.is_contiguous() or order.get_device() != index:
         raise ValueError("order [P] int64, contiguous, on the rows' device, expected")
+    if order.size(0) > _INT_MAX:
+        raise ValueError("fewer than 2^31 pairs expected")
     return order.size(0)
 
 
@@ -621,8 +624,8 @@ def _bf16_operands(x, weight, n):
     if x.dim() != 2 or x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16:
         raise TypeError("x [R, K] and weight [E * n, K] bfloat16 expected")
     (R, K), index = x.shape, x.get_device()
-    if K < 64 or K % 64:
-        raise ValueError(f"K is a positive multiple of 64, not {K}")
+    if K < 64 or K % 64 or K > _INT_MAX:
+        raise ValueError(f"K is a positive multiple of 64 below 2^31, not {K}")
     if n < 1 or weight.dim() != 2 or weight.size(1) != K or weight.size(0) % n or not weight.is_contiguous() \
             or weight.get_device() != index:
         raise ValueError(f"weight [E * {n}, {K}], contiguous, on the rows' device, expected")
@@ -678,6 +681,8 @@ def direct_layer(x, topk_idx, topk_weight, num_experts, gemv, grouped):
         return torch.zeros_like(x)
     if x.get_device() < 0:
         raise ValueError(f"the kernels run on a GPU, not on {x.device}")
+    if topk_idx.device != x.device or topk_weight.device != x.device:
+        raise ValueError(f"topk_idx and topk_weight on {x.device} expected")
     with torch.cuda.device(x.device):
         if T <= LINE_ROWS:
             ids = topk_idx.reshape(-1).to(torch.int64)

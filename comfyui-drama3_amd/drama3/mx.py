@@ -21,6 +21,7 @@ import torch
 from . import _lib, kernels
 
 BLOCK, STAGE = 32, 256
+MAX_COLS = 2 ** 31 - 2 * STAGE  # (whole stages of them in 32 bits)
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
@@ -57,8 +58,8 @@ class MxBank:
 
 
 def _check_cols(cols):
-    if cols < BLOCK or cols % BLOCK:
-        raise ValueError(f"microscaled rows have a positive multiple of {BLOCK} columns, not {cols}")
+    if cols < BLOCK or cols % BLOCK or cols > MAX_COLS:
+        raise ValueError(f"microscaled rows have a positive multiple of {BLOCK} columns, up to {MAX_COLS}, not {cols}")
 
 
 def _check_rows(r):
@@ -66,6 +67,8 @@ def _check_rows(r):
     codes, scale, bits = r.codes, r.scale, r.bits
     if bits != 8 and bits != 4:
         raise ValueError(f"microscaled rows have 4 or 8 bits an element, not {bits}")
+    if r.cols > MAX_COLS:
+        raise ValueError(f"microscaled rows have up to {MAX_COLS} columns, not {r.cols}")
     if codes.dtype is not torch.uint8 or scale.dtype is not torch.uint8:
         raise TypeError("codes and scale must be uint8")
     R, C, index = codes.size(0), -(-r.cols // STAGE) * STAGE, codes.get_device()

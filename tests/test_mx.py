@@ -139,3 +139,43 @@ def test_c_entries_refuse():
     assert lib.d3_mx_quantize(None, 0, 64, 0, 64, 4, None, None, None) == 0
     assert lib.d3_mx_grouped(None, None, 4, 0, None, 1, 0, None, 0, None, None, 0, 16, 32, 0, 0, None, None) == 0
     assert lib.d3_bf16_gemv(None, 0, None, 0, None, 0, 16, 64, 0, 0, None, None) == 0
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The C entries take 32-bit sizes, which ctypes would cut to their low bits."""
+    far = 2 ** 32
+    with pytest.raises(ValueError):
+        mx.quantize(torch.zeros(1, device="meta").expand(1, far + 32))
+    with pytest.raises(ValueError):
+        mx.gemv(mx.MxRows(torch.empty(1, far // 2 + 128, dtype=torch.uint8, device="meta"),
+                          torch.empty(1, far // 32 + 8, dtype=torch.uint8, device="meta"), 4, far + 256),
+                torch.zeros(1, dtype=torch.int64), _bank())
+    with pytest.raises(ValueError):
+        kernels.pair_ids(torch.empty(far + 1, dtype=torch.int64, device="meta"), 1, -1)
+    order = torch.empty(4, dtype=torch.int64)
+    assert kernels.check_groups(_groups((0, 0, 4)), order, 2, 2, -1) == 4
+    for groups, order, k in ((_groups((0, 0, 4)), order, far + 1),
+                             (_groups((0, 0, 4)), torch.empty(far + 1, dtype=torch.int64, device="meta"), 2),
+                             (torch.empty(far + 1, 5, dtype=torch.int32, device="meta"), order, 2)):
+        with pytest.raises(ValueError):
+            kernels.check_groups(groups, order, k, 2, -1)
+    lib, p = _lib.lib(), ctypes.c_void_p(4096)
+    for cols in (2 ** 31 - 32, 2 ** 31 - 224):
+        assert lib.d3_mx_quantize(p, 0, 64, 1, cols, 4, p, p, None) == -1
+        assert lib.d3_mx_dequantize(p, p, 1, cols, 4, 0, p, None) == -1
+
+
+def test_layer_refuses_routes_elsewhere():
+    """Routes or weights that are not on the rows' device would be read through a pointer of another memory."""
+    x, ids, weights = torch.zeros(2, 64), torch.zeros(2, 1, dtype=torch.int64), torch.ones(2, 1)
+
+    class OnGpu(torch.Tensor):  # rows that say they are on a GPU
+        def get_device(self):
+            return 0
+
+        @property
+        def device(self):
+            return torch.device("cuda:0")
+
+    with pytest.raises(ValueError, match="topk_idx and topk_weight"):
+        kernels.direct_layer(x.as_subclass(OnGpu), ids, weights, 2, None, None)
