@@ -3,6 +3,11 @@
 // on their way. A wave streams its tiles of 16 weight rows from memory straight into the MFMA operands, DEPTH stages
 // ahead; nothing but the accumulators is shared along K, so there is no barrier in the loop. The pass's rows lie whole in
 // LDS (SEG stages at a time), read by all waves.
+//
+// Short prompts run near what memory gives: 77 rows of top-8 of 256 experts (FFN 512) on e4m3 rows, first bank, 48 us (260 MB of
+// weights at 5.4 TB/s); of 128 experts, bf16, second bank, 75 us (400 MB at 5.3). A line's experts are few bytes, and
+// its time a launch and one round trip of loads: 8 pairs of the first bank 4.5 us (e2m1 weights, 13 MB) and 11 us (bf16, 50 MB
+// at 4.6 TB/s).
 #pragma once
 #include "ragged.hpp"
 

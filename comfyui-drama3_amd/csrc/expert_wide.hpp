@@ -6,6 +6,13 @@
 // item begin during the last stages of this. The rows, which other columns' workgroups read too, are copied a stage ahead;
 // the weights come from HBM and are copied by halves of a stage (a step), three (bf16: four) ahead, so that there are always
 // some on their way: with whole stages, one ahead, a stage of bf16 took 4200 clocks, of which the products take 2200.
+//
+// Bound by what comes from HBM and the memory-side cache (each XCD reads the rows of its experts for itself), the first
+// products of each workgroup and the epilogues beside it. 4096 rows, top-8 of 128 experts, first bank (FFN 768) with SwiGLU:
+// bf16 232 us, 0.96 GB read past the L2s and 50 MB written at 4.3 TB/s (223 us with the products left out; the matrix units
+// work 47% of the time); e2m1 rows on e2m1 weights 83 us, 0.27 GB read and 50 MB written at 3.9 TB/s (34%). An e4m3 row's
+// float32 result takes two products a step (ragged.hpp), and passes of 160 rows read the weights twice as often: 150 us
+// (second bank).
 #pragma once
 #include "expert_stream.hpp"
 
@@ -127,7 +134,7 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
   constexpr int COPIES = ROWS / PER / 8;                // of the rows, per wave
   constexpr int SCOPIES = F::SCALED ? (ROWS + 255) / 256 : 0;  // of the rows' scale words, per wave
   // LDS: RING steps' weights, two stages' rows, and of microscaled ones the rows' scales of two stages and the weights' scale
-  // words of two pairs of stages (tile, lane); all of a CU's 160 KB for bf16 and e2m1
+  // words of two pairs of stages (tile, lane): all of a CU's 160 KB (e4m3: 156)
   constexpr int RING = F::SCALED ? 4 : 5, XSCALE = 2048 * SCOPIES, WSCALE = F::SCALED ? 16 * 256 : 0;
   constexpr int AT_ROWS = RING * STEP, AT_XSCALE = AT_ROWS + 2 * STAGE, AT_WSCALE = AT_XSCALE + 2 * XSCALE;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[AT_WSCALE + 2 * WSCALE];
@@ -295,7 +302,8 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
       read_x(0);
       if constexpr (F::SCALED) {
 #pragma unroll
-        for (int n = 0; n < 4; n++) sw[n] = *(const uint32_t*)(smem + AT_WSCALE + pair * WSCALE + 256 * (4 * wn + n) + 4 * lane) >> (16 * (st & 1));
+        for (int n = 0; n < 4; n++)
+          sw[n] = *(const uint32_t*)(smem + AT_WSCALE + pair * WSCALE + 256 * (4 * wn + n) + 4 * lane) >> (16 * (st & 1));
       }
       read_x(1);
       // The next stage's rows, of this item or the next, go out between the products: those that this item's rows need

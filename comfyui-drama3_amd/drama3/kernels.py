@@ -650,7 +650,7 @@ def grouped_bf16(x, groups, weight, n, order=None, k=1, swiglu=False, dtype=torc
     """grouped_int8's products on a bank of bfloat16 weights [E * n, K]: [P, n] for the places of `groups` [g, 5] int32,
     place p row order[p] // k of the bfloat16 rows x [R, K] (its own row p without order), order and groups as
     expert_groups makes them. dtype and `swiglu` as for gemv_bf16. Places in no group are left as `out` had them (unset
-    without it), as are groups whose expert or places lie outside the bank or the pairs."""
+    without it), as are groups whose expert or places lie outside the bank or the pairs. Groups must not share places."""
     x, R, K, E, index = _bf16_operands(x, weight, n)
     P = check_groups(groups, order, k, R, index)
     out = product_out(x, P, n, swiglu, dtype, out)

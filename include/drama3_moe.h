@@ -424,7 +424,7 @@ int d3_mx_dequantize(const void* codes, const void* scale, int32_t rows, int32_t
  * gemv: pair p multiplies row p / (pairs / rows) with expert ids[p] (int64); an id outside [0, E) gives zeros.
  * grouped: groups [n_groups, 5] int32 = (expert, ., ., first, rows) as d3_expert_groups makes them; place p of a group
  * multiplies row order[p] / k (row p when order is NULL). Places in no group, and groups whose expert or rows lie
- * outside the bank or the pairs, are left alone. */
+ * outside the bank or the pairs, are left alone; groups must not share places. */
 int d3_mx_gemv(const void* codes, const void* scale, int32_t bits, int32_t rows, const int64_t* ids, int32_t pairs,
                const void* w, const void* w_scale, int32_t E, int32_t N, int32_t K, int32_t swiglu, int32_t out_bf16,
                void* out, void* stream);
