@@ -4,9 +4,9 @@
 // ahead; nothing but the accumulators is shared along K, so there is no barrier in the loop. The pass's rows lie whole in
 // LDS (SEG stages at a time), read by all waves.
 //
-// Short prompts run near what memory gives: 77 rows of top-8 of 256 experts (FFN 512) on e4m3 rows, first bank, 48 us (260 MB of
-// weights at 5.4 TB/s); of 128 experts, bf16, second bank, 75 us (400 MB at 5.3). A line's experts are few bytes, and
-// its time a launch and one round trip of loads: 8 pairs of the first bank 4.5 us (e2m1 weights, 13 MB) and 11 us (bf16, 50 MB
+// Short prompts run near what memory gives: 77 rows of top-8 of 256 experts (FFN 512) on e4m3 rows, first bank, 44 us (260 MB of
+// weights at 5.9 TB/s); of 128 experts, bf16, second bank, 75 us (400 MB at 5.3). A line's experts are few bytes, and
+// its time a launch and one round trip of loads: 8 pairs of the first bank 4.4 us (e2m1 weights, 13 MB) and 11 us (bf16, 50 MB
 // at 4.6 TB/s).
 #pragma once
 #include "ragged.hpp"
@@ -22,9 +22,17 @@ template <class F, int SEG> constexpr int st_pitch() { return (SEG * F::ROW + 25
 template <class F, int SEG, int MT> constexpr int st_waves() { return 16 * MT * st_pitch<F, SEG>() > 80000 ? 1 : 2; }
 D3_INLINE int st_piece(int r, int j) { return 16 * (j ^ (r & 15)); }
 
+// 16 bytes of weights; ONCE: nontemporal, for weights that no other workgroup reads. (Only where a load takes whole lines, as
+// of microscaled tiles: a load of bf16 rows takes half of each, and with the hint both halves come from HBM: 10.6 -> 14.8 us.)
+template <bool ONCE>
+D3_INLINE i32x4 weights_16(const uint8_t* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load((const i32x4*)p);
+  else return *(const i32x4*)p;
+}
+
 // NT tiles of weight rows a wave; SWIGLU with NT 2: a gate tile and its up tile, with NT 1 (gemv): those of two
 // neighbouring waves
-template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH, int SEG>
+template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH, int SEG, bool ONCE>
 __global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
     expert_stream_kernel(ExpertProduct a, int columns, int per) {
   constexpr int ROWS = GEMV ? 1 : 16 * MT, PITCH = st_pitch<F, SEG>(), SPITCH = 8 * SEG + 4;
@@ -92,7 +100,7 @@ __global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int s = 0; s < 2; s++)
-            buf[d][n][s] = *(const i32x4*)(wp[n] + (size_t)(s0 + st) * F::A_STAGE + s * F::A_STEP);
+            buf[d][n][s] = weights_16<ONCE>(wp[n] + (size_t)(s0 + st) * F::A_STAGE + s * F::A_STEP);
       };
 #pragma unroll
       for (int d = 0; d < DEPTH; d++) load(d, min(d, n_st - 1));
@@ -154,7 +162,7 @@ __global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
         uint32_t sw[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) sw[n] = F::SCALED ? sa[n][st / 2] : 0u;
-        if (d & 1) products.template operator()<1>(d, st, sw);
+        if (st & 1) products.template operator()<1>(d, st, sw);
         else products.template operator()<0>(d, st, sw);
       };
       if constexpr (F::SCALED) {  // at most SEG / DEPTH turns, unrolled: the scale words stay in registers
@@ -225,19 +233,38 @@ int st_columns(int N) {
   return (N / 16 + per - 1) / per;
 }
 
-template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH, int SEG>
+template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH, int SEG, bool ONCE>
 void launch_stream_of(const ExpertProduct& a, int passes, int per, hipStream_t s) {
   const int columns = st_columns<GEMV, SWIGLU, NT>(a.N);
   per = per < columns ? per : columns;
-  hipLaunchKernelGGL((expert_stream_kernel<F, GEMV, SWIGLU, OUT_BF16, NT, MT, DEPTH, SEG>),
+  hipLaunchKernelGGL((expert_stream_kernel<F, GEMV, SWIGLU, OUT_BF16, NT, MT, DEPTH, SEG, ONCE>),
                      dim3((unsigned)((columns + per - 1) / per * passes)), dim3(ST_THREADS), 0, s, a, columns, per);
 }
 
+template <class F, bool GEMV, int MT, int DEPTH, int SEG, bool ONCE>
+void launch_stream_out(const ExpertProduct& a, bool swiglu, bool out_bf16, int passes, int per, hipStream_t s) {
+  constexpr int NT = GEMV ? 1 : 2;
+  if (swiglu) launch_stream_of<F, GEMV, true, true, NT, MT, DEPTH, SEG, ONCE>(a, passes, per, s);
+  else if (out_bf16) launch_stream_of<F, GEMV, false, true, NT, MT, DEPTH, SEG, ONCE>(a, passes, per, s);
+  else launch_stream_of<F, GEMV, false, false, NT, MT, DEPTH, SEG, ONCE>(a, passes, per, s);
+}
+
+// DEPTH for microscaled rows of fewer than 8 stages: no more loads than there are stages
 template <class F>
 void launch_gemv(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
-  if (swiglu) launch_stream_of<F, true, true, true, 1, 1, 8, F::SEG>(a, a.pairs, 1, s);
-  else if (out_bf16) launch_stream_of<F, true, false, true, 1, 1, 8, F::SEG>(a, a.pairs, 1, s);
-  else launch_stream_of<F, true, false, false, 1, 1, 8, F::SEG>(a, a.pairs, 1, s);
+  // Few pairs, of which hardly two meet in an expert, read its weights once. Of 128 experts (e4m3 rows), us without / with: first
+  // bank 8 pairs 5.0 / 4.4, 16 7.1 / 6.8, 32 10.1 / 10.3, 128 30 / 34; second bank 16 pairs 5.5 / 5.0, 32 7.8 / 8.3; 40 of 256
+  // experts, second bank: 6.1 / 5.0.
+  if constexpr (F::SCALED) {
+    if ((int64_t)6 * a.pairs <= a.E) {
+      if (a.stages >= 8) launch_stream_out<F, true, 1, 8, F::SEG, true>(a, swiglu, out_bf16, a.pairs, 1, s);
+      else if (a.stages >= 4) launch_stream_out<F, true, 1, 4, F::SEG, true>(a, swiglu, out_bf16, a.pairs, 1, s);
+      else if (a.stages == 3) launch_stream_out<F, true, 1, 3, F::SEG, true>(a, swiglu, out_bf16, a.pairs, 1, s);
+      else launch_stream_out<F, true, 1, 2, F::SEG, true>(a, swiglu, out_bf16, a.pairs, 1, s);
+      return;
+    }
+  }
+  launch_stream_out<F, true, 1, 8, F::SEG, false>(a, swiglu, out_bf16, a.pairs, 1, s);
 }
 
 template <class F, int MT, int SEG>
@@ -247,9 +274,14 @@ void launch_stream(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream
   // columns in turn. Second bank of 128 experts (2048 x 768, e4m3), 256 rows: 32 us with two, 38 with one; first bank
   // (8 stages): 51 with one, 53 with two.
   const int per = F::SCALED && a.stages < 6 ? 6 / a.stages : 1;
-  if (swiglu) launch_stream_of<F, false, true, true, 2, MT, 4, SEG>(a, passes, per, s);
-  else if (out_bf16) launch_stream_of<F, false, false, true, 2, MT, 4, SEG>(a, passes, per, s);
-  else launch_stream_of<F, false, false, false, 2, MT, 4, SEG>(a, passes, per, s);
+  // Up to 16 rows an expert its weights go by in one pass, mostly: nontemporal where a column is long (first bank, 77 rows
+  // of 256 experts 48.6 -> 44.4 us, 100 of 128 40.7 -> 36.1; second bank, 256 rows, Zipf: 32.0 -> 33.5, so not there).
+  constexpr bool ONCE = F::SCALED && MT == 1 && SEG == F::SEG;
+  if constexpr (F::SCALED && SEG < F::SEG) {  // (second bank, 256 rows of 128 experts: 31.3 -> 29.2 us)
+    if (a.stages == 3) return launch_stream_out<F, false, MT, 3, SEG, ONCE>(a, swiglu, out_bf16, passes, per, s);
+    if (a.stages < 3) return launch_stream_out<F, false, MT, 2, SEG, ONCE>(a, swiglu, out_bf16, passes, per, s);
+  }
+  launch_stream_out<F, false, MT, 4, SEG, ONCE>(a, swiglu, out_bf16, passes, per, s);
 }
 
 }  // namespace d3

@@ -390,3 +390,25 @@ def test_banks_beyond_32_bit_offsets(fmt):
     small.w, small.E = w, E
     assert torch.equal(small.gemv(ids), want)
     assert torch.equal(small.grouped(groups), want_grouped)
+
+
+@pytest.mark.parametrize("K", [64, 256, 512, 768, 1024, 1280, 2048, 2368])
+@pytest.mark.parametrize("fmt", ["mx4", "mx8"])
+def test_few_pairs_of_many_experts(fmt, K):
+    """Decode lines of fewer pairs than a sixth of the experts, at every number of stages that their loads go by, the same
+    expert twice, ids outside; bit for bit the results of the same pairs among more. And groups of few rows."""
+    case = Case(fmt, 48, 96, K, 2, spread=1.0)
+    ids = torch.tensor([47, 3, 3, 0, 20, 48, 47, -1], device=DEV)
+    row, ok = torch.arange(8, device=DEV) // 4, (ids >= 0) & (ids < 48)
+    many = ids.view(2, 4).repeat_interleave(4, dim=1).flatten()  # four times each
+    for how in ({}, {"dtype": torch.bfloat16}, {"swiglu": True}):
+        got = case.gemv(ids, **how)
+        assert not got[~ok].any()
+        case.check(got[ok], row[ok], ids[ok], "swiglu" in how)
+        assert torch.equal(case.gemv(many, **how)[::4], got)
+    one = Case(fmt, 48, 96, K, 1)
+    assert torch.equal(one.gemv(ids), torch.cat([one.gemv(ids[i:i + 1]) for i in range(8)]))
+    rows = Case(fmt, 10, 96, K, sum(FEW))
+    ids, order, _, groups = _pairs(10, FEW)
+    for how in ({}, {"swiglu": True}):
+        rows.check(rows.grouped(groups, order=order, **how), order, ids[order], "swiglu" in how)
