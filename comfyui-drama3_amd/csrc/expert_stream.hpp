@@ -5,7 +5,7 @@
 // LDS (SEG stages at a time), read by all waves.
 //
 // Short prompts run near what memory gives: 77 rows of top-8 of 256 experts (FFN 512) on e4m3 rows, first bank, 44 us (260 MB of
-// weights at 5.9 TB/s); of 128 experts, bf16, second bank, 75 us (400 MB at 5.3). A line's experts are few bytes, and
+// weights at 5.9 TB/s); of 128 experts, bf16, second bank, 68 us (400 MB at 5.9). A line's experts are few bytes, and
 // its time a launch and one round trip of loads: 8 pairs of the first bank 4.4 us (e2m1 weights, 13 MB) and 11 us (bf16, 50 MB
 // at 4.6 TB/s).
 #pragma once
@@ -22,12 +22,37 @@ template <class F, int SEG> constexpr int st_pitch() { return (SEG * F::ROW + 25
 template <class F, int SEG, int MT> constexpr int st_waves() { return 16 * MT * st_pitch<F, SEG>() > 80000 ? 1 : 2; }
 D3_INLINE int st_piece(int r, int j) { return 16 * (j ^ (r & 15)); }
 
-// 16 bytes of weights; ONCE: nontemporal, for weights that no other workgroup reads. (Only where a load takes whole lines, as
-// of microscaled tiles: a load of bf16 rows takes half of each, and with the hint both halves come from HBM: 10.6 -> 14.8 us.)
+// 16 bytes of weights; ONCE: nontemporal, for weights that hardly another workgroup reads. (Only where a load takes whole lines:
+// with the hint, a line that two loads take halves of comes from HBM twice, 10.6 -> 14.8 us for a bf16 decode line.)
 template <bool ONCE>
 D3_INLINE i32x4 weights_16(const uint8_t* p) {
   if constexpr (ONCE) return __builtin_nontemporal_load((const i32x4*)p);
   else return *(const i32x4*)p;
+}
+
+// bf16 rows are loaded by whole lines in the grouped products: the first load of a stage takes rows 0 - 7 of the tile, lane (q, c)
+// piece 4 (c >> 3) + q of row c & 7, the second rows 8 - 15, piece 4 (1 - (c >> 3)) + q of row 8 + (c & 7). (A decode line is
+// latency, and takes the operands as they are: 10.8 us, 12.1 by lines.)
+template <class F, bool LINES>
+D3_INLINE size_t st_base(size_t tile, int stages, int lane) {
+  if constexpr (!LINES) return F::a_base(tile, stages, lane);
+  else return (tile * 16 + (lane & 7)) * ((size_t)stages * F::A_STAGE) + 64 * ((lane >> 3) & 1) + 16 * (lane >> 4);
+}
+// from a stage's first load to its second
+template <class F, bool LINES>
+D3_INLINE int64_t st_second(int stages, int lane) {
+  if constexpr (!LINES) return F::A_STEP;
+  else return (int64_t)8 * stages * F::A_STAGE + (lane & 8 ? -64 : 64);
+}
+// what the lines' loads brought, as the operands of the stage's steps: of 16 lanes the first 8 of the first load and the last
+// 8 of the second are step 0's, in their places, the others step 1's, 8 lanes on
+D3_INLINE void steps_of_lines(i32x4& first, i32x4& second) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int a = first[i], b = second[i], turned = __builtin_amdgcn_update_dpp(0, a, 0x128, 0xF, 0x3, false);  // row_ror 8
+    first[i] = __builtin_amdgcn_update_dpp(a, b, 0xE4, 0xF, 0xC, false);
+    second[i] = __builtin_amdgcn_update_dpp(turned, b, 0x128, 0xF, 0xC, false);
+  }
 }
 
 // NT tiles of weight rows a wave; SWIGLU with NT 2: a gate tile and its up tile, with NT 1 (gemv): those of two
@@ -35,6 +60,7 @@ D3_INLINE i32x4 weights_16(const uint8_t* p) {
 template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH, int SEG, bool ONCE>
 __global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
     expert_stream_kernel(ExpertProduct a, int columns, int per) {
+  constexpr bool LINES = !GEMV && !F::SCALED;
   constexpr int ROWS = GEMV ? 1 : 16 * MT, PITCH = st_pitch<F, SEG>(), SPITCH = 8 * SEG + 4;
   __shared__ __attribute__((aligned(1024))) uint8_t xs[ROWS * PITCH];
   __shared__ __attribute__((aligned(16))) uint8_t ss[F::SCALED ? ROWS * SPITCH : 16];
@@ -87,10 +113,11 @@ __global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       const size_t t = (size_t)pass.expert * tiles + tile[n];
-      wp[n] = a.w + F::a_base(t, S, lane);
+      wp[n] = a.w + st_base<F, LINES>(t, S, lane);
       sp[n] = F::SCALED ? a.w_scale + (t * 64 + lane) * mx_lane_scales(S) : nullptr;
     }
     const size_t row_bytes = (size_t)S * F::ROW;
+    const int64_t second = st_second<F, LINES>(S, lane);
     for (int s0 = 0; s0 < S; s0 += SEG) {
       const int n_st = min(SEG, S - s0);
       i32x4 buf[DEPTH][NT][2];
@@ -100,7 +127,7 @@ __global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int s = 0; s < 2; s++)
-            buf[d][n][s] = weights_16<ONCE>(wp[n] + (size_t)(s0 + st) * F::A_STAGE + s * F::A_STEP);
+            buf[d][n][s] = weights_16<ONCE>(wp[n] + (size_t)(s0 + st) * F::A_STAGE + (s ? second : 0));
       };
 #pragma unroll
       for (int d = 0; d < DEPTH; d++) load(d, min(d, n_st - 1));
@@ -151,12 +178,15 @@ __global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
             }
         }
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT; n++) {
+          i32x4 w[2] = {buf[d][n][0], buf[d][n][1]};
+          if constexpr (LINES) steps_of_lines(w[0], w[1]);
 #pragma unroll
           for (int m = 0; m < MT; m++) {
-            acc[n][m] = step_product<F, !OUT_BF16, 2 * ODD, 0>(buf[d][n][0], b[m][0], acc[n][m], sw[n], sb[m]);
-            acc[n][m] = step_product<F, !OUT_BF16, 2 * ODD + 1, 1>(buf[d][n][1], b[m][1], acc[n][m], sw[n], sb[m]);
+            acc[n][m] = step_product<F, !OUT_BF16, 2 * ODD, 0>(w[0], b[m][0], acc[n][m], sw[n], sb[m]);
+            acc[n][m] = step_product<F, !OUT_BF16, 2 * ODD + 1, 1>(w[1], b[m][1], acc[n][m], sw[n], sb[m]);
           }
+        }
       };
       auto run = [&](int d, int st) __attribute__((always_inline)) {
         uint32_t sw[NT];
@@ -274,9 +304,11 @@ void launch_stream(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream
   // columns in turn. Second bank of 128 experts (2048 x 768, e4m3), 256 rows: 32 us with two, 38 with one; first bank
   // (8 stages): 51 with one, 53 with two.
   const int per = F::SCALED && a.stages < 6 ? 6 / a.stages : 1;
-  // Up to 16 rows an expert its weights go by in one pass, mostly: nontemporal where a column is long (first bank, 77 rows
-  // of 256 experts 48.6 -> 44.4 us, 100 of 128 40.7 -> 36.1; second bank, 256 rows, Zipf: 32.0 -> 33.5, so not there).
-  constexpr bool ONCE = F::SCALED && MT == 1 && SEG == F::SEG;
+  // Up to 16 rows an expert its weights go by in one pass, mostly: nontemporal, e2m1 where a column is long (first bank, 77
+  // rows of 256 experts 48.6 -> 44.4 us, 100 of 128 40.7 -> 36.1; second bank, 256 rows, Zipf: 32.0 -> 33.5, so not there), bf16
+  // (16 rows of 128 experts 103 -> 91 and 51 -> 43 us, 77 rows on the second bank 79 -> 68), and up to 32 rows bf16's long
+  // columns (256 rows of 128 experts 184 -> 163 us, Zipf 186 either way; second bank, 700 rows of 256 experts 134 -> 141).
+  constexpr bool LONG = SEG == F::SEG, ONCE = F::SCALED ? MT == 1 && LONG : MT == 1 || LONG;
   if constexpr (F::SCALED && SEG < F::SEG) {  // (second bank, 256 rows of 128 experts: 31.3 -> 29.2 us)
     if (a.stages == 3) return launch_stream_out<F, false, MT, 3, SEG, ONCE>(a, swiglu, out_bf16, passes, per, s);
     if (a.stages < 3) return launch_stream_out<F, false, MT, 2, SEG, ONCE>(a, swiglu, out_bf16, passes, per, s);

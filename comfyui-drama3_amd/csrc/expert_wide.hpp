@@ -441,7 +441,7 @@ bool wide_fits(const ExpertProduct& a) {
 // us with 16 / 32 / wide: first bank, e4m3 rows, 256 rows (16 to an expert) 51 / 46 / 52, 400 rows 67 / 50 / 53, 700 rows
 // 73 wide and 74 streamed (256 experts, Zipf); second bank 16 to an expert 31 / 36 / 43 (few stages: a 32-row pass has
 // less to stream than it takes to set up), 25 to an expert 40 / 41 / 42, 44 to an expert 60 streamed, 47 wide; bf16 first
-// bank 16 to an expert 182 / 187 / 190, 25: 238 / 185 / 192; second bank 16: 100 / 91 / 102.
+// bank 16 to an expert 182 / 163 / 190, 25: 238 / 174 / 192; second bank 16: 100 / 89 / 102.
 template <class F>
 void launch_grouped(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
   if (wide_fits<F>(a)) return launch_wide<F>(a, swiglu, out_bf16, s);
