@@ -35,6 +35,24 @@ D3_INLINE void dma4(uint32_t lds, const void* base, uint32_t off) {
                : "memory");
 }
 
+// dma16; ONCE: nontemporal, for weights that no other workgroup reads (whole lines: what two copies take halves of would come
+// from HBM twice)
+template <bool ONCE>
+D3_INLINE void dma16_weights(uint32_t lds, const void* base, uint32_t off) {
+  if constexpr (!ONCE) {
+    dma16(lds, base, off);
+  } else {
+    const uint64_t at = (uint64_t)base;
+    const uint64_t sbase = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at) |
+                           (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32;
+    uint64_t from;
+    asm volatile("s_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0 nt"
+                 : "=&s"(from)
+                 : "{m0}"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(sbase)
+                 : "memory");
+  }
+}
+
 // all but the N last of this wave's loads have come
 template <int N>
 D3_INLINE void wait_loads() {
@@ -55,8 +73,7 @@ D3_INLINE int wx_piece(int r, int t) {
   if constexpr (F::ROW != 128) return t ^ (r & 15);
   const int p = t ^ ((r >> 1) & 7);
   return F::SCALED ? ((p & 3) << 1) | (p >> 2) : p;
-}
-// the same of bf16 weights by the step, 64 bytes a row: piece q of row r of 16
+}// the same of bf16 weights by the step, 64 bytes a row: piece q of row r of 16
 D3_INLINE int wx_step_slot(int r, int q) { return q ^ ((4 - (r >> 2)) & 3); }
 
 // The passes go by what they cost: those of most tiles first (three classes of them), so that the items of a turn take
@@ -127,7 +144,7 @@ D3_INLINE void store_pair(uint16_t* row, i32x2 v0, i32x2 v1, bool stored, int ti
     *(i32x4*)(row + 16 * (q & 1) + 8 * (q >> 1)) = i32x4{(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
 }
 
-template <class F, bool SWIGLU, bool OUT_BF16>
+template <class F, bool SWIGLU, bool OUT_BF16, bool ONCE>
 __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduct a, int columns) {
   constexpr int TILES = wx_tiles<F>(), ROWS = 16 * TILES, STEP = WX_N * 64, STAGE = ROWS * F::ROW;
   constexpr int PER = 1024 / F::ROW, LANES = 64 / PER;  // rows of a 1 KB copy, lanes to a row of it
@@ -142,9 +159,17 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
   const int q = lane >> 4, c = lane & 15, wn = w & 3, wm = w >> 2;
   const int S = a.stages, bank_tiles = a.N / 16, half = bank_tiles / 2;
   const uint32_t lds0 = lds_address(smem);
-  // a lane's place in a step of a tile
-  const uint32_t woff = F::SCALED ? 16 * lane
-                                  : (uint32_t)((lane >> 2) * S * 128 + 16 * wx_step_slot(lane >> 2, lane & 3));
+  // A step of bf16 weights is half lines of memory. LINES: a half of a stage is both steps of two of a wave's four tiles
+  // instead of one step of all, which reads the rows' operands twice from LDS.
+  constexpr bool LINES = ONCE && !F::SCALED;
+  // a lane's place in a copy of 1 KB: a step of a tile; LINES, 8 rows of a stage of it
+  uint32_t woff[2];
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const int r = LINES ? 8 * k + (lane >> 3) : lane >> 2;
+    woff[k] = F::SCALED ? 16 * lane
+                        : (uint32_t)(r * S * 128 + 16 * (LINES ? wx_piece<F>(r, lane & 7) : wx_step_slot(r, lane & 3)));
+  }
 
   // The workgroup's items. Two passes that follow each other (mostly one expert's) go to one XCD with all columns of each, so
   // that their weights and rows are read once into its L2; its items are dealt to its workgroups in turn. Those that are left
@@ -188,7 +213,8 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
     t.rows = __builtin_amdgcn_readlane(table.rows, l);
     taken++;
   };
-  // where an item's weights lie: wave w copies the tiles in places 2 w and 2 w + 1, and their scales
+  // where an item's weights lie: wave w copies the tiles in places 2 w and 2 w + 1, and their scales; LINES, one of the first
+  // two and one of the last two of wave w / 2's tiles
   struct Weights {
     const uint8_t *src[2], *word[2];
   };
@@ -196,7 +222,7 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       // the expert's tile in the place of the 16 (a place past the expert's last tile repeats that)
-      const int slot = 2 * w + i, part = max(t.part, 0);
+      const int slot = !LINES ? 2 * w + i : 4 * (w >> 1) + 2 * i + (w & 1), part = max(t.part, 0);
       const int unit = t.part < 0 ? 2 * (slot >> 2) + (slot & 1) : 4 * part + (slot >> 2);
       const int tile = SWIGLU ? min(8 * t.column + unit, half - 1) + ((slot >> 1) & 1) * half
                               : min(16 * t.column + (t.part < 0 ? slot : 8 * part + (slot >> 1)), bank_tiles - 1);
@@ -227,14 +253,17 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
   };
   Item cur, nxt;
   Weights at, at_next;
-  // the copies of step s of stage st (from the next item where this one ends) to step buffer `to`
+  // the copies of half s of stage st (from the next item where this one ends) to buffer `to`: step s of every
+  // tile; LINES, both steps of the first or the last two tiles of every wave
   auto load_weights = [&](int st, int s, int to) __attribute__((always_inline)) {
     const bool here = st < S || nxt.rows == 0;
     st = st < S ? st : nxt.rows ? st - S : S - 1;
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-      dma16(lds0 + to * STEP + (2 * w + i) * 1024, (here ? at.src[i] : at_next.src[i]) + (size_t)st * F::A_STAGE + s * F::A_STEP,
-            woff);
+    for (int i = 0; i < 2; i++) {
+      const int t = LINES ? s : i;
+      dma16_weights<ONCE>(lds0 + to * STEP + (2 * w + i) * 1024, (here ? at.src[t] : at_next.src[t]) +
+                          (size_t)st * F::A_STAGE + (LINES ? 0 : s * F::A_STEP), woff[i]);
+    }
   };
   auto load_rows = [&](int k, int st, int buf) __attribute__((always_inline)) {
     dma16(lds0 + AT_ROWS + buf * STAGE + (uint32_t)(w + 8 * k) * 1024, a.x + (size_t)st * F::ROW, xoff[k]);
@@ -288,14 +317,19 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
       i32x4 wa[4], b[4][F::PIECES];
       uint32_t sw[4] = {0, 0, 0, 0}, sb[4] = {0, 0, 0, 0};
       auto read_w = [&](int s) __attribute__((always_inline)) {
-        const uint8_t* from = smem + ring * STEP + 4 * wn * 1024 +
-                              (F::SCALED ? 16 * lane : c * 64 + 16 * wx_step_slot(c, q));
+        // step s of the wave's four tiles; LINES: steps 0 and 1 of two of them
+        const uint8_t* from = smem + ring * STEP + 4 * wn * 1024;
 #pragma unroll
-        for (int n = 0; n < 4; n++) wa[n] = *(const i32x4*)(from + 1024 * n);
+        for (int n = 0; n < 4; n++)
+          wa[n] = *(const i32x4*)(F::SCALED ? from + 1024 * n + 16 * lane
+                                  : LINES   ? from + 2048 * (n >> 1) + 128 * c + 16 * wx_slot<F>(c, 4 * (n & 1) + q)
+                                            : from + 1024 * n + 64 * c + 16 * wx_step_slot(c, q));
       };
-      auto read_x = [&](int i) __attribute__((always_inline)) {  // operand i: tile i % NT, step i / NT
+      // operand i: tile i % NT, step i / NT; LINES: step i & 1 of tile i / 2, all again for the other weights
+      auto read_x = [&](int i) __attribute__((always_inline)) {
+        const int step = LINES ? i & 1 : i / NT, j = LINES ? i % (2 * NT) / 2 : i % NT;
 #pragma unroll
-        for (int k = 0; k < F::PIECES; k++) b[i & 3][k] = *(const i32x4*)(xlane[i / NT][k] + (i % NT) * 32 * F::ROW);
+        for (int k = 0; k < F::PIECES; k++) b[i & 3][k] = *(const i32x4*)(xlane[step][k] + j * 32 * F::ROW);
         if constexpr (F::SCALED) sb[i & 3] = *(const uint16_t*)(slane + (i % NT) * 256);
       };
       read_w(0);
@@ -323,11 +357,22 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
       auto products = [&]<int s>() __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-          if (s * NT + j + 2 < 2 * NT) read_x(s * NT + j + 2);
-          __builtin_amdgcn_sched_barrier(0);  // the reads first
+          const int i = (LINES ? 2 : 1) * (s * NT + j);
+          if constexpr (!LINES) {
+            if (i + 2 < 2 * NT) read_x(i + 2);
+            __builtin_amdgcn_sched_barrier(0);  // the reads first
 #pragma unroll
-          for (int n = 0; n < 4; n++)
-            acc[j][n] = step_product<F, !OUT_BF16, s, s>(wa[n], b[(s * NT + j) & 3], acc[j][n], sw[n], sb[(s * NT + j) & 3]);
+            for (int n = 0; n < 4; n++)
+              acc[j][n] = step_product<F, !OUT_BF16, s, s>(wa[n], b[i & 3], acc[j][n], sw[n], sb[i & 3]);
+          } else {
+            if (i + 2 < 4 * NT) read_x(i + 2), read_x(i + 3);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+              for (int n = 0; n < 2; n++)
+                acc[j][2 * s + n] = step_product<F, false, 0, 0>(wa[2 * n + k], b[(i + k) & 3], acc[j][2 * s + n], 0, 0);
+          }
           if (s == 0) {
             constexpr int SPREAD = (MINE + NT - 1) / NT;
 #pragma unroll
@@ -419,15 +464,24 @@ inline int device_cus() {
   return n;
 }
 
-template <class F>
-void launch_wide(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
+template <class F, bool ONCE>
+void launch_wide_of(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
   const int columns = (a.N + WX_N - 1) / WX_N, passes = most_passes(a.pairs, a.n_groups, 16 * wx_tiles<F>());
   const int64_t items = (int64_t)2 * passes * columns;  // shared ones twice
   const int cus = std::max(device_cus() & ~7, 8);       // as many for each XCD
   const dim3 grid((unsigned)std::min<int64_t>((items + 7) & ~7, cus)), block(WX_THREADS);
-  if (swiglu) hipLaunchKernelGGL((expert_wide_kernel<F, true, true>), grid, block, 0, s, a, columns);
-  else if (out_bf16) hipLaunchKernelGGL((expert_wide_kernel<F, false, true>), grid, block, 0, s, a, columns);
-  else hipLaunchKernelGGL((expert_wide_kernel<F, false, false>), grid, block, 0, s, a, columns);
+  if (swiglu) hipLaunchKernelGGL((expert_wide_kernel<F, true, true, ONCE>), grid, block, 0, s, a, columns);
+  else if (out_bf16) hipLaunchKernelGGL((expert_wide_kernel<F, false, true, ONCE>), grid, block, 0, s, a, columns);
+  else hipLaunchKernelGGL((expert_wide_kernel<F, false, false, ONCE>), grid, block, 0, s, a, columns);
+}
+
+// Where an expert's rows are one pass, mostly, its weights are read once: nontemporal. us without / with (first bank,
+// 128 experts): bf16 512 rows 191 / 182, 1024 197 / 193, 4096 247 / 242 and on the second bank 183 / 175; e4m3 1024 rows
+// 61 / 57; e2m1 4096 rows the same; bf16 rows of 13 passes an expert 193 / 201.
+template <class F>
+void launch_wide(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
+  if ((int64_t)a.pairs <= (int64_t)16 * wx_tiles<F>() * a.n_groups) launch_wide_of<F, true>(a, swiglu, out_bf16, s);
+  else launch_wide_of<F, false>(a, swiglu, out_bf16, s);
 }
 
 // Whether a grouped product runs in wide passes: by the rows an expert has on average. (The copies to LDS take 32-bit
@@ -438,10 +492,10 @@ bool wide_fits(const ExpertProduct& a) {
 }
 
 // Wide passes, or streamed ones of 32 rows, or of 16, by the rows an expert has on average. Top-8 of 128 experts (FFN 768),
-// us with 16 / 32 / wide: first bank, e4m3 rows, 256 rows (16 to an expert) 51 / 46 / 52, 400 rows 67 / 50 / 53, 700 rows
+// us with 16 / 32 / wide: first bank, e4m3 rows, 256 rows (16 to an expert) 54 / 46 / 52, 400 rows 67 / 50 / 53, 700 rows
 // 73 wide and 74 streamed (256 experts, Zipf); second bank 16 to an expert 31 / 36 / 43 (few stages: a 32-row pass has
 // less to stream than it takes to set up), 25 to an expert 40 / 41 / 42, 44 to an expert 60 streamed, 47 wide; bf16 first
-// bank 16 to an expert 182 / 163 / 190, 25: 238 / 174 / 192; second bank 16: 100 / 89 / 102.
+// bank 16 to an expert 196 / 164 / 190, 25: 238 / 174 / 192; second bank 16: 100 / 89 / 102.
 template <class F>
 void launch_grouped(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
   if (wide_fits<F>(a)) return launch_wide<F>(a, swiglu, out_bf16, s);

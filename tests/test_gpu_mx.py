@@ -412,3 +412,17 @@ def test_few_pairs_of_many_experts(fmt, K):
     ids, order, _, groups = _pairs(10, FEW)
     for how in ({}, {"swiglu": True}):
         rows.check(rows.grouped(groups, order=order, **how), order, ids[order], "swiglu" in how)
+
+
+@pytest.mark.parametrize("n, K", [(96, 320), (544, 512), (288, 2048)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_experts_of_many_passes(fmt, n, K):
+    """More rows to an expert than a wide pass takes, on average too: several passes read an expert's weights. Bit for bit what
+    the pairs give one by one."""
+    counts = [700, 0, 1301]
+    case = Case(fmt, 3, n, K, sum(counts))
+    ids, order, _, groups = _pairs(3, counts)
+    for how in ({}, {"dtype": torch.bfloat16}, {"swiglu": True}):
+        got = case.grouped(groups, order=order, **how)
+        assert torch.equal(got, case.gemv(ids, **how)[order])
+        case.check(got[::37], order[::37], ids[order[::37]], "swiglu" in how)
