@@ -9,8 +9,8 @@
 //
 // Bound by what comes from HBM and the memory-side cache (each XCD reads the rows of its experts for itself), the first
 // products of each workgroup and the epilogues beside it. 4096 rows, top-8 of 128 experts, first bank (FFN 768) with SwiGLU:
-// bf16 232 us, 0.96 GB read past the L2s and 50 MB written at 4.3 TB/s (223 us with the products left out; the matrix units
-// work 47% of the time); e2m1 rows on e2m1 weights 83 us, 0.27 GB read and 50 MB written at 3.9 TB/s (34%). An e4m3 row's
+// bf16 230 us, 0.96 GB read past the L2s and 50 MB written at 4.4 TB/s (10 us less with the products left out; the matrix units
+// work 47% of the time); e2m1 rows on e2m1 weights 81 us, 0.27 GB read and 50 MB written at 3.9 TB/s (34%). An e4m3 row's
 // float32 result takes two products a step (ragged.hpp), and passes of 160 rows read the weights twice as often: 150 us
 // (second bank).
 #pragma once
