@@ -183,8 +183,8 @@ __global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
           if constexpr (LINES) steps_of_lines(w[0], w[1]);
 #pragma unroll
           for (int m = 0; m < MT; m++) {
-            acc[n][m] = step_product<F, !OUT_BF16, 2 * ODD, 0>(w[0], b[m][0], acc[n][m], sw[n], sb[m]);
-            acc[n][m] = step_product<F, !OUT_BF16, 2 * ODD + 1, 1>(w[1], b[m][1], acc[n][m], sw[n], sb[m]);
+            acc[n][m] = step_product<F, 2 * ODD, 0>(w[0], b[m][0], acc[n][m], sw[n], sb[m]);
+            acc[n][m] = step_product<F, 2 * ODD + 1, 1>(w[1], b[m][1], acc[n][m], sw[n], sb[m]);
           }
         }
       };

@@ -10,9 +10,9 @@
 // Bound by what comes from HBM and the memory-side cache (each XCD reads the rows of its experts for itself), the first
 // products of each workgroup and the epilogues beside it. 4096 rows, top-8 of 128 experts, first bank (FFN 768) with SwiGLU:
 // bf16 230 us, 0.96 GB read past the L2s and 50 MB written at 4.4 TB/s (10 us less with the products left out; the matrix units
-// work 47% of the time); e2m1 rows on e2m1 weights 81 us, 0.27 GB read and 50 MB written at 3.9 TB/s (34%). An e4m3 row's
-// float32 result takes two products a step (ragged.hpp), and passes of 160 rows read the weights twice as often: 150 us
-// (second bank).
+// work 47% of the time); e2m1 rows on e2m1 weights 81 us, 0.27 GB read and 50 MB written at 3.9 TB/s (34%). An e4m3 row
+// takes two products a step (ragged.hpp), and its passes of 160 rows read the weights twice as often: 214 us, 150 us on the
+// second bank.
 #pragma once
 #include "expert_stream.hpp"
 
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
             __builtin_amdgcn_sched_barrier(0);  // the reads first
 #pragma unroll
             for (int n = 0; n < 4; n++)
-              acc[j][n] = step_product<F, !OUT_BF16, s, s>(wa[n], b[i & 3], acc[j][n], sw[n], sb[i & 3]);
+              acc[j][n] = step_product<F, s, s>(wa[n], b[i & 3], acc[j][n], sw[n], sb[i & 3]);
           } else {
             if (i + 2 < 4 * NT) read_x(i + 2), read_x(i + 3);
             __builtin_amdgcn_sched_barrier(0);
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(WX_THREADS, 2) expert_wide_kernel(ExpertProduc
             for (int k = 0; k < 2; k++)
 #pragma unroll
               for (int n = 0; n < 2; n++)
-                acc[j][2 * s + n] = step_product<F, false, 0, 0>(wa[2 * n + k], b[(i + k) & 3], acc[j][2 * s + n], 0, 0);
+                acc[j][2 * s + n] = step_product<F, 0, 0>(wa[2 * n + k], b[(i + k) & 3], acc[j][2 * s + n], 0, 0);
           }
           if (s == 0) {
             constexpr int SPREAD = (MINE + NT - 1) / NT;

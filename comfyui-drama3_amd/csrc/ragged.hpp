@@ -59,8 +59,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 //
 // Against e4m3, v_mfma_scale aligns a block's 32 products to the largest one's exponent and keeps 13 bits below it (measured:
 // of 256 - 256 + 2^-n it gives 2^-5 and nothing smaller; e2m1 against e2m1 loses nothing). e4m3 spans 18 binades, so
-// small elements beside a block's large ones are cut: 7e-6 of a result's norm on normally distributed rows with a
-// few large channels, where float32 sums give 2e-7. Of each part every product keeps all its bits: e2m1 is a multiple
+// small elements beside a block's large ones are cut, each by up to 2^-13 of the block's largest product: 7e-6 of a result's
+// norm on normally distributed rows with a few channels eight times as large, where float32 sums give 2e-7, and without a
+// bound where large products cancel. Of each part every product keeps all its bits: e2m1 is a multiple
 // of 1/2, high of 1/4 and low of 2^-9, so products are multiples of 2^-3 with exponents up to 8 + 2 = 10, and of 2^-10 with
 // exponents up to 0 + 2 = 2 (4000 random blocks of each part came out exactly, with the border at 1 or 8 they did not).
 D3_INLINE void split_e4m3(i32x8 b, i32x8& low, i32x8& high) {
@@ -74,9 +75,9 @@ D3_INLINE void split_e4m3(i32x8 b, i32x8& low, i32x8& high) {
 }
 
 // acc + a . b over a step. sa, sb: scale words, byte OA and OB of them. (The upper half of an e2m1 operand is not
-// read.) EXACT: e4m3 rows in two parts, for results that are kept in float32; those that are rounded to bf16 (2e-3
-// of their norm) take the instruction's own sums, at half the products.
-template <class F, bool EXACT, int OA, int OB>
+// read.) e4m3 rows in two parts whatever becomes of the result: what the instruction cuts goes by a block's largest product,
+// not by the sum, and where large products cancel, rounding the sum to bf16 does not hide it.
+template <class F, int OA, int OB>
 D3_INLINE f32x4 step_product(i32x4 a, const i32x4 (&b)[F::PIECES], f32x4 acc, uint32_t sa, uint32_t sb) {
   if constexpr (F::SCALED) {
     const i32x8 A = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
@@ -85,7 +86,6 @@ D3_INLINE f32x4 step_product(i32x4 a, const i32x4 (&b)[F::PIECES], f32x4 acc, ui
       return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc, 4, 4, OA, (int)sa, OB, (int)sb);
     } else {
       const i32x8 B = __builtin_shufflevector(b[0], b[F::PIECES - 1], 0, 1, 2, 3, 4, 5, 6, 7);
-      if constexpr (!EXACT) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc, 4, 0, OA, (int)sa, OB, (int)sb);
       i32x8 low, high;
       split_e4m3(B, low, high);
       acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, high, acc, 4, 0, OA, (int)sa, OB, (int)sb);

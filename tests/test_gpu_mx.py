@@ -426,3 +426,53 @@ def test_experts_of_many_passes(fmt, n, K):
         got = case.grouped(groups, order=order, **how)
         assert torch.equal(got, case.gemv(ids, **how)[order])
         case.check(got[::37], order[::37], ids[order[::37]], "swiglu" in how)
+
+
+# per number of rows: streamed (20 rows an expert), and wide passes
+SUMS = [[20, 19], [300, 77]]
+
+
+@pytest.mark.parametrize("counts", SUMS)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_bfloat16_result_is_the_float32_one_rounded(fmt, counts):
+    """Sums are the same whatever becomes of them: a bfloat16 result is the float32 one to nearest, ties to even, bit for bit."""
+    case = Case(fmt, 2, 96, 832, sum(counts), spread=2.0)
+    ids, order, _, groups = _pairs(2, counts)
+    assert torch.equal(case.gemv(ids, dtype=torch.bfloat16), case.gemv(ids).to(torch.bfloat16))
+    assert torch.equal(case.grouped(groups, order=order, dtype=torch.bfloat16),
+                       case.grouped(groups, order=order).to(torch.bfloat16))
+
+
+def _cancelling(bits, E, n, K, R):
+    """A Case whose every fourth block holds two products of the formats' largest elements that cancel, beside 30 that are a
+    thousandth of them or less, as the other blocks' are."""
+    case = Case(f"mx{bits}", E, n, K, R)
+    rng = np.random.default_rng(41)
+    big = np.arange(K) // 32 % 4 == 1
+    x = rng.uniform(-1, 1, (R, K)) * (0.0625 if bits == 8 else 0.5)
+    w = rng.uniform(-1, 1, (E * n, K)) * 6
+    x[:, big & (np.arange(K) % 32 < 2)] = 448.0 if bits == 8 else 6.0
+    w[:, big & (np.arange(K) % 32 == 0)], w[:, big & (np.arange(K) % 32 == 1)] = 6.0, -6.0
+    w[:, ~big & (np.arange(K) % 32 == 0)] = 6.0  # (the weights' scales are 1)
+    (xc, xs), (wc, ws) = omx.quantize(x, bits), omx.quantize(w, 4)
+    case.x = mx.rows_from(dev(omx.pack(xc, bits)), dev(xs), bits)
+    case.w = mx.bank(mx.rows_from(dev(omx.pack(wc, 4)), dev(ws), 4), E)
+    case.xv, case.wv = dev(omx.values(xc, xs, bits)), dev(omx.values(wc, ws, 4)).view(E, n, K)
+    return case
+
+
+@pytest.mark.parametrize("how", [{}, {"dtype": torch.bfloat16}, {"swiglu": True}])
+@pytest.mark.parametrize("counts", SUMS)
+@pytest.mark.parametrize("bits", [4, 8])
+def test_small_products_beside_large_ones_that_cancel(bits, counts, how):
+    """A result is what the small products of its blocks add up to, within the bound of float32 sums (`want`'s for results that
+    are kept) and the result's own rounding."""
+    case = _cancelling(bits, 2, 96, 768, sum(counts))
+    ids, order, _, groups = _pairs(2, counts)
+    rows = torch.arange(sum(counts), device=DEV)
+    for got, row in ((case.gemv(ids, **how), rows), (case.grouped(groups, order=order, **how), order)):
+        for part in range(0, len(row), 32):
+            at = row[part:part + 32]
+            want, off = case.want(at, ids[at], "swiglu" in how, False)
+            eps = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24
+            assert torch.all((got[part:part + 32].double() - want).abs() <= off + eps * (want.abs() + off) + 1e-37)
