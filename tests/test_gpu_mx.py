@@ -476,3 +476,62 @@ def test_small_products_beside_large_ones_that_cancel(bits, counts, how):
             want, off = case.want(at, ids[at], "swiglu" in how, False)
             eps = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24
             assert torch.all((got[part:part + 32].double() - want).abs() <= off + eps * (want.abs() + off) + 1e-37)
+
+
+@pytest.mark.parametrize("down", [4, 10, 16])
+@pytest.mark.parametrize("apart", [1, 2, 8])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_small_blocks_beside_large_ones_that_cancel(bits, apart, down):
+    """The same across blocks: a block of the formats' largest products and, `apart` blocks on (in the same step's products or
+    another's), its negative; what is between them and behind is 2^-down as large in its scales."""
+    E, n, K, R = 2, 32, 512, 80
+    case = Case(f"mx{bits}", E, n, K, R)
+    rng = np.random.default_rng(100 * apart + down)
+    first = 2
+    x = rng.uniform(-1, 1, (R, K)) * 2.0 ** -down
+    w = rng.uniform(-1, 1, (E * n, K)) * 6
+    large = 32 * first + np.arange(32)
+    x[:, large] = rng.uniform(0.5, 1, (R, 32)) * (448 if bits == 8 else 6)
+    x[:, large + 32 * apart] = -x[:, large]
+    w[:, large + 32 * apart] = w[:, large]
+    (xc, xs), (wc, ws) = omx.quantize(x, bits), omx.quantize(w, 4)
+    case.x = mx.rows_from(dev(omx.pack(xc, bits)), dev(xs), bits)
+    case.w = mx.bank(mx.rows_from(dev(omx.pack(wc, 4)), dev(ws), 4), E)
+    case.xv, case.wv = dev(omx.values(xc, xs, bits)), dev(omx.values(wc, ws, 4)).view(E, n, K)
+    ids = torch.arange(R, device=DEV) % E
+    order, _, groups = kernels.expert_groups(ids.view(-1, 1), E)
+    rows = torch.arange(R, device=DEV)
+    for got, row in ((case.gemv(ids), rows), (case.grouped(groups, order=order), order)):
+        want, off = case.want(row, ids[row], False, False)
+        err = (got.double() - want).abs()
+        assert torch.all(err <= off + 2.0 ** -24 * want.abs()), float((err / off).max())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_products_at_every_scale_code(bits):
+    """Rows of every scale code from 0 to 254 against weights of codes that bring the products back into float32's range,
+    the smallest and the largest code among both."""
+    E, n, K, R = 8, 32, 512, 255
+    case = Case(f"mx{bits}", E, n, K, R)
+    codes, _ = omx.quantize(case.xv.cpu().numpy(), bits)
+    wcodes, _ = omx.quantize(case.wv.flatten(0, 1).cpu().numpy(), 4)
+    xs = np.repeat(np.arange(255)[:, None], K // 32, axis=1).astype(np.uint8)
+    level = np.array([0, 1, 60, 120, 134, 190, 253, 254])
+    ws = np.repeat(level, n)[:, None].repeat(K // 32, axis=1).astype(np.uint8)
+    case.x = mx.rows_from(dev(omx.pack(codes, bits)), dev(xs), bits)
+    case.w = mx.bank(mx.rows_from(dev(omx.pack(wcodes, 4)), dev(ws), 4), E)
+    case.xv, case.wv = dev(omx.values(codes, xs, bits)), dev(omx.values(wcodes, ws, 4)).view(E, n, K)
+    # (row, expert) of products between 2^-100 and 2^90 a scale
+    row, expert = (torch.from_numpy(a).to(DEV) for a in np.nonzero(np.abs(np.arange(255)[:, None] + level - 249) <= 95))
+    ids = torch.full((R * E,), -1, dtype=torch.int64, device=DEV)
+    ids[row * E + expert] = expert
+    got = case.gemv(ids)[row * E + expert]
+    case.check(got, row, expert)
+    # the same pairs grouped, in wide passes
+    order = row * E + expert
+    order = order[torch.argsort(expert, stable=True)]
+    counts = torch.bincount(expert, minlength=E)
+    groups = torch.stack([torch.arange(E, device=DEV)] * 2 + [torch.zeros_like(counts), counts.cumsum(0) - counts, counts],
+                         dim=1).to(torch.int32)
+    grouped = case.grouped(groups, order=order, k=E)
+    assert torch.equal(grouped, case.gemv(ids)[order])
