@@ -556,20 +556,20 @@ def fp8_linear(x, weight, scale):
 
 # ------------------------------------------------------------- products of unquantized and of microscaled (mx.py) banks
 _INT_MAX = 2 ** 31 - 1  # of the C entries' sizes, which ctypes would cut to their low bits
-_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def launch(name, index, *args):
     """C entry `name` with `args` and torch's current stream of device `index`, that device the current one. (The stream's
-    handle as torch's own generated code asks for it: a Stream object costs 2 us, as much as the launch.)"""
+    handle as torch's own generated code asks for it: a Stream object costs 2 us, as much as the launch. A torch without GPU
+    support has neither binding, and imports this module all the same.)"""
     if index < 0:
         raise ValueError(f"{name}: the kernels run on a GPU, not on the CPU")
-    fn = getattr(_lib.lib(), name)
-    if index == _current():
-        rc = fn(*args, _raw_stream(index))
+    fn, stream = getattr(_lib.lib(), name), torch._C._cuda_getCurrentRawStream
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(*args, stream(index))
     if rc:
         _lib.check(rc, name)
 

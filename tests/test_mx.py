@@ -1,5 +1,8 @@
 """Microscaled rows and banks without a GPU: the oracle's formats, the banks' layout, and what the entry points refuse."""
 import ctypes
+import pathlib
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -179,3 +182,24 @@ def test_layer_refuses_routes_elsewhere():
 
     with pytest.raises(ValueError, match="topk_idx and topk_weight"):
         kernels.direct_layer(x.as_subclass(OnGpu), ids, weights, 2, None, None)
+
+
+def test_modules_import_without_gpu_bindings():
+    """A torch built without GPU support has no current stream or device to ask for: the package imports there, and the
+    products refuse rows that are not on a GPU."""
+    code = """
+import torch
+for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+from drama3 import formats, kernels, loader, moe, mx, offload
+try:
+    mx.quantize(torch.zeros(2, 64))
+except ValueError as e:
+    assert "GPU" in str(e)
+else:
+    raise AssertionError("not refused")
+"""
+    root = pathlib.Path(mx.__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
