@@ -503,6 +503,8 @@ class QuantHostBank(HostBank):
     @classmethod
     def from_fields(cls, num_experts, kind, fields, pin, codebook=None):
         """A bank given as its kernel kind and field dict (a converted file's tensors, drama3/loader.py)."""
+        if kind not in ("int8", "w4", "w6"):
+            raise ValueError(f"a store's banks are int8, fp8, w4 or w6, not {kind!r} (bf16 and mx4: ExpertTable)")
         self = cls.__new__(cls)
         in_features = fields["_qdata"].shape[1] * 8 // (8 if kind == "int8" else int(kind[1]))
         self._setup(num_experts, kind, fields, pin, {} if codebook is None else {"codebook": codebook}, in_features)

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from drama3 import _lib, kernels, mx
+from drama3 import _lib, kernels, mx, offload
 from oracle import mx as omx
 
 
@@ -203,3 +203,13 @@ else:
     root = pathlib.Path(mx.__file__).resolve().parents[1]
     done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr
+
+
+@pytest.mark.parametrize("kind", ["bf16", "mx4", "int4"])
+def test_store_refuses_kinds_it_does_not_take(kind):
+    """A store's slot cache reads the four reference formats: the other kinds are refused by name, and nothing is added."""
+    fields = {"weight": torch.zeros((64, 256), dtype=torch.uint8), "scale": torch.zeros((64, 16), dtype=torch.uint8)}
+    store = offload.ExpertStore(0, False)
+    with pytest.raises(ValueError, match=kind):
+        store.add_fields(kind, fields, fields, 2)
+    assert not store.banks
