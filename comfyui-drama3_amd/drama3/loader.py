@@ -105,6 +105,9 @@ def write_experts(path, kind, layers, config=None):
     fields), (codebooks)), ...} with flat fields and `experts` rows per bank given by the fields' first dimension /
     experts in config["num_experts"]."""
     from safetensors.torch import save_file
+    formats = {v: k for k, v in KINDS.items()}
+    if kind not in formats:
+        raise ValueError(f"a converted file holds {', '.join(formats)} banks, not {kind!r}")
     experts = int(config["num_experts"])
     out = {}
     for layer, (banks, codebooks) in layers.items():
@@ -130,5 +133,4 @@ def write_experts(path, kind, layers, config=None):
                 conf = {"format": "asym_w4a8_int8" if kind == "w4" else "w6a8_int8", "group_size": 16,
                         "convrot_groupsize": 256, "num_experts": experts}
             out[m + "comfy_quant"] = torch.tensor(list(json.dumps(conf).encode()), dtype=torch.uint8)
-    fmt = {v: k for k, v in KINDS.items()}[kind]
-    save_file(out, str(path), metadata={"drama3_format": fmt, "drama3_config": json.dumps(config or {})})
+    save_file(out, str(path), metadata={"drama3_format": formats[kind], "drama3_config": json.dumps(config or {})})

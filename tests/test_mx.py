@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from drama3 import _lib, kernels, mx, offload
+from drama3 import _lib, kernels, loader, mx, offload
 from oracle import mx as omx
 
 
@@ -213,3 +213,11 @@ def test_store_refuses_kinds_it_does_not_take(kind):
     with pytest.raises(ValueError, match=kind):
         store.add_fields(kind, fields, fields, 2)
     assert not store.banks
+
+
+@pytest.mark.parametrize("kind", ["bf16", "mx4"])
+def test_files_refuse_kinds_they_do_not_hold(kind, tmp_path):
+    fields = {"weight": torch.zeros((64, 256), dtype=torch.uint8), "scale": torch.zeros((64, 16), dtype=torch.uint8)}
+    with pytest.raises(ValueError, match=kind):
+        loader.write_experts(tmp_path / "x.safetensors", kind, {0: ((fields, fields), (None, None))}, {"num_experts": 2})
+    assert not list(tmp_path.iterdir())
