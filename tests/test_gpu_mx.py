@@ -535,3 +535,113 @@ def test_products_at_every_scale_code(bits):
                          dim=1).to(torch.int32)
     grouped = case.grouped(groups, order=order, k=E)
     assert torch.equal(grouped, case.gemv(ids)[order])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_pairs_of_a_row(fmt):
+    """How many pairs each row has follows from the ids' number: three rows with one expert each, then with three."""
+    case = Case(fmt, 5, 96, 320, 3, spread=1.0)
+    ids = dev(np.array([4, 0, 2, 2, 4, 1, 0, 3, 2], np.int64))
+    row = torch.arange(3, device=DEV)
+    one, three = case.gemv(ids[[0, 4, 8]]), case.gemv(ids)
+    case.check(one, row, ids[[0, 4, 8]])
+    assert torch.equal(one, three[[0, 4, 8]])
+
+
+@pytest.mark.parametrize("n, K", [(288, 768), (96, 1280), (160, 2368)])
+@pytest.mark.parametrize("fmt", ["mx4", "mx8"])
+def test_wide_passes_of_an_odd_number_of_stages(fmt, n, K):
+    """Wide passes where an item ends inside a pair of stages, whose scale words lie together: the next item's start in the other
+    buffer."""
+    case = Case(fmt, len(MANY), n, K, sum(MANY), spread=1.0)
+    ids, order, _, groups = _pairs(len(MANY), MANY)
+    for how in ({}, {"dtype": torch.bfloat16}, {"swiglu": True}):
+        got = case.grouped(groups, order=order, **how)
+        case.check(got, order, ids[order], "swiglu" in how)
+        assert torch.equal(got, case.gemv(ids, **how)[order])
+
+
+@pytest.mark.parametrize("E, rows, n", [(10, 300, 800), (70, 33, 800), (300, 34, 96)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_more_items_of_an_odd_number_of_stages(fmt, E, rows, n):
+    """The same where a workgroup walks several items."""
+    K = 192 if fmt == "bf16" else 768
+    counts = np.random.default_rng(E).integers(rows - 1, rows + 2, E)
+    counts[3], counts[5] = 0, 7 * rows
+    case = Case(fmt, E, n, K, int(counts.sum()))
+    ids, order, _, groups = _pairs(E, counts)
+    for how in ({}, {"swiglu": True}, {"dtype": torch.bfloat16}):
+        got = case.grouped(groups, order=order, **how)
+        assert torch.equal(got, case.gemv(ids, **how)[order])
+        at = torch.arange(0, len(order), 499, device=DEV)
+        case.check(got[at], order[at], ids[order[at]], "swiglu" in how)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_what_is_not_finite_stays_in_its_row_of_a_wide_pass(fmt):
+    """A NaN row and an infinite (microscaled: NaN) weight beside the rows of a pass whose last tile is not full."""
+    case = Case(fmt, 2, 64, 768, 150)
+    pair = torch.arange(150, device=DEV)
+    ids = pair % 2
+    order, _, groups = kernels.expert_groups(ids.view(-1, 1), 2)
+    before = case.grouped(groups, order=order)[torch.argsort(order)]
+    if fmt == "bf16":
+        case.x[6, 100] = float("nan")
+        case.w[64 + 9, 3] = float("inf")
+    else:
+        case.x.scale[6, 3] = 255
+        rows = mx.bank_rows(case.w)
+        rows.scale[64 + 9, 0] = 255
+        case.w = mx.bank(rows, 2)
+    got = case.grouped(groups, order=order)[torch.argsort(order)]
+    bad = (pair == 6)[:, None] | ((ids == 1)[:, None] & (torch.arange(64, device=DEV) == 9))
+    assert not torch.isfinite(got[bad]).any()
+    assert torch.equal(got[~bad], before[~bad])
+
+
+@pytest.mark.parametrize("fmt", ["mx8", "bf16"])
+def test_wide_passes_beyond_32_bit_offsets(fmt):
+    """The last experts of a bank of more than 4 GiB, 40 rows each."""
+    n, K = 2048, 2048
+    E = 560 if fmt == "bf16" else 2100
+    small = Case(fmt, 2, n, K, 80)
+    groups = torch.tensor([[0, 0, 0, 0, 39], [1, 0, 0, 39, 41]], dtype=torch.int32, device=DEV)
+    want = small.grouped(groups)
+    at = torch.tensor([0, 38, 39, 79], device=DEV)
+    small.check(want[at], at, (at >= 39).long())
+    if fmt == "bf16":
+        w = torch.zeros((E * n, K), dtype=torch.bfloat16, device=DEV)
+        w[-2 * n:] = small.w
+    else:
+        w = mx.MxBank(torch.zeros((E * n, K // 2), dtype=torch.uint8, device=DEV),
+                      torch.zeros((E * n, K // 32), dtype=torch.uint8, device=DEV), E, n, K)
+        w.weight[-2 * n:], w.scale[-2 * n:] = small.w.weight, small.w.scale
+    assert (w if fmt == "bf16" else w.weight).nbytes > 2 ** 32
+    small.w, small.E = w, E
+    assert torch.equal(small.grouped(groups + torch.tensor([E - 2, 0, 0, 0, 0], dtype=torch.int32, device=DEV)), want)
+
+
+@pytest.mark.parametrize("fmt", ["mx8", "bf16"])
+def test_rows_beyond_32_bit_offsets(fmt):
+    """The last rows of more than 4 GiB of them, some with an expert of few pairs and some with one of many."""
+    K, last = 2048, 64
+    R = 2 ** 32 // (K * (2 if fmt == "bf16" else 1)) + last
+    case = Case(fmt, 2, 64, K, last)
+    for counts in ((3, 5), (64, 64)):
+        pairs = torch.cat([torch.arange(c, device=DEV) for c in counts])
+        groups = torch.tensor([[0, 0, 0, 0, counts[0]], [1, 0, 0, counts[0], counts[1]]], dtype=torch.int32, device=DEV)
+        want = case.grouped(groups, order=pairs)
+        case.check(want, pairs, torch.arange(2, device=DEV).repeat_interleave(torch.tensor(counts, device=DEV)))
+        many = Case.__new__(Case)
+        many.__dict__.update(case.__dict__, R=R)
+        if fmt == "bf16":
+            many.x = torch.zeros((R, K), dtype=torch.bfloat16, device=DEV)
+            many.x[-last:] = case.x
+            assert many.x.nbytes > 2 ** 32
+        else:
+            many.x = mx.MxRows(torch.zeros((R, K), dtype=torch.uint8, device=DEV),
+                               torch.zeros((R, K // 32), dtype=torch.uint8, device=DEV), 8, K)
+            many.x.codes[-last:], many.x.scale[-last:] = case.x.codes, case.x.scale
+            assert many.x.codes.nbytes > 2 ** 32
+        assert torch.equal(many.grouped(groups, order=R - last + pairs), want)
+        del many
