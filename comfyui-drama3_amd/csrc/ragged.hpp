@@ -103,7 +103,9 @@ D3_INLINE i32x2 bf16_4(f32x4 v) {
   return __builtin_bit_cast(i32x2, __builtin_convertvector(v, bf16x4));
 }
 // SiLU(gate) * up in float32, then rounded to bf16 as the rows that the next product reads. exp and the reciprocal are the
-// hardware's, within 2 and 1 units of the last place: about 2^-21 of the value, which the rounding's 2^-9 hides.
+// hardware's, within 2 and 1 units of the last place, and exp takes a rounded gate / ln 2, |gate| 2^-23 of the value more: within
+// (2^-21 + |gate| 2^-23) of it in all, 2^-16 at |gate| = 87, which the rounding's 2^-8 hides. (Below, SiLU is under 2^-118 and
+// its reciprocal may come out as zero.)
 D3_INLINE i32x2 swiglu_4(f32x4 gate, f32x4 up) {
   f32x4 h;
 #pragma unroll

@@ -333,7 +333,8 @@ def prompt_groups(topk_idx, num_experts):
 
 
 def prompt_expert_groups(topk_idx, num_experts):
-    """expert_groups (without a plan) over many workgroups: (order, inverse, groups) of a long prompt's pairs."""
+    """expert_groups (without a plan) over many workgroups: (order, inverse, groups) of a long prompt's pairs. Within a group
+    the pairs' order is not fixed, so order and inverse of two calls do not go together."""
     ids = topk_idx.reshape(-1).contiguous()
     if ids.dtype != torch.int64:
         ids = ids.long()
@@ -648,8 +649,8 @@ def gemv_bf16(x, ids, weight, n, swiglu=False, dtype=torch.float32, out=None):
 
 def grouped_bf16(x, groups, weight, n, order=None, k=1, swiglu=False, dtype=torch.float32, out=None):
     """grouped_int8's products on a bank of bfloat16 weights [E * n, K]: [P, n] for the places of `groups` [g, 5] int32,
-    place p row order[p] // k of the bfloat16 rows x [R, K] (its own row p without order), order and groups as
-    expert_groups makes them. dtype and `swiglu` as for gemv_bf16. Places in no group are left as `out` had them (unset
+    place p row order[p] // k of the bfloat16 rows x [R, K] (its own row p without order; an order outside the rows reads the
+    nearest one), order and groups as expert_groups makes them. dtype and `swiglu` as for gemv_bf16. Places in no group are left as `out` had them (unset
     without it), as are groups whose expert or places lie outside the bank or the pairs. Groups must not share places."""
     x, R, K, E, index = _bf16_operands(x, weight, n)
     P = check_groups(groups, order, k, R, index)

@@ -185,8 +185,8 @@ def gemv(rows, ids, bank, swiglu=False, dtype=torch.float32, out=None):
 
 def grouped(rows, groups, bank, order=None, k=1, swiglu=False, dtype=torch.float32, out=None):
     """[P, N] of pairs grouped by expert: groups [g, 5] int32 (expert, ., ., first place, rows) and order [P] int64 as
-    kernels.expert_groups makes them; place p multiplies row order[p] // k (its own row p without order) with its group's
-    expert. dtype and `swiglu` as for gemv. Places in no group are left as `out` had them (unset without it), as are groups
+    kernels.expert_groups makes them; place p multiplies row order[p] // k (its own row p without order; an order outside the
+    rows reads the nearest one) with its group's expert. dtype and `swiglu` as for gemv. Places in no group are left as `out` had them (unset without it), as are groups
     whose expert or places lie outside the bank or the pairs. Groups must not share places."""
     codes, scale, R, index = _check_rows(rows)
     weight, wscale = _check_bank(bank, rows.cols, index)

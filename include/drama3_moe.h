@@ -395,7 +395,9 @@ int d3_decode_codes(int32_t bits, const void* rows, const void* scales, const fl
                     void* out, void* stream);
 
 /* d3_expert_groups over many workgroups, for long prompts (no counterpart in the reference, whose grouping is torch's sort
- * and bincount): the same order, inverse and groups; scratch int32 [>= d3_prompt_pass_ints(E, P)], needs no clearing; P >= 1. */
+ * and bincount): the same groups, and order and inverse by the same rules. Within a group the pairs' order is not fixed, here
+ * as there, so an order goes with the inverse of its own call only. scratch int32 [>= d3_prompt_pass_ints(E, P)], needs no
+ * clearing; P >= 1. */
 int d3_prompt_expert_groups(const int64_t* ids, int32_t P, int32_t E, int64_t* order, int32_t* inverse, int32_t* groups,
                             int32_t* scratch, int64_t scratch_ints, void* stream);
 
@@ -423,8 +425,8 @@ int d3_mx_dequantize(const void* codes, const void* scale, int32_t rows, int32_t
  * row and expert alone, not on the other pairs of the call.
  * gemv: pair p multiplies row p / (pairs / rows) with expert ids[p] (int64); an id outside [0, E) gives zeros.
  * grouped: groups [n_groups, 5] int32 = (expert, ., ., first, rows) as d3_expert_groups makes them; place p of a group
- * multiplies row order[p] / k (row p when order is NULL). Places in no group, and groups whose expert or rows lie
- * outside the bank or the pairs, are left alone; groups must not share places. */
+ * multiplies row order[p] / k (row p when order is NULL; an order outside the rows reads the nearest one). Places in no group,
+ * and groups whose expert or rows lie outside the bank or the pairs, are left alone; groups must not share places. */
 int d3_mx_gemv(const void* codes, const void* scale, int32_t bits, int32_t rows, const int64_t* ids, int32_t pairs,
                const void* w, const void* w_scale, int32_t E, int32_t N, int32_t K, int32_t swiglu, int32_t out_bf16,
                void* out, void* stream);
