@@ -4,10 +4,10 @@
 // ahead; nothing but the accumulators is shared along K, so there is no barrier in the loop. The pass's rows lie whole in
 // LDS (SEG stages at a time), read by all waves.
 //
-// Short prompts run near what memory gives: 77 rows of top-8 of 256 experts (FFN 512) on e4m3 rows, first bank, 44 us (260 MB of
-// weights at 5.9 TB/s); of 128 experts, bf16, second bank, 68 us (400 MB at 5.9). A line's experts are few bytes, and
-// its time a launch and one round trip of loads: 8 pairs of the first bank 4.4 us (e2m1 weights, 13 MB) and 11 us (bf16, 50 MB
-// at 4.6 TB/s).
+// Short prompts run near what memory gives: 77 rows of top-8 of 256 experts (FFN 512) on e4m3 rows, first bank, 46 us (260 MB of
+// weights at 5.6 TB/s; 44 with one product a step, ragged.hpp); of 128 experts, bf16, second bank, 65 us (400 MB at 6.1). A
+// line's experts are few bytes, and its time a launch and one round trip of loads: 8 pairs of the first bank 6.0 us (e2m1
+// weights, 13 MB, e4m3 rows; 4.4 with one product a step) and 11 us (bf16, 50 MB at 4.6 TB/s).
 #pragma once
 #include "ragged.hpp"
 
@@ -282,9 +282,9 @@ void launch_stream_out(const ExpertProduct& a, bool swiglu, bool out_bf16, int p
 // DEPTH for microscaled rows of fewer than 8 stages: no more loads than there are stages
 template <class F>
 void launch_gemv(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
-  // Few pairs, of which hardly two meet in an expert, read its weights once. Of 128 experts (e4m3 rows), us without / with: first
-  // bank 8 pairs 5.0 / 4.4, 16 7.1 / 6.8, 32 10.1 / 10.3, 128 30 / 34; second bank 16 pairs 5.5 / 5.0, 32 7.8 / 8.3; 40 of 256
-  // experts, second bank: 6.1 / 5.0.
+  // Few pairs, of which hardly two meet in an expert, read its weights once. Of 128 experts (e4m3 rows), us without / with:
+  // first bank 8 pairs 6.7 / 6.0, 16 9.4 / 8.9, 32 12.6 / 12.5, 64 20.0 / 21.4, 128 37.5 / 40.2; second bank 16 pairs 5.5 /
+  // 5.0, 32 7.8 / 8.3; 40 of 256 experts, second bank: 6.1 / 5.0.
   if constexpr (F::SCALED) {
     if ((int64_t)6 * a.pairs <= a.E) {
       if (a.stages >= 8) launch_stream_out<F, true, 1, 8, F::SEG, true>(a, swiglu, out_bf16, a.pairs, 1, s);
@@ -302,12 +302,13 @@ void launch_stream(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream
   const int passes = most_passes(a.pairs, a.n_groups, 16 * MT);
   // A workgroup finds its pass and copies the rows before it streams anything: with few stages to a column it takes some
   // columns in turn. Second bank of 128 experts (2048 x 768, e4m3), 256 rows: 32 us with two, 38 with one; first bank
-  // (8 stages): 51 with one, 53 with two.
+  // (8 stages): 58 with one, 59 with two.
   const int per = F::SCALED && a.stages < 6 ? 6 / a.stages : 1;
-  // Up to 16 rows an expert its weights go by in one pass, mostly: nontemporal, e2m1 where a column is long (first bank, 77
-  // rows of 256 experts 48.6 -> 44.4 us, 100 of 128 40.7 -> 36.1; second bank, 256 rows, Zipf: 32.0 -> 33.5, so not there), bf16
-  // (16 rows of 128 experts 103 -> 91 and 51 -> 43 us, 77 rows on the second bank 79 -> 68), and up to 32 rows bf16's long
-  // columns (256 rows of 128 experts 184 -> 163 us, Zipf 186 either way; second bank, 700 rows of 256 experts 134 -> 141).
+  // Up to 16 rows an expert its weights go by in one pass, mostly: nontemporal, e2m1 where a column is long (first bank, e4m3
+  // rows, 77 of 256 experts 53.8 -> 48.6 us, 100 of 128 42.8 -> 40.0; second bank, 256 rows, Zipf: 32.0 -> 33.5, so not
+  // there), bf16 (16 rows of 128 experts 103 -> 91 and 51 -> 43 us, 77 rows on the second bank 79 -> 68), and up to 32 rows
+  // bf16's long columns (256 rows of 128 experts 184 -> 163 us, Zipf 186 either way; second bank, 700 rows of 256 experts 134
+  // -> 141).
   constexpr bool LONG = SEG == F::SEG, ONCE = F::SCALED ? MT == 1 && LONG : MT == 1 || LONG;
   if constexpr (F::SCALED && SEG < F::SEG) {  // (second bank, 256 rows of 128 experts: 31.3 -> 29.2 us)
     if (a.stages == 3) return launch_stream_out<F, false, MT, 3, SEG, ONCE>(a, swiglu, out_bf16, passes, per, s);

@@ -7,12 +7,12 @@
 // the weights come from HBM and are copied by halves of a stage (a step), three (bf16: four) ahead, so that there are always
 // some on their way: with whole stages, one ahead, a stage of bf16 took 4200 clocks, of which the products take 2200.
 //
-// Bound by what comes from HBM and the memory-side cache (each XCD reads the rows of its experts for itself), the first
-// products of each workgroup and the epilogues beside it. 4096 rows, top-8 of 128 experts, first bank (FFN 768) with SwiGLU:
-// bf16 230 us, 0.96 GB read past the L2s and 50 MB written at 4.4 TB/s (10 us less with the products left out; the matrix units
-// work 47% of the time); e2m1 rows on e2m1 weights 81 us, 0.27 GB read and 50 MB written at 3.9 TB/s (34%). An e4m3 row
-// takes two products a step (ragged.hpp), and its passes of 160 rows read the weights twice as often: 214 us, 150 us on the
-// second bank.
+// Bound by what comes from HBM and the memory-side cache (each XCD reads the rows of its experts for itself), the 7 us until
+// a workgroup's first products and the epilogues (2 us an item) beside it. 4096 rows, top-8 of 128 experts, first bank (FFN 768)
+// with SwiGLU: bf16 228 us, 0.97 GB read past the L2s and 50 MB written at 4.5 TB/s (12% less with the products left out; the
+// matrix units work 51% of the time); e2m1 rows on e2m1 weights 80 us, 0.28 GB read and 50 MB written at 4.1 TB/s (29%; 35%).
+// An e4m3 row takes two products a step (ragged.hpp), and its passes of 160 rows read the weights twice as often: 215 us,
+// products before all (93 without them), 150 us on the second bank (124).
 #pragma once
 #include "expert_stream.hpp"
 
@@ -477,7 +477,7 @@ void launch_wide_of(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStrea
 
 // Where an expert's rows are one pass, mostly, its weights are read once: nontemporal. us without / with (first bank,
 // 128 experts): bf16 512 rows 191 / 182, 1024 197 / 193, 4096 247 / 242 and on the second bank 183 / 175; e4m3 1024 rows
-// 61 / 57; e2m1 4096 rows the same; bf16 rows of 13 passes an expert 193 / 201.
+// 84 / 83; e2m1 4096 rows the same; bf16 rows of 13 passes an expert 193 / 201.
 template <class F>
 void launch_wide(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
   if ((int64_t)a.pairs <= (int64_t)16 * wx_tiles<F>() * a.n_groups) launch_wide_of<F, true>(a, swiglu, out_bf16, s);
@@ -492,10 +492,11 @@ bool wide_fits(const ExpertProduct& a) {
 }
 
 // Wide passes, or streamed ones of 32 rows, or of 16, by the rows an expert has on average. Top-8 of 128 experts (FFN 768),
-// us with 16 / 32 / wide: first bank, e4m3 rows, 256 rows (16 to an expert) 54 / 46 / 52, 400 rows 67 / 50 / 53, 700 rows
-// 73 wide and 74 streamed (256 experts, Zipf); second bank 16 to an expert 31 / 36 / 43 (few stages: a 32-row pass has
-// less to stream than it takes to set up), 25 to an expert 40 / 41 / 42, 44 to an expert 60 streamed, 47 wide; bf16 first
-// bank 16 to an expert 196 / 164 / 190, 25: 238 / 174 / 192; second bank 16: 100 / 89 / 102.
+// us with 16 / 32 / wide: first bank, e4m3 rows, 150 rows (9 to an expert) 43 / 56 / 71, 256 rows 57 / 59 / 72 (Zipf 59 / 64
+// / 83), 300 rows 69 / 61 / 70, 400 rows 77 / 65 / 69, 500 rows 89 / 74 / 72, 1024 rows 139 / 114 / 83; second bank 16 to an
+// expert 31 / 36 / 43 (few stages: a 32-row pass has less to stream than it takes to set up), 25 to an expert 40 / 41 / 42,
+// 44 to an expert 60 streamed, 47 wide; bf16 first bank 16 to an expert 196 / 164 / 190, 25: 238 / 174 / 192; second bank 16:
+// 100 / 89 / 102.
 template <class F>
 void launch_grouped(const ExpertProduct& a, bool swiglu, bool out_bf16, hipStream_t s) {
   if (wide_fits<F>(a)) return launch_wide<F>(a, swiglu, out_bf16, s);

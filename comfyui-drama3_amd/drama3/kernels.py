@@ -661,8 +661,8 @@ def grouped_bf16(x, groups, weight, n, order=None, k=1, swiglu=False, dtype=torc
 
 
 # Rows up to which a layer's pairs read their experts one by one (gemv). Both products of 128 experts (e4m3 rows), us by lines /
-# by groups without the grouping's launch, which is 5: 4 rows 18 / 20, 8 rows 29 / 28, 16 rows 50 / 39; bf16 55 / 58, 104 / 99,
-# 188 / 132.
+# by groups without the grouping's launch, which is 5: 4 rows 20 / 23, 8 rows 32 / 29, 16 rows 55 / 43; bf16 57 / 58, 105 / 99,
+# 191 / 135.
 LINE_ROWS = 8
 # Pairs from which the grouping runs over many workgroups: one takes 1 ns a pair, the two launches of many about 8 us.
 GROUPING_PAIRS = 8192

@@ -2,7 +2,7 @@
 
 A microscaled row holds elements of 4 bits (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) or 8 (e4m3) with one
 power-of-two scale (e8m0) per 32 columns. MI355X multiplies both operands as they are stored, scales included, so a bank
-of e2m1 weights costs 17/32 byte a weight and no decoding:
+of e2m1 weights costs 17/32 byte a weight and no decoding. Sums are float32, also of results that are then rounded to bfloat16:
 
     gate_up, down = mx.quantize_bank(w_gate_up), mx.quantize_bank(w_down)   # [E, 2I, H], [E, H, I] float -> MxBank
     rows = mx.quantize(x, 8)                                                # [T, H] -> MxRows (e4m3; 4: e2m1)
