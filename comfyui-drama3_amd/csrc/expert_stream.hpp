@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(ST_THREADS, (st_waves<F, SEG, MT>()))
   __shared__ f32x4 other[2][GEMV && SWIGLU ? ST_THREADS / 64 : 1][4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, c = lane & 15;
-  const int strips = (columns + per - 1) / per, at = blockIdx.x / strips, column0 = (blockIdx.x % strips) * per;
+  const int at = blockIdx.y, column0 = blockIdx.x * per;
   Pass pass;
   int my_row;  // lane r: row r of the pass
   if constexpr (GEMV) {
@@ -263,12 +263,13 @@ int st_columns(int N) {
   return (N / 16 + per - 1) / per;
 }
 
+// (the passes along y: HIP launches nothing, without an error, where a dimension of the grid has 2^32 threads)
 template <class F, bool GEMV, bool SWIGLU, bool OUT_BF16, int NT, int MT, int DEPTH, int SEG, bool ONCE>
 void launch_stream_of(const ExpertProduct& a, int passes, int per, hipStream_t s) {
   const int columns = st_columns<GEMV, SWIGLU, NT>(a.N);
   per = per < columns ? per : columns;
   hipLaunchKernelGGL((expert_stream_kernel<F, GEMV, SWIGLU, OUT_BF16, NT, MT, DEPTH, SEG, ONCE>),
-                     dim3((unsigned)((columns + per - 1) / per * passes)), dim3(ST_THREADS), 0, s, a, columns, per);
+                     dim3((unsigned)((columns + per - 1) / per), (unsigned)passes), dim3(ST_THREADS), 0, s, a, columns, per);
 }
 
 template <class F, bool GEMV, int MT, int DEPTH, int SEG, bool ONCE>

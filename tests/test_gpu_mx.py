@@ -645,3 +645,31 @@ def test_rows_beyond_32_bit_offsets(fmt):
             assert many.x.codes.nbytes > 2 ** 32
         assert torch.equal(many.grouped(groups, order=R - last + pairs), want)
         del many
+
+
+@pytest.mark.parametrize("fmt, n, P", [("mx4", 16, 2 ** 24 + 16), ("bf16", 128, 2 ** 23 + 5)])
+def test_lines_of_more_than_2_32_threads(fmt, n, P):
+    """A gemv of more pairs than one dimension of a launch has threads for: all of them come out, as the first ones do."""
+    case = Case(fmt, 2, n, 64, 1)
+    ids = torch.arange(P, device=DEV) % 2
+    out = torch.full((P, n), float("nan"), dtype=torch.bfloat16, device=DEV)
+    case.gemv(ids, dtype=torch.bfloat16, out=out)
+    case.check(out[:2], torch.zeros(2, dtype=torch.int64, device=DEV), ids[:2])
+    for part in (out[:P // 2 * 2].view(-1, 2 * n), out[P - 2:][ids[P - 2:]].view(-1, 2 * n)):
+        assert torch.all(part == out[:2].view(-1))
+
+
+def test_groups_of_more_than_2_32_threads():
+    """The same of a grouped product: 2^24 and some passes of 32 rows."""
+    P, E = 2 ** 29 + 100, 7
+    case = Case("bf16", E, 16, 64, 1)
+    counts = torch.full((E,), P // E, dtype=torch.int64, device=DEV)
+    counts[-1] += P - int(counts.sum())
+    first = counts.cumsum(0) - counts
+    e = torch.arange(E, device=DEV)
+    groups = torch.stack((e, e, e * 0, first, counts), dim=1).to(torch.int32)
+    out = torch.full((P, 16), float("nan"), dtype=torch.bfloat16, device=DEV)
+    case.grouped(groups, order=torch.zeros(P, dtype=torch.int64, device=DEV), dtype=torch.bfloat16, out=out)
+    case.check(out[first], e * 0, e)
+    for g in range(E):
+        assert torch.all(out[first[g]:first[g] + counts[g]] == out[first[g]])
