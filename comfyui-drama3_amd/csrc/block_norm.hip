@@ -1,0 +1,410 @@
+// The end of one block and the start of the next, in one pass over the rows, and its backward pass:
+//
+//   v = y                            h = residual + scale gate v
+//   v = y rstd(y) post  (post given) n = h rstd(h) weight            rstd(z) = 1 / sqrt(mean(z^2) + eps)
+//
+// with post and weight read as 1 + w where they are kept as offsets. Sums, h inside the pass and all products are float32; h and
+// n are each rounded once, to the stream's and the block's type (n comes from h before its rounding).
+//
+// HBM-bound: a row is read once, held in registers through its sums, and written once. A lane takes 8 columns at a time;
+// 64, 256 or 1024 lanes a row, so that a lane holds at most 32 columns.
+//
+// Backward, for dh and dn (gradients of h and n), with z^ = z rstd(z) and m(z) the mean over a row:
+//   a = dn weight        dresidual = dh + rstd(h) (a - h^ m(a h^))        dv = scale dresidual
+//   dgate = dv v         b = dv gate post        dy = rstd(y) (b - y^ m(b y^))
+//   dweight = sum_t dn h^,  dpost = sum_t dv gate y^,  dgate summed over the columns (a gate per row) or rows (per channel)
+// Sums over the rows: a workgroup's lanes keep their columns' over the rows that it walks, and a second launch adds the
+// workgroups' in a fixed order, so they are the same bits from call to call.
+#include "common.hpp"
+#include "../../include/drama3_moe.h"
+
+#include <string>
+#include <type_traits>
+
+namespace d3 {
+int fail(const std::string& msg);
+int hip_fail(hipError_t err, const char* what);
+
+namespace {
+
+typedef d3_add_norm_desc Desc;
+struct bf16_t {
+  uint16_t bits;
+};
+// (rows may start at any element)
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// columns col .. col + 7 of a row as float (zeros past H), and back
+template <class T>
+D3_INLINE void load8(const T* row, int col, int H, float (&v)[8]) {
+  if (col + 8 <= H) {
+    if constexpr (std::is_same_v<T, bf16_t>) {
+      const u32x4_at2 w = *(const u32x4_at2*)(row + col);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    } else {
+      const f32x4_at4 a = *(const f32x4_at4*)(row + col), b = *(const f32x4_at4*)(row + col + 4);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      v[i] = 0.0f;
+      if (col + i < H) {
+        if constexpr (std::is_same_v<T, bf16_t>) v[i] = bf16_to_f32(row[col + i].bits);
+        else v[i] = row[col + i];
+      }
+    }
+  }
+}
+template <class T>
+D3_INLINE void store8(T* row, int col, int H, const float (&v)[8]) {
+  if (col + 8 <= H) {
+    if constexpr (std::is_same_v<T, bf16_t>) {
+      u32x4_at2 w;
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[i] = f32_to_bf16(v[2 * i]) | f32_to_bf16(v[2 * i + 1]) << 16;
+      *(u32x4_at2*)(row + col) = w;
+    } else {
+      *(f32x4_at4*)(row + col) = f32x4_at4{v[0], v[1], v[2], v[3]};
+      *(f32x4_at4*)(row + col + 4) = f32x4_at4{v[4], v[5], v[6], v[7]};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (col + i < H) {
+        if constexpr (std::is_same_v<T, bf16_t>) row[col + i].bits = (uint16_t)f32_to_bf16(v[i]);
+        else row[col + i] = v[i];
+      }
+    }
+  }
+}
+// the same of a norm's weight or a gate, whose type goes by the call (1: bf16, 0: float32)
+D3_INLINE void load8_of(const void* row, int type, int col, int H, float (&v)[8]) {
+  if (type) load8((const bf16_t*)row, col, H, v);
+  else load8((const float*)row, col, H, v);
+}
+D3_INLINE float load1_of(const void* p, int type, int64_t i) {
+  return type ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i];
+}
+
+// a row's sum over its LANES lanes, the same in all of them; `slot`: LDS of this sum alone until two barriers later
+template <int LANES>
+D3_INLINE float row_sum(float v, float* slot) {
+  v = wave_sum_f32(v);
+  if constexpr (LANES > 64) {
+    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = slot[0];
+#pragma unroll
+    for (int i = 1; i < LANES / 64; i++) v += slot[i];
+  }
+  return v;
+}
+
+constexpr int GATE_ROW = 1, GATE_CHANNEL = 2, GATE_FULL = 3;  // gate_kind; 0: none
+
+// the gate's values at a row's columns
+D3_INLINE void gate8(const Desc& d, int row, int col, float (&g)[8]) {
+  const int64_t at = d.gate_kind == GATE_CHANNEL ? 0 : (int64_t)row * d.gate_stride;
+  if (d.gate_kind == GATE_ROW) {
+    const float one = load1_of(d.gate, d.gate_type, at);
+#pragma unroll
+    for (int i = 0; i < 8; i++) g[i] = one;
+  } else {
+    load8_of((const uint8_t*)d.gate + at * (d.gate_type ? 2 : 4), d.gate_type, col, d.H, g);
+  }
+}
+
+// a norm's weight, as it multiplies
+D3_INLINE void weight8(const void* w, int type, int offset, int col, int H, float (&v)[8]) {
+  load8_of(w, type, col, H, v);
+  if (offset) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] += 1.0f;
+  }
+}
+
+// LANES lanes a row, CH times 8 columns a lane
+template <class TY, class TS, int LANES, int CH>
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) add_norm_kernel(Desc d) {
+  constexpr int ROWS = LANES < 256 ? 256 / LANES : 1;
+  __shared__ float slots[2][LANES / 64];
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
+  if (row >= d.T) return;  // (whole waves, and then without barriers)
+  float h[CH][8], w[CH][8];
+#pragma unroll
+  for (int j = 0; j < CH; j++) load8((const TS*)d.residual + row * d.residual_stride, 8 * (lane + LANES * j), d.H, h[j]);
+  if (d.weight) {  // (on its way during the sums)
+#pragma unroll
+    for (int j = 0; j < CH; j++) weight8(d.weight, d.weight_type, d.unit_offset, 8 * (lane + LANES * j), d.H, w[j]);
+  }
+  if (d.y) {
+    float v[CH][8];
+#pragma unroll
+    for (int j = 0; j < CH; j++) load8((const TY*)d.y + row * d.y_stride, 8 * (lane + LANES * j), d.H, v[j]);
+    if (d.post) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < CH; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum += v[j][i] * v[j][i];
+      const float rstd = rsqrtf(row_sum<LANES>(sum, slots[0]) / (float)d.H + d.eps);
+      if (d.rstd && lane == 0) d.rstd[d.T + row] = rstd;
+#pragma unroll
+      for (int j = 0; j < CH; j++) {
+        float p[8];
+        weight8(d.post, d.post_type, d.unit_offset, 8 * (lane + LANES * j), d.H, p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[j][i] *= rstd * p[i];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < CH; j++) {
+      float g[8] = {1, 1, 1, 1, 1, 1, 1, 1};
+      if (d.gate_kind) gate8(d, (int)row, 8 * (lane + LANES * j), g);
+#pragma unroll
+      for (int i = 0; i < 8; i++) h[j][i] += d.scale * (g[i] * v[j][i]);
+      if (d.h) store8((TS*)d.h + row * d.H, 8 * (lane + LANES * j), d.H, h[j]);
+    }
+  }
+  if (!d.weight) return;
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < CH; j++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum += h[j][i] * h[j][i];
+  const float rstd = rsqrtf(row_sum<LANES>(sum, slots[1]) / (float)d.H + d.eps);
+  if (d.rstd && lane == 0) d.rstd[row] = rstd;
+#pragma unroll
+  for (int j = 0; j < CH; j++) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[j][i] *= h[j][i] * rstd;
+    store8((TY*)d.n + row * d.H, 8 * (lane + LANES * j), d.H, w[j]);
+  }
+}
+
+template <class TY, class TS, int LANES, int CH>
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) add_norm_backward_kernel(Desc d, int groups) {
+  constexpr int ROWS = LANES < 256 ? 256 / LANES : 1;
+  __shared__ float slots[2][3][LANES / 64];
+  const int lane = threadIdx.x % LANES, group = blockIdx.x * ROWS + threadIdx.x / LANES;
+  if (group >= groups) return;  // (whole waves, and then without barriers)
+  float sum_w[CH][8] = {}, sum_p[CH][8] = {}, sum_g[CH][8] = {};
+  int turn = 0;
+  for (int64_t row = group; row < d.T; row += groups, turn ^= 1) {
+    float dr[CH][8], v[CH][8];
+#pragma unroll
+    for (int j = 0; j < CH; j++) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) dr[j][i] = 0.0f;
+      if (d.dh) load8((const TS*)d.dh + row * d.H, 8 * (lane + LANES * j), d.H, dr[j]);
+      if (d.y) load8((const TY*)d.y + row * d.y_stride, 8 * (lane + LANES * j), d.H, v[j]);
+    }
+    if (d.dn) {
+      float a[CH][8], hat[CH][8], sum = 0.0f;
+      const float rstd = d.rstd[row];
+#pragma unroll
+      for (int j = 0; j < CH; j++) {
+        float w[8];
+        load8((const TY*)d.dn + row * d.H, 8 * (lane + LANES * j), d.H, a[j]);
+        load8((const TS*)d.h + row * d.residual_stride, 8 * (lane + LANES * j), d.H, hat[j]);
+        weight8(d.weight, d.weight_type, d.unit_offset, 8 * (lane + LANES * j), d.H, w);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          hat[j][i] *= rstd;
+          sum_w[j][i] += a[j][i] * hat[j][i];
+          a[j][i] *= w[i];
+          sum += a[j][i] * hat[j][i];
+        }
+      }
+      const float mean = row_sum<LANES>(sum, slots[turn][0]) / (float)d.H;
+#pragma unroll
+      for (int j = 0; j < CH; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) dr[j][i] += rstd * (a[j][i] - hat[j][i] * mean);
+    }
+#pragma unroll
+    for (int j = 0; j < CH; j++)
+      if (d.dresidual) store8((TS*)d.dresidual + row * d.H, 8 * (lane + LANES * j), d.H, dr[j]);
+    if (!d.y || !(d.dy || d.dpost || d.dgate)) continue;
+    const float rstd = d.post ? d.rstd[d.T + row] : 1.0f;
+    float sum_row = 0.0f, sum_b = 0.0f;
+#pragma unroll
+    for (int j = 0; j < CH; j++) {
+      const int col = 8 * (lane + LANES * j);
+      float p[8] = {1, 1, 1, 1, 1, 1, 1, 1}, g[8] = {1, 1, 1, 1, 1, 1, 1, 1}, full[8];
+      if (d.post) weight8(d.post, d.post_type, d.unit_offset, col, d.H, p);
+      if (d.gate_kind) gate8(d, (int)row, col, g);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float dv = d.scale * dr[j][i];
+        if (d.post) v[j][i] *= rstd;  // y^
+        full[i] = dv * (v[j][i] * p[i]);
+        sum_g[j][i] += full[i];
+        sum_row += full[i];
+        const float dnormed = dv * g[i];
+        sum_p[j][i] += dnormed * v[j][i];
+        dr[j][i] = dnormed * p[i];  // b
+        sum_b += dr[j][i] * v[j][i];
+      }
+      if (d.dgate && d.gate_kind == GATE_FULL) {
+        if (d.gate_type) store8((bf16_t*)d.dgate + row * d.H, col, d.H, full);
+        else store8((float*)d.dgate + row * d.H, col, d.H, full);
+      }
+    }
+    if (d.dgate && d.gate_kind == GATE_ROW) {
+      sum_row = row_sum<LANES>(sum_row, slots[turn][1]);
+      if (lane == 0) {
+        if (d.gate_type) ((uint16_t*)d.dgate)[row] = (uint16_t)f32_to_bf16(sum_row);
+        else ((float*)d.dgate)[row] = sum_row;
+      }
+    }
+    if (!d.dy) continue;
+    if (d.post) {
+      const float mean = row_sum<LANES>(sum_b, slots[turn][2]) / (float)d.H;
+#pragma unroll
+      for (int j = 0; j < CH; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) dr[j][i] = rstd * (dr[j][i] - v[j][i] * mean);
+    }
+#pragma unroll
+    for (int j = 0; j < CH; j++) store8((TY*)d.dy + row * d.H, 8 * (lane + LANES * j), d.H, dr[j]);
+  }
+  float* part = d.partials + (int64_t)group * d.H;
+  const int64_t step = (int64_t)groups * d.H;
+#pragma unroll
+  for (int j = 0; j < CH; j++) {
+    const int col = 8 * (lane + LANES * j);
+    float* to = part;
+    if (d.dweight) store8(to, col, d.H, sum_w[j]), to += step;
+    if (d.dpost) store8(to, col, d.H, sum_p[j]), to += step;
+    if (d.dgate && d.gate_kind == GATE_CHANNEL) store8(to, col, d.H, sum_g[j]);
+  }
+}
+
+// the workgroups' sums over the rows added up: 64 columns a workgroup, 16 waves of which each adds every 16th group
+struct Sums {
+  void* out[3];
+  int type[3];
+};
+__global__ void __launch_bounds__(1024) add_groups_kernel(const float* partials, int groups, int H, Sums s) {
+  __shared__ float part[16][64];
+  const int col = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const float* from = partials + (int64_t)blockIdx.y * groups * H;
+  float sum = 0.0f;
+  if (col < H) {
+#pragma unroll 8
+    for (int g = w; g < groups; g += 16) sum += from[(int64_t)g * H + col];
+  }
+  part[w][threadIdx.x & 63] = sum;
+  __syncthreads();
+  if (w || col >= H) return;
+  for (int i = 1; i < 16; i++) sum += part[i][threadIdx.x];
+  if (s.type[blockIdx.y]) ((uint16_t*)s.out[blockIdx.y])[col] = (uint16_t)f32_to_bf16(sum);
+  else ((float*)s.out[blockIdx.y])[col] = sum;
+}
+
+constexpr int MAX_H = 16384;
+
+// f(lanes, chunks) for rows of H columns, chunks of 8 to a lane
+template <class F>
+void by_width(int H, F f) {
+  const int units = (H + 7) / 8;
+  using std::integral_constant;
+  if (units <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (units <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (units <= 256) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (units <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  else if (units <= 1024) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+  else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+}
+template <class F>
+void by_types(const Desc& d, F f) {
+  if (d.y_type) {
+    if (d.stream_type) f(bf16_t{}, bf16_t{});
+    else f(bf16_t{}, float{});
+  } else {
+    if (d.stream_type) f(float{}, bf16_t{});
+    else f(float{}, float{});
+  }
+}
+
+int rows_of(int H) { return (H + 7) / 8 <= 128 ? 4 : 1; }
+
+// groups of rows whose sums over the rows a backward pass keeps apart
+int groups_of(int T, int H) {
+  const int most = 1024;
+  return T < most ? T : most;
+}
+
+int check(const char* what, const Desc* d) {
+  const std::string at = what;
+  if (!d) return fail(at + ": null descriptor");
+  if (d->T < 0 || d->H < 1 || d->H > MAX_H) return fail(at + ": H must be 1 to 16384, T not negative");
+  if ((d->y_type | d->stream_type | d->weight_type | d->post_type | d->gate_type) & ~1) return fail(at + ": types are 0 (float32) or 1 (bf16)");
+  if (d->gate_kind < 0 || d->gate_kind > 3 || (d->gate_kind && !d->gate)) return fail(at + ": gate_kind is 0 to 3, with a gate from 1 on");
+  if (d->T > 0 && (d->post || d->gate_kind) && !d->y) return fail(at + ": post and gate go with y");
+  return 0;
+}
+
+}  // namespace
+}  // namespace d3
+
+using namespace d3;
+
+extern "C" int64_t d3_add_norm_partials(int32_t T, int32_t H) {
+  if (T < 0 || H < 1) return 0;
+  return 3 * (int64_t)groups_of(T, H) * H;
+}
+
+extern "C" int d3_add_norm(const d3_add_norm_desc* desc, void* stream) {
+  if (const int rc = check("d3_add_norm", desc)) return rc;
+  const Desc& d = *desc;
+  if (d.T == 0) return 0;
+  if (!d.residual || (d.y && !d.h) || (d.weight && !d.n) || !(d.y || d.weight)) return fail("d3_add_norm: null pointer");
+  by_types(d, [&](auto y, auto s) {
+    by_width(d.H, [&](auto lanes, auto chunks) {
+      constexpr int L = decltype(lanes)::value, rows = L < 256 ? 256 / L : 1;
+      add_norm_kernel<decltype(y), decltype(s), L, decltype(chunks)::value>
+          <<<(unsigned)(((int64_t)d.T + rows - 1) / rows), L < 256 ? 256 : L, 0, (hipStream_t)stream>>>(d);
+    });
+  });
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : hip_fail(e, "d3_add_norm launch");
+}
+
+extern "C" int d3_add_norm_backward(const d3_add_norm_desc* desc, void* stream) {
+  if (const int rc = check("d3_add_norm_backward", desc)) return rc;
+  const Desc& d = *desc;
+  if ((d.dn || d.dweight) && !d.weight) return fail("d3_add_norm_backward: dn and dweight go with weight");
+  if ((d.dpost && !d.post) || (d.dgate && !d.gate_kind) || (d.dy && !d.y))
+    return fail("d3_add_norm_backward: dpost, dgate and dy go with post, gate and y");
+  const int parts = !!d.dweight + !!d.dpost + (d.dgate && d.gate_kind == GATE_CHANNEL);
+  const int groups = groups_of(d.T, d.H);
+  if (d.T > 0) {
+    if (!(d.dh || d.dn) || (d.dn && (!d.h || !d.rstd)) || (d.post && !d.rstd)) return fail("d3_add_norm_backward: null pointer");
+    if (parts && (!d.partials || d.partials_floats < (int64_t)parts * groups * d.H))
+      return fail("d3_add_norm_backward: partials too small (d3_add_norm_partials)");
+    by_types(d, [&](auto y, auto s) {
+      by_width(d.H, [&](auto lanes, auto chunks) {
+        constexpr int L = decltype(lanes)::value, rows = L < 256 ? 256 / L : 1;
+        add_norm_backward_kernel<decltype(y), decltype(s), L, decltype(chunks)::value>
+            <<<(groups + rows - 1) / rows, L < 256 ? 256 : L, 0, (hipStream_t)stream>>>(d, groups);
+      });
+    });
+  }
+  if (parts) {
+    Sums sums{};
+    int i = 0;
+    if (d.dweight) sums.out[i] = d.dweight, sums.type[i++] = d.weight_type;
+    if (d.dpost) sums.out[i] = d.dpost, sums.type[i++] = d.post_type;
+    if (d.dgate && d.gate_kind == GATE_CHANNEL) sums.out[i] = d.dgate, sums.type[i++] = d.gate_type;
+    add_groups_kernel<<<dim3((d.H + 63) / 64, parts), 1024, 0, (hipStream_t)stream>>>(d.partials, groups, d.H, sums);
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : hip_fail(e, "d3_add_norm_backward launch");
+}

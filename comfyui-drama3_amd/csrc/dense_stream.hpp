@@ -1,0 +1,151 @@
+// Dense products of few rows: the weights stream from memory straight into the matrix instruction's operands. A workgroup
+// takes 16 weight rows (with SwiGLU 8 units, gate and up rows by turns) against 16, 32 or 64 rows of x; its 8 waves each
+// take an eighth of K and the sums are added in LDS, so that even the narrow weights of one shared expert (64 workgroups)
+// come in one round of loads a wave.
+#pragma once
+#include "dense_tile.hpp"
+
+namespace d3 {
+
+constexpr int ST_WAVES = 8, ST_THREADS = 64 * ST_WAVES, ST_AT_ONCE = 4;  // stages of 64 k whose loads a wave sends together
+
+// this wave's part of the sums of 16 weight rows (lane's own at w) with 16 RT rows of x (lane's own at x[t])
+template <int RT>
+D3_INLINE void stream_sums(const uint16_t* w, const uint16_t* const (&x)[RT], int K, int wave, f32x4 (&acc)[RT]) {
+  const int q = (threadIdx.x & 63) >> 4, stages = (K + 63) / 64;
+  const int first = stages * wave / ST_WAVES, last = stages * (wave + 1) / ST_WAVES;
+#pragma unroll
+  for (int t = 0; t < RT; t++) acc[t] = f32x4{0, 0, 0, 0};
+  int s = first;
+  for (; s + ST_AT_ONCE <= last && (s + ST_AT_ONCE) * 64 <= K; s += ST_AT_ONCE) {
+    i32x4 wv[2 * ST_AT_ONCE], xv[RT][2 * ST_AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < 2 * ST_AT_ONCE; i++) wv[i] = *(const i32x4*)(w + s * 64 + i * 32 + 8 * q);
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+      for (int i = 0; i < 2 * ST_AT_ONCE; i++) xv[t][i] = *(const i32x4*)(x[t] + s * 64 + i * 32 + 8 * q);
+#pragma unroll
+    for (int i = 0; i < 2 * ST_AT_ONCE; i++)
+#pragma unroll
+      for (int t = 0; t < RT; t++) acc[t] = mfma_bf16(wv[i], xv[t][i], acc[t]);
+  }
+  for (; s < last; s++) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int k = s * 64 + i * 32 + 8 * q;
+      i32x4 wv{0, 0, 0, 0}, xv[RT];
+      if (k < K) wv = *(const i32x4*)(w + k);
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        xv[t] = i32x4{0, 0, 0, 0};
+        if (k < K) xv[t] = *(const i32x4*)(x[t] + k);
+      }
+#pragma unroll
+      for (int t = 0; t < RT; t++) acc[t] = mfma_bf16(wv, xv[t], acc[t]);
+    }
+  }
+}
+
+// the waves' parts added up, in their order: wave t < RT returns tile t's
+template <int RT>
+D3_INLINE f32x4 join_waves(f32x4 (*part)[RT][64], const f32x4 (&acc)[RT], int wave) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int t = 0; t < RT; t++) part[wave][t][lane] = acc[t];
+  __syncthreads();
+  f32x4 sum{0, 0, 0, 0};
+  if (wave < RT) {
+    sum = part[0][wave][lane];
+#pragma unroll
+    for (int i = 1; i < ST_WAVES; i++) sum += part[i][wave][lane];
+  }
+  return sum;
+}
+
+template <int RT, int END, bool LORA>
+__global__ void __launch_bounds__(ST_THREADS) dense_stream_kernel(Dense a) {
+  __shared__ f32x4 part[ST_WAVES][RT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c = lane & 15;
+  const int m0 = blockIdx.y * (16 * RT), n0 = blockIdx.x * (END == END_SWIGLU ? 8 : 16);
+  const int n = END == END_SWIGLU ? n0 + (c >> 1) + (c & 1) * a.half : min(n0 + c, a.N - 1);
+  const uint16_t* x[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) x[t] = a.x + min(m0 + 16 * t + c, a.M - 1) * a.ldx;
+  f32x4 acc[RT];
+  stream_sums<RT>(a.w + n * a.ldw, x, a.K, wave, acc);
+  if constexpr (LORA) {
+    // the rows' adapters, an eighth of them to each wave: lane l has row l's
+    const int m = m0 + lane;
+    const int64_t id = lane < 16 * RT && m < a.M ? a.ids[m] : -1;
+    uint64_t open = __ballot(id >= 0 && id < a.adapters);
+    for (int i = 0; open; i++) {
+      const int leader = __ffsll((unsigned long long)open) - 1;
+      const int64_t now = __shfl(id, leader);
+      const uint64_t rows = __ballot(id == now);
+      open &= ~rows;
+      if (i % ST_WAVES != wave) continue;
+      const uint16_t* b = a.b + ((size_t)now * a.N + n) * a.rank;
+      for (int r = 8 * q; r - 8 * q < a.rank; r += 32) {
+        i32x4 bv{0, 0, 0, 0}, pv[RT];
+        if (r < a.rank) bv = *(const i32x4*)(b + r);
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+          pv[t] = i32x4{0, 0, 0, 0};
+          if ((rows >> (16 * t + c) & 1) && r < a.rank) pv[t] = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + c) * a.rank + r);
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+          // (the other rows keep their sums, also where this adapter holds infinities or NaN)
+          const f32x4 with = mfma_bf16(bv, pv[t], acc[t]);
+          acc[t] = rows >> (16 * t + c) & 1 ? with : acc[t];
+        }
+      }
+    }
+  }
+  const f32x4 v = join_waves<RT>(part, acc, wave);
+  const int m = m0 + 16 * wave + c;
+  if (wave >= RT || m >= a.M) return;
+  if constexpr (END == END_SWIGLU) {
+    // results 4 q .. 4 q + 3: gate and up of units n0 + 2 q and n0 + 2 q + 1
+    const int u = n0 + 2 * q;
+    if (a.pre) {
+      *(f32x2*)(a.pre + (size_t)m * 2 * a.half + u) = f32x2{v[0], v[2]};
+      *(f32x2*)(a.pre + (size_t)m * 2 * a.half + a.half + u) = f32x2{v[1], v[3]};
+    }
+    const f32x4 h{v[0] * sigmoid(v[0]) * v[1], v[2] * sigmoid(v[2]) * v[3], 0, 0};
+    *(int*)(a.out + m * a.ldo + u) = round4(h)[0];
+  } else {
+    if (n0 + 4 * q < a.N) *(i32x2*)(a.out + m * a.ldo + n0 + 4 * q) = round4(v);
+  }
+}
+
+// p[m, r] = alpha[a] sum_k x[m, k] A[a, r, k] for the adapter a of each row m, rounded to bf16 (the operand of the second product:
+// a relative 2^-9 of what the adapter adds). A workgroup takes 16 ranks and 16 RT rows, one adapter that they name
+// after the other (blockIdx.z of them at the start, gridDim.z apart); rows without one are not written, nor read later.
+template <int RT>
+__global__ void __launch_bounds__(ST_THREADS) lora_inner_kernel(const uint16_t* x, int64_t ldx, const uint16_t* A, const float* alpha,
+                                                                const int64_t* ids, int M, int K, int rank, int adapters, uint16_t* p) {
+  __shared__ f32x4 part[ST_WAVES][RT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c = lane & 15;
+  const int m0 = blockIdx.y * (16 * RT), r0 = blockIdx.x * 16;
+  const int64_t id = lane < 16 * RT && m0 + lane < M ? ids[m0 + lane] : -1;
+  uint64_t open = __ballot(id >= 0 && id < adapters);
+  const uint16_t* xr[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) xr[t] = x + min(m0 + 16 * t + c, M - 1) * ldx;
+  for (int i = 0; open; i++) {
+    const int64_t now = __shfl(id, __ffsll((unsigned long long)open) - 1);
+    const uint64_t rows = __ballot(id == now);
+    open &= ~rows;
+    if (i % (int)gridDim.z != (int)blockIdx.z) continue;
+    f32x4 acc[RT];
+    stream_sums<RT>(A + ((size_t)now * rank + min(r0 + c, rank - 1)) * K, xr, K, wave, acc);
+    const f32x4 v = join_waves<RT>(part, acc, wave) * alpha[now];
+    if (wave < RT && (rows >> (16 * wave + c) & 1) && r0 + 4 * q < rank)
+      *(i32x2*)(p + (size_t)(m0 + 16 * wave + c) * rank + r0 + 4 * q) = round4(v);
+    __syncthreads();  // (the sums are read: the next adapter's may take their place)
+  }
+}
+
+}  // namespace d3

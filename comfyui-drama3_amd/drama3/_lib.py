@@ -44,6 +44,37 @@ class MoeA8PrefillDesc(ctypes.Structure):
     ]
 
 
+class AddNormDesc(ctypes.Structure):
+    """d3_add_norm_desc (include/drama3_moe.h)."""
+    _fields_ = [
+        ("y", c_void_p), ("residual", c_void_p), ("weight", c_void_p), ("post", c_void_p), ("gate", c_void_p),
+        ("dh", c_void_p), ("dn", c_void_p), ("h", c_void_p), ("n", c_void_p), ("rstd", c_void_p), ("dy", c_void_p),
+        ("dresidual", c_void_p), ("dweight", c_void_p), ("dpost", c_void_p), ("dgate", c_void_p), ("partials", c_void_p),
+        ("partials_floats", c_int64), ("y_stride", c_int64), ("residual_stride", c_int64), ("gate_stride", c_int64),
+        ("y_type", c_int32), ("stream_type", c_int32), ("weight_type", c_int32), ("post_type", c_int32),
+        ("gate_type", c_int32), ("gate_kind", c_int32), ("T", c_int32), ("H", c_int32), ("scale", ctypes.c_float),
+        ("eps", ctypes.c_float), ("unit_offset", c_int32),
+    ]
+
+
+class DenseDesc(ctypes.Structure):
+    """d3_dense_desc (include/drama3_moe.h)."""
+    _fields_ = [
+        ("x", c_void_p), ("w", c_void_p), ("out", c_void_p), ("pre", c_void_p), ("a", c_void_p), ("b", c_void_p),
+        ("alpha", c_void_p), ("ids", c_void_p), ("inner", c_void_p), ("x_stride", c_int64), ("T", c_int32), ("N", c_int32),
+        ("K", c_int32), ("swiglu", c_int32), ("rank", c_int32), ("adapters", c_int32),
+    ]
+
+
+class GatedFfnBackwardDesc(ctypes.Structure):
+    """d3_gated_ffn_backward_desc (include/drama3_moe.h)."""
+    _fields_ = [
+        ("dout", c_void_p), ("x", c_void_p), ("gate_up", c_void_p), ("down", c_void_p), ("pre", c_void_p),
+        ("hidden", c_void_p), ("dgate_up_rows", c_void_p), ("dx", c_void_p), ("dgate_up", c_void_p), ("ddown", c_void_p),
+        ("x_stride", c_int64), ("T", c_int32), ("H", c_int32), ("I", c_int32), ("O", c_int32),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "d3_last_error": (ctypes.c_char_p, []),
@@ -131,6 +162,11 @@ SIGNATURES = {
                                c_int32, c_void_p, c_void_p]),
     "d3_bf16_grouped": (c_int32, [c_void_p, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_int32,
                                   c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
+    "d3_add_norm_partials": (c_int64, [c_int32, c_int32]),
+    "d3_add_norm": (c_int32, [ctypes.POINTER(AddNormDesc), c_void_p]),
+    "d3_add_norm_backward": (c_int32, [ctypes.POINTER(AddNormDesc), c_void_p]),
+    "d3_dense": (c_int32, [ctypes.POINTER(DenseDesc), c_void_p]),
+    "d3_gated_ffn_backward": (c_int32, [ctypes.POINTER(GatedFfnBackwardDesc), c_void_p]),
     "d3_await_cpu": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32,
                                c_void_p]),
 }

@@ -441,6 +441,105 @@ int d3_bf16_grouped(const void* x, int32_t rows, const int64_t* order, int32_t k
                     int32_t n_groups, const void* w, int32_t E, int32_t N, int32_t K, int32_t swiglu, int32_t out_bf16,
                     void* out, void* stream);
 
+/* ---- Around the routed experts, on unquantized weights (no counterpart in the reference) ----------------------------
+ * The end of one block and the start of the next, for rows [T, H], H up to 16384:
+ *   v = y, or y rstd(y) post with post     h = residual + scale gate v     n = h rstd(h) weight
+ *   rstd(z) = 1 / sqrt(mean(z^2) + eps); post and weight read as 1 + w with unit_offset.
+ * Types are 0 (float32) or 1 (bf16): h, residual and their gradients have stream_type, y, n and theirs y_type. gate_kind: 0
+ * none, 1 a value per row (gate[t * gate_stride]), 2 per channel, 3 per element (rows gate_stride apart). Rows of y and
+ * residual are their strides apart (elements), all others H. Float32 inside; n comes from h before h is rounded.
+ *   d3_add_norm: h (with y; without, h is residual and is not written) and n (with weight). rstd [2, T] may be NULL:
+ *     rstd(h), and rstd(y) with post.
+ *   d3_add_norm_backward: from dh and dn (either may be NULL: zero), y, h (rows residual_stride apart) and rstd as the
+ *     forward call left them: dy, dresidual, dweight, dpost, dgate, each where it is not NULL, of its input's type and
+ *     shape. partials: d3_add_norm_partials(T, H) floats, need no clearing. Sums over the rows are made in a fixed order.
+ *     T = 0 gives zeros. */
+typedef struct d3_add_norm_desc {
+  const void* y;
+  const void* residual;
+  const void* weight;
+  const void* post;
+  const void* gate;
+  const void* dh;
+  const void* dn;
+  void* h;
+  void* n;
+  float* rstd;
+  void* dy;
+  void* dresidual;
+  void* dweight;
+  void* dpost;
+  void* dgate;
+  float* partials;
+  int64_t partials_floats;
+  int64_t y_stride;
+  int64_t residual_stride;
+  int64_t gate_stride;
+  int32_t y_type;
+  int32_t stream_type;
+  int32_t weight_type;
+  int32_t post_type;
+  int32_t gate_type;
+  int32_t gate_kind;
+  int32_t T;
+  int32_t H;
+  float scale;
+  float eps;
+  int32_t unit_offset;
+} d3_add_norm_desc;
+int64_t d3_add_norm_partials(int32_t T, int32_t H);
+int d3_add_norm(const d3_add_norm_desc* desc, void* stream);
+int d3_add_norm_backward(const d3_add_norm_desc* desc, void* stream);
+
+/* Dense products of bf16 rows x [T, K] (x_stride elements apart) with bf16 weights w [N, K], float32 sums: out [T, N] bf16; with
+ * swiglu (N / 2 gate rows, then as many up rows) out [T, N / 2] = SiLU(gate) * up, and pre [T, N] float32 = gate and up where
+ * it is not NULL. K, N (swiglu: N / 2) and x_stride multiples of 8, rows 16-byte aligned.
+ * With adapters > 0 every row has its adapter's low-rank product added before anything else: alpha[i] (x[t] a[i]^T) b[i]^T,
+ * i = ids[t] (int64; a row with an id outside [0, adapters) has none), a [adapters, rank, K] and b [adapters, N, rank]
+ * bf16, alpha [adapters] float32, rank a multiple of 8; inner [T, rank] bf16 is workspace that needs no clearing. */
+typedef struct d3_dense_desc {
+  const void* x;
+  const void* w;
+  void* out;
+  float* pre;
+  const void* a;
+  const void* b;
+  const float* alpha;
+  const int64_t* ids;
+  void* inner;
+  int64_t x_stride;
+  int32_t T;
+  int32_t N;
+  int32_t K;
+  int32_t swiglu;
+  int32_t rank;
+  int32_t adapters;
+} d3_dense_desc;
+int d3_dense(const d3_dense_desc* desc, void* stream);
+
+/* Gradients of out = down(SiLU(gate) * up), (gate, up) = x gate_up^T, for rows x [T, H], gate_up [2 I, H] and down [O, I], from
+ * dout [T, O] (all bf16) and what d3_dense left: pre [T, 2 I] float32 and hidden [T, I] = SiLU(gate) * up. dgate_up_rows [T, 2 I]
+ * bf16 is workspace: the gradients of gate and up. dx [T, H], dgate_up [2 I, H] and ddown [O, I] bf16, each where it is not
+ * NULL. H, I, O multiples of 8. T = 0 writes nothing. */
+typedef struct d3_gated_ffn_backward_desc {
+  const void* dout;
+  const void* x;
+  const void* gate_up;
+  const void* down;
+  const float* pre;
+  const void* hidden;
+  void* dgate_up_rows;
+  void* dx;
+  void* dgate_up;
+  void* ddown;
+  int64_t x_stride;
+  int32_t T;
+  int32_t H;
+  int32_t I;
+  int32_t O;
+} d3_gated_ffn_backward_desc;
+int d3_gated_ffn_backward(const d3_gated_ffn_backward_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

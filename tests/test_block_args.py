@@ -1,0 +1,193 @@
+"""Argument checks of drama3.block that run before any launch (no GPU needed), and of its C entries and descriptors."""
+import ctypes
+import pathlib
+import subprocess
+
+import pytest
+import torch
+
+from drama3 import _lib, block
+
+BF, F32 = torch.bfloat16, torch.float32
+HEADER = pathlib.Path(__file__).resolve().parents[1] / "include" / "drama3_moe.h"
+
+
+def z(*shape, dtype=BF):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("error, match, call", [
+    (TypeError, "x .T, K. bfloat16", lambda: block.gated_ffn(z(2, 16, dtype=F32), z(32, 16), z(16, 16))),
+    (TypeError, "x .T, K. bfloat16", lambda: block.gated_ffn(z(2, 2, 16), z(32, 16), z(16, 16))),
+    (ValueError, "multiple of 8 columns", lambda: block.gated_ffn(z(2, 20), z(32, 20), z(16, 16))),
+    (ValueError, "gate_up", lambda: block.gated_ffn(z(2, 16), z(32, 24), z(16, 16))),
+    (TypeError, "gate_up bfloat16", lambda: block.gated_ffn(z(2, 16), z(32, 16, dtype=F32), z(16, 16))),
+    (ValueError, "multiples of 8 each", lambda: block.gated_ffn(z(2, 16), z(24, 16), z(16, 8))),
+    (ValueError, "down", lambda: block.gated_ffn(z(2, 16), z(32, 16), z(16, 32))),
+    (ValueError, "down", lambda: block.gated_ffn(z(2, 16), z(32, 16), z(12, 16))),
+    (ValueError, "ids go with", lambda: block.gated_ffn(z(2, 16), z(32, 16), z(16, 16), ids=torch.zeros(2, dtype=torch.int64))),
+    (ValueError, "on a GPU", lambda: block.gated_ffn(z(2, 16), z(32, 16), z(16, 16))),
+    (ValueError, "dout", lambda: block.gated_ffn_backward(z(2, 24), z(2, 16), z(32, 16), z(16, 16), (z(2, 32, dtype=F32), z(2, 16)))),
+    (ValueError, "dout", lambda: block.gated_ffn_backward(z(3, 16), z(2, 16), z(32, 16), z(16, 16), (z(2, 32, dtype=F32), z(2, 16)))),
+    (ValueError, "saved", lambda: block.gated_ffn_backward(z(2, 16), z(2, 16), z(32, 16), z(16, 16), (z(2, 32), z(2, 16)))),
+    (ValueError, "saved", lambda: block.gated_ffn_backward(z(2, 16), z(2, 16), z(32, 16), z(16, 16), (z(1, 32, dtype=F32), z(2, 16)))),
+])
+def test_gated_ffn_refusals(error, match, call):
+    with pytest.raises(error, match=match):
+        call()
+
+
+def lora(T=2, K=16, N=24, rank=8, count=3, **changed):
+    args = {"x": z(T, K), "weight": z(N, K), "a": z(count, rank, K), "b": z(count, N, rank), "alpha": z(count, dtype=F32),
+            "ids": torch.zeros(T, dtype=torch.int64)}
+    return block.lora_linear(**{**args, **changed})
+
+
+@pytest.mark.parametrize("error, match, changed", [
+    (ValueError, "rank a multiple of 8", {"a": z(3, 12, 16), "b": z(3, 24, 12)}),
+    (ValueError, "adapters a", {"a": z(3, 8, 24)}),
+    (ValueError, "adapters a", {"b": z(2, 24, 8)}),
+    (TypeError, "adapters a", {"a": z(3, 8, 16, dtype=F32)}),
+    (ValueError, "alpha", {"alpha": z(3)}),
+    (ValueError, "alpha", {"alpha": z(4, dtype=F32)}),
+    (ValueError, "ids", {"ids": torch.zeros(2, dtype=torch.int32)}),
+    (ValueError, "ids", {"ids": torch.zeros(3, dtype=torch.int64)}),
+    (ValueError, "ids", {"ids": None}),
+    (ValueError, "weight", {"weight": z(24, 24)}),
+    (RuntimeError, "no backward", {"a": z(3, 8, 16).requires_grad_()}),
+    (ValueError, "on a GPU", {}),
+])
+def test_lora_linear_refusals(error, match, changed):
+    with pytest.raises(error, match=match):
+        lora(**changed)
+
+
+def test_gated_ffn_with_adapters_has_no_backward():
+    with pytest.raises(RuntimeError, match="no backward"):
+        block.gated_ffn(z(2, 16).requires_grad_(), z(32, 16), z(16, 16), ids=torch.zeros(2, dtype=torch.int64),
+                        down_lora=(z(1, 8, 16), z(1, 16, 8), z(1, dtype=F32)))
+
+
+def norm(**changed):
+    args = {"y": z(3, 10), "residual": z(3, 10, dtype=F32), "weight": z(10, dtype=F32)}
+    return block.add_norm(**{**args, **changed})
+
+
+@pytest.mark.parametrize("error, match, changed", [
+    (TypeError, "y .T, H.", {"y": None}),
+    (TypeError, "y .T, H.", {"y": z(3, 10, dtype=torch.float16)}),
+    (ValueError, "y .3, 10.", {"y": z(3, 12)}),
+    (TypeError, "residual", {"residual": z(3, 10, dtype=torch.float64)}),
+    (TypeError, "residual", {"residual": z(30)}),
+    (ValueError, "weight", {"weight": z(12)}),
+    (ValueError, "weight", {"weight": z(1, 10)}),
+    (ValueError, "post", {"post": z(10, dtype=torch.float16)}),
+    (ValueError, "gate", {"gate": z(3)}),
+    (ValueError, "gate", {"gate": z(2, 1)}),
+    (ValueError, "gate", {"gate": z(3, 10, dtype=torch.float16)}),
+    (ValueError, "1 to 16384 columns", {"y": z(1, 16385), "residual": z(1, 16385), "weight": z(16385)}),
+    (ValueError, "on a GPU", {}),
+])
+def test_add_norm_refusals(error, match, changed):
+    with pytest.raises(error, match=match):
+        norm(**changed)
+
+
+@pytest.mark.parametrize("match, changed", [
+    ("dh or dn", {"dh": None, "dn": None}),
+    ("dh of", {"dh": z(3, 10)}),
+    ("dn of", {"dn": z(3, 10, dtype=F32)}),
+    ("dn goes with weight", {"weight": None}),
+    ("rstd", {"rstd": z(3, dtype=F32)}),
+    ("rstd", {"rstd": None}),
+])
+def test_add_norm_backward_refusals(match, changed):
+    args = {"dh": z(3, 10, dtype=F32), "dn": z(3, 10), "y": z(3, 10), "h": z(3, 10, dtype=F32), "rstd": z(2, 3, dtype=F32),
+            "weight": z(10)}
+    with pytest.raises(ValueError, match=match):
+        block.add_norm_backward(**{**args, **changed})
+
+
+def test_norm_refusals():
+    with pytest.raises(TypeError):
+        block.norm(z(2, 8), z(8), dtype=torch.float16)
+    with pytest.raises(ValueError, match="weight"):
+        block.norm(z(2, 8), None)
+
+
+@pytest.mark.parametrize("form, name", [(block._GatedFfn, "gated_ffn"), (block._AddNorm, "add_norm"), (block._Norm, "add_norm")])
+def test_autograd_backward_is_refused_under_capture(form, name, monkeypatch):
+    """The autograd forms' backward passes, of which this is the first check."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    grads = (z(2, 8),) * (2 if form is block._AddNorm else 1)
+    with pytest.raises(RuntimeError, match=f"{name}_backward"):
+        form.backward(None, *grads)
+
+
+P = 1 << 20  # an address that passes the checks of alignment; nothing is launched on it
+
+
+@pytest.mark.parametrize("match, changed", [
+    (b"multiples of 8", {"K": 12}),
+    (b"multiples of 8", {"N": 20}),
+    (b"multiples of 8 each", {"N": 24, "swiglu": 1}),
+    (b"negative", {"T": -1}),
+    (b"2\\^31", {"N": 1 << 20, "K": 1 << 12}),
+    (b"null pointer", {"x": None}),
+    (b"null pointer", {"w": P + 8}),
+    (b"null pointer", {"x_stride": 12}),
+    (b"null pointer", {"x_stride": 8}),
+    (b"rank", {"adapters": 1, "rank": 12}),
+    (b"null pointer", {"adapters": 1, "rank": 8}),
+    (b"aligned", {"adapters": 1, "rank": 8, "a": P + 2, "b": P, "alpha": P, "ids": P, "inner": P}),
+])
+def test_dense_entry_refuses(match, changed):
+    d = _lib.DenseDesc(**{**dict(x=P, w=P, out=P, x_stride=16, T=2, N=16, K=16), **changed})
+    assert _lib.lib().d3_dense(ctypes.byref(d), None) == -1
+    assert match.replace(b"\\", b"") in _lib.lib().d3_last_error()
+
+
+def test_entries_refuse_null_descriptors():
+    for name in ("d3_dense", "d3_gated_ffn_backward", "d3_add_norm", "d3_add_norm_backward"):
+        assert getattr(_lib.lib(), name)(None, None) == -1, name
+
+
+@pytest.mark.parametrize("changed", [{"H": 12}, {"I": 4}, {"O": 0}, {"T": -1}, {"dout": None}, {"pre": P + 4}, {"dx": P, "gate_up": None},
+                                     {"dgate_up": P, "x": None}, {"ddown": P, "hidden": None}, {"I": 1 << 20, "H": 1 << 12}])
+def test_ffn_backward_entry_refuses(changed):
+    args = dict(dout=P, x=P, gate_up=P, down=P, pre=P, hidden=P, dgate_up_rows=P, x_stride=16, T=2, H=16, I=16, O=16)
+    d = _lib.GatedFfnBackwardDesc(**{**args, **changed})
+    assert _lib.lib().d3_gated_ffn_backward(ctypes.byref(d), None) == -1
+
+
+@pytest.mark.parametrize("changed", [{"H": 0}, {"H": 16385}, {"T": -1}, {"y_type": 2}, {"gate_kind": 4}, {"gate_kind": 1},
+                                     {"residual": None}, {"h": None}, {"n": None}, {"y": None, "post": P}, {"y": None, "weight": None}])
+def test_add_norm_entry_refuses(changed):
+    args = dict(y=P, residual=P, weight=P, h=P, n=P, T=2, H=16, y_stride=16, residual_stride=16, scale=1.0, eps=1e-6)
+    d = _lib.AddNormDesc(**{**args, **changed})
+    assert _lib.lib().d3_add_norm(ctypes.byref(d), None) == -1
+
+
+@pytest.mark.parametrize("changed", [{"dh": None, "dn": None}, {"weight": None}, {"rstd": None}, {"h": None}, {"partials_floats": 31},
+                                     {"partials": None}, {"dpost": P}, {"dgate": P}, {"y": None}])
+def test_add_norm_backward_entry_refuses(changed):
+    args = dict(y=P, h=P, weight=P, dh=P, dn=P, rstd=P, dy=P, dresidual=P, dweight=P, partials=P, partials_floats=32, T=2, H=16,
+                y_stride=16, residual_stride=16, scale=1.0)
+    d = _lib.AddNormDesc(**{**args, **changed})
+    assert _lib.lib().d3_add_norm_backward(ctypes.byref(d), None) == -1
+
+
+@pytest.mark.parametrize("struct, cname", [(_lib.AddNormDesc, "d3_add_norm_desc"), (_lib.DenseDesc, "d3_dense_desc"),
+                                           (_lib.GatedFfnBackwardDesc, "d3_gated_ffn_backward_desc")])
+def test_descriptor_layout_matches_header(struct, cname, tmp_path):
+    fields = [f[0] for f in struct._fields_]
+    prog = tmp_path / "layout.c"
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{HEADER}"', "int main(void) {",
+             f'  printf("size %zu\\n", sizeof({cname}));']
+    lines += [f'  printf("{f} %zu\\n", offsetof({cname}, {f}));' for f in fields]
+    prog.write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-std=c11", "-o", str(exe), str(prog)], check=True, capture_output=True)
+    got = dict(line.split() for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines())
+    assert int(got["size"]) == ctypes.sizeof(struct)
+    assert {f: int(got[f]) for f in fields} == {f: getattr(struct, f).offset for f in fields}
