@@ -358,7 +358,7 @@ using namespace d3;
 
 extern "C" int64_t d3_add_norm_partials(int32_t T, int32_t H) {
   if (T < 0 || H < 1) return 0;
-  return 3 * (int64_t)groups_of(T, H) * H;
+  return (int64_t)groups_of(T, H) * H;
 }
 
 extern "C" int d3_add_norm(const d3_add_norm_desc* desc, void* stream) {

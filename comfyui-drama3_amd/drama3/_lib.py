@@ -11,6 +11,7 @@ import ctypes
 import functools
 import os
 import pathlib
+import struct
 import threading
 
 import torch
@@ -57,22 +58,24 @@ class AddNormDesc(ctypes.Structure):
     ]
 
 
-class DenseDesc(ctypes.Structure):
-    """d3_dense_desc (include/drama3_moe.h)."""
-    _fields_ = [
-        ("x", c_void_p), ("w", c_void_p), ("out", c_void_p), ("pre", c_void_p), ("a", c_void_p), ("b", c_void_p),
-        ("alpha", c_void_p), ("ids", c_void_p), ("inner", c_void_p), ("x_stride", c_int64), ("T", c_int32), ("N", c_int32),
-        ("K", c_int32), ("swiglu", c_int32), ("rank", c_int32), ("adapters", c_int32),
-    ]
+class Layout:
+    """A descriptor struct of include/drama3_moe.h as its fields' names and format codes in order: pack(...) gives its bytes (a
+    ctypes.Structure of as many fields takes four times as long to fill)."""
+
+    def __init__(self, **runs):
+        self.fields = [(name, code) for code, names in runs.values() for name in names.split()]
+        self.struct = struct.Struct("".join(code for _, code in self.fields))  # native sizes and alignment
+        self.pack = self.struct.pack
 
 
-class GatedFfnBackwardDesc(ctypes.Structure):
-    """d3_gated_ffn_backward_desc (include/drama3_moe.h)."""
-    _fields_ = [
-        ("dout", c_void_p), ("x", c_void_p), ("gate_up", c_void_p), ("down", c_void_p), ("pre", c_void_p),
-        ("hidden", c_void_p), ("dgate_up_rows", c_void_p), ("dx", c_void_p), ("dgate_up", c_void_p), ("ddown", c_void_p),
-        ("x_stride", c_int64), ("T", c_int32), ("H", c_int32), ("I", c_int32), ("O", c_int32),
-    ]
+ADD_NORM = Layout(
+    pointers=("Q", "y residual weight post gate dh dn h n rstd dy dresidual dweight dpost dgate partials"),
+    wide=("q", "partials_floats y_stride residual_stride gate_stride"),
+    ints=("i", "y_type stream_type weight_type post_type gate_type gate_kind T H"), floats=("f", "scale eps"),
+    last=("i", "unit_offset"))
+DENSE = Layout(pointers=("Q", "x w out pre a b alpha ids inner"), wide=("q", "x_stride"), ints=("i", "T N K swiglu rank adapters"))
+GATED_FFN_BACKWARD = Layout(pointers=("Q", "dout x gate_up down pre hidden dgate_up_rows dx dgate_up ddown"), wide=("q", "x_stride"),
+                            ints=("i", "T H I O"))
 
 
 # name -> (restype, argtypes)
@@ -163,10 +166,10 @@ SIGNATURES = {
     "d3_bf16_grouped": (c_int32, [c_void_p, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_int32,
                                   c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "d3_add_norm_partials": (c_int64, [c_int32, c_int32]),
-    "d3_add_norm": (c_int32, [ctypes.POINTER(AddNormDesc), c_void_p]),
-    "d3_add_norm_backward": (c_int32, [ctypes.POINTER(AddNormDesc), c_void_p]),
-    "d3_dense": (c_int32, [ctypes.POINTER(DenseDesc), c_void_p]),
-    "d3_gated_ffn_backward": (c_int32, [ctypes.POINTER(GatedFfnBackwardDesc), c_void_p]),
+    "d3_add_norm": (c_int32, [c_void_p, c_void_p]),
+    "d3_add_norm_backward": (c_int32, [c_void_p, c_void_p]),
+    "d3_dense": (c_int32, [c_void_p, c_void_p]),
+    "d3_gated_ffn_backward": (c_int32, [c_void_p, c_void_p]),
     "d3_await_cpu": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32,
                                c_void_p]),
 }

@@ -11,8 +11,6 @@ Gradients: gated_ffn (without adapters), add_norm and norm are differentiable (t
 their autograd backward is refused, since torch may then touch a stream outside the capture; a captured training step calls
 gated_ffn_forward and gated_ffn_backward, add_norm_forward and add_norm_backward, which the autograd forms are made of.
 """
-import ctypes
-
 import torch
 
 from . import _lib, kernels
@@ -27,12 +25,22 @@ def _no_capture(name):
         raise RuntimeError(f"{name}: autograd's backward pass is not captured; call {name}_backward in the captured step")
 
 
+def _any_grad(*tensors):
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
 # ---------------------------------------------------------------------------------------------------------- products
 MAX_ROW_STRIDE = 2 ** 23  # of a product's rows, in elements
 
 
-def _rows(x, what, cols=None, rows=None, index=None):
-    """Rows [T, K] bfloat16 as the products read them: columns side by side, 16-byte aligned (else a copy that is so)."""
+def _refuse_rows(x, what, cols, rows, index):
     if x.dim() != 2 or x.dtype is not torch.bfloat16:
         raise TypeError(f"{what} [T, K] bfloat16 expected")
     T, K = x.shape
@@ -40,40 +48,45 @@ def _rows(x, what, cols=None, rows=None, index=None):
         raise ValueError(f"{what} [{'T' if rows is None else rows}, {'K' if cols is None else cols}] expected, not {[T, K]}")
     if K < 8 or K % 8 or K > MAX_ROW_STRIDE or T > _INT_MAX:
         raise ValueError(f"{what} has a positive multiple of 8 columns up to {MAX_ROW_STRIDE}, not {K}")
-    if index is not None and x.get_device() != index:
+    if x.get_device() != index:
         raise ValueError(f"{what} on the rows' device expected")
-    if T == 1:
-        return x if x.stride(1) == 1 and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+
+
+def _rows(x, what, index, cols=None, rows=None):
+    """Rows x [T, K] bfloat16, checked, and as the products read them, (x, T, K, row stride): columns side by side, 16-byte aligned
+    (else a copy that is so)."""
+    _refuse_rows(x, what, cols, rows, index)
+    T, K = x.shape
+    at = x.data_ptr()
+    if x.is_contiguous():
+        return (x if at % 16 == 0 else x.clone()), T, K, K
     stride = x.stride(0)
-    if x.stride(1) != 1 or stride < K or stride % 8 or stride > MAX_ROW_STRIDE or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
-def _stride(x):
-    return x.stride(0) if x.size(0) > 1 else x.size(1)
+    if x.stride(1) != 1 or stride < K or stride % 8 or stride > MAX_ROW_STRIDE or at % 16:
+        return x.clone(memory_format=torch.contiguous_format), T, K, K
+    return x, T, K, stride
 
 
 def _weight(w, what, n, k, index):
-    """A weight [n, k] bfloat16, contiguous, 16-byte aligned (n None: any multiple of 8)."""
-    if w.dim() != 2 or w.dtype is not torch.bfloat16:
+    """(w, its rows): a weight [n, k] bfloat16, checked, contiguous and 16-byte aligned (n None: any multiple of 8)."""
+    if w.dtype is not torch.bfloat16 or w.dim() != 2:
         raise TypeError(f"{what} bfloat16, two-dimensional, expected")
-    if w.size(1) != k or (n is not None and w.size(0) != n) or w.size(0) < 8 or w.size(0) % 8:
-        raise ValueError(f"{what} [{'a multiple of 8' if n is None else n}, {k}] expected, not {list(w.shape)}")
-    if w.numel() > _INT_MAX:
+    N, K = w.shape
+    if K != k or N < 8 or N % 8 or (n is not None and N != n):
+        raise ValueError(f"{what} [{'a multiple of 8' if n is None else n}, {k}] expected, not {[N, K]}")
+    if N * K > _INT_MAX:
         raise ValueError(f"{what}: fewer than 2^31 elements expected")
     if w.get_device() != index:
         raise ValueError(f"{what} on the rows' device expected")
-    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+    return (w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)), N
 
 
 def _adapters(lora, ids, T, n, k, index):
     """(a, b, alpha, ids, rank, adapters) of rows' adapters, checked."""
     a, b, alpha = lora
-    if a.dim() != 3 or b.dim() != 3 or a.dtype is not torch.bfloat16 or b.dtype is not torch.bfloat16:
+    if a.dtype is not torch.bfloat16 or b.dtype is not torch.bfloat16 or a.dim() != 3 or b.dim() != 3:
         raise TypeError("adapters a [A, rank, K] and b [A, N, rank] bfloat16 expected")
-    count, rank, _ = a.shape
-    if a.shape != (count, rank, k) or b.shape != (count, n, rank) or rank < 8 or rank % 8:
+    count, rank, K = a.shape
+    if K != k or b.shape != (count, n, rank) or rank < 8 or rank % 8:
         raise ValueError(f"adapters a [A, rank, {k}] and b [A, {n}, rank] expected, rank a multiple of 8, not {list(a.shape)} and "
                          f"{list(b.shape)}")
     if rank * max(n, k) > _INT_MAX or count > _INT_MAX:
@@ -82,23 +95,28 @@ def _adapters(lora, ids, T, n, k, index):
         raise ValueError(f"alpha [{count}] float32 expected")
     if ids is None or ids.dtype is not torch.int64 or ids.shape != (T,):
         raise ValueError(f"ids [{T}] int64 expected: every row's adapter")
-    if any(t.get_device() != index for t in (a, b, alpha, ids)):
+    if a.get_device() != index or b.get_device() != index or alpha.get_device() != index or ids.get_device() != index:
         raise ValueError("adapters and ids on the rows' device expected")
-    a, b = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (a, b))
+    if not a.is_contiguous() or a.data_ptr() % 16:
+        a = a.clone(memory_format=torch.contiguous_format)
+    if not b.is_contiguous() or b.data_ptr() % 16:
+        b = b.clone(memory_format=torch.contiguous_format)
     return a, b, alpha.contiguous(), ids.contiguous(), rank, count
 
 
-def _dense(x, w, index, swiglu=False, pre=None, lora=None, ids=None):
+def _dense(x, T, K, stride, w, N, index, swiglu=False, pre=None, lora=None, ids=None):
     """[T, N] bfloat16 of checked rows and weight (swiglu: [T, N / 2])."""
-    (T, K), N = x.shape, w.size(0)
     out = x.new_empty((T, N // 2 if swiglu else N))
-    d = _lib.DenseDesc(x=x.data_ptr(), w=w.data_ptr(), out=out.data_ptr(), pre=_lib.ptr(pre), x_stride=_stride(x), T=T, N=N, K=K,
-                       swiglu=swiglu)
-    if lora is not None:
-        a, b, alpha, ids, d.rank, d.adapters = _adapters(lora, ids, T, N, K, index)
-        inner = x.new_empty((T, d.rank))
-        d.a, d.b, d.alpha, d.ids, d.inner = (t.data_ptr() for t in (a, b, alpha, ids, inner))
-    kernels.launch("d3_dense", index, ctypes.byref(d))
+    if lora is None:
+        kernels.launch("d3_dense", index, _lib.DENSE.pack(
+            x.data_ptr(), w.data_ptr(), out.data_ptr(), 0 if pre is None else pre.data_ptr(), 0, 0, 0, 0, 0, stride, T, N, K, swiglu,
+            0, 0))
+    else:
+        a, b, alpha, ids, rank, count = _adapters(lora, ids, T, N, K, index)
+        inner = x.new_empty((T, rank))
+        kernels.launch("d3_dense", index, _lib.DENSE.pack(
+            x.data_ptr(), w.data_ptr(), out.data_ptr(), 0, a.data_ptr(), b.data_ptr(), alpha.data_ptr(), ids.data_ptr(),
+            inner.data_ptr(), stride, T, N, K, swiglu, rank, count))
     return out
 
 
@@ -108,20 +126,20 @@ def lora_linear(x, weight, a, b, alpha, ids):
     int64; a row whose id is outside 0 .. A - 1 (-1, say) has none. [T, N] bfloat16, rounded once; sums in float32, the inner
     product x a^T alpha rounded to bfloat16 between its two products. Widths and rank are multiples of 8 (pad adapters of smaller
     rank with zeros). For decode lines and for prompts packed into one pass."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, a, b, alpha)):
+    if torch.is_grad_enabled() and _any_grad(x, weight, a, b, alpha):
         raise RuntimeError("lora_linear has no backward pass: call it under torch.no_grad()")
     index = x.get_device()
-    x = _rows(x, "x")
-    return _dense(x, _weight(weight, "weight", None, x.size(1), index), index, lora=(a, b, alpha), ids=ids)
+    x, T, K, stride = _rows(x, "x", index)
+    weight, N = _weight(weight, "weight", None, K, index)
+    return _dense(x, T, K, stride, weight, N, index, lora=(a, b, alpha), ids=ids)
 
 
-def _ffn_operands(x, gate_up, down):
-    index = x.get_device()
-    x = _rows(x, "x")
-    gate_up = _weight(gate_up, "gate_up", None, x.size(1), index)
-    if gate_up.size(0) % 16:
-        raise ValueError(f"gate and up rows are multiples of 8 each, not {gate_up.size(0)} in all")
-    return x, gate_up, _weight(down, "down", None, gate_up.size(0) // 2, index), index
+def _ffn_weights(gate_up, down, H, index):
+    """(gate_up, down, I, O), checked."""
+    gate_up, N = _weight(gate_up, "gate_up", None, H, index)
+    if N % 16:
+        raise ValueError(f"gate and up rows are multiples of 8 each, not {N} in all")
+    return (gate_up, N // 2) + _weight(down, "down", None, N // 2, index)
 
 
 def gated_ffn_forward(x, gate_up, down):
@@ -129,10 +147,12 @@ def gated_ffn_forward(x, gate_up, down):
     sums are kept unrounded: their rounding to bfloat16 would add as much error to the gradients as the gradients' own. Autograd does
     not see it."""
     with torch.no_grad():
-        x, gate_up, down, index = _ffn_operands(x, gate_up, down)
-        pre = x.new_empty((x.size(0), gate_up.size(0)), dtype=torch.float32)
-        hidden = _dense(x, gate_up, index, swiglu=True, pre=pre)
-        return _dense(hidden, down, index), (pre, hidden)
+        index = x.get_device()
+        x, T, H, stride = _rows(x, "x", index)
+        gate_up, I, down, O = _ffn_weights(gate_up, down, H, index)
+        pre = x.new_empty((T, 2 * I), dtype=torch.float32)
+        hidden = _dense(x, T, H, stride, gate_up, 2 * I, index, True, pre)
+        return _dense(hidden, T, I, I, down, O, index), (pre, hidden)
 
 
 def gated_ffn_backward(dout, x, gate_up, down, saved, needs=(True, True, True)):
@@ -140,11 +160,11 @@ def gated_ffn_backward(dout, x, gate_up, down, saved, needs=(True, True, True)):
     they went in and `saved` as gated_ffn_forward returned it; None where `needs` says so. Sums in float32; the gradients of gate
     and up are rounded to bfloat16 as the operands of the products that follow. The same bits from call to call."""
     with torch.no_grad():
-        x, gate_up, down, index = _ffn_operands(x, gate_up, down)
-        (T, H), I, O = x.shape, down.size(1), down.size(0)
+        index = x.get_device()
+        x, T, H, stride = _rows(x, "x", index)
+        gate_up, I, down, O = _ffn_weights(gate_up, down, H, index)
         pre, hidden = saved
-        dout = _rows(dout, "dout", O, T, index)
-        dout = dout if dout.is_contiguous() else dout.contiguous()
+        dout = _rows(dout, "dout", index, O, T)[0].contiguous()
         if pre.shape != (T, 2 * I) or pre.dtype is not torch.float32 or hidden.shape != (T, I) or \
                 hidden.dtype is not torch.bfloat16 or not (pre.is_contiguous() and hidden.is_contiguous()) or \
                 pre.get_device() != index or hidden.get_device() != index:
@@ -152,11 +172,9 @@ def gated_ffn_backward(dout, x, gate_up, down, saved, needs=(True, True, True)):
         new = x.new_zeros if T == 0 else x.new_empty
         dx, dgate_up, ddown = (new(shape) if need else None for need, shape in zip(needs, ((T, H), (2 * I, H), (O, I))))
         rows = x.new_empty((T, 2 * I))
-        d = _lib.GatedFfnBackwardDesc(
-            dout=dout.data_ptr(), x=x.data_ptr(), gate_up=gate_up.data_ptr(), down=down.data_ptr(), pre=pre.data_ptr(),
-            hidden=hidden.data_ptr(), dgate_up_rows=rows.data_ptr(), dx=_lib.ptr(dx), dgate_up=_lib.ptr(dgate_up),
-            ddown=_lib.ptr(ddown), x_stride=_stride(x), T=T, H=H, I=I, O=O)
-        kernels.launch("d3_gated_ffn_backward", index, ctypes.byref(d))
+        kernels.launch("d3_gated_ffn_backward", index, _lib.GATED_FFN_BACKWARD.pack(
+            dout.data_ptr(), x.data_ptr(), gate_up.data_ptr(), down.data_ptr(), pre.data_ptr(), hidden.data_ptr(), rows.data_ptr(),
+            _at(dx), _at(dgate_up), _at(ddown), stride, T, H, I, O))
         return dx, dgate_up, ddown
 
 
@@ -187,27 +205,32 @@ def gated_ffn(x, gate_up, down, *, gate_up_lora=None, down_lora=None, ids=None):
             raise ValueError("ids go with gate_up_lora or down_lora")
         if torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad):
             return _GatedFfn.apply(x, gate_up, down)
-    elif torch.is_grad_enabled() and any(
-            t.requires_grad for t in (x, gate_up, down, *(gate_up_lora or ()), *(down_lora or ()))):
+    elif torch.is_grad_enabled() and _any_grad(x, gate_up, down, *(gate_up_lora or ()), *(down_lora or ())):
         raise RuntimeError("gated_ffn with adapters has no backward pass: call it under torch.no_grad()")
-    x, gate_up, down, index = _ffn_operands(x, gate_up, down)
-    hidden = _dense(x, gate_up, index, swiglu=True, lora=gate_up_lora, ids=ids)
-    return _dense(hidden, down, index, lora=down_lora, ids=ids)
+    index = x.get_device()
+    x, T, H, stride = _rows(x, "x", index)
+    gate_up, I, down, O = _ffn_weights(gate_up, down, H, index)
+    hidden = _dense(x, T, H, stride, gate_up, 2 * I, index, True, lora=gate_up_lora, ids=ids)
+    return _dense(hidden, T, I, I, down, O, index, lora=down_lora, ids=ids)
 
 
 # ------------------------------------------------------------------------------------------------------------- norms
-def _float_rows(t, what, shape=None):
-    """Rows [T, H] float32 or bfloat16 with columns side by side (else a copy that has them so)."""
-    if t.dim() != 2 or t.dtype not in _TYPES:
+def _float_rows(t, what, index, shape=None):
+    """(rows [T, H], their stride), checked, float32 or bfloat16, with columns side by side (else a copy that has them so)."""
+    if t.dtype not in _TYPES or t.dim() != 2:
         raise TypeError(f"{what} [T, H] float32 or bfloat16 expected")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{what} {list(shape)} expected, not {list(t.shape)}")
-    return t if t.stride(1) == 1 and t.stride(0) >= t.size(1) else t.contiguous()
+    if t.get_device() != index:
+        raise ValueError(f"{what} on the rows' device expected")
+    if t.is_contiguous():
+        return t, t.size(1)
+    if t.stride(1) == 1 and t.stride(0) >= t.size(1):
+        return t, t.stride(0)
+    return t.contiguous(), t.size(1)
 
 
 def _norm_weight(w, what, H, index):
-    if w is None:
-        return None
     if w.dtype not in _TYPES or w.shape != (H,):
         raise ValueError(f"{what} [{H}] float32 or bfloat16 expected")
     if w.get_device() != index:
@@ -216,56 +239,54 @@ def _norm_weight(w, what, H, index):
 
 
 def _norm_gate(gate, T, H, index):
-    """(gate, kind): 1 a value per row ([T, 1]), 2 per channel ([H] or [1, H]), 3 per element."""
-    if gate is None:
-        return None, 0
+    """(gate, kind, row stride): 1 a value per row ([T, 1]), 2 per channel ([H] or [1, H]), 3 per element."""
     if gate.dtype not in _TYPES or gate.get_device() != index:
         raise ValueError("gate float32 or bfloat16 on the rows' device expected")
-    if gate.dim() == 1 and gate.shape == (H,):
-        return gate.contiguous(), 2
-    if gate.dim() == 2:
-        if gate.shape == (T, H):
-            return (gate if gate.stride(1) == 1 and gate.stride(0) >= H else gate.contiguous()), 3
-        if gate.shape == (T, 1):
-            return gate.contiguous(), 1
-        if gate.shape == (1, H):
-            return gate.contiguous(), 2
-    raise ValueError(f"gate [{T}, 1], [{H}], [1, {H}] or [{T}, {H}] expected, not {list(gate.shape)}")
+    shape = gate.shape
+    if shape == (T, H):
+        return _float_rows(gate, "gate", index) + (3,)
+    if shape == (T, 1):
+        return gate.contiguous(), 1, 1
+    if shape == (H,) or shape == (1, H):
+        return gate.contiguous(), 0, 2
+    raise ValueError(f"gate [{T}, 1], [{H}], [1, {H}] or [{T}, {H}] expected, not {list(shape)}")
 
 
-def _norm_desc(y, residual, weight, post, gate, scale, eps, unit_offset, out_dtype=None):
-    """(descriptor, tensors that it points to, device index) of a call's inputs, checked."""
-    residual = _float_rows(residual, "residual")
-    (T, H), index = residual.shape, residual.get_device()
-    if not 1 <= H <= MAX_NORM_COLS or T > _INT_MAX:
-        raise ValueError(f"rows of 1 to {MAX_NORM_COLS} columns, not {H}")
-    if y is not None:
-        y = _float_rows(y, "y", (T, H))
-        if y.get_device() != index:
-            raise ValueError("y on residual's device expected")
-        out_dtype = y.dtype
-    weight, post = _norm_weight(weight, "weight", H, index), _norm_weight(post, "post", H, index)
-    gate, kind = _norm_gate(gate, T, H, index)
-    d = _lib.AddNormDesc(
-        y=_lib.ptr(y), residual=residual.data_ptr(), weight=_lib.ptr(weight), post=_lib.ptr(post), gate=_lib.ptr(gate),
-        y_stride=0 if y is None else y.stride(0), residual_stride=residual.stride(0),
-        gate_stride=0 if gate is None else gate.stride(0), y_type=_TYPES[out_dtype], stream_type=_TYPES[residual.dtype],
-        weight_type=0 if weight is None else _TYPES[weight.dtype], post_type=0 if post is None else _TYPES[post.dtype],
-        gate_type=0 if gate is None else _TYPES[gate.dtype], gate_kind=kind, T=T, H=H, scale=float(scale), eps=float(eps),
-        unit_offset=bool(unit_offset))
-    return d, (y, residual, weight, post, gate), index
+class _NormCall:
+    """A norm's inputs, checked (y None: the norm alone, n of type out_dtype)."""
+
+    def __init__(self, y, residual, weight, post, gate, out_dtype=None):
+        index = self.index = residual.get_device()
+        self.residual, self.residual_stride = residual, _ = _float_rows(residual, "residual", index)
+        T, H = self.T, self.H = residual.shape
+        if not 1 <= H <= MAX_NORM_COLS or T > _INT_MAX:
+            raise ValueError(f"rows of 1 to {MAX_NORM_COLS} columns, not {H}")
+        self.y, self.y_stride = (None, 0) if y is None else _float_rows(y, "y", index, (T, H))
+        self.out_dtype = out_dtype if y is None else y.dtype
+        self.weight = None if weight is None else _norm_weight(weight, "weight", H, index)
+        self.post = None if post is None else _norm_weight(post, "post", H, index)
+        self.gate, self.gate_stride, self.gate_kind = (None, 0, 0) if gate is None else _norm_gate(gate, T, H, index)
+
+    def launch(self, name, scale, eps, unit_offset, dh=0, dn=0, h=0, n=0, rstd=0, dy=0, dresidual=0, dweight=0, dpost=0, dgate=0,
+               partials=0, floats=0):
+        y, weight, post, gate = self.y, self.weight, self.post, self.gate
+        kernels.launch(name, self.index, _lib.ADD_NORM.pack(
+            0 if y is None else y.data_ptr(), self.residual.data_ptr(), 0 if weight is None else weight.data_ptr(),
+            0 if post is None else post.data_ptr(), 0 if gate is None else gate.data_ptr(), dh, dn, h, n, rstd, dy, dresidual, dweight,
+            dpost, dgate, partials, floats, self.y_stride, self.residual_stride, self.gate_stride, _TYPES[self.out_dtype],
+            _TYPES[self.residual.dtype], 0 if weight is None else _TYPES[weight.dtype], 0 if post is None else _TYPES[post.dtype],
+            0 if gate is None else _TYPES[gate.dtype], self.gate_kind, self.T, self.H, scale, eps, unit_offset))
 
 
 def _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, stats):
     if y is None:
         raise TypeError("y [T, H] float32 or bfloat16 expected")
-    d, (y, residual, weight, post, gate), index = _norm_desc(y, residual, weight, post, gate, scale, eps, unit_offset)
-    T, H = d.T, d.H
-    h = residual.new_empty((T, H))
-    n = None if weight is None else y.new_empty((T, H))
-    rstd = residual.new_empty((2, T), dtype=torch.float32) if stats else None
-    d.h, d.n, d.rstd = h.data_ptr(), _lib.ptr(n), _lib.ptr(rstd)
-    kernels.launch("d3_add_norm", index, ctypes.byref(d))
+    c = _NormCall(y, residual, weight, post, gate)
+    T, H = c.T, c.H
+    h = c.residual.new_empty((T, H))
+    n = None if weight is None else c.y.new_empty((T, H))
+    rstd = h.new_empty((2, T), dtype=torch.float32) if stats else None
+    c.launch("d3_add_norm", scale, eps, unit_offset, h=h.data_ptr(), n=_at(n), rstd=_at(rstd))
     return h, n, rstd
 
 
@@ -282,37 +303,42 @@ def add_norm_backward(dh, dn, y, h, rstd, weight, *, post=None, gate=None, scale
     gradient has its input's type and shape; None where the input is absent or `needs` says so. Float32 inside, from h as it is
     stored; sums over the rows (dweight, dpost, a gate per channel) are the same bits from call to call."""
     with torch.no_grad():
-        return _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, scale, unit_offset, needs,
-                                  h.dtype if y is None else y.dtype)
+        if y is None:
+            raise TypeError("y [T, H] float32 or bfloat16 expected")
+        return _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, scale, unit_offset, needs, None)
 
 
 def _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, scale, unit_offset, needs, out_dtype):
-    gate_in = gate
-    d, (y, h, weight, post, gate), index = _norm_desc(y, h, weight, post, gate, scale, 0.0, unit_offset, out_dtype)
-    T, H = d.T, d.H
+    c = _NormCall(y, h, weight, post, gate, out_dtype)
+    T, H, index, h = c.T, c.H, c.index, c.residual
     if dh is None and dn is None:
         raise ValueError("dh or dn expected")
     if weight is None and dn is not None:
         raise ValueError("dn goes with weight")
-    if rstd is None or rstd.dtype != torch.float32 or rstd.shape != (2, T) or not rstd.is_contiguous() or rstd.get_device() != index:
+    if rstd is None or rstd.dtype is not torch.float32 or rstd.shape != (2, T) or not rstd.is_contiguous() or \
+            rstd.get_device() != index:
         raise ValueError(f"rstd [2, {T}] float32 of add_norm_forward expected")
-    if dh is not None and (dh.dtype != h.dtype or dh.shape != (T, H) or dh.get_device() != index):
-        raise ValueError("dh of h's type and shape, on its device, expected")
-    if dn is not None and (dn.dtype != out_dtype or dn.shape != (T, H) or dn.get_device() != index):
-        raise ValueError("dn of n's type and shape, on its device, expected")
-    dh, dn = (None if t is None else t.contiguous() for t in (dh, dn))
+    if dh is not None:
+        if dh.dtype is not h.dtype or dh.shape != (T, H) or dh.get_device() != index:
+            raise ValueError("dh of h's type and shape, on its device, expected")
+        dh = dh.contiguous()
+    if dn is not None:
+        if dn.dtype is not c.out_dtype or dn.shape != (T, H) or dn.get_device() != index:
+            raise ValueError("dn of n's type and shape, on its device, expected")
+        dn = dn.contiguous()
     if not any(needs):
         return (None,) * 5
-    new = lambda like, need, *shape: h.new_empty(shape, dtype=like.dtype) if like is not None and need else None  # noqa: E731
-    dy, dresidual = new(y, needs[0], T, H), new(h, needs[1], T, H)
-    dweight, dpost = new(weight, needs[2], H), new(post, needs[3], H)
-    dgate = new(gate, needs[4], *gate_in.shape) if gate_in is not None else None
-    floats = _lib.lib().d3_add_norm_partials(T, H)
-    partials = h.new_empty(floats, dtype=torch.float32) if any(t is not None for t in (dweight, dpost, dgate)) else None
-    d.dh, d.dn, d.h, d.rstd = _lib.ptr(dh), _lib.ptr(dn), h.data_ptr(), rstd.data_ptr()
-    d.dy, d.dresidual, d.dweight, d.dpost, d.dgate = (_lib.ptr(t) for t in (dy, dresidual, dweight, dpost, dgate))
-    d.partials, d.partials_floats = _lib.ptr(partials), floats
-    kernels.launch("d3_add_norm_backward", index, ctypes.byref(d))
+    new = h.new_empty
+    dy = new((T, H), dtype=c.out_dtype) if y is not None and needs[0] else None
+    dresidual = new((T, H)) if needs[1] else None
+    dweight = new((H,), dtype=weight.dtype) if weight is not None and needs[2] else None
+    dpost = new((H,), dtype=post.dtype) if post is not None and needs[3] else None
+    dgate = new(gate.shape, dtype=gate.dtype) if gate is not None and needs[4] else None
+    parts = (dweight is not None) + (dpost is not None) + (dgate is not None and c.gate_kind == 2)
+    floats = parts * _lib.lib().d3_add_norm_partials(T, H)
+    partials = new((floats,), dtype=torch.float32) if parts else None
+    c.launch("d3_add_norm_backward", scale, 0.0, unit_offset, _at(dh), _at(dn), h.data_ptr(), 0, rstd.data_ptr(), _at(dy),
+             _at(dresidual), _at(dweight), _at(dpost), _at(dgate), _at(partials), floats)
     return dy, dresidual, dweight, dpost, dgate
 
 
@@ -332,7 +358,7 @@ class _AddNorm(torch.autograd.Function):
         if dh is None and dn is None:
             return (None,) * 8
         y, h, rstd, weight, post, gate = ctx.saved_tensors
-        grads = _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, *ctx.options, ctx.needs_input_grad[:5], y.dtype)
+        grads = _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, *ctx.options, ctx.needs_input_grad[:5], None)
         return grads + (None,) * 3
 
 
@@ -342,8 +368,7 @@ def add_norm(y, residual, weight, *, post=None, gate=None, scale=1.0, eps=1e-6, 
     block as well). y and residual [T, H], float32 or bfloat16 each; weight and post [H]; gate a value per row [T, 1], per
     channel [H] or per element [T, H]. rms(z) = sqrt(mean(z^2) + eps); with unit_offset weight and post are read as 1 + w.
     weight None: n is None. Float32 inside, h and n each rounded once (n comes from h before its rounding). Differentiable."""
-    wants = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, residual, weight, post, gate))
-    if wants:
+    if torch.is_grad_enabled() and _any_grad(y, residual, weight, post, gate):
         return _AddNorm.apply(y, residual, weight, post, gate, scale, eps, unit_offset)
     return _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, False)[:2]
 
@@ -371,11 +396,10 @@ class _Norm(torch.autograd.Function):
 def _norm(x, weight, eps, unit_offset, dtype, stats):
     if weight is None:
         raise ValueError("weight [H] expected")
-    d, (_, x, weight, _, _), index = _norm_desc(None, x, weight, None, None, 1.0, eps, unit_offset, dtype)
-    n = x.new_empty((d.T, d.H), dtype=dtype)
-    rstd = x.new_empty((2, d.T), dtype=torch.float32) if stats else None
-    d.n, d.rstd = n.data_ptr(), _lib.ptr(rstd)
-    kernels.launch("d3_add_norm", index, ctypes.byref(d))
+    c = _NormCall(None, x, weight, None, None, dtype)
+    n = c.residual.new_empty((c.T, c.H), dtype=dtype)
+    rstd = n.new_empty((2, c.T), dtype=torch.float32) if stats else None
+    c.launch("d3_add_norm", 1.0, eps, unit_offset, n=n.data_ptr(), rstd=_at(rstd))
     return n, rstd
 
 

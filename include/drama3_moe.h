@@ -452,7 +452,8 @@ int d3_bf16_grouped(const void* x, int32_t rows, const int64_t* order, int32_t k
  *     rstd(h), and rstd(y) with post.
  *   d3_add_norm_backward: from dh and dn (either may be NULL: zero), y, h (rows residual_stride apart) and rstd as the
  *     forward call left them: dy, dresidual, dweight, dpost, dgate, each where it is not NULL, of its input's type and
- *     shape. partials: d3_add_norm_partials(T, H) floats, need no clearing. Sums over the rows are made in a fixed order.
+ *     shape. partials: d3_add_norm_partials(T, H) floats for each of dweight, dpost and a dgate per channel, need no clearing.
+ *     Sums over the rows are made in a fixed order.
  *     T = 0 gives zeros. */
 typedef struct d3_add_norm_desc {
   const void* y;

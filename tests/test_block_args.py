@@ -1,6 +1,6 @@
 """Argument checks of drama3.block that run before any launch (no GPU needed), and of its C entries and descriptors."""
-import ctypes
 import pathlib
+import struct
 import subprocess
 
 import pytest
@@ -124,6 +124,14 @@ def test_autograd_backward_is_refused_under_capture(form, name, monkeypatch):
         form.backward(None, *grads)
 
 
+def call(entry, layout, **fields):
+    """The entry's return code for a descriptor of these fields, zeros elsewhere."""
+    left = dict(fields)
+    data = layout.pack(*(left.pop(name, None) or (0.0 if code == "f" else 0) for name, code in layout.fields))
+    assert not left, left
+    return getattr(_lib.lib(), entry)(data, None)
+
+
 P = 1 << 20  # an address that passes the checks of alignment; nothing is launched on it
 
 
@@ -142,8 +150,7 @@ P = 1 << 20  # an address that passes the checks of alignment; nothing is launch
     (b"aligned", {"adapters": 1, "rank": 8, "a": P + 2, "b": P, "alpha": P, "ids": P, "inner": P}),
 ])
 def test_dense_entry_refuses(match, changed):
-    d = _lib.DenseDesc(**{**dict(x=P, w=P, out=P, x_stride=16, T=2, N=16, K=16), **changed})
-    assert _lib.lib().d3_dense(ctypes.byref(d), None) == -1
+    assert call("d3_dense", _lib.DENSE, **{**dict(x=P, w=P, out=P, x_stride=16, T=2, N=16, K=16), **changed}) == -1
     assert match.replace(b"\\", b"") in _lib.lib().d3_last_error()
 
 
@@ -156,16 +163,14 @@ def test_entries_refuse_null_descriptors():
                                      {"dgate_up": P, "x": None}, {"ddown": P, "hidden": None}, {"I": 1 << 20, "H": 1 << 12}])
 def test_ffn_backward_entry_refuses(changed):
     args = dict(dout=P, x=P, gate_up=P, down=P, pre=P, hidden=P, dgate_up_rows=P, x_stride=16, T=2, H=16, I=16, O=16)
-    d = _lib.GatedFfnBackwardDesc(**{**args, **changed})
-    assert _lib.lib().d3_gated_ffn_backward(ctypes.byref(d), None) == -1
+    assert call("d3_gated_ffn_backward", _lib.GATED_FFN_BACKWARD, **{**args, **changed}) == -1
 
 
 @pytest.mark.parametrize("changed", [{"H": 0}, {"H": 16385}, {"T": -1}, {"y_type": 2}, {"gate_kind": 4}, {"gate_kind": 1},
                                      {"residual": None}, {"h": None}, {"n": None}, {"y": None, "post": P}, {"y": None, "weight": None}])
 def test_add_norm_entry_refuses(changed):
     args = dict(y=P, residual=P, weight=P, h=P, n=P, T=2, H=16, y_stride=16, residual_stride=16, scale=1.0, eps=1e-6)
-    d = _lib.AddNormDesc(**{**args, **changed})
-    assert _lib.lib().d3_add_norm(ctypes.byref(d), None) == -1
+    assert call("d3_add_norm", _lib.ADD_NORM, **{**args, **changed}) == -1
 
 
 @pytest.mark.parametrize("changed", [{"dh": None, "dn": None}, {"weight": None}, {"rstd": None}, {"h": None}, {"partials_floats": 31},
@@ -173,21 +178,25 @@ def test_add_norm_entry_refuses(changed):
 def test_add_norm_backward_entry_refuses(changed):
     args = dict(y=P, h=P, weight=P, dh=P, dn=P, rstd=P, dy=P, dresidual=P, dweight=P, partials=P, partials_floats=32, T=2, H=16,
                 y_stride=16, residual_stride=16, scale=1.0)
-    d = _lib.AddNormDesc(**{**args, **changed})
-    assert _lib.lib().d3_add_norm_backward(ctypes.byref(d), None) == -1
+    assert call("d3_add_norm_backward", _lib.ADD_NORM, **{**args, **changed}) == -1
 
 
-@pytest.mark.parametrize("struct, cname", [(_lib.AddNormDesc, "d3_add_norm_desc"), (_lib.DenseDesc, "d3_dense_desc"),
-                                           (_lib.GatedFfnBackwardDesc, "d3_gated_ffn_backward_desc")])
-def test_descriptor_layout_matches_header(struct, cname, tmp_path):
-    fields = [f[0] for f in struct._fields_]
+@pytest.mark.parametrize("layout, cname", [(_lib.ADD_NORM, "d3_add_norm_desc"), (_lib.DENSE, "d3_dense_desc"),
+                                           (_lib.GATED_FFN_BACKWARD, "d3_gated_ffn_backward_desc")])
+def test_descriptor_layout_matches_header(layout, cname, tmp_path):
+    """Every field sits at the offset and has the size that the C compiler gives it in the header."""
     prog = tmp_path / "layout.c"
-    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{HEADER}"', "int main(void) {",
-             f'  printf("size %zu\\n", sizeof({cname}));']
-    lines += [f'  printf("{f} %zu\\n", offsetof({cname}, {f}));' for f in fields]
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{HEADER}"', "int main(void) {", f"  {cname} d;",
+             '  printf("size %zu 0\\n", sizeof(d));']
+    lines += [f'  printf("{f} %zu %zu\\n", offsetof({cname}, {f}), sizeof(d.{f}));' for f, _ in layout.fields]
     prog.write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
     exe = tmp_path / "layout"
     subprocess.run(["gcc", "-std=c11", "-o", str(exe), str(prog)], check=True, capture_output=True)
-    got = dict(line.split() for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines())
-    assert int(got["size"]) == ctypes.sizeof(struct)
-    assert {f: int(got[f]) for f in fields} == {f: getattr(struct, f).offset for f in fields}
+    got = {n: (int(a), int(b)) for n, a, b in (line.split() for line in subprocess.run(
+        [str(exe)], check=True, capture_output=True, text=True).stdout.splitlines())}
+    size = got.pop("size")[0]
+    assert 0 <= size - layout.struct.size < 8  # (the end of the struct is padded to its alignment)
+    codes = "".join(code for _, code in layout.fields)
+    for i, (name, code) in enumerate(layout.fields):
+        assert got[name] == (struct.calcsize(codes[:i + 1]) - struct.calcsize(code), struct.calcsize(code)), name
+    assert len(got) == len(layout.fields)
