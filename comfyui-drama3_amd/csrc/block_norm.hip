@@ -18,6 +18,7 @@
 #include "common.hpp"
 #include "../../include/drama3_moe.h"
 
+#include <algorithm>
 #include <string>
 #include <type_traits>
 
@@ -35,29 +36,47 @@ struct bf16_t {
 typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// columns col .. col + 7 of a row as float (zeros past H), and back
+// columns col .. col + 7 of a row as they are stored (zeros past H)
 template <class T>
-D3_INLINE void load8(const T* row, int col, int H, float (&v)[8]) {
-  if (col + 8 <= H) {
-    if constexpr (std::is_same_v<T, bf16_t>) {
-      const u32x4_at2 w = *(const u32x4_at2*)(row + col);
-#pragma unroll
-      for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+struct Eight;
+template <>
+struct Eight<bf16_t> {
+  u32x4_at2 w;
+    D3_INLINE void get(const bf16_t* row, int col, int H) {
+    if (col + 8 <= H) {
+      w = *(const u32x4_at2*)(row + col);
     } else {
-      const f32x4_at4 a = *(const f32x4_at4*)(row + col), b = *(const f32x4_at4*)(row + col + 4);
 #pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = a[i], v[4 + i] = b[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      v[i] = 0.0f;
-      if (col + i < H) {
-        if constexpr (std::is_same_v<T, bf16_t>) v[i] = bf16_to_f32(row[col + i].bits);
-        else v[i] = row[col + i];
+      for (int i = 0; i < 4; i++) {
+        w[i] = col + 2 * i < H ? row[col + 2 * i].bits : 0u;
+        if (col + 2 * i + 1 < H) w[i] |= (uint32_t)row[col + 2 * i + 1].bits << 16;
       }
     }
   }
+  D3_INLINE float operator[](int i) const { return i & 1 ? __uint_as_float(w[i / 2] & 0xFFFF0000u) : __uint_as_float(w[i / 2] << 16); }
+};
+template <>
+struct Eight<float> {
+  f32x4_at4 a, b;
+    D3_INLINE void get(const float* row, int col, int H) {
+    if (col + 8 <= H) {
+      a = *(const f32x4_at4*)(row + col), b = *(const f32x4_at4*)(row + col + 4);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        a[i] = col + i < H ? row[col + i] : 0.0f;
+        b[i] = col + 4 + i < H ? row[col + 4 + i] : 0.0f;
+      }
+    }
+  }
+  D3_INLINE float operator[](int i) const { return i < 4 ? a[i] : b[i - 4]; }
+};
+template <class T>
+D3_INLINE void load8(const T* row, int col, int H, float (&v)[8]) {
+  Eight<T> e;
+  e.get(row, col, H);
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = e[i];
 }
 template <class T>
 D3_INLINE void store8(T* row, int col, int H, const float (&v)[8]) {
@@ -90,16 +109,16 @@ D3_INLINE float load1_of(const void* p, int type, int64_t i) {
   return type ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i];
 }
 
-// a row's sum over its LANES lanes, the same in all of them; `slot`: LDS of this sum alone until two barriers later
-template <int LANES>
+// A row's sum over its lanes, the same in all of them: a wave's (WAVE) or the workgroup's, whose `slot` is LDS of this sum alone
+// until two barriers later.
+template <bool WAVE>
 D3_INLINE float row_sum(float v, float* slot) {
   v = wave_sum_f32(v);
-  if constexpr (LANES > 64) {
+  if constexpr (!WAVE) {
     if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
     __syncthreads();
     v = slot[0];
-#pragma unroll
-    for (int i = 1; i < LANES / 64; i++) v += slot[i];
+    for (int i = 1; i < (int)blockDim.x / 64; i++) v += slot[i];
   }
   return v;
 }
@@ -127,37 +146,42 @@ D3_INLINE void weight8(const void* w, int type, int offset, int col, int H, floa
   }
 }
 
-// LANES lanes a row, CH times 8 columns a lane
-template <class TY, class TS, int LANES, int CH>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) add_norm_kernel(Desc d) {
-  constexpr int ROWS = LANES < 256 ? 256 / LANES : 1;
-  __shared__ float slots[2][LANES / 64];
-  const int lane = threadIdx.x % LANES;
-  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
+// Lanes: WAVE a wave a row and four rows a workgroup, else a row a workgroup, of which lane l has the 8 columns from 8 l and CH - 1
+// times as many lanes further on.
+template <bool WAVE>
+D3_INLINE int lane_of() { return WAVE ? (int)threadIdx.x & 63 : (int)threadIdx.x; }
+template <bool WAVE>
+D3_INLINE int lanes_of() { return WAVE ? 64 : (int)blockDim.x; }
+
+template <class TY, class TS, bool WAVE, int CH, int MOST>
+__global__ void __launch_bounds__(MOST) add_norm_kernel(Desc d) {
+  __shared__ float slots[2][16];
+  const int lane = lane_of<WAVE>(), lanes = lanes_of<WAVE>();
+  const int64_t row = WAVE ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x;
   if (row >= d.T) return;  // (whole waves, and then without barriers)
   float h[CH][8], w[CH][8];
 #pragma unroll
-  for (int j = 0; j < CH; j++) load8((const TS*)d.residual + row * d.residual_stride, 8 * (lane + LANES * j), d.H, h[j]);
+  for (int j = 0; j < CH; j++) load8((const TS*)d.residual + row * d.residual_stride, 8 * (lane + lanes * j), d.H, h[j]);
   if (d.weight) {  // (on its way during the sums)
 #pragma unroll
-    for (int j = 0; j < CH; j++) weight8(d.weight, d.weight_type, d.unit_offset, 8 * (lane + LANES * j), d.H, w[j]);
+    for (int j = 0; j < CH; j++) weight8(d.weight, d.weight_type, d.unit_offset, 8 * (lane + lanes * j), d.H, w[j]);
   }
   if (d.y) {
     float v[CH][8];
 #pragma unroll
-    for (int j = 0; j < CH; j++) load8((const TY*)d.y + row * d.y_stride, 8 * (lane + LANES * j), d.H, v[j]);
+    for (int j = 0; j < CH; j++) load8((const TY*)d.y + row * d.y_stride, 8 * (lane + lanes * j), d.H, v[j]);
     if (d.post) {
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < CH; j++)
 #pragma unroll
         for (int i = 0; i < 8; i++) sum += v[j][i] * v[j][i];
-      const float rstd = rsqrtf(row_sum<LANES>(sum, slots[0]) / (float)d.H + d.eps);
+      const float rstd = rsqrtf(row_sum<WAVE>(sum, slots[0]) / (float)d.H + d.eps);
       if (d.rstd && lane == 0) d.rstd[d.T + row] = rstd;
 #pragma unroll
       for (int j = 0; j < CH; j++) {
         float p[8];
-        weight8(d.post, d.post_type, d.unit_offset, 8 * (lane + LANES * j), d.H, p);
+        weight8(d.post, d.post_type, d.unit_offset, 8 * (lane + lanes * j), d.H, p);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[j][i] *= rstd * p[i];
       }
@@ -165,10 +189,10 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) add_norm_kernel(Des
 #pragma unroll
     for (int j = 0; j < CH; j++) {
       float g[8] = {1, 1, 1, 1, 1, 1, 1, 1};
-      if (d.gate_kind) gate8(d, (int)row, 8 * (lane + LANES * j), g);
+      if (d.gate_kind) gate8(d, (int)row, 8 * (lane + lanes * j), g);
 #pragma unroll
       for (int i = 0; i < 8; i++) h[j][i] += d.scale * (g[i] * v[j][i]);
-      if (d.h) store8((TS*)d.h + row * d.H, 8 * (lane + LANES * j), d.H, h[j]);
+      if (d.h) store8((TS*)d.h + row * d.H, 8 * (lane + lanes * j), d.H, h[j]);
     }
   }
   if (!d.weight) return;
@@ -177,150 +201,206 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) add_norm_kernel(Des
   for (int j = 0; j < CH; j++)
 #pragma unroll
     for (int i = 0; i < 8; i++) sum += h[j][i] * h[j][i];
-  const float rstd = rsqrtf(row_sum<LANES>(sum, slots[1]) / (float)d.H + d.eps);
+  const float rstd = rsqrtf(row_sum<WAVE>(sum, slots[1]) / (float)d.H + d.eps);
   if (d.rstd && lane == 0) d.rstd[row] = rstd;
 #pragma unroll
   for (int j = 0; j < CH; j++) {
 #pragma unroll
     for (int i = 0; i < 8; i++) w[j][i] *= h[j][i] * rstd;
-    store8((TY*)d.n + row * d.H, 8 * (lane + LANES * j), d.H, w[j]);
+    store8((TY*)d.n + row * d.H, 8 * (lane + lanes * j), d.H, w[j]);
   }
 }
 
-template <class TY, class TS, int LANES, int CH>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) add_norm_backward_kernel(Desc d, int groups) {
-  constexpr int ROWS = LANES < 256 ? 256 / LANES : 1;
-  __shared__ float slots[2][3][LANES / 64];
-  const int lane = threadIdx.x % LANES, group = blockIdx.x * ROWS + threadIdx.x / LANES;
+// SIDE: there is a post norm or a gate; without them dy = scale dresidual, and y is not read. The next row's loads are on
+// their way during a row's sums. What all rows share (weight, post, a gate per channel) stays in registers: loads come back in
+// order, so one that a row waits for would wait for the next row's as well.
+template <class TY, class TS, bool SIDE, bool WAVE, int CH, int MOST>
+__global__ void __launch_bounds__(MOST) add_norm_backward_kernel(Desc d, int groups) {
+  __shared__ float slots[2][3][16];
+  const int lane = lane_of<WAVE>(), lanes = lanes_of<WAVE>(), group = WAVE ? (int)(blockIdx.x * 4 + threadIdx.x / 64) : (int)blockIdx.x;
   if (group >= groups) return;  // (whole waves, and then without barriers)
-  float sum_w[CH][8] = {}, sum_p[CH][8] = {}, sum_g[CH][8] = {};
-  int turn = 0;
-  for (int64_t row = group; row < d.T; row += groups, turn ^= 1) {
-    float dr[CH][8], v[CH][8];
+  constexpr int SC = SIDE ? CH : 1;
+  float sum_w[CH][8] = {}, sum_p[SC][8] = {}, sum_g[SC][8] = {}, w[CH][8] = {}, p[SC][8], g[SC][8];
+  float next_g[SC][8], next_rstd = 0.0f, next_rstd_y = 1.0f;
+  Eight<TS> next_dh[CH], next_h[CH];
+  Eight<TY> next_dn[CH], next_y[SC];
+#pragma unroll
+  for (int j = 0; j < CH; j++) {
+    const int col = 8 * (lane + lanes * j);
+    if (d.weight) weight8(d.weight, d.weight_type, d.unit_offset, col, d.H, w[j]);
+    if constexpr (SIDE) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) p[j][i] = g[j][i] = next_g[j][i] = 1.0f;
+      if (d.post) weight8(d.post, d.post_type, d.unit_offset, col, d.H, p[j]);
+      if (d.gate_kind == GATE_CHANNEL) gate8(d, 0, col, g[j]);
+    }
+  }
+  auto get = [&](int64_t row) {
+    if (d.dn) next_rstd = d.rstd[row];
+    if (SIDE && d.post) next_rstd_y = d.rstd[d.T + row];
 #pragma unroll
     for (int j = 0; j < CH; j++) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) dr[j][i] = 0.0f;
-      if (d.dh) load8((const TS*)d.dh + row * d.H, 8 * (lane + LANES * j), d.H, dr[j]);
-      if (d.y) load8((const TY*)d.y + row * d.y_stride, 8 * (lane + LANES * j), d.H, v[j]);
+      const int col = 8 * (lane + lanes * j);
+      if (d.dh) next_dh[j].get((const TS*)d.dh + row * d.H, col, d.H);
+      if (d.dn) {
+        next_dn[j].get((const TY*)d.dn + row * d.H, col, d.H);
+        next_h[j].get((const TS*)d.h + row * d.residual_stride, col, d.H);
+      }
+      if constexpr (SIDE) {
+        next_y[j].get((const TY*)d.y + row * d.y_stride, col, d.H);
+        if (d.gate_kind == GATE_ROW || d.gate_kind == GATE_FULL) gate8(d, (int)row, col, next_g[j]);
+      }
     }
-    if (d.dn) {
-      float a[CH][8], hat[CH][8], sum = 0.0f;
-      const float rstd = d.rstd[row];
+  };
+  get(group);  // (there are no more groups than rows)
+  int turn = 0;
+  for (int64_t row = group; row < d.T; row += groups, turn ^= 1) {
+    float dr[CH][8], a[CH][8], hat[CH][8], v[SC][8];
+    const float rstd = next_rstd, rstd_y = next_rstd_y;
 #pragma unroll
-      for (int j = 0; j < CH; j++) {
-        float w[8];
-        load8((const TY*)d.dn + row * d.H, 8 * (lane + LANES * j), d.H, a[j]);
-        load8((const TS*)d.h + row * d.residual_stride, 8 * (lane + LANES * j), d.H, hat[j]);
-        weight8(d.weight, d.weight_type, d.unit_offset, 8 * (lane + LANES * j), d.H, w);
+    for (int j = 0; j < CH; j++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          hat[j][i] *= rstd;
-          sum_w[j][i] += a[j][i] * hat[j][i];
-          a[j][i] *= w[i];
-          sum += a[j][i] * hat[j][i];
+      for (int i = 0; i < 8; i++) {
+        dr[j][i] = d.dh ? next_dh[j][i] : 0.0f;
+        if (d.dn) a[j][i] = next_dn[j][i], hat[j][i] = next_h[j][i] * rstd;
+        if constexpr (SIDE) {
+          v[j][i] = next_y[j][i];
+          if (d.gate_kind != GATE_CHANNEL) g[j][i] = next_g[j][i];
         }
       }
-      const float mean = row_sum<LANES>(sum, slots[turn][0]) / (float)d.H;
+    if (row + groups < d.T) get(row + groups);
+    if (d.dn) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < CH; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          sum_w[j][i] += a[j][i] * hat[j][i];
+          a[j][i] *= w[j][i];
+          sum += a[j][i] * hat[j][i];
+        }
+      const float mean = row_sum<WAVE>(sum, slots[turn][0]) / (float)d.H;
 #pragma unroll
       for (int j = 0; j < CH; j++)
 #pragma unroll
         for (int i = 0; i < 8; i++) dr[j][i] += rstd * (a[j][i] - hat[j][i] * mean);
     }
+    if (d.dresidual) {
 #pragma unroll
-    for (int j = 0; j < CH; j++)
-      if (d.dresidual) store8((TS*)d.dresidual + row * d.H, 8 * (lane + LANES * j), d.H, dr[j]);
-    if (!d.y || !(d.dy || d.dpost || d.dgate)) continue;
-    const float rstd = d.post ? d.rstd[d.T + row] : 1.0f;
-    float sum_row = 0.0f, sum_b = 0.0f;
+      for (int j = 0; j < CH; j++) store8((TS*)d.dresidual + row * d.H, 8 * (lane + lanes * j), d.H, dr[j]);
+    }
+    if constexpr (!SIDE) {
+      if (d.dy) {
 #pragma unroll
-    for (int j = 0; j < CH; j++) {
-      const int col = 8 * (lane + LANES * j);
-      float p[8] = {1, 1, 1, 1, 1, 1, 1, 1}, g[8] = {1, 1, 1, 1, 1, 1, 1, 1}, full[8];
-      if (d.post) weight8(d.post, d.post_type, d.unit_offset, col, d.H, p);
-      if (d.gate_kind) gate8(d, (int)row, col, g);
+        for (int j = 0; j < CH; j++) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float dv = d.scale * dr[j][i];
-        if (d.post) v[j][i] *= rstd;  // y^
-        full[i] = dv * (v[j][i] * p[i]);
-        sum_g[j][i] += full[i];
-        sum_row += full[i];
-        const float dnormed = dv * g[i];
-        sum_p[j][i] += dnormed * v[j][i];
-        dr[j][i] = dnormed * p[i];  // b
-        sum_b += dr[j][i] * v[j][i];
+          for (int i = 0; i < 8; i++) dr[j][i] *= d.scale;
+          store8((TY*)d.dy + row * d.H, 8 * (lane + lanes * j), d.H, dr[j]);
+        }
       }
-      if (d.dgate && d.gate_kind == GATE_FULL) {
-        if (d.gate_type) store8((bf16_t*)d.dgate + row * d.H, col, d.H, full);
-        else store8((float*)d.dgate + row * d.H, col, d.H, full);
+    } else {
+      float sum_row = 0.0f, sum_b = 0.0f;
+#pragma unroll
+      for (int j = 0; j < CH; j++) {
+        const int col = 8 * (lane + lanes * j);
+        float full[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float dv = d.scale * dr[j][i];
+          v[j][i] *= rstd_y;  // y^
+          full[i] = dv * (v[j][i] * p[j][i]);
+          sum_g[j][i] += full[i];
+          sum_row += full[i];
+          const float dnormed = dv * g[j][i];
+          sum_p[j][i] += dnormed * v[j][i];
+          dr[j][i] = dnormed * p[j][i];  // b
+          sum_b += dr[j][i] * v[j][i];
+        }
+        if (d.dgate && d.gate_kind == GATE_FULL) {
+          if (d.gate_type) store8((bf16_t*)d.dgate + row * d.H, col, d.H, full);
+          else store8((float*)d.dgate + row * d.H, col, d.H, full);
+        }
+      }
+      if (d.dgate && d.gate_kind == GATE_ROW) {
+        sum_row = row_sum<WAVE>(sum_row, slots[turn][1]);
+        if (lane == 0) {
+          if (d.gate_type) ((uint16_t*)d.dgate)[row] = (uint16_t)f32_to_bf16(sum_row);
+          else ((float*)d.dgate)[row] = sum_row;
+        }
+      }
+      if (d.dy) {
+        if (d.post) {
+          const float mean = row_sum<WAVE>(sum_b, slots[turn][2]) / (float)d.H;
+#pragma unroll
+          for (int j = 0; j < CH; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) dr[j][i] = rstd_y * (dr[j][i] - v[j][i] * mean);
+        }
+#pragma unroll
+        for (int j = 0; j < CH; j++) store8((TY*)d.dy + row * d.H, 8 * (lane + lanes * j), d.H, dr[j]);
       }
     }
-    if (d.dgate && d.gate_kind == GATE_ROW) {
-      sum_row = row_sum<LANES>(sum_row, slots[turn][1]);
-      if (lane == 0) {
-        if (d.gate_type) ((uint16_t*)d.dgate)[row] = (uint16_t)f32_to_bf16(sum_row);
-        else ((float*)d.dgate)[row] = sum_row;
-      }
-    }
-    if (!d.dy) continue;
-    if (d.post) {
-      const float mean = row_sum<LANES>(sum_b, slots[turn][2]) / (float)d.H;
-#pragma unroll
-      for (int j = 0; j < CH; j++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) dr[j][i] = rstd * (dr[j][i] - v[j][i] * mean);
-    }
-#pragma unroll
-    for (int j = 0; j < CH; j++) store8((TY*)d.dy + row * d.H, 8 * (lane + LANES * j), d.H, dr[j]);
   }
   float* part = d.partials + (int64_t)group * d.H;
   const int64_t step = (int64_t)groups * d.H;
 #pragma unroll
   for (int j = 0; j < CH; j++) {
-    const int col = 8 * (lane + LANES * j);
+    const int col = 8 * (lane + lanes * j);
     float* to = part;
     if (d.dweight) store8(to, col, d.H, sum_w[j]), to += step;
-    if (d.dpost) store8(to, col, d.H, sum_p[j]), to += step;
-    if (d.dgate && d.gate_kind == GATE_CHANNEL) store8(to, col, d.H, sum_g[j]);
+    if constexpr (SIDE) {
+      if (d.dpost) store8(to, col, d.H, sum_p[j]), to += step;
+      if (d.dgate && d.gate_kind == GATE_CHANNEL) store8(to, col, d.H, sum_g[j]);
+    }
   }
 }
 
-// the workgroups' sums over the rows added up: 64 columns a workgroup, 16 waves of which each adds every 16th group
+// the groups' sums over the rows added up: 32 columns a workgroup, 4 a lane, so that its 1024 lanes each add every 128th
+// group, whose sums are then added in LDS
 struct Sums {
   void* out[3];
   int type[3];
 };
 __global__ void __launch_bounds__(1024) add_groups_kernel(const float* partials, int groups, int H, Sums s) {
-  __shared__ float part[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  __shared__ float part[128][32];
+  const int lane = threadIdx.x & 7, slice = threadIdx.x >> 3, col = blockIdx.x * 32 + 4 * lane;
   const float* from = partials + (int64_t)blockIdx.y * groups * H;
-  float sum = 0.0f;
-  if (col < H) {
+  f32x4 sum{0, 0, 0, 0};
+  if (col + 4 <= H) {
 #pragma unroll 8
-    for (int g = w; g < groups; g += 16) sum += from[(int64_t)g * H + col];
+    for (int g = slice; g < groups; g += 128) sum += *(const f32x4_at4*)(from + (int64_t)g * H + col);
+  } else {
+    for (int g = slice; g < groups; g += 128)
+      for (int i = 0; i < 4; i++)
+        if (col + i < H) sum[i] += from[(int64_t)g * H + col + i];
   }
-  part[w][threadIdx.x & 63] = sum;
+  *(f32x4*)&part[slice][4 * lane] = sum;
   __syncthreads();
-  if (w || col >= H) return;
-  for (int i = 1; i < 16; i++) sum += part[i][threadIdx.x];
-  if (s.type[blockIdx.y]) ((uint16_t*)s.out[blockIdx.y])[col] = (uint16_t)f32_to_bf16(sum);
-  else ((float*)s.out[blockIdx.y])[col] = sum;
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5, out = blockIdx.x * 32 + c;
+  float all = (part[r][c] + part[r + 32][c]) + (part[r + 64][c] + part[r + 96][c]);
+  part[r][c] = all;  // (no other lane reads or writes these four)
+  __syncthreads();
+  if (r || out >= H) return;
+#pragma unroll
+  for (int i = 1; i < 32; i++) all += part[i][c];
+  if (s.type[blockIdx.y]) ((uint16_t*)s.out[blockIdx.y])[out] = (uint16_t)f32_to_bf16(all);
+  else ((float*)s.out[blockIdx.y])[out] = all;
 }
 
 constexpr int MAX_H = 16384;
 
-// f(lanes, chunks) for rows of H columns, chunks of 8 to a lane
-template <class F>
+// f(WAVE, CH, MOST, lanes) for rows of H columns: MOST lanes at 8 columns each, then 512 at more. 1391 rows of 5120, 640 lanes
+// against 320: forward 17.2 us and 15.5, backward 28 and 48 (of which a CU holds one row at a time either way).
+template <int MOST, class F>
 void by_width(int H, F f) {
   const int units = (H + 7) / 8;
-  using std::integral_constant;
-  if (units <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  else if (units <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  else if (units <= 256) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-  else if (units <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  else if (units <= 1024) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
-  else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+  auto lanes = [&](int ch) { return ((units + ch - 1) / ch + 63) / 64 * 64; };
+  using std::bool_constant, std::integral_constant;
+  if (units <= 64) f(bool_constant<true>{}, integral_constant<int, 1>{}, integral_constant<int, 256>{}, 256);
+  else if (units <= 128) f(bool_constant<true>{}, integral_constant<int, 2>{}, integral_constant<int, 256>{}, 256);
+  else if (units <= MOST) f(bool_constant<false>{}, integral_constant<int, 1>{}, integral_constant<int, MOST>{}, lanes(1));
+  else if (units <= 1024) f(bool_constant<false>{}, integral_constant<int, 2>{}, integral_constant<int, 512>{}, lanes(2));
+  else f(bool_constant<false>{}, integral_constant<int, 4>{}, integral_constant<int, 512>{}, lanes(4));
 }
 template <class F>
 void by_types(const Desc& d, F f) {
@@ -333,12 +413,11 @@ void by_types(const Desc& d, F f) {
   }
 }
 
-int rows_of(int H) { return (H + 7) / 8 <= 128 ? 4 : 1; }
-
-// groups of rows whose sums over the rows a backward pass keeps apart
+// Groups of rows whose sums over the rows a backward pass keeps apart: as many as the CUs hold at once (12 waves each), since
+// each writes float32 sums of H columns that the second launch reads.
 int groups_of(int T, int H) {
-  const int most = 1024;
-  return T < most ? T : most;
+  const int units = (H + 7) / 8, most = units <= 128 ? 256 * 8 : 256 * std::max(1, 12 / ((units + 63) / 64));
+  return std::min(T, most);
 }
 
 int check(const char* what, const Desc* d) {
@@ -367,10 +446,10 @@ extern "C" int d3_add_norm(const d3_add_norm_desc* desc, void* stream) {
   if (d.T == 0) return 0;
   if (!d.residual || (d.y && !d.h) || (d.weight && !d.n) || !(d.y || d.weight)) return fail("d3_add_norm: null pointer");
   by_types(d, [&](auto y, auto s) {
-    by_width(d.H, [&](auto lanes, auto chunks) {
-      constexpr int L = decltype(lanes)::value, rows = L < 256 ? 256 / L : 1;
-      add_norm_kernel<decltype(y), decltype(s), L, decltype(chunks)::value>
-          <<<(unsigned)(((int64_t)d.T + rows - 1) / rows), L < 256 ? 256 : L, 0, (hipStream_t)stream>>>(d);
+    by_width<512>(d.H, [&](auto wave, auto chunks, auto most, int lanes) {
+      constexpr bool W = decltype(wave)::value;
+      add_norm_kernel<decltype(y), decltype(s), W, decltype(chunks)::value, decltype(most)::value>
+          <<<W ? (unsigned)(((int64_t)d.T + 3) / 4) : (unsigned)d.T, lanes, 0, (hipStream_t)stream>>>(d);
     });
   });
   const hipError_t e = hipGetLastError();
@@ -390,10 +469,14 @@ extern "C" int d3_add_norm_backward(const d3_add_norm_desc* desc, void* stream) 
     if (parts && (!d.partials || d.partials_floats < (int64_t)parts * groups * d.H))
       return fail("d3_add_norm_backward: partials too small (d3_add_norm_partials)");
     by_types(d, [&](auto y, auto s) {
-      by_width(d.H, [&](auto lanes, auto chunks) {
-        constexpr int L = decltype(lanes)::value, rows = L < 256 ? 256 / L : 1;
-        add_norm_backward_kernel<decltype(y), decltype(s), L, decltype(chunks)::value>
-            <<<(groups + rows - 1) / rows, L < 256 ? 256 : L, 0, (hipStream_t)stream>>>(d, groups);
+      by_width<768>(d.H, [&](auto wave, auto chunks, auto most, int lanes) {
+        constexpr bool W = decltype(wave)::value;
+        constexpr int CH = decltype(chunks)::value, MOST = decltype(most)::value;
+        const int grid = W ? (groups + 3) / 4 : groups;
+        if (d.y && (d.post || d.gate_kind))
+          add_norm_backward_kernel<decltype(y), decltype(s), true, W, CH, MOST><<<grid, lanes, 0, (hipStream_t)stream>>>(d, groups);
+        else
+          add_norm_backward_kernel<decltype(y), decltype(s), false, W, CH, MOST><<<grid, lanes, 0, (hipStream_t)stream>>>(d, groups);
       });
     });
   }
@@ -403,7 +486,7 @@ extern "C" int d3_add_norm_backward(const d3_add_norm_desc* desc, void* stream) 
     if (d.dweight) sums.out[i] = d.dweight, sums.type[i++] = d.weight_type;
     if (d.dpost) sums.out[i] = d.dpost, sums.type[i++] = d.post_type;
     if (d.dgate && d.gate_kind == GATE_CHANNEL) sums.out[i] = d.dgate, sums.type[i++] = d.gate_type;
-    add_groups_kernel<<<dim3((d.H + 63) / 64, parts), 1024, 0, (hipStream_t)stream>>>(d.partials, groups, d.H, sums);
+    add_groups_kernel<<<dim3((d.H + 31) / 32, parts), 1024, 0, (hipStream_t)stream>>>(d.partials, groups, d.H, sums);
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : hip_fail(e, "d3_add_norm_backward launch");
