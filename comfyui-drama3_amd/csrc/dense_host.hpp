@@ -2,6 +2,7 @@
 #pragma once
 #include "dense_stream.hpp"
 
+#include <algorithm>
 #include <string>
 
 namespace d3 {
@@ -9,7 +10,9 @@ int fail(const std::string& msg);
 int hip_fail(hipError_t err, const char* what);
 
 using Wide = Tile<2, 4, 8, 4, 2>;    // 256 x 256, 8 waves, one workgroup a CU
+using Long = Tile<2, 4, 8, 2, 3>;    // 256 x 128, 8 waves, one workgroup a CU
 using Narrow = Tile<2, 2, 4, 4, 2>;  // 128 x 128, 4 waves, two workgroups a CU
+using Small = Tile<2, 2, 2, 2, 4>;   // 64 x 64, 4 waves, two workgroups a CU
 
 constexpr int64_t MAX_LD = 1 << 23;  // (a tile's rows within 32-bit byte offsets)
 
@@ -22,19 +25,33 @@ inline int dense_tiles(const Dense& a, bool swiglu) {
 }
 
 template <class C, bool XT, bool WT, int END, bool LORA = false>
-inline void launch_tile(Dense a, hipStream_t stream) {
-  a.splits = 1, a.split_stages = (a.K + 63) / 64;
+inline void launch_tile(const Dense& a, hipStream_t stream) {
   const int tiles = dense_tiles<C>(a, END == END_SWIGLU);
   dense_tile_kernel<C, XT, WT, END, LORA><<<tiles, C::THREADS, 0, stream>>>(a, a, tiles);
 }
 
-// the tile's size: 256 x 256 where that still gives every CU one
+// The tile's size by what a stage of each takes, us, times the turns in which the 256 CUs take the tiles: 1.66 (256 x 256),
+// 0.86 (256 x 128), 0.9 for two of 128 x 128 (0.5 for one), 0.18 (64 x 64), measured with every CU at work. So the large
+// ones, which read least, where they come out even, and small ones for few rows. Measured, us, in this order:
+//   4096 x 4096 x 11008  285 295 308 -     4096 x 2048 x 6144  124  89  88 -     4096 x 12288 x 2048 (SwiGLU) 196 216 230 -
+//   1391 x 1536 x 2048     -   -  26 22     509 x 1024 x 2048    -   -  19 10
 template <bool XT, bool WT, int END, bool LORA = false>
 inline void launch_tiles(const Dense& a, hipStream_t stream) {
-  if constexpr (!LORA) {  // (with adapters the wide tile's sums do not stay in registers)
-    if (dense_tiles<Wide>(a, END == END_SWIGLU) >= 256) return launch_tile<Wide, XT, WT, END, LORA>(a, stream);
+  constexpr bool SWIGLU = END == END_SWIGLU;
+  auto turns = [](int tiles, int at_once) { return (tiles + at_once - 1) / at_once; };
+  const int narrow_tiles = dense_tiles<Narrow>(a, SWIGLU);
+  const float wide = 1.66f * turns(dense_tiles<Wide>(a, SWIGLU), 256), tall = 0.86f * turns(dense_tiles<Long>(a, SWIGLU), 256);
+  const float narrow = narrow_tiles <= 256 ? 0.5f : 0.9f * turns(narrow_tiles, 512);
+  const float small = 0.18f * turns(dense_tiles<Small>(a, SWIGLU), 256);
+  if (!LORA && wide <= std::min({tall, narrow, small})) {  // (with adapters the wide tile's sums do not stay in registers)
+    if constexpr (!LORA) launch_tile<Wide, XT, WT, END, LORA>(a, stream);
+  } else if (tall <= std::min(narrow, small)) {
+    launch_tile<Long, XT, WT, END, LORA>(a, stream);
+  } else if (narrow <= small) {
+    launch_tile<Narrow, XT, WT, END, LORA>(a, stream);
+  } else {
+    launch_tile<Small, XT, WT, END, LORA>(a, stream);
   }
-  launch_tile<Narrow, XT, WT, END, LORA>(a, stream);
 }
 
 template <int RT, int END, bool LORA>

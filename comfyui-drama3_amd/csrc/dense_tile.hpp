@@ -14,6 +14,8 @@
 #pragma once
 #include "wide_tile.hpp"
 
+#include <type_traits>
+
 namespace d3 {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -24,7 +26,6 @@ enum DenseEnd {
   END_ROWS,     // out bf16
   END_SWIGLU,   // w holds `half` gate rows, then as many up rows: out [M, half] = SiLU(gate) * up, and pre where it is given
   END_DSWIGLU,  // the sums are the gradient of SiLU(gate) * up: out [M, 2 half] = the gradients of gate and up (from pre)
-  END_PART,     // float32 sums of a part of K, part `split` of the workspace
 };
 
 struct Dense {
@@ -33,9 +34,7 @@ struct Dense {
   int64_t ldx, ldw, ldo;  // elements from row to row as they are stored (ldo: of out)
   uint16_t* out;
   float* pre;     // [M, 2 half]: gate and up before the activation
-  float* parts;   // [splits, M, N]
   int M, N, K, half;
-  int splits, split_stages;  // K in `splits` runs of split_stages stages
   // adapters: out += p(m) . b[ids[m]](n), p [M, rank] of this row's own adapter; rows with an id outside have none
   const uint16_t* p;
   const uint16_t* b;  // [adapters, N, rank]
@@ -43,8 +42,17 @@ struct Dense {
   int rank, adapters;
 };
 
-// 16 bytes a lane from base + off into LDS at lds + 16 * lane (dma16's rules), base a scalar already
-D3_INLINE void copy16(uint32_t lds, const uint8_t* base, uint32_t off) { dma16(lds, base, off); }
+// dma16 as an instruction that the compiler may move other memory accesses past: its place among the barriers (which
+// nothing passes) is what the LDS that it writes needs
+D3_INLINE void copy16(uint32_t lds, const uint8_t* base, uint32_t off) {
+  const uint64_t at = (uint64_t)base;
+  const uint64_t sbase = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at) |
+                         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32;
+  uint64_t from;
+  asm volatile("s_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+               : "=&s"(from)
+               : "{m0}"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(sbase));
+}
 
 template <int N>
 D3_INLINE void loads_but() {
@@ -56,14 +64,16 @@ D3_INLINE f32x4 mfma_bf16(i32x4 a, i32x4 b, f32x4 acc) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
 }
 
-// which turn row k's chunks take
-D3_INLINE int t_turn(int k) { return (k & 3) | ((k >> 3) & 1) << 2; }
+// which turn row k's chunks take: bits of k that tell 8 rows 0 .. 3, 8 .. 11 apart (of 64 columns two rows share a group of banks)
+template <int ROWS>
+D3_INLINE int t_turn(int k) { return ROWS >= 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1; }
+template <int ROWS> constexpr int t_turns = ROWS >= 128 ? 7 : 3;
 
 // One operand's side of a tile: ROWS m or n. T: transposed. W waves copy it, PER kilobytes each.
 template <int ROWS, bool T, int W>
 struct Side {
   static constexpr int BYTES = ROWS * 128, PER = BYTES / 1024 / W;
-  static_assert(BYTES % (1024 * W) == 0 && ROWS % 128 == 0);
+  static_assert(BYTES % (1024 * W) == 0 && ROWS % 64 == 0);
   const uint8_t* base;  // of the next stage to copy
   uint32_t step;        // bytes from stage to stage
   uint32_t off[PER];
@@ -71,28 +81,41 @@ struct Side {
   static D3_INLINE int row_of(int i, int w, int lane) { return T ? ((w * PER + i) * 1024 + lane * 16) / (2 * ROWS) : (w * PER + i) * 8 + (lane >> 3); }
   static D3_INLINE int col_of(int i, int w, int lane) {
     const int r = row_of(i, w, lane);
-    if constexpr (!T) return 8 * ((lane & 7) ^ ((r >> 1) & 7));
-    const int at = (lane * 16) % (2 * ROWS), c = at >> 5;  // (a copy holds whole rows of k, or half a row of 256 m)
-    return 16 * ((c & ~7) | ((c & 7) ^ t_turn(r))) + ((at >> 4) & 1) * 8;
+    if constexpr (!T) return 8 * wt_slot(r, lane & 7);
+    const int at = (lane * 16) % (2 * ROWS), c = at >> 5;
+    return 16 * ((c & ~t_turns<ROWS>) | ((c & t_turns<ROWS>) ^ t_turn<ROWS>(r))) + ((at >> 4) & 1) * 8;
   }
+  // which of a stage's k that is
+  static D3_INLINE int k_of(int i, int w, int lane) { return T ? row_of(i, w, lane) : col_of(i, w, lane); }
 };
 
-// MFMA operand `t` (16 m or n) of k-step s: lane (q, c) holds k = 8 q .. 8 q + 7 of row c
+// Where a lane's operands of k-step s lie in a side's stage, those of MFMA tile 0: lane (q, c) holds k = 8 q .. 8 q + 7 of row c.
 template <int ROWS, bool T>
-D3_INLINE i32x4 operand(uint32_t side, int t, int s, int lane) {
+D3_INLINE uint32_t operand_at(int s, int lane) {
+  const int q = lane >> 4, c = lane & 15;
+  if constexpr (!T) return c * 128 + wt_slot(c, 4 * s + q) * 16;
+  const int k = 8 * q + (c >> 2);
+  return k * (2 * ROWS) + t_turn<ROWS>(k) * 32 + (c & 3) * 8 + s * 64 * ROWS;
+}
+// the operand of tile t, `at` the place above in this stage's buffer (whose address, like a row of k's, ends in zeros where t's turn goes)
+template <int ROWS, bool T>
+D3_INLINE i32x4 operand(uint32_t at, int t) {
   typedef __attribute__((address_space(3))) const i32x4 lds_i32x4;
   typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-  const int q = lane >> 4, c = lane & 15;
   if constexpr (!T) {
-    const uint32_t at = side + (t * 16 + c) * 128 + ((4 * s + q) ^ ((c >> 1) & 7)) * 16;
-    return *(lds_i32x4*)(uintptr_t)at;
+    return *(lds_i32x4*)(uintptr_t)(at + t * 2048);
   } else {
-    const int k = 8 * q + (c >> 2);
-    const uint32_t at = (side + k * (2 * ROWS) + (t & ~7) * 32 + (t_turn(k) ^ (t & 7)) * 32 + (c & 3) * 8) + s * 64 * ROWS;
-    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)at);
-    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)(at + 8 * ROWS));
+    const uint32_t here = (at ^ ((t & t_turns<ROWS>) * 32)) + (t & ~t_turns<ROWS>) * 32;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)here);
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)(here + 8 * ROWS));
     return __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
+}
+// v, of which the compiler forgets what it knows: what is computed from it here is neither kept from earlier nor made ahead of a loop
+// (registers that the wide tile does not have: a reload from scratch memory would wait for all copies on their way)
+D3_INLINE uint32_t anew(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // SiLU(g) u and its gradients from the float32 sums. The sigmoid's exponential and reciprocal are the hardware's
@@ -100,10 +123,21 @@ D3_INLINE i32x4 operand(uint32_t side, int t, int s, int lane) {
 // is infinite and the sigmoid 0, as in the limit.
 D3_INLINE float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
-// Four results of a row, rounded to bf16 and stored; n a multiple of 4, N of 8.
+// four results rounded to bf16
 D3_INLINE i32x2 round4(f32x4 v) {
   typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(i32x2, __builtin_convertvector(v, bf16x4));
+}
+
+// A row's results of two neighbouring MFMA tiles (of `tiles` whose columns are all there), lane (q, c) holding 4 of each, as 16-byte
+// stores, 64 bytes a row in a row: the odd q's of the first tile change places with the even ones of the second, so
+// that a lane holds 8 in a row of one tile. `at`: the row's first of the 32 columns; `stored`: columns from there on that
+// there are (0: none, the whole wave calls all the same).
+D3_INLINE void store_two(uint16_t* at, i32x2 v0, i32x2 v1, int stored) {
+  const int q = (threadIdx.x & 63) >> 4, n = 16 * (q & 1) + 8 * (q >> 1);
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v0[0], (uint32_t)v1[0], false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)v0[1], (uint32_t)v1[1], false, false);
+  if (n < stored) *(i32x4*)(at + n) = i32x4{(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
 }
 
 // The tile of a workgroup among nm x nn: those of an XCD (workgroup i runs on XCD i % 8) lie side by side, and go by
@@ -144,13 +178,8 @@ D3_INLINE void add_adapters(const Dense& a, f32x4 (&acc)[C::NT][C::MT], int m0, 
       if (open[t]) now = __builtin_amdgcn_readlane(id[t], __ffs((int)open[t]) - 1);
     if (now < 0) break;
     const uint16_t* b = a.b + (size_t)now * a.N * a.rank;
-    uint32_t some = 0;  // which of the wave's tiles have rows of it
 #pragma unroll
-    for (int t = 0; t < C::MT; t++) {
-      const uint32_t rows = (uint32_t)__ballot(id[t] == now) & 0xFFFFu;
-      open[t] &= ~rows;
-      some |= (rows ? 1u : 0u) << t;
-    }
+    for (int t = 0; t < C::MT; t++) open[t] &= ~(uint32_t)__ballot(id[t] == now);
     for (int r0 = 0; r0 < a.rank; r0 += 32) {
       const int r = r0 + 8 * q;
       i32x4 bv[C::NT];
@@ -161,7 +190,6 @@ D3_INLINE void add_adapters(const Dense& a, f32x4 (&acc)[C::NT][C::MT], int m0, 
       }
 #pragma unroll
       for (int t = 0; t < C::MT; t++) {
-        if (!(some >> t & 1)) continue;
         const bool mine = id[t] == now;
         i32x4 pv{0, 0, 0, 0};
         if (mine && r < a.rank) pv = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + c) * a.rank + r);
@@ -176,6 +204,12 @@ D3_INLINE void add_adapters(const Dense& a, f32x4 (&acc)[C::NT][C::MT], int m0, 
   }
 }
 
+// The loop over the stages is one stream of MFMA groups (NT products of one row tile each). Beside each group go the LDS reads of
+// the operands that the half stage after needs, into the registers that the group has just read, and, in a stage's second
+// half, its share of the copies of the stage BUFS later: with all copies at the start of a stage the waves stood in line
+// to send them, and copies and products took turns (256 x 256 on 4096 x 4096 x 11008: 285 us, 321 so before; 4096 x
+// 6144 x 2048 transposed twice 90, 114). A stage's one barrier stands after group BAR of its second half, when the reads of its own
+// operands are long done.
 template <class C, bool XT, bool WT, int END, bool LORA>
 __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, Dense two, int tiles_one) {
   constexpr int TM = C::TM, TN = C::TN, W = C::WAVES, BUFS = C::BUFS;
@@ -191,8 +225,7 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, De
   const int columns = END == END_SWIGLU ? a.half : a.N, nm = (a.M + TM - 1) / TM, nn = (columns + UN - 1) / UN;
   int tm, tn;
   place((int)blockIdx.x - (second ? tiles_one : 0), nm, nn, tm, tn);
-  const int m0 = tm * TM, n0 = tn * UN, split = blockIdx.y;
-  const int all_stages = (a.K + 63) / 64, first = split * a.split_stages, stages = min(a.split_stages, all_stages - first);
+  const int m0 = tm * TM, n0 = tn * UN, stages = (a.K + 63) / 64;
   const uint32_t lds = lds_address(smem);
 
   // the rows of w (n) of a tile's row r, gate and up rows by turns of the waves' tiles
@@ -208,8 +241,8 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, De
   SW sw;
   sx.step = XT ? (uint32_t)(128 * a.ldx) : 128u;
   sw.step = WT ? (uint32_t)(128 * a.ldw) : 128u;
-  sx.base = (const uint8_t*)(a.x + (XT ? (int64_t)first * 64 * a.ldx + m0 : m0 * a.ldx + (int64_t)first * 64));
-  sw.base = (const uint8_t*)(a.w + (WT ? (int64_t)first * 64 * a.ldw + n0 : (END == END_SWIGLU ? 0 : n0 * a.ldw) + (int64_t)first * 64));
+  sx.base = (const uint8_t*)(a.x + (XT ? m0 : m0 * a.ldx));
+  sw.base = (const uint8_t*)(a.w + (WT ? n0 : END == END_SWIGLU ? 0 : n0 * a.ldw));
 #pragma unroll
   for (int i = 0; i < SX::PER; i++) {
     const int r = SX::row_of(i, w, lane), col = SX::col_of(i, w, lane);
@@ -221,43 +254,42 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, De
     sw.off[i] = WT ? (uint32_t)(r * a.ldw + min(col, a.N - 8 - n0)) * 2
                    : (uint32_t)((w_row(r) - (END == END_SWIGLU ? 0 : n0)) * a.ldw + col) * 2;
   }
-  // how many k of stage s there are, and its copies: the lanes of k past K read from k 0 of the stage instead (cleared later)
-  auto copy = [&](int s) {
-    const int left = a.K - (first + s) * 64;
-    const uint32_t at = lds + (s % BUFS) * STAGE + w * (SX::PER * 1024);
-    const uint32_t at_w = lds + (s % BUFS) * STAGE + SX::BYTES + w * (SW::PER * 1024);
-    if (left >= 64) {
-#pragma unroll
-      for (int i = 0; i < SX::PER; i++) copy16(at + i * 1024, sx.base, sx.off[i]);
-#pragma unroll
-      for (int i = 0; i < SW::PER; i++) copy16(at_w + i * 1024, sw.base, sw.off[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < SX::PER; i++) {
-        const int k = XT ? SX::row_of(i, w, lane) : SX::col_of(i, w, lane);
-        copy16(at + i * 1024, sx.base, k < left ? sx.off[i] : sx.off[i] - (uint32_t)(XT ? k * a.ldx : k) * 2);
-      }
-#pragma unroll
-      for (int i = 0; i < SW::PER; i++) {
-        const int k = WT ? SW::row_of(i, w, lane) : SW::col_of(i, w, lane);
-        copy16(at_w + i * 1024, sw.base, k < left ? sw.off[i] : sw.off[i] - (uint32_t)(WT ? k * a.ldw : k) * 2);
-      }
-    }
-    sx.base += sx.step;
-    sw.base += sw.step;
+  constexpr int PIECES = SX::PER + SW::PER;
+  auto piece = [&](int i, int buf) {
+    const uint32_t at = lds + buf * STAGE;
+    if (i < SX::PER) copy16(at + (w * SX::PER + i) * 1024, sx.base, sx.off[i]);
+    else copy16(at + SX::BYTES + (w * SW::PER + i - SX::PER) * 1024, sw.base, sw.off[i - SX::PER]);
   };
-  auto clear = [&](int s) {
-    const int left = a.K - (first + s) * 64;
+  // before stage s is copied: where it ends past K (it is the last one then), the lanes of k past K read from its k 0
+  auto ready = [&](int s) {
+    const int left = a.K - s * 64;
+    if (left >= 64) return;
+    const int l = (int)anew(lane);
+#pragma unroll
+    for (int i = 0; i < SX::PER; i++) {
+      const int k = SX::k_of(i, w, l);
+      if (k >= left) sx.off[i] -= (uint32_t)(XT ? k * a.ldx : k) * 2;
+    }
+#pragma unroll
+    for (int i = 0; i < SW::PER; i++) {
+      const int k = SW::k_of(i, w, l);
+      if (k >= left) sw.off[i] -= (uint32_t)(WT ? k * a.ldw : k) * 2;
+    }
+  };
+  // and once it has come, each lane clears what it copied of them
+  auto clear = [&](int s, int buf) {
+    const int left = a.K - s * 64;
     if (left >= 64) return;
     typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
-    const uint32_t at = lds + (s % BUFS) * STAGE + w * (SX::PER * 1024) + lane * 16;
-    const uint32_t at_w = lds + (s % BUFS) * STAGE + SX::BYTES + w * (SW::PER * 1024) + lane * 16;
+    const int l = (int)anew(lane);
+    const uint32_t at = lds + buf * STAGE + w * (SX::PER * 1024) + l * 16;
+    const uint32_t at_w = lds + buf * STAGE + SX::BYTES + w * (SW::PER * 1024) + l * 16;
 #pragma unroll
     for (int i = 0; i < SX::PER; i++)
-      if ((XT ? SX::row_of(i, w, lane) : SX::col_of(i, w, lane)) >= left) *(lds_i32x4*)(uintptr_t)(at + i * 1024) = i32x4{0, 0, 0, 0};
+      if (SX::k_of(i, w, l) >= left) *(lds_i32x4*)(uintptr_t)(at + i * 1024) = i32x4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < SW::PER; i++)
-      if ((WT ? SW::row_of(i, w, lane) : SW::col_of(i, w, lane)) >= left) *(lds_i32x4*)(uintptr_t)(at_w + i * 1024) = i32x4{0, 0, 0, 0};
+      if (SW::k_of(i, w, l) >= left) *(lds_i32x4*)(uintptr_t)(at_w + i * 1024) = i32x4{0, 0, 0, 0};
   };
 
   f32x4 acc[C::NT][C::MT];
@@ -266,30 +298,80 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, De
 #pragma unroll
     for (int t = 0; t < C::MT; t++) acc[u][t] = f32x4{0, 0, 0, 0};
 
+  for (int s = 0; s < BUFS && s < stages; s++) {
+    ready(s);
 #pragma unroll
-  for (int s = 0; s < BUFS - 1; s++)
-    if (s < stages) copy(s);
-  for (int s = 0; s < stages; s++) {
-    // stage s has come, of every wave, and stage s - 1 is read: its place may be overwritten
-    if (s + BUFS - 2 < stages) loads_but<(BUFS - 2) * (SX::PER + SW::PER)>();
-    else loads_but<0>();
-    clear(s);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + BUFS - 1 < stages) copy(s + BUFS - 1);
-    const uint32_t at = lds + (s % BUFS) * STAGE;
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      i32x4 xv[C::MT], wv[C::NT];
-#pragma unroll
-      for (int u = 0; u < C::NT; u++) wv[u] = operand<TN, WT>(at + SX::BYTES, wn * C::NT + u, k, lane);
-#pragma unroll
-      for (int t = 0; t < C::MT; t++) xv[t] = operand<TM, XT>(at, wm * C::MT + t, k, lane);
-#pragma unroll
-      for (int t = 0; t < C::MT; t++)
-#pragma unroll
-        for (int u = 0; u < C::NT; u++) acc[u][t] = mfma_bf16(wv[u], xv[t], acc[u][t]);
-    }
+    for (int i = 0; i < PIECES; i++) piece(i, s);
+    sx.base += sx.step, sw.base += sw.step;
   }
+  if (stages >= BUFS) loads_but<(BUFS - 1) * PIECES>();
+  else loads_but<0>();
+  clear(0, 0);
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  // this wave's operands of half stage k
+  const uint32_t x_at[2] = {operand_at<TM, XT>(0, lane) + (XT ? 0 : wm * C::MT * 2048), operand_at<TM, XT>(1, lane) + (XT ? 0 : wm * C::MT * 2048)};
+  const uint32_t w_at[2] = {operand_at<TN, WT>(0, lane) + (WT ? 0 : wn * C::NT * 2048), operand_at<TN, WT>(1, lane) + (WT ? 0 : wn * C::NT * 2048)};
+  auto x_operand = [&](uint32_t at, int t) { return operand<TM, XT>(at, XT ? wm * C::MT + t : t); };
+  auto w_operand = [&](uint32_t at, int u) { return operand<TN, WT>(at, WT ? wn * C::NT + u : u); };
+  i32x4 xv[C::MT], wv[2][C::NT];
+  {
+    const uint32_t x0 = lds + x_at[0], w0 = lds + SX::BYTES + w_at[0];
+#pragma unroll
+    for (int u = 0; u < C::NT; u++) wv[0][u] = w_operand(w0, u);
+#pragma unroll
+    for (int t = 0; t < C::MT; t++) xv[t] = x_operand(x0, t);
+  }
+  int buf = 0;
+  // stage s; COPY: stage s + BUFS is to be copied; NEXT: there is a stage s + 1
+  auto stage = [&](int s, auto copy, auto next) {
+    constexpr bool COPY = decltype(copy)::value, NEXT = decltype(next)::value;
+    constexpr int MT = C::MT, NT = C::NT, BAR = MT > 4 ? 1 : 0;
+    const int after = buf + 1 == BUFS ? 0 : buf + 1;
+    const uint32_t x1 = anew(lds + buf * STAGE + x_at[1]), w1 = anew(lds + buf * STAGE + SX::BYTES + w_at[1]);
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+#pragma unroll
+      for (int u = 0; u < NT; u++) acc[u][t] = mfma_bf16(wv[0][u], xv[t], acc[u][t]);
+      xv[t] = x_operand(x1, t);
+#pragma unroll
+      for (int u = t * NT / MT; u < (t + 1) * NT / MT; u++) wv[1][u] = w_operand(w1, u);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const uint32_t x0 = anew(lds + after * STAGE + x_at[0]), w0 = anew(lds + after * STAGE + SX::BYTES + w_at[0]);
+    if constexpr (COPY) ready(s + BUFS);
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+#pragma unroll
+      for (int u = 0; u < NT; u++) acc[u][t] = mfma_bf16(wv[1][u], xv[t], acc[u][t]);
+      if constexpr (NEXT) {
+        if (t == BAR) {
+          // stage s + 1 has come, of every wave, and stage s is read: its place is free
+          if (COPY || s + BUFS == stages) loads_but<(BUFS - 2) * PIECES>();
+          else loads_but<0>();
+          if constexpr (!COPY) clear(s + 1, after);
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+          for (int v = 0; v < BAR; v++) xv[v] = x_operand(x0, v);
+        }
+        if (t >= BAR) {
+#pragma unroll
+          for (int u = t == BAR ? 0 : t * NT / MT; u < (t + 1) * NT / MT; u++) wv[0][u] = w_operand(w0, u);
+          xv[t] = x_operand(x0, t);
+          if constexpr (COPY) {
+#pragma unroll
+            for (int i = (t - BAR) * PIECES / (MT - BAR); i < (t - BAR + 1) * PIECES / (MT - BAR); i++) piece(i, buf);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (COPY) sx.base += sx.step, sw.base += sw.step;
+    buf = after;
+  };
+  int s = 0;
+  for (; s + BUFS < stages; s++) stage(s, std::true_type{}, std::true_type{});
+  for (; s + 1 < stages; s++) stage(s, std::false_type{}, std::true_type{});
+  stage(s, std::false_type{}, std::false_type{});
 
   const int mw = m0 + wm * C::MT * 16;  // this wave's first row
   if constexpr (LORA) {
@@ -301,42 +383,54 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, De
 #pragma unroll
   for (int t = 0; t < C::MT; t++) {
     const int m = mw + 16 * t + c;
-    if (m >= a.M) continue;
+    const bool row = m < a.M;  // (every lane goes on: store_two exchanges between them)
     if constexpr (END == END_SWIGLU) {
 #pragma unroll
-      for (int u = 0; u < C::NT / 2; u++) {
-        const int n = n0 + wn * (8 * C::NT) + 16 * u + 4 * q;
-        if (n >= a.half) continue;
-        const f32x4 g = acc[u][t], up = acc[u + C::NT / 2][t];
-        if (a.pre) {
-          *(f32x4*)(a.pre + (size_t)m * 2 * a.half + n) = g;
-          *(f32x4*)(a.pre + (size_t)m * 2 * a.half + a.half + n) = up;
-        }
-        f32x4 h;
+      for (int u = 0; u < C::NT / 2; u += 2) {
+        const int n = n0 + wn * (8 * C::NT) + 16 * u;  // of two tiles' units the first
+        i32x2 h[2] = {};
 #pragma unroll
-        for (int i = 0; i < 4; i++) h[i] = g[i] * sigmoid(g[i]) * up[i];
-        *(i32x2*)(a.out + m * a.ldo + n) = round4(h);
+        for (int v = 0; v < 2 && u + v < C::NT / 2; v++) {
+          const f32x4 g = acc[u + v][t], up = acc[u + v + C::NT / 2][t];
+          const int at = n + 16 * v + 4 * q;
+          if (a.pre && row && at < a.half) {
+            *(f32x4*)(a.pre + (size_t)m * 2 * a.half + at) = g;
+            *(f32x4*)(a.pre + (size_t)m * 2 * a.half + a.half + at) = up;
+          }
+          f32x4 s;
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[i] = g[i] * sigmoid(g[i]) * up[i];
+          h[v] = round4(s);
+        }
+        store_two(a.out + m * a.ldo + n, h[0], h[1], row ? (C::NT / 2 > 1 ? a.half - n : min(16, a.half - n)) : 0);
       }
     } else {
 #pragma unroll
-      for (int u = 0; u < C::NT; u++) {
-        const int n = n0 + (wn * C::NT + u) * 16 + 4 * q;
-        if (n >= a.N) continue;
+      for (int u = 0; u < C::NT; u += 2) {
+        const int n = n0 + (wn * C::NT + u) * 16;
         if constexpr (END == END_ROWS) {
-          *(i32x2*)(a.out + m * a.ldo + n) = round4(acc[u][t]);
-        } else if constexpr (END == END_PART) {
-          *(f32x4*)(a.parts + ((size_t)split * a.M + m) * a.N + n) = acc[u][t];
+          store_two(a.out + m * a.ldo + n, round4(acc[u][t]), round4(acc[u + 1][t]), row ? a.N - n : 0);
         } else {
-          const f32x4 g = *(const f32x4*)(a.pre + (size_t)m * 2 * a.half + n), up = *(const f32x4*)(a.pre + (size_t)m * 2 * a.half + a.half + n);
-          f32x4 dg, du;
+          i32x2 dg[2], du[2];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float s = sigmoid(g[i]), silu = g[i] * s;
-            dg[i] = acc[u][t][i] * up[i] * (s + silu * (1.0f - s));
-            du[i] = acc[u][t][i] * silu;
+          for (int v = 0; v < 2; v++) {
+            const int at = n + 16 * v + 4 * q;
+            f32x4 g{0, 0, 0, 0}, up{0, 0, 0, 0};
+            if (row && at < a.N) {
+              g = *(const f32x4*)(a.pre + (size_t)m * 2 * a.half + at);
+              up = *(const f32x4*)(a.pre + (size_t)m * 2 * a.half + a.half + at);
+            }
+            f32x4 g1, u1;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const float s = sigmoid(g[i]), silu = g[i] * s, d = acc[u + v][t][i];
+              g1[i] = d * up[i] * (s + silu * (1.0f - s));
+              u1[i] = d * silu;
+            }
+            dg[v] = round4(g1), du[v] = round4(u1);
           }
-          *(i32x2*)(a.out + m * a.ldo + n) = round4(dg);
-          *(i32x2*)(a.out + m * a.ldo + a.half + n) = round4(du);
+          store_two(a.out + m * a.ldo + n, dg[0], dg[1], row ? a.N - n : 0);
+          store_two(a.out + m * a.ldo + a.half + n, du[0], du[1], row ? a.N - n : 0);
         }
       }
     }

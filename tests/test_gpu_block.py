@@ -115,7 +115,9 @@ FFN_SHAPES = [  # rows, hidden, ffn, out: row counts at every kernel's borders, 
     (1, 8, 8, 8), (1, 2048, 512, 2048), (2, 72, 24, 40), (15, 2048, 768, 2048), (16, 264, 136, 264), (17, 512, 64, 8), (31, 64, 72, 520),
     (33, 200, 8, 1000), (63, 1000, 264, 64), (64, 2048, 512, 2048), (65, 2048, 512, 2048), (100, 8, 2048, 16), (127, 136, 128, 128),
     (128, 64, 64, 72), (129, 72, 1032, 200), (255, 320, 200, 256), (256, 256, 256, 256), (257, 1000, 264, 520), (300, 2048, 768, 2048),
-    (509, 2048, 512, 2048), (1391, 2048, 768, 2048), (2050, 2056, 2056, 2064)]
+    (509, 2048, 512, 2048), (1391, 2048, 768, 2048), (2050, 2056, 2056, 2064),
+    # every size of tile in every product, with ends inside tiles and stages
+    (777, 4104, 4104, 4104), (1500, 1032, 2056, 1544), (2600, 2568, 2056, 4104), (3333, 2056, 3976, 2056), (4000, 3080, 1000, 2056)]
 
 
 @pytest.mark.parametrize("T, H, I, O", FFN_SHAPES)
