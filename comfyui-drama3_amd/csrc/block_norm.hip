@@ -157,7 +157,7 @@ template <class TY, class TS, bool WAVE, int CH, int MOST>
 __global__ void __launch_bounds__(MOST) add_norm_kernel(Desc d) {
   __shared__ float slots[2][16];
   const int lane = lane_of<WAVE>(), lanes = lanes_of<WAVE>();
-  const int64_t row = WAVE ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x;
+  const int64_t row = WAVE ? (int64_t)blockIdx.y * 4 + threadIdx.x / 64 : blockIdx.y;
   if (row >= d.T) return;  // (whole waves, and then without barriers)
   float h[CH][8], w[CH][8];
 #pragma unroll
@@ -445,11 +445,12 @@ extern "C" int d3_add_norm(const d3_add_norm_desc* desc, void* stream) {
   const Desc& d = *desc;
   if (d.T == 0) return 0;
   if (!d.residual || (d.y && !d.h) || (d.weight && !d.n) || !(d.y || d.weight)) return fail("d3_add_norm: null pointer");
+  // (rows along y: a grid's x has room for 2^32 threads)
   by_types(d, [&](auto y, auto s) {
     by_width<512>(d.H, [&](auto wave, auto chunks, auto most, int lanes) {
       constexpr bool W = decltype(wave)::value;
       add_norm_kernel<decltype(y), decltype(s), W, decltype(chunks)::value, decltype(most)::value>
-          <<<W ? (unsigned)(((int64_t)d.T + 3) / 4) : (unsigned)d.T, lanes, 0, (hipStream_t)stream>>>(d);
+          <<<dim3(1, W ? (unsigned)(((int64_t)d.T + 3) / 4) : (unsigned)d.T), lanes, 0, (hipStream_t)stream>>>(d);
     });
   });
   const hipError_t e = hipGetLastError();

@@ -12,7 +12,7 @@ extern "C" int d3_gated_ffn_backward(const d3_gated_ffn_backward_desc* d, void* 
   if (H < 8 || H % 8 || I < 8 || I % 8 || O < 8 || O % 8) return fail(what + ": widths must be positive multiples of 8");
   if (2 * (int64_t)I * H > INT32_MAX || (int64_t)O * I > INT32_MAX) return fail(what + ": a weight of more than 2^31 elements");
   if (2 * (int64_t)I > MAX_LD || H > MAX_LD || O > MAX_LD) return fail(what + ": widths of more than 2^23");
-  if ((int64_t)((T + 127) / 128) * ((2 * I + H + 127) / 128 + 1) > INT32_MAX) return fail(what + ": too many rows for one launch");
+  if ((int64_t)((T + 15) / 16) * (std::max({2 * I, H, O}) / 8) > INT32_MAX) return fail(what + ": too many rows for one launch");
   if (T == 0) return 0;
   const hipStream_t s = (hipStream_t)stream;
   if (bad_rows(d->dout, O, O) || bad_rows(d->dgate_up_rows, 2 * (int64_t)I, I) || bad_rows(d->down, I, I) || bad_rows(d->pre, 2 * (int64_t)I, I))

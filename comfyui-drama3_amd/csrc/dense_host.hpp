@@ -27,7 +27,7 @@ inline int dense_tiles(const Dense& a, bool swiglu) {
 template <class C, bool XT, bool WT, int END, bool LORA = false>
 inline void launch_tile(const Dense& a, hipStream_t stream) {
   const int tiles = dense_tiles<C>(a, END == END_SWIGLU);
-  dense_tile_kernel<C, XT, WT, END, LORA><<<tiles, C::THREADS, 0, stream>>>(a, a, tiles);
+  dense_tile_kernel<C, XT, WT, END, LORA><<<dim3(1, tiles), C::THREADS, 0, stream>>>(a, a, tiles);
 }
 
 // The tile's size by what a stage of each takes, us, times the turns in which the 256 CUs take the tiles: 1.66 (256 x 256),

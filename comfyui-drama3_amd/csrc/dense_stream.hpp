@@ -25,6 +25,7 @@ D3_INLINE void stream_sums(const uint16_t* w, const uint16_t* const (&x)[RT], in
     for (int t = 0; t < RT; t++)
 #pragma unroll
       for (int i = 0; i < 2 * ST_AT_ONCE; i++) xv[t][i] = *(const i32x4*)(x[t] + s * 64 + i * 32 + 8 * q);
+    __builtin_amdgcn_sched_barrier(0);  // (all loads on their way before the first product)
 #pragma unroll
     for (int i = 0; i < 2 * ST_AT_ONCE; i++)
 #pragma unroll
@@ -86,18 +87,23 @@ __global__ void __launch_bounds__(ST_THREADS) dense_stream_kernel(Dense a) {
       open &= ~rows;
       if (i % ST_WAVES != wave) continue;
       const uint16_t* b = a.b + ((size_t)now * a.N + n) * a.rank;
-      for (int r = 8 * q; r - 8 * q < a.rank; r += 32) {
-        i32x4 bv{0, 0, 0, 0}, pv[RT];
-        if (r < a.rank) bv = *(const i32x4*)(b + r);
+      for (int r0 = 0; r0 < a.rank; r0 += 64) {
+        i32x4 bv[2], pv[2][RT];
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-          pv[t] = i32x4{0, 0, 0, 0};
-          if ((rows >> (16 * t + c) & 1) && r < a.rank) pv[t] = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + c) * a.rank + r);
+        for (int h = 0; h < 2; h++) {
+          const int r = r0 + 32 * h + 8 * q;
+          bv[h] = i32x4{0, 0, 0, 0};
+          if (r < a.rank) bv[h] = *(const i32x4*)(b + r);
+#pragma unroll
+          for (int t = 0; t < RT; t++) {
+            pv[h][t] = i32x4{0, 0, 0, 0};
+            if ((rows >> (16 * t + c) & 1) && r < a.rank) pv[h][t] = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + c) * a.rank + r);
+          }
         }
 #pragma unroll
         for (int t = 0; t < RT; t++) {
           // (the other rows keep their sums, also where this adapter holds infinities or NaN)
-          const f32x4 with = mfma_bf16(bv, pv[t], acc[t]);
+          const f32x4 with = mfma_bf16(bv[1], pv[1][t], mfma_bf16(bv[0], pv[0][t], acc[t]));
           acc[t] = rows >> (16 * t + c) & 1 ? with : acc[t];
         }
       }
@@ -117,34 +123,6 @@ __global__ void __launch_bounds__(ST_THREADS) dense_stream_kernel(Dense a) {
     *(int*)(a.out + m * a.ldo + u) = round4(h)[0];
   } else {
     if (n0 + 4 * q < a.N) *(i32x2*)(a.out + m * a.ldo + n0 + 4 * q) = round4(v);
-  }
-}
-
-// p[m, r] = alpha[a] sum_k x[m, k] A[a, r, k] for the adapter a of each row m, rounded to bf16 (the operand of the second product:
-// a relative 2^-9 of what the adapter adds). A workgroup takes 16 ranks and 16 RT rows, one adapter that they name
-// after the other (blockIdx.z of them at the start, gridDim.z apart); rows without one are not written, nor read later.
-template <int RT>
-__global__ void __launch_bounds__(ST_THREADS) lora_inner_kernel(const uint16_t* x, int64_t ldx, const uint16_t* A, const float* alpha,
-                                                                const int64_t* ids, int M, int K, int rank, int adapters, uint16_t* p) {
-  __shared__ f32x4 part[ST_WAVES][RT][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c = lane & 15;
-  const int m0 = blockIdx.y * (16 * RT), r0 = blockIdx.x * 16;
-  const int64_t id = lane < 16 * RT && m0 + lane < M ? ids[m0 + lane] : -1;
-  uint64_t open = __ballot(id >= 0 && id < adapters);
-  const uint16_t* xr[RT];
-#pragma unroll
-  for (int t = 0; t < RT; t++) xr[t] = x + min(m0 + 16 * t + c, M - 1) * ldx;
-  for (int i = 0; open; i++) {
-    const int64_t now = __shfl(id, __ffsll((unsigned long long)open) - 1);
-    const uint64_t rows = __ballot(id == now);
-    open &= ~rows;
-    if (i % (int)gridDim.z != (int)blockIdx.z) continue;
-    f32x4 acc[RT];
-    stream_sums<RT>(A + ((size_t)now * rank + min(r0 + c, rank - 1)) * K, xr, K, wave, acc);
-    const f32x4 v = join_waves<RT>(part, acc, wave) * alpha[now];
-    if (wave < RT && (rows >> (16 * wave + c) & 1) && r0 + 4 * q < rank)
-      *(i32x2*)(p + (size_t)(m0 + 16 * wave + c) * rank + r0 + 4 * q) = round4(v);
-    __syncthreads();  // (the sums are read: the next adapter's may take their place)
   }
 }
 

@@ -158,51 +158,71 @@ struct Tile {
   static constexpr int TM = 16 * WM * MT, TN = 16 * WN * NT;
 };
 
-// A row of m's adapters: the products of p and b, added for one adapter after the other that the wave's rows name.
+// The adapters of a wave's rows: the products of p and b, added for one adapter after the other that the rows name. The ids are read
+// before the loop over the stages, and the first adapter's operands before its last stage (most tiles have one).
 template <class C>
-D3_INLINE void add_adapters(const Dense& a, f32x4 (&acc)[C::NT][C::MT], int m0, const int (&n)[C::NT], int lane) {
-  const int q = lane >> 4, c = lane & 15;
-  int id[C::MT];        // -1: none
+struct RowAdapters {
+  int id[C::MT];         // of row c of tile t; -1: none
   uint32_t open[C::MT];  // rows whose adapter is still to come
+  int now;
+  i32x4 bv[C::NT], pv[C::MT];
+
+  D3_INLINE void begin(const Dense& a, int m0, int lane) {
 #pragma unroll
-  for (int t = 0; t < C::MT; t++) {
-    const int m = m0 + 16 * t + c;
-    const int64_t named = m < a.M ? a.ids[m] : -1;
-    id[t] = named >= 0 && named < a.adapters ? (int)named : -1;
-    open[t] = (uint32_t)__ballot(id[t] >= 0) & 0xFFFFu;
+    for (int t = 0; t < C::MT; t++) {
+      const int m = m0 + 16 * t + (lane & 15);
+      const int64_t named = m < a.M ? a.ids[m] : -1;
+      id[t] = named >= 0 && named < a.adapters ? (int)named : -1;
+    }
   }
-  while (true) {
-    int now = -1;
+  // the operands of ranks r0 .. r0 + 31 of adapter `now`, n this lane's rows of b
+  D3_INLINE void load(const Dense& a, int m0, const int (&n)[C::NT], int lane, int r0) {
+    const int r = r0 + 8 * (lane >> 4);
+    const uint16_t* b = a.b + (size_t)now * a.N * a.rank;
+#pragma unroll
+    for (int u = 0; u < C::NT; u++) {
+      bv[u] = i32x4{0, 0, 0, 0};
+      if (r < a.rank) bv[u] = *(const i32x4*)(b + (size_t)n[u] * a.rank + r);
+    }
+#pragma unroll
+    for (int t = 0; t < C::MT; t++) {
+      pv[t] = i32x4{0, 0, 0, 0};
+      if (id[t] == now && r < a.rank) pv[t] = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + (lane & 15)) * a.rank + r);
+    }
+  }
+  D3_INLINE void next() {
+    now = -1;
 #pragma unroll
     for (int t = C::MT - 1; t >= 0; t--)
       if (open[t]) now = __builtin_amdgcn_readlane(id[t], __ffs((int)open[t]) - 1);
-    if (now < 0) break;
-    const uint16_t* b = a.b + (size_t)now * a.N * a.rank;
+  }
+  D3_INLINE void first(const Dense& a, int m0, const int (&n)[C::NT], int lane) {
 #pragma unroll
-    for (int t = 0; t < C::MT; t++) open[t] &= ~(uint32_t)__ballot(id[t] == now);
-    for (int r0 = 0; r0 < a.rank; r0 += 32) {
-      const int r = r0 + 8 * q;
-      i32x4 bv[C::NT];
+    for (int t = 0; t < C::MT; t++) open[t] = (uint32_t)__ballot(id[t] >= 0) & 0xFFFFu;
+    next();
+    if (now >= 0) load(a, m0, n, lane, 0);
+  }
+  D3_INLINE void add(const Dense& a, f32x4 (&acc)[C::NT][C::MT], int m0, const int (&n)[C::NT], int lane) {
+    while (now >= 0) {
+      for (int r0 = 0;;) {
 #pragma unroll
-      for (int u = 0; u < C::NT; u++) {
-        bv[u] = i32x4{0, 0, 0, 0};
-        if (r < a.rank) bv[u] = *(const i32x4*)(b + (size_t)n[u] * a.rank + r);
+        for (int t = 0; t < C::MT; t++)
+#pragma unroll
+          for (int u = 0; u < C::NT; u++) {
+            // (the other rows keep their sums, also where this adapter holds infinities or NaN)
+            const f32x4 with = mfma_bf16(bv[u], pv[t], acc[u][t]);
+            acc[u][t] = id[t] == now ? with : acc[u][t];
+          }
+        if ((r0 += 32) >= a.rank) break;
+        load(a, m0, n, lane, r0);
       }
 #pragma unroll
-      for (int t = 0; t < C::MT; t++) {
-        const bool mine = id[t] == now;
-        i32x4 pv{0, 0, 0, 0};
-        if (mine && r < a.rank) pv = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + c) * a.rank + r);
-#pragma unroll
-        for (int u = 0; u < C::NT; u++) {
-          // (the other rows keep their sums, also where this adapter holds infinities or NaN)
-          const f32x4 with = mfma_bf16(bv[u], pv, acc[u][t]);
-          acc[u][t] = mine ? with : acc[u][t];
-        }
-      }
+      for (int t = 0; t < C::MT; t++) open[t] &= ~(uint32_t)__ballot(id[t] == now);
+      next();
+      if (now >= 0) load(a, m0, n, lane, 0);
     }
   }
-}
+};
 
 // The loop over the stages is one stream of MFMA groups (NT products of one row tile each). Beside each group go the LDS reads of
 // the operands that the half stage after needs, into the registers that the group has just read, and, in a stage's second
@@ -217,14 +237,14 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, De
   using SW = Side<TN, WT, W>;
   constexpr int STAGE = SX::BYTES + SW::BYTES;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[BUFS * STAGE];
-  const bool second = (int)blockIdx.x >= tiles_one;
+  const bool second = (int)blockIdx.y >= tiles_one;  // (along y: a grid's x has room for 2^32 threads)
   const Dense& a = second ? two : one;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, c = lane & 15, wn = w % C::WN, wm = w / C::WN;
   constexpr int UN = END == END_SWIGLU ? TN / 2 : TN;  // columns of out to a tile
   const int columns = END == END_SWIGLU ? a.half : a.N, nm = (a.M + TM - 1) / TM, nn = (columns + UN - 1) / UN;
   int tm, tn;
-  place((int)blockIdx.x - (second ? tiles_one : 0), nm, nn, tm, tn);
+  place((int)blockIdx.y - (second ? tiles_one : 0), nm, nn, tm, tn);
   const int m0 = tm * TM, n0 = tn * UN, stages = (a.K + 63) / 64;
   const uint32_t lds = lds_address(smem);
 
@@ -298,6 +318,9 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, De
 #pragma unroll
     for (int t = 0; t < C::MT; t++) acc[u][t] = f32x4{0, 0, 0, 0};
 
+  const int mw = m0 + wm * C::MT * 16;  // this wave's first row
+  [[maybe_unused]] RowAdapters<C> adapters;
+  if constexpr (LORA) adapters.begin(a, mw, lane);
   for (int s = 0; s < BUFS && s < stages; s++) {
     ready(s);
 #pragma unroll
@@ -371,15 +394,17 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, De
   int s = 0;
   for (; s + BUFS < stages; s++) stage(s, std::true_type{}, std::true_type{});
   for (; s + 1 < stages; s++) stage(s, std::false_type{}, std::true_type{});
-  stage(s, std::false_type{}, std::false_type{});
-
-  const int mw = m0 + wm * C::MT * 16;  // this wave's first row
   if constexpr (LORA) {
     int n[C::NT];
 #pragma unroll
     for (int u = 0; u < C::NT; u++) n[u] = w_row((wn * C::NT + u) * 16 + c);
-    add_adapters<C>(a, acc, mw, n, lane);
+    adapters.first(a, mw, n, lane);
+    stage(s, std::false_type{}, std::false_type{});
+    adapters.add(a, acc, mw, n, lane);
+  } else {
+    stage(s, std::false_type{}, std::false_type{});
   }
+
 #pragma unroll
   for (int t = 0; t < C::MT; t++) {
     const int m = mw + 16 * t + c;
