@@ -9,10 +9,12 @@ namespace d3 {
 int fail(const std::string& msg);
 int hip_fail(hipError_t err, const char* what);
 
-using Wide = Tile<2, 4, 8, 4, 2>;    // 256 x 256, 8 waves, one workgroup a CU
-using Long = Tile<2, 4, 8, 2, 3>;    // 256 x 128, 8 waves, one workgroup a CU
-using Narrow = Tile<2, 2, 4, 4, 2>;  // 128 x 128, 4 waves, two workgroups a CU
-using Small = Tile<2, 2, 2, 2, 4>;   // 64 x 64, 4 waves, two workgroups a CU
+using Wide = Tile<2, 4, 8, 4, 2>;        // 256 x 256, 8 waves, one workgroup a CU
+using Long = Tile<2, 4, 8, 2, 3, 2>;     // 256 x 128, 8 waves, one workgroup a CU
+using Narrow = Tile<2, 2, 4, 4, 2, 2>;   // 128 x 128, 4 waves, two workgroups a CU
+using Small = Tile<2, 2, 2, 2, 4, 8>;    // 64 x 64, 4 waves, two workgroups a CU
+using Thin = Tile<4, 1, 1, 2, 6, 8>;     // 64 x 32, 4 waves, two workgroups a CU
+using Flat = Tile<2, 2, 1, 2, 6>;        // 32 x 64, the same for a transposed w, of which LDS holds 64 columns at least
 
 constexpr int64_t MAX_LD = 1 << 23;  // (a tile's rows within 32-bit byte offsets)
 
@@ -31,41 +33,40 @@ inline void launch_tile(const Dense& a, hipStream_t stream) {
 }
 
 // The tile's size by what a stage of each takes, us, times the turns in which the 256 CUs take the tiles: 1.66 (256 x 256),
-// 0.86 (256 x 128), 0.9 for two of 128 x 128 (0.5 for one), 0.18 (64 x 64), measured with every CU at work. So the large
-// ones, which read least, where they come out even, and small ones for few rows. Measured, us, in this order:
-//   4096 x 4096 x 11008  285 295 308 -     4096 x 2048 x 6144  124  89  88 -     4096 x 12288 x 2048 (SwiGLU) 196 216 230 -
-//   1391 x 1536 x 2048     -   -  26 22     509 x 1024 x 2048    -   -  19 10
+// 0.86 (256 x 128), 0.9 for two of 128 x 128 (0.5 for one), 0.18 (64 x 64), 0.155 (64 x 32), measured with every CU at
+// work. So the large ones, which read least, where they come out even, and small ones for few rows. Measured, us, in this order:
+//   4096 x 4096 x 11008  285 295 308   -   -     4096 x 2048 x 6144  124  89  88   -   -
+//   4096 x 12288 x 2048  196 216 230   -   -  (SwiGLU)                1391 x 1536 x 2048   -   -  26  22   -  (SwiGLU)
+//    509 x 1024 x 2048     -   -  19 8.1 7.4  (SwiGLU)                  61 x 4096 x 2048   -  21  20 7.9 7.1
 template <bool XT, bool WT, int END, bool LORA = false>
 inline void launch_tiles(const Dense& a, hipStream_t stream) {
   constexpr bool SWIGLU = END == END_SWIGLU;
+  using Least = std::conditional_t<WT, Flat, Thin>;
   auto turns = [](int tiles, int at_once) { return (tiles + at_once - 1) / at_once; };
   const int narrow_tiles = dense_tiles<Narrow>(a, SWIGLU);
   const float wide = 1.66f * turns(dense_tiles<Wide>(a, SWIGLU), 256), tall = 0.86f * turns(dense_tiles<Long>(a, SWIGLU), 256);
   const float narrow = narrow_tiles <= 256 ? 0.5f : 0.9f * turns(narrow_tiles, 512);
-  const float small = 0.18f * turns(dense_tiles<Small>(a, SWIGLU), 256);
+  const float small = 0.18f * turns(dense_tiles<Small>(a, SWIGLU), 256), least = 0.155f * turns(dense_tiles<Least>(a, SWIGLU), 256);
   if (!LORA && wide <= std::min({tall, narrow, small})) {  // (with adapters the wide tile's sums do not stay in registers)
     if constexpr (!LORA) launch_tile<Wide, XT, WT, END, LORA>(a, stream);
   } else if (tall <= std::min(narrow, small)) {
     launch_tile<Long, XT, WT, END, LORA>(a, stream);
   } else if (narrow <= small) {
     launch_tile<Narrow, XT, WT, END, LORA>(a, stream);
-  } else {
+  } else if (XT || small <= least) {
     launch_tile<Small, XT, WT, END, LORA>(a, stream);
+  } else {
+    if constexpr (!XT) launch_tile<Least, XT, WT, END, LORA>(a, stream);
   }
 }
 
-template <int RT, int END, bool LORA>
-inline void launch_stream(const Dense& a, hipStream_t stream) {
-  const int columns = END == END_SWIGLU ? (a.half + 7) / 8 : (a.N + 15) / 16;
-  dense_stream_kernel<RT, END, LORA><<<dim3(columns, (a.M + 16 * RT - 1) / (16 * RT)), ST_THREADS, 0, stream>>>(a);
-}
-
-// products of rows with rows (both operands with their k side by side)
+// Products of rows with rows (both operands with their k side by side): up to 16 rows by streaming the weights, where a CU has
+// no more than one of their 16-row columns, else by tiles. Both, us: 5 x 1024 x 2048 (SwiGLU) 5.1 and 6.9, 16 rows 6.1 and
+// 6.9; 4 x 4096 x 4096 8.3 and 11.1, 16 rows 10.1 and 10.9; 4 x 6144 x 4096 12.9 and 11.1, 16 rows 16.8 and 11.3.
 template <int END, bool LORA>
 inline void launch_dense(const Dense& a, hipStream_t stream) {
-  if (a.M <= 16) launch_stream<1, END, LORA>(a, stream);
-  else if (a.M <= 32) launch_stream<2, END, LORA>(a, stream);
-  else if (a.M <= 64) launch_stream<4, END, LORA>(a, stream);
+  const int columns = END == END_SWIGLU ? (a.half + 7) / 8 : (a.N + 15) / 16;
+  if (a.M <= 16 && columns <= 256) dense_stream_kernel<END, LORA><<<columns, ST_THREADS, 0, stream>>>(a);
   else launch_tiles<false, false, END, LORA>(a, stream);
 }
 

@@ -73,7 +73,7 @@ template <int ROWS> constexpr int t_turns = ROWS >= 128 ? 7 : 3;
 template <int ROWS, bool T, int W>
 struct Side {
   static constexpr int BYTES = ROWS * 128, PER = BYTES / 1024 / W;
-  static_assert(BYTES % (1024 * W) == 0 && ROWS % 64 == 0);
+  static_assert(BYTES % (1024 * W) == 0 && (!T || ROWS % 64 == 0));
   const uint8_t* base;  // of the next stage to copy
   uint32_t step;        // bytes from stage to stage
   uint32_t off[PER];
@@ -152,20 +152,24 @@ D3_INLINE void place(int at, int nm, int nn, int& tm, int& tn) {
   tn = t / high;
 }
 
-template <int WM_, int WN_, int MT_, int NT_, int BUFS_>
+template <int WM_, int WN_, int MT_, int NT_, int BUFS_, int DEPTH_ = 1>
 struct Tile {
-  static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, BUFS = BUFS_, WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, BUFS = BUFS_, DEPTH = DEPTH_, WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int TM = 16 * WM * MT, TN = 16 * WN * NT;
 };
 
-// The adapters of a wave's rows: the products of p and b, added for one adapter after the other that the rows name. The ids are read
-// before the loop over the stages, and the first adapter's operands before its last stage (most tiles have one).
+// The adapters of a wave's rows: the products of p and b, by steps of 32 ranks and one adapter that the rows name. DEPTH steps'
+// operands are on their way at once (decode lines name about as many adapters as rows); the first of them from before the
+// last stage on, the ids from before the first.
 template <class C>
 struct RowAdapters {
+  static constexpr int DEPTH = C::DEPTH;
   int id[C::MT];         // of row c of tile t; -1: none
-  uint32_t open[C::MT];  // rows whose adapter is still to come
-  int now;
-  i32x4 bv[C::NT], pv[C::MT];
+  uint32_t open[C::MT];  // rows whose adapter is still to come in this run of ranks
+  int now, r0;           // the next step's
+  int who[DEPTH];        // the steps' adapters; -1: none
+  uint32_t at[C::NT];    // this lane's rows of an adapter's b, in bytes
+  i32x4 bv[DEPTH][C::NT], pv[C::MT];
 
   D3_INLINE void begin(const Dense& a, int m0, int lane) {
 #pragma unroll
@@ -175,51 +179,72 @@ struct RowAdapters {
       id[t] = named >= 0 && named < a.adapters ? (int)named : -1;
     }
   }
-  // the operands of ranks r0 .. r0 + 31 of adapter `now`, n this lane's rows of b
-  D3_INLINE void load(const Dense& a, int m0, const int (&n)[C::NT], int lane, int r0) {
-    const int r = r0 + 8 * (lane >> 4);
-    const uint16_t* b = a.b + (size_t)now * a.N * a.rank;
-#pragma unroll
-    for (int u = 0; u < C::NT; u++) {
-      bv[u] = i32x4{0, 0, 0, 0};
-      if (r < a.rank) bv[u] = *(const i32x4*)(b + (size_t)n[u] * a.rank + r);
-    }
-#pragma unroll
-    for (int t = 0; t < C::MT; t++) {
-      pv[t] = i32x4{0, 0, 0, 0};
-      if (id[t] == now && r < a.rank) pv[t] = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + (lane & 15)) * a.rank + r);
-    }
-  }
+  // the next adapter that a row names
   D3_INLINE void next() {
     now = -1;
 #pragma unroll
     for (int t = C::MT - 1; t >= 0; t--)
       if (open[t]) now = __builtin_amdgcn_readlane(id[t], __ffs((int)open[t]) - 1);
+#pragma unroll
+    for (int t = 0; t < C::MT; t++) open[t] &= ~(uint32_t)__ballot(id[t] == now);
   }
+  // sends the next step's loads
+  D3_INLINE void load(const Dense& a, int i, int lane) {
+    who[i] = now;
+    if (now < 0) return;
+    const uint8_t* b = (const uint8_t*)(a.b + (size_t)now * a.N * a.rank + r0);
+#pragma unroll
+    for (int u = 0; u < C::NT; u++) {
+      if (r0 + 32 <= a.rank) {
+        bv[i][u] = *(const i32x4*)(b + at[u]);
+      } else {
+        bv[i][u] = i32x4{0, 0, 0, 0};
+        if (r0 + 8 * (lane >> 4) < a.rank) bv[i][u] = *(const i32x4*)(b + at[u]);
+      }
+    }
+    next();
+  }
+  // the rows' inner products of ranks r0 .. r0 + 31 (where a row has an adapter: what the others hold is not used), and the first
+  // steps with them
+  D3_INLINE void ranks(const Dense& a, int m0, int lane) {
+    const int r = r0 + 8 * (lane >> 4);
+#pragma unroll
+    for (int t = 0; t < C::MT; t++) {
+      pv[t] = i32x4{0, 0, 0, 0};
+      if (id[t] >= 0 && r < a.rank) pv[t] = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + (lane & 15)) * a.rank + r);
+      open[t] = (uint32_t)__ballot(id[t] >= 0) & 0xFFFFu;
+    }
+    next();
+#pragma unroll
+    for (int i = 0; i < DEPTH; i++) load(a, i, lane);
+  }
+  // n: this lane's rows of b
   D3_INLINE void first(const Dense& a, int m0, const int (&n)[C::NT], int lane) {
 #pragma unroll
-    for (int t = 0; t < C::MT; t++) open[t] = (uint32_t)__ballot(id[t] >= 0) & 0xFFFFu;
-    next();
-    if (now >= 0) load(a, m0, n, lane, 0);
+    for (int u = 0; u < C::NT; u++) at[u] = (uint32_t)(n[u] * a.rank + 8 * (lane >> 4)) * 2;
+    r0 = 0;
+    ranks(a, m0, lane);
   }
-  D3_INLINE void add(const Dense& a, f32x4 (&acc)[C::NT][C::MT], int m0, const int (&n)[C::NT], int lane) {
-    while (now >= 0) {
-      for (int r0 = 0;;) {
+  D3_INLINE void add(const Dense& a, f32x4 (&acc)[C::NT][C::MT], int m0, int lane) {
+    while (true) {
+      while (who[0] >= 0) {
 #pragma unroll
-        for (int t = 0; t < C::MT; t++)
+        for (int i = 0; i < DEPTH; i++) {
+          if (who[i] >= 0) {
 #pragma unroll
-          for (int u = 0; u < C::NT; u++) {
-            // (the other rows keep their sums, also where this adapter holds infinities or NaN)
-            const f32x4 with = mfma_bf16(bv[u], pv[t], acc[u][t]);
-            acc[u][t] = id[t] == now ? with : acc[u][t];
+            for (int t = 0; t < C::MT; t++)
+#pragma unroll
+              for (int u = 0; u < C::NT; u++) {
+                // (the other rows keep their sums, also where this adapter holds infinities or NaN)
+                const f32x4 with = mfma_bf16(bv[i][u], pv[t], acc[u][t]);
+                acc[u][t] = id[t] == who[i] ? with : acc[u][t];
+              }
+            load(a, i, lane);
           }
-        if ((r0 += 32) >= a.rank) break;
-        load(a, m0, n, lane, r0);
+        }
       }
-#pragma unroll
-      for (int t = 0; t < C::MT; t++) open[t] &= ~(uint32_t)__ballot(id[t] == now);
-      next();
-      if (now >= 0) load(a, m0, n, lane, 0);
+      if ((r0 += 32) >= a.rank) return;
+      ranks(a, m0, lane);
     }
   }
 };
@@ -400,7 +425,7 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, De
     for (int u = 0; u < C::NT; u++) n[u] = w_row((wn * C::NT + u) * 16 + c);
     adapters.first(a, mw, n, lane);
     stage(s, std::false_type{}, std::false_type{});
-    adapters.add(a, acc, mw, n, lane);
+    adapters.add(a, acc, mw, lane);
   } else {
     stage(s, std::false_type{}, std::false_type{});
   }
