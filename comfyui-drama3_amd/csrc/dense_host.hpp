@@ -29,8 +29,14 @@ inline int dense_tiles(const Dense& a, bool swiglu) {
 template <class C, bool XT, bool WT, int END, bool LORA = false>
 inline void launch_tile(const Dense& a, hipStream_t stream) {
   const int tiles = dense_tiles<C>(a, END == END_SWIGLU);
-  dense_tile_kernel<C, XT, WT, END, LORA><<<dim3(1, tiles), C::THREADS, 0, stream>>>(a, a, tiles);
+  dense_tile_kernel<C, XT, WT, END, LORA><<<dim3(1, tiles), C::THREADS, 0, stream>>>(a);
 }
+
+enum TileSize { WIDE, LONG, NARROW, SMALL, LEAST };
+struct TilePlan {
+  TileSize size;
+  float cost;
+};
 
 // The tile's size by what a stage of each takes, us, times the turns in which the 256 CUs take the tiles: 1.66 (256 x 256),
 // 0.86 (256 x 128), 0.9 for two of 128 x 128 (0.5 for one), 0.18 (64 x 64), 0.155 (64 x 32), measured with every CU at
@@ -38,26 +44,63 @@ inline void launch_tile(const Dense& a, hipStream_t stream) {
 //   4096 x 4096 x 11008  285 295 308   -   -     4096 x 2048 x 6144  124  89  88   -   -
 //   4096 x 12288 x 2048  196 216 230   -   -  (SwiGLU)                1391 x 1536 x 2048   -   -  26  22   -  (SwiGLU)
 //    509 x 1024 x 2048     -   -  19 8.1 7.4  (SwiGLU)                  61 x 4096 x 2048   -  21  20 7.9 7.1
-template <bool XT, bool WT, int END, bool LORA = false>
-inline void launch_tiles(const Dense& a, hipStream_t stream) {
+template <bool XT, bool WT, int END, bool LORA>
+inline TilePlan plan_tiles(const Dense& a) {
   constexpr bool SWIGLU = END == END_SWIGLU;
   using Least = std::conditional_t<WT, Flat, Thin>;
   auto turns = [](int tiles, int at_once) { return (tiles + at_once - 1) / at_once; };
-  const int narrow_tiles = dense_tiles<Narrow>(a, SWIGLU);
-  const float wide = 1.66f * turns(dense_tiles<Wide>(a, SWIGLU), 256), tall = 0.86f * turns(dense_tiles<Long>(a, SWIGLU), 256);
-  const float narrow = narrow_tiles <= 256 ? 0.5f : 0.9f * turns(narrow_tiles, 512);
-  const float small = 0.18f * turns(dense_tiles<Small>(a, SWIGLU), 256), least = 0.155f * turns(dense_tiles<Least>(a, SWIGLU), 256);
-  if (!LORA && wide <= std::min({tall, narrow, small})) {  // (with adapters the wide tile's sums do not stay in registers)
-    if constexpr (!LORA) launch_tile<Wide, XT, WT, END, LORA>(a, stream);
-  } else if (tall <= std::min(narrow, small)) {
-    launch_tile<Long, XT, WT, END, LORA>(a, stream);
-  } else if (narrow <= small) {
-    launch_tile<Narrow, XT, WT, END, LORA>(a, stream);
-  } else if (XT || small <= least) {
-    launch_tile<Small, XT, WT, END, LORA>(a, stream);
-  } else {
-    if constexpr (!XT) launch_tile<Least, XT, WT, END, LORA>(a, stream);
+  const int narrow = dense_tiles<Narrow>(a, SWIGLU);
+  TilePlan best{LONG, 0.86f * turns(dense_tiles<Long>(a, SWIGLU), 256)};
+  auto try_size = [&](TileSize size, float cost) {
+    if (cost < best.cost) best = TilePlan{size, cost};
+  };
+  if (!LORA) try_size(WIDE, 1.66f * turns(dense_tiles<Wide>(a, SWIGLU), 256));  // (with adapters its sums do not stay in registers)
+  try_size(NARROW, narrow <= 256 ? 0.5f : 0.9f * turns(narrow, 512));
+  try_size(SMALL, 0.18f * turns(dense_tiles<Small>(a, SWIGLU), 256));
+  if (!XT) try_size(LEAST, 0.155f * turns(dense_tiles<Least>(a, SWIGLU), 256));
+  return best;
+}
+
+template <bool XT, bool WT, int END, bool LORA>
+inline void launch_plan(TileSize size, const Dense& a, hipStream_t stream) {
+  if constexpr (!LORA) {
+    if (size == WIDE) return launch_tile<Wide, XT, WT, END, LORA>(a, stream);
   }
+  if (size == LONG) launch_tile<Long, XT, WT, END, LORA>(a, stream);
+  else if (size == NARROW) launch_tile<Narrow, XT, WT, END, LORA>(a, stream);
+  else if (size == SMALL) launch_tile<Small, XT, WT, END, LORA>(a, stream);
+  if constexpr (!XT) {
+    if (size == LEAST) launch_tile<std::conditional_t<WT, Flat, Thin>, XT, WT, END, LORA>(a, stream);
+  }
+}
+
+// a's rows from m on
+template <bool XT>
+inline Dense rows_from(Dense a, int m, int rows) {
+  a.x += XT ? m : m * a.ldx;
+  a.out += m * a.ldo;
+  if (a.pre) a.pre += (int64_t)m * 2 * a.half;
+  if (a.ids) a.ids += m, a.p += (int64_t)m * a.rank;
+  a.M = rows;
+  return a;
+}
+
+// The whole product by one size of tile, or the rows that fill whole turns of 256 x 128 tiles by those and the rest by
+// what suits it, where that is 8% less (the second launch takes 3 us): 5000 x 4096 x 2048 is 2.5 turns.
+template <bool XT, bool WT, int END, bool LORA = false>
+inline void launch_tiles(const Dense& a, hipStream_t stream) {
+  const TilePlan whole = plan_tiles<XT, WT, END, LORA>(a);
+  const int columns = dense_tiles<Long>(Dense{.M = 1, .N = a.N, .K = a.K, .half = a.half}, END == END_SWIGLU);
+  const int full = dense_tiles<Long>(a, END == END_SWIGLU) / 256, rows = 256 * full / columns * Long::TM;
+  if (full >= 1 && rows > 0 && rows < a.M) {
+    const Dense rest = rows_from<XT>(a, rows, a.M - rows);
+    const TilePlan left = plan_tiles<XT, WT, END, LORA>(rest);
+    if (0.86f * full + left.cost < 0.92f * whole.cost) {
+      launch_tile<Long, XT, WT, END, LORA>(rows_from<XT>(a, 0, rows), stream);
+      return launch_plan<XT, WT, END, LORA>(left.size, rest, stream);
+    }
+  }
+  launch_plan<XT, WT, END, LORA>(whole.size, a, stream);
 }
 
 // Products of rows with rows (both operands with their k side by side): up to 16 rows by streaming the weights, where a CU has

@@ -256,20 +256,18 @@ struct RowAdapters {
 // 6144 x 2048 transposed twice 90, 114). A stage's one barrier stands after group BAR of its second half, when the reads of its own
 // operands are long done.
 template <class C, bool XT, bool WT, int END, bool LORA>
-__global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense one, Dense two, int tiles_one) {
+__global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense a) {
   constexpr int TM = C::TM, TN = C::TN, W = C::WAVES, BUFS = C::BUFS;
   using SX = Side<TM, XT, W>;
   using SW = Side<TN, WT, W>;
   constexpr int STAGE = SX::BYTES + SW::BYTES;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[BUFS * STAGE];
-  const bool second = (int)blockIdx.y >= tiles_one;  // (along y: a grid's x has room for 2^32 threads)
-  const Dense& a = second ? two : one;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, c = lane & 15, wn = w % C::WN, wm = w / C::WN;
   constexpr int UN = END == END_SWIGLU ? TN / 2 : TN;  // columns of out to a tile
   const int columns = END == END_SWIGLU ? a.half : a.N, nm = (a.M + TM - 1) / TM, nn = (columns + UN - 1) / UN;
   int tm, tn;
-  place((int)blockIdx.y - (second ? tiles_one : 0), nm, nn, tm, tn);
+  place((int)blockIdx.y, nm, nn, tm, tn);  // (along y: a grid's x has room for 2^32 threads)
   const int m0 = tm * TM, n0 = tn * UN, stages = (a.K + 63) / 64;
   const uint32_t lds = lds_address(smem);
 

@@ -3,6 +3,7 @@
     out = block.gated_ffn(n, gate_up, down)                          # a layer's shared expert, or a dense layer
     out = block.lora_linear(x, weight, a, b, alpha, ids)             # a projection beside every row's own adapter
     h, n = block.add_norm(y, residual, weight)                       # end of one block, start of the next
+    h, n = block.sparse_block(n, h, router, gate_up, down, 8, shared=(s_gate_up, s_down), next_weight=weight)  # all of it
 
 The reference has no kernels for these. Nothing waits on the host; outputs and workspaces are allocated per call, so calls on
 different streams are independent and each can be captured in a graph. The C entries are in include/drama3_moe.h.
@@ -118,6 +119,17 @@ def _dense(x, T, K, stride, w, N, index, swiglu=False, pre=None, lora=None, ids=
             x.data_ptr(), w.data_ptr(), out.data_ptr(), 0, a.data_ptr(), b.data_ptr(), alpha.data_ptr(), ids.data_ptr(),
             inner.data_ptr(), stride, T, N, K, swiglu, rank, count))
     return out
+
+
+def linear(x, weight):
+    """x weight^T of rows x [T, K] and a weight [N, K] (bfloat16): [T, N] bfloat16, float32 sums rounded once. A router's logits,
+    say; widths are multiples of 8. No backward pass."""
+    if torch.is_grad_enabled() and _any_grad(x, weight):
+        raise RuntimeError("linear has no backward pass: call it under torch.no_grad()")
+    index = x.get_device()
+    x, T, K, stride = _rows(x, "x", index)
+    weight, N = _weight(weight, "weight", None, K, index)
+    return _dense(x, T, K, stride, weight, N, index)
 
 
 def lora_linear(x, weight, a, b, alpha, ids):
@@ -412,3 +424,42 @@ def norm(x, weight, *, eps=1e-6, unit_offset=False, dtype=None):
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)):
         return _Norm.apply(x, weight, eps, unit_offset, dtype)
     return _norm(x, weight, eps, unit_offset, dtype, False)[0]
+
+
+# ------------------------------------------------------------------------------------------------------- the whole block
+def gate_weight(shared_gate):
+    """A shared expert's gate [H] bfloat16 as sparse_block reads it, laid out once: [8, H], zeros below."""
+    if shared_gate.dim() != 1 or shared_gate.dtype is not torch.bfloat16:
+        raise TypeError("shared_gate [H] bfloat16 expected")
+    out = shared_gate.new_zeros((8, shared_gate.numel()))
+    out[0] = shared_gate
+    return out
+
+
+def sparse_block(n, h, router, gate_up, down, topk, *, shared=None, shared_gate=None, shared_lora=(None, None), ids=None,
+                 next_weight=None, scale=1.0, eps=1e-6, unit_offset=False):
+    """A block's expert half on unquantized weights, from its normalized rows n [T, H] bfloat16 and the residual stream h [T, H] to
+    the next block's: (h, n) as add_norm returns them with `next_weight` (n None without it). router [E, H] gives the logits (E a
+    multiple of 8), kernels.route the experts, kernels.bf16_layer the routed layer on banks gate_up [E * 2I, H] and down [E * H, I].
+    shared = (gate_up, down): the shared expert, gated_ffn with `shared_lora` = (gate_up_lora, down_lora) of the rows' adapters
+    `ids`; it enters times sigmoid(n . gate) where shared_gate (gate_weight's) is given. The routed and the shared output are each
+    added to the stream, times `scale`, and rounded to its type. Any number of rows; nothing waits on the host. No backward pass."""
+    tensors = (n, h, router, gate_up, down, shared_gate, next_weight, *(shared or ()))
+    if torch.is_grad_enabled() and _any_grad(*tensors):
+        raise RuntimeError("sparse_block has no backward pass: call it under torch.no_grad()")
+    if shared is None and (shared_gate is not None or ids is not None or tuple(shared_lora) != (None, None)):
+        raise ValueError("shared_gate, shared_lora and ids go with shared")
+    if shared_gate is not None and shared_gate.dim() != 2:
+        raise ValueError("shared_gate as gate_weight lays it out expected")
+    options = {"scale": scale, "eps": eps, "unit_offset": unit_offset}
+    logits = linear(n, router)
+    if n.shape[0] == 0:
+        return add_norm(n, h, next_weight, **options)
+    experts, weights = kernels.route(logits, topk)
+    routed = kernels.bf16_layer(n, experts, weights, gate_up, down, router.shape[0])
+    if shared is None:
+        return add_norm(routed, h, next_weight, **options)
+    y = gated_ffn(n, *shared, gate_up_lora=shared_lora[0], down_lora=shared_lora[1], ids=ids)
+    gate = None if shared_gate is None else torch.sigmoid(linear(n, shared_gate)[:, :1])
+    h, _ = add_norm(routed, h, None, scale=scale)
+    return add_norm(y, h, next_weight, gate=gate, **options)

@@ -115,6 +115,20 @@ def test_norm_refusals():
         block.norm(z(2, 8), None)
 
 
+@pytest.mark.parametrize("error, match, call", [
+    (RuntimeError, "no backward", lambda: block.linear(z(2, 16).requires_grad_(), z(8, 16))),
+    (ValueError, "weight", lambda: block.linear(z(2, 16), z(12, 16))),
+    (TypeError, "shared_gate", lambda: block.gate_weight(z(16, dtype=F32))),
+    (ValueError, "go with shared", lambda: block.sparse_block(z(2, 16), z(2, 16), z(8, 16), z(8, 16), z(8, 16), 2, shared_gate=z(8, 16))),
+    (ValueError, "gate_weight", lambda: block.sparse_block(z(2, 16), z(2, 16), z(8, 16), z(8, 16), z(8, 16), 2, shared=(z(16, 16), z(16, 8)),
+                                                          shared_gate=z(16))),
+    (RuntimeError, "no backward", lambda: block.sparse_block(z(2, 16), z(2, 16).requires_grad_(), z(8, 16), z(8, 16), z(8, 16), 2)),
+])
+def test_sparse_block_refusals(error, match, call):
+    with pytest.raises(error, match=match):
+        call()
+
+
 @pytest.mark.parametrize("form, name", [(block._GatedFfn, "gated_ffn"), (block._AddNorm, "add_norm"), (block._Norm, "add_norm")])
 def test_autograd_backward_is_refused_under_capture(form, name, monkeypatch):
     """The autograd forms' backward passes, of which this is the first check."""

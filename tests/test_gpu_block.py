@@ -6,7 +6,7 @@ entry. A float32 sum of n products is taken to be off by at most n 2^-23 of the 
 import pytest
 import torch
 
-from drama3 import block
+from drama3 import block, kernels
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -574,6 +574,62 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@pytest.mark.parametrize("T", [0, 1, 3, 40, 300])
+@pytest.mark.parametrize("with_shared", [False, True])
+def test_sparse_block(T, with_shared):
+    """A block's expert half: router, routed experts, the shared expert with its rows' adapters and its gate, the residual stream
+    in float32 and the next norm. The routed experts' own error is taken from their layer (tested in test_gpu_direct_layer.py)."""
+    H, I, E, k, S = 512, 192, 16, 4, 136
+    gen = gen_of(T)
+    n, h = randn(gen, T, H), randn(gen, T, H, dtype=F32)
+    router, gate = randn(gen, E, H, scale=0.05), randn(gen, H, scale=0.05)
+    banks = randn(gen, E * 2 * I, H, scale=0.05), randn(gen, E * H, I, scale=0.05)
+    shared = randn(gen, 2 * S, H, scale=0.05), randn(gen, H, S, scale=0.05)
+    loras = lora_inputs(max(T, 1), H, 2 * S, 8, 3)[2:], lora_inputs(max(T, 1), S, H, 16, 3, seed=1)[2:]
+    ids = ids_of("mixed", T, 3)
+    weight = randn(gen, H, dtype=F32)
+    options = dict(shared=shared, shared_gate=block.gate_weight(gate), shared_lora=loras, ids=ids) if with_shared else {}
+    got_h, got_n = block.sparse_block(n, h, router, *banks, k, next_weight=weight, scale=0.5, **options)
+    assert got_h.dtype == F32 and got_n.dtype == BF and got_h.shape == got_n.shape == (T, H)
+    if T == 0:
+        return
+    experts, weights = kernels.route(block.linear(n, router), k)
+    routed = kernels.bf16_layer(n, experts, weights, *banks, E).to(F64)
+    want, err = h.to(F64) + 0.5 * routed, 4 * HALF[F32] * (h.to(F64).abs() + routed.abs())
+    if with_shared:
+        ref = Ffn(n, *shared, loras, ids)
+        v, e = dot(n.to(F64), gate.to(F64)[:, None])
+        e = rounded(v, e)  # the logit is rounded, and so is its sigmoid, whose slope is at most 1 / 4
+        g = torch.sigmoid(v)
+        want, err = want + 0.5 * g * ref.out, err + 0.5 * (g * ref.e_out + (0.25 * e + HALF[BF] * g) * (ref.out.abs() + ref.e_out)) \
+            + 8 * HALF[F32] * (want.abs() + ref.out.abs())
+    within(got_h, want, err + 1e-30)
+    rms = (want * want).mean(1, keepdim=True).sqrt()
+    rel = ((got_n.to(F64) - want / rms * weight.to(F64)).norm() / (want / rms * weight.to(F64)).norm()).item()
+    assert rel < 2.0 ** -8 + (err.norm() / want.norm()).item()
+
+
+def test_sparse_block_captured():
+    H, I, E = 512, 192, 16
+    gen = gen_of(3)
+    n, h = randn(gen, 20, H), randn(gen, 20, H)
+    args = randn(gen, E, H), randn(gen, E * 2 * I, H, scale=0.05), randn(gen, E * H, I, scale=0.05), 4
+    options = dict(shared=(randn(gen, 2 * I, H, scale=0.05), randn(gen, H, I, scale=0.05)), shared_gate=block.gate_weight(randn(gen, H)),
+                   next_weight=randn(gen, H))
+    block.sparse_block(n, h, *args, **options)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block.sparse_block(n, h, *args, **options)
+    for _ in range(3):
+        n.copy_(torch.randn(n.shape, device=DEV))
+        want = block.sparse_block(n, h, *args, **options)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
 
 
 def test_training_step_by_autograd():
