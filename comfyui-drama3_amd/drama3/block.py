@@ -41,23 +41,18 @@ def _at(t):
 MAX_ROW_STRIDE = 2 ** 23  # of a product's rows, in elements
 
 
-def _refuse_rows(x, what, cols, rows, index):
-    if x.dim() != 2 or x.dtype is not torch.bfloat16:
+def _rows(x, what, index, cols=None, rows=None):
+    """Rows x [T, K] bfloat16, checked, and as the products read them, (x, T, K, row stride): columns side by side, 16-byte aligned
+    (else a copy that is so)."""
+    if x.dtype is not torch.bfloat16 or x.dim() != 2:
         raise TypeError(f"{what} [T, K] bfloat16 expected")
     T, K = x.shape
-    if cols is not None and K != cols or rows is not None and T != rows:
-        raise ValueError(f"{what} [{'T' if rows is None else rows}, {'K' if cols is None else cols}] expected, not {[T, K]}")
+    if cols is not None and (K != cols or T != rows):
+        raise ValueError(f"{what} [{rows}, {cols}] expected, not {[T, K]}")
     if K < 8 or K % 8 or K > MAX_ROW_STRIDE or T > _INT_MAX:
         raise ValueError(f"{what} has a positive multiple of 8 columns up to {MAX_ROW_STRIDE}, not {K}")
     if x.get_device() != index:
         raise ValueError(f"{what} on the rows' device expected")
-
-
-def _rows(x, what, index, cols=None, rows=None):
-    """Rows x [T, K] bfloat16, checked, and as the products read them, (x, T, K, row stride): columns side by side, 16-byte aligned
-    (else a copy that is so)."""
-    _refuse_rows(x, what, cols, rows, index)
-    T, K = x.shape
     at = x.data_ptr()
     if x.is_contiguous():
         return (x if at % 16 == 0 else x.clone()), T, K, K
@@ -228,77 +223,80 @@ def gated_ffn(x, gate_up, down, *, gate_up_lora=None, down_lora=None, ids=None):
 
 # ------------------------------------------------------------------------------------------------------------- norms
 def _float_rows(t, what, index, shape=None):
-    """(rows [T, H], their stride), checked, float32 or bfloat16, with columns side by side (else a copy that has them so)."""
-    if t.dtype not in _TYPES or t.dim() != 2:
+    """(rows [T, H], their stride, type), checked, float32 or bfloat16, with columns side by side (else a copy that has them so)."""
+    kind = _TYPES.get(t.dtype)
+    if kind is None or t.dim() != 2:
         raise TypeError(f"{what} [T, H] float32 or bfloat16 expected")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{what} {list(shape)} expected, not {list(t.shape)}")
     if t.get_device() != index:
         raise ValueError(f"{what} on the rows' device expected")
     if t.is_contiguous():
-        return t, t.size(1)
+        return t, t.size(1), kind
     if t.stride(1) == 1 and t.stride(0) >= t.size(1):
-        return t, t.stride(0)
-    return t.contiguous(), t.size(1)
+        return t, t.stride(0), kind
+    return t.contiguous(), t.size(1), kind
 
 
 def _norm_weight(w, what, H, index):
-    if w.dtype not in _TYPES or w.shape != (H,):
+    """(weight, type), checked; (None, 0) without one."""
+    if w is None:
+        return None, 0
+    kind = _TYPES.get(w.dtype)
+    if kind is None or w.dim() != 1 or w.size(0) != H:
         raise ValueError(f"{what} [{H}] float32 or bfloat16 expected")
     if w.get_device() != index:
         raise ValueError(f"{what} on the rows' device expected")
-    return w.contiguous()
+    return w.contiguous(), kind
 
 
 def _norm_gate(gate, T, H, index):
-    """(gate, kind, row stride): 1 a value per row ([T, 1]), 2 per channel ([H] or [1, H]), 3 per element."""
-    if gate.dtype not in _TYPES or gate.get_device() != index:
+    """(gate, type, kind, row stride): 1 a value per row ([T, 1]), 2 per channel ([H] or [1, H]), 3 per element, 0 without one."""
+    if gate is None:
+        return None, 0, 0, 0
+    dtype, shape = _TYPES.get(gate.dtype), gate.shape
+    if dtype is None or gate.get_device() != index:
         raise ValueError("gate float32 or bfloat16 on the rows' device expected")
-    shape = gate.shape
     if shape == (T, H):
-        return _float_rows(gate, "gate", index) + (3,)
+        gate, stride, _ = _float_rows(gate, "gate", index)
+        return gate, dtype, 3, stride
     if shape == (T, 1):
-        return gate.contiguous(), 1, 1
+        return gate.contiguous(), dtype, 1, 1
     if shape == (H,) or shape == (1, H):
-        return gate.contiguous(), 0, 2
+        return gate.contiguous(), dtype, 2, 0
     raise ValueError(f"gate [{T}, 1], [{H}], [1, {H}] or [{T}, {H}] expected, not {list(shape)}")
 
 
-class _NormCall:
-    """A norm's inputs, checked (y None: the norm alone, n of type out_dtype)."""
+def _norm_launch(name, index, y, residual, weight, post, gate, T, H, out_type, scale, eps, unit_offset, dh=0, dn=0, h=0, n=0, rstd=0,
+                 dy=0, dresidual=0, dweight=0, dpost=0, dgate=0, partials=0, floats=0):
+    """C entry `name` on inputs as the functions above return them."""
+    (y, y_stride, _), (residual, stride, stream_type) = y, residual
+    (weight, weight_type), (post, post_type), (gate, gate_type, gate_kind, gate_stride) = weight, post, gate
+    kernels.launch(name, index, _lib.ADD_NORM.pack(
+        _at(y), residual.data_ptr(), _at(weight), _at(post), _at(gate), dh, dn, h, n, rstd, dy, dresidual, dweight, dpost, dgate,
+        partials, floats, y_stride, stride, gate_stride, out_type, stream_type, weight_type, post_type, gate_type, gate_kind, T, H,
+        scale, eps, unit_offset))
 
-    def __init__(self, y, residual, weight, post, gate, out_dtype=None):
-        index = self.index = residual.get_device()
-        self.residual, self.residual_stride = residual, _ = _float_rows(residual, "residual", index)
-        T, H = self.T, self.H = residual.shape
-        if not 1 <= H <= MAX_NORM_COLS or T > _INT_MAX:
-            raise ValueError(f"rows of 1 to {MAX_NORM_COLS} columns, not {H}")
-        self.y, self.y_stride = (None, 0) if y is None else _float_rows(y, "y", index, (T, H))
-        self.out_dtype = out_dtype if y is None else y.dtype
-        self.weight = None if weight is None else _norm_weight(weight, "weight", H, index)
-        self.post = None if post is None else _norm_weight(post, "post", H, index)
-        self.gate, self.gate_stride, self.gate_kind = (None, 0, 0) if gate is None else _norm_gate(gate, T, H, index)
 
-    def launch(self, name, scale, eps, unit_offset, dh=0, dn=0, h=0, n=0, rstd=0, dy=0, dresidual=0, dweight=0, dpost=0, dgate=0,
-               partials=0, floats=0):
-        y, weight, post, gate = self.y, self.weight, self.post, self.gate
-        kernels.launch(name, self.index, _lib.ADD_NORM.pack(
-            0 if y is None else y.data_ptr(), self.residual.data_ptr(), 0 if weight is None else weight.data_ptr(),
-            0 if post is None else post.data_ptr(), 0 if gate is None else gate.data_ptr(), dh, dn, h, n, rstd, dy, dresidual, dweight,
-            dpost, dgate, partials, floats, self.y_stride, self.residual_stride, self.gate_stride, _TYPES[self.out_dtype],
-            _TYPES[self.residual.dtype], 0 if weight is None else _TYPES[weight.dtype], 0 if post is None else _TYPES[post.dtype],
-            0 if gate is None else _TYPES[gate.dtype], self.gate_kind, self.T, self.H, scale, eps, unit_offset))
+def _norm_shape(residual):
+    T, H = residual.shape
+    if not 1 <= H <= MAX_NORM_COLS or T > _INT_MAX:
+        raise ValueError(f"rows of 1 to {MAX_NORM_COLS} columns, not {H}")
+    return T, H
 
 
 def _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, stats):
+    index = residual.get_device()
+    r = _float_rows(residual, "residual", index)
+    T, H = _norm_shape(residual)
     if y is None:
         raise TypeError("y [T, H] float32 or bfloat16 expected")
-    c = _NormCall(y, residual, weight, post, gate)
-    T, H = c.T, c.H
-    h = c.residual.new_empty((T, H))
-    n = None if weight is None else c.y.new_empty((T, H))
+    b = _float_rows(y, "y", index, residual.shape)
+    w, p, g = _norm_weight(weight, "weight", H, index), _norm_weight(post, "post", H, index), _norm_gate(gate, T, H, index)
+    h = residual.new_empty((T, H))
+    n = None if weight is None else y.new_empty((T, H))
     rstd = h.new_empty((2, T), dtype=torch.float32) if stats else None
-    c.launch("d3_add_norm", scale, eps, unit_offset, h=h.data_ptr(), n=_at(n), rstd=_at(rstd))
+    _norm_launch("d3_add_norm", index, b, r, w, p, g, T, H, b[2], scale, eps, unit_offset, 0, 0, h.data_ptr(), _at(n), _at(rstd))
     return h, n, rstd
 
 
@@ -321,8 +319,12 @@ def add_norm_backward(dh, dn, y, h, rstd, weight, *, post=None, gate=None, scale
 
 
 def _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, scale, unit_offset, needs, out_dtype):
-    c = _NormCall(y, h, weight, post, gate, out_dtype)
-    T, H, index, h = c.T, c.H, c.index, c.residual
+    index = h.get_device()
+    r = _float_rows(h, "h", index)
+    T, H = _norm_shape(h)
+    b = (None, 0, _TYPES[out_dtype]) if y is None else _float_rows(y, "y", index, h.shape)
+    out_dtype = out_dtype if y is None else y.dtype
+    w, p, g = _norm_weight(weight, "weight", H, index), _norm_weight(post, "post", H, index), _norm_gate(gate, T, H, index)
     if dh is None and dn is None:
         raise ValueError("dh or dn expected")
     if weight is None and dn is not None:
@@ -335,22 +337,22 @@ def _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, scale, unit_offse
             raise ValueError("dh of h's type and shape, on its device, expected")
         dh = dh.contiguous()
     if dn is not None:
-        if dn.dtype is not c.out_dtype or dn.shape != (T, H) or dn.get_device() != index:
+        if dn.dtype is not out_dtype or dn.shape != (T, H) or dn.get_device() != index:
             raise ValueError("dn of n's type and shape, on its device, expected")
         dn = dn.contiguous()
     if not any(needs):
         return (None,) * 5
     new = h.new_empty
-    dy = new((T, H), dtype=c.out_dtype) if y is not None and needs[0] else None
+    dy = new((T, H), dtype=out_dtype) if y is not None and needs[0] else None
     dresidual = new((T, H)) if needs[1] else None
     dweight = new((H,), dtype=weight.dtype) if weight is not None and needs[2] else None
     dpost = new((H,), dtype=post.dtype) if post is not None and needs[3] else None
     dgate = new(gate.shape, dtype=gate.dtype) if gate is not None and needs[4] else None
-    parts = (dweight is not None) + (dpost is not None) + (dgate is not None and c.gate_kind == 2)
+    parts = (dweight is not None) + (dpost is not None) + (dgate is not None and g[2] == 2)
     floats = parts * _lib.lib().d3_add_norm_partials(T, H)
     partials = new((floats,), dtype=torch.float32) if parts else None
-    c.launch("d3_add_norm_backward", scale, 0.0, unit_offset, _at(dh), _at(dn), h.data_ptr(), 0, rstd.data_ptr(), _at(dy),
-             _at(dresidual), _at(dweight), _at(dpost), _at(dgate), _at(partials), floats)
+    _norm_launch("d3_add_norm_backward", index, b, r, w, p, g, T, H, b[2], scale, 0.0, unit_offset, _at(dh), _at(dn), r[0].data_ptr(), 0,
+                 rstd.data_ptr(), _at(dy), _at(dresidual), _at(dweight), _at(dpost), _at(dgate), _at(partials), floats)
     return dy, dresidual, dweight, dpost, dgate
 
 
@@ -408,10 +410,13 @@ class _Norm(torch.autograd.Function):
 def _norm(x, weight, eps, unit_offset, dtype, stats):
     if weight is None:
         raise ValueError("weight [H] expected")
-    c = _NormCall(None, x, weight, None, None, dtype)
-    n = c.residual.new_empty((c.T, c.H), dtype=dtype)
-    rstd = n.new_empty((2, c.T), dtype=torch.float32) if stats else None
-    c.launch("d3_add_norm", 1.0, eps, unit_offset, n=n.data_ptr(), rstd=_at(rstd))
+    index = x.get_device()
+    r = _float_rows(x, "x", index)
+    T, H = _norm_shape(x)
+    n = x.new_empty((T, H), dtype=dtype)
+    rstd = n.new_empty((2, T), dtype=torch.float32) if stats else None
+    _norm_launch("d3_add_norm", index, (None, 0, 0), r, _norm_weight(weight, "weight", H, index), (None, 0), (None, 0, 0, 0), T, H,
+                 _TYPES[dtype], 1.0, eps, unit_offset, n=n.data_ptr(), rstd=_at(rstd))
     return n, rstd
 
 
