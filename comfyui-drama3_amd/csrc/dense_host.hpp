@@ -10,8 +10,8 @@ int fail(const std::string& msg);
 int hip_fail(hipError_t err, const char* what);
 
 using Wide = Tile<2, 4, 8, 4, 2>;        // 256 x 256, 8 waves, one workgroup a CU
-using Long = Tile<2, 4, 8, 2, 3, 2>;     // 256 x 128, 8 waves, one workgroup a CU
-using Narrow = Tile<2, 2, 4, 4, 2, 2>;   // 128 x 128, 4 waves, two workgroups a CU
+using Long = Tile<2, 4, 4, 4, 3, 2>;     // 128 x 256, the same
+using Square = Tile<2, 4, 4, 2, 4, 2>;   // 128 x 128, the same
 using Small = Tile<2, 2, 2, 2, 4, 8>;    // 64 x 64, 4 waves, two workgroups a CU
 using Thin = Tile<4, 1, 1, 2, 6, 8>;     // 64 x 32, 4 waves, two workgroups a CU
 using Flat = Tile<2, 2, 1, 2, 6>;        // 32 x 64, the same for a transposed w, of which LDS holds 64 columns at least
@@ -32,32 +32,32 @@ inline void launch_tile(const Dense& a, hipStream_t stream) {
   dense_tile_kernel<C, XT, WT, END, LORA><<<dim3(1, tiles), C::THREADS, 0, stream>>>(a);
 }
 
-enum TileSize { WIDE, LONG, NARROW, SMALL, LEAST };
+enum TileSize { WIDE, LONG, SQUARE, SMALL, LEAST };
 struct TilePlan {
   TileSize size;
   float cost;
 };
+constexpr float LONG_COST = 0.82f;
 
-// The tile's size by what a stage of each takes, us, times the turns in which the 256 CUs take the tiles: 1.66 (256 x 256),
-// 0.86 (256 x 128), 0.9 for two of 128 x 128 (0.5 for one), 0.18 (64 x 64), 0.155 (64 x 32), measured with every CU at
-// work. So the large ones, which read least, where they come out even, and small ones for few rows. Measured, us, in this order:
-//   4096 x 4096 x 11008  285 295 308   -   -     4096 x 2048 x 6144  124  89  88   -   -
-//   4096 x 12288 x 2048  196 216 230   -   -  (SwiGLU)                1391 x 1536 x 2048   -   -  26  22   -  (SwiGLU)
-//    509 x 1024 x 2048     -   -  19 8.1 7.4  (SwiGLU)                  61 x 4096 x 2048   -  21  20 7.9 7.1
+// The tile's size by what a stage of each takes, us, times the turns in which the 256 CUs take the tiles: 1.5 (256 x 256),
+// 0.82 (128 x 256), 0.45 (128 x 128), 0.17 (64 x 64), 0.155 (64 x 32), measured with the CUs at work. So the large ones, which read
+// least, where they come out even, and small ones for few rows. Measured, us, in this order (t: transposed operands):
+//   4096 x 4096 x 11008    266 276 317   -   -     4096 x 2048 x 6144    115  80  91   -   -     4096 x 12288 x 2048  154 170 200  -  -
+//   12288 x 2048 x 4096 tt 177 177 211   -   -     2048 x 6144 x 4096 tt  86 107 106   -   -     1391 x 1536 x 2048    -   -  16  19  -
+//    509 x 1024 x 2048       -   -   - 8.1 7.4       61 x 4096 x 2048      -   -   - 7.9 7.1     1391 x 2048 x 1536 t   -   -  13  16  -
 template <bool XT, bool WT, int END, bool LORA>
 inline TilePlan plan_tiles(const Dense& a) {
   constexpr bool SWIGLU = END == END_SWIGLU;
   using Least = std::conditional_t<WT, Flat, Thin>;
-  auto turns = [](int tiles, int at_once) { return (tiles + at_once - 1) / at_once; };
-  const int narrow = dense_tiles<Narrow>(a, SWIGLU);
-  TilePlan best{LONG, 0.86f * turns(dense_tiles<Long>(a, SWIGLU), 256)};
+  auto turns = [](int tiles) { return (float)((tiles + 255) / 256); };
+  TilePlan best{LONG, LONG_COST * turns(dense_tiles<Long>(a, SWIGLU))};
   auto try_size = [&](TileSize size, float cost) {
     if (cost < best.cost) best = TilePlan{size, cost};
   };
-  if (!LORA) try_size(WIDE, 1.66f * turns(dense_tiles<Wide>(a, SWIGLU), 256));  // (with adapters its sums do not stay in registers)
-  try_size(NARROW, narrow <= 256 ? 0.5f : 0.9f * turns(narrow, 512));
-  try_size(SMALL, 0.18f * turns(dense_tiles<Small>(a, SWIGLU), 256));
-  if (!XT) try_size(LEAST, 0.155f * turns(dense_tiles<Least>(a, SWIGLU), 256));
+  if (!LORA) try_size(WIDE, 1.5f * turns(dense_tiles<Wide>(a, SWIGLU)));  // (with adapters its sums do not stay in registers)
+  try_size(SQUARE, 0.45f * turns(dense_tiles<Square>(a, SWIGLU)));
+  try_size(SMALL, 0.17f * turns(dense_tiles<Small>(a, SWIGLU)));
+  if (!XT) try_size(LEAST, 0.155f * turns(dense_tiles<Least>(a, SWIGLU)));
   return best;
 }
 
@@ -67,7 +67,7 @@ inline void launch_plan(TileSize size, const Dense& a, hipStream_t stream) {
     if (size == WIDE) return launch_tile<Wide, XT, WT, END, LORA>(a, stream);
   }
   if (size == LONG) launch_tile<Long, XT, WT, END, LORA>(a, stream);
-  else if (size == NARROW) launch_tile<Narrow, XT, WT, END, LORA>(a, stream);
+  else if (size == SQUARE) launch_tile<Square, XT, WT, END, LORA>(a, stream);
   else if (size == SMALL) launch_tile<Small, XT, WT, END, LORA>(a, stream);
   if constexpr (!XT) {
     if (size == LEAST) launch_tile<std::conditional_t<WT, Flat, Thin>, XT, WT, END, LORA>(a, stream);
@@ -85,7 +85,7 @@ inline Dense rows_from(Dense a, int m, int rows) {
   return a;
 }
 
-// The whole product by one size of tile, or the rows that fill whole turns of 256 x 128 tiles by those and the rest by
+// The whole product by one size of tile, or the rows that fill whole turns of 128 x 256 tiles by those and the rest by
 // what suits it, where that is 8% less (the second launch takes 3 us): 5000 x 4096 x 2048 is 2.5 turns.
 template <bool XT, bool WT, int END, bool LORA = false>
 inline void launch_tiles(const Dense& a, hipStream_t stream) {
@@ -95,7 +95,7 @@ inline void launch_tiles(const Dense& a, hipStream_t stream) {
   if (full >= 1 && rows > 0 && rows < a.M) {
     const Dense rest = rows_from<XT>(a, rows, a.M - rows);
     const TilePlan left = plan_tiles<XT, WT, END, LORA>(rest);
-    if (0.86f * full + left.cost < 0.92f * whole.cost) {
+    if (LONG_COST * full + left.cost < 0.92f * whole.cost) {
       launch_tile<Long, XT, WT, END, LORA>(rows_from<XT>(a, 0, rows), stream);
       return launch_plan<XT, WT, END, LORA>(left.size, rest, stream);
     }
