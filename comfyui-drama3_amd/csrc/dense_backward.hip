@@ -8,7 +8,7 @@ extern "C" int d3_gated_ffn_backward(const d3_gated_ffn_backward_desc* d, void* 
   const std::string what = "d3_gated_ffn_backward";
   if (!d) return fail(what + ": null descriptor");
   const int T = d->T, H = d->H, I = d->I, O = d->O;
-  if (T < 0) return fail(what + ": negative sizes");
+  if (T < 0 || T > MAX_ROWS) return fail(what + ": 0 to 2^30 rows");
   if (H < 8 || H % 8 || I < 8 || I % 8 || O < 8 || O % 8) return fail(what + ": widths must be positive multiples of 8");
   if (2 * (int64_t)I * H > INT32_MAX || (int64_t)O * I > INT32_MAX) return fail(what + ": a weight of more than 2^31 elements");
   if (2 * (int64_t)I > MAX_LD || H > MAX_LD || O > MAX_LD) return fail(what + ": widths of more than 2^23");
@@ -28,23 +28,23 @@ extern "C" int d3_gated_ffn_backward(const d3_gated_ffn_backward_desc* d, void* 
     a.out = (uint16_t*)d->dgate_up_rows, a.ldo = 2 * (int64_t)I, a.pre = (float*)d->pre;
     launch_tiles<false, true, END_DSWIGLU>(a, s);
   }
+  DenseSet set{};
+  set.rows = -1;
   if (d->dx) {
-    Dense a{};
+    Dense& a = set.product[set.rows = set.count++];
     a.x = (const uint16_t*)d->dgate_up_rows, a.ldx = 2 * (int64_t)I, a.w = (const uint16_t*)d->gate_up, a.ldw = H, a.M = T, a.N = H, a.K = 2 * I;
     a.out = (uint16_t*)d->dx, a.ldo = H;
-    launch_tiles<false, true, END_ROWS>(a, s);
   }
   if (d->dgate_up) {
-    Dense a{};
+    Dense& a = set.product[set.count++];
     a.x = (const uint16_t*)d->dgate_up_rows, a.ldx = 2 * (int64_t)I, a.w = (const uint16_t*)d->x, a.ldw = d->x_stride, a.M = 2 * I, a.N = H, a.K = T;
     a.out = (uint16_t*)d->dgate_up, a.ldo = H;
-    launch_tiles<true, true, END_ROWS>(a, s);
   }
   if (d->ddown) {
-    Dense a{};
+    Dense& a = set.product[set.count++];
     a.x = (const uint16_t*)d->dout, a.ldx = O, a.w = (const uint16_t*)d->hidden, a.ldw = I, a.M = O, a.N = I, a.K = T;
     a.out = (uint16_t*)d->ddown, a.ldo = I;
-    launch_tiles<true, true, END_ROWS>(a, s);
   }
+  if (set.count) launch_dense_set(set, s);
   return launched("d3_gated_ffn_backward launch");
 }

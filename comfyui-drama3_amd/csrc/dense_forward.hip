@@ -7,7 +7,7 @@ using namespace d3;
 namespace {
 
 int check_dense(const std::string& what, const Dense& a) {
-  if (a.M < 0) return fail(what + ": negative sizes");
+  if (a.M < 0 || a.M > MAX_ROWS) return fail(what + ": 0 to 2^30 rows");
   if (a.K < 8 || a.K % 8 || a.N < 8 || a.N % 8) return fail(what + ": widths must be positive multiples of 8");
   if ((int64_t)a.N * a.K > INT32_MAX) return fail(what + ": a weight of more than 2^31 elements");
   if (a.M == 0) return 0;

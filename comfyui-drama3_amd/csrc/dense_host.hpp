@@ -17,6 +17,7 @@ using Thin = Tile<4, 1, 1, 2, 6, 8>;     // 64 x 32, 4 waves, two workgroups a C
 using Flat = Tile<2, 2, 1, 2, 6>;        // 32 x 64, the same for a transposed w, of which LDS holds 64 columns at least
 
 constexpr int64_t MAX_LD = 1 << 23;  // (a tile's rows within 32-bit byte offsets)
+constexpr int MAX_ROWS = 1 << 30;
 
 inline bool bad_rows(const void* p, int64_t ld, int64_t cols) { return !p || ((uintptr_t)p & 15u) || ld % 8 || ld < cols || ld > MAX_LD; }
 
@@ -40,7 +41,7 @@ struct TilePlan {
 constexpr float LONG_COST = 0.82f;
 
 // The tile's size by what a stage of each takes, us, times the turns in which the 256 CUs take the tiles: 1.5 (256 x 256),
-// 0.82 (128 x 256), 0.45 (128 x 128), 0.17 (64 x 64), 0.155 (64 x 32), measured with the CUs at work. So the large ones, which read
+// 0.82 (128 x 256), 0.45 (128 x 128; 0.5 in several turns), 0.17 (64 x 64), 0.155 (64 x 32), measured with the CUs at work. So the large ones, which read
 // least, where they come out even, and small ones for few rows. Measured, us, in this order (t: transposed operands):
 //   4096 x 4096 x 11008    266 276 317   -   -     4096 x 2048 x 6144    115  80  91   -   -     4096 x 12288 x 2048  154 170 200  -  -
 //   12288 x 2048 x 4096 tt 177 177 211   -   -     2048 x 6144 x 4096 tt  86 107 106   -   -     1391 x 1536 x 2048    -   -  16  19  -
@@ -55,7 +56,8 @@ inline TilePlan plan_tiles(const Dense& a) {
     if (cost < best.cost) best = TilePlan{size, cost};
   };
   if (!LORA) try_size(WIDE, 1.5f * turns(dense_tiles<Wide>(a, SWIGLU)));  // (with adapters its sums do not stay in registers)
-  try_size(SQUARE, 0.45f * turns(dense_tiles<Square>(a, SWIGLU)));
+  const float square = turns(dense_tiles<Square>(a, SWIGLU));
+  try_size(SQUARE, (square > 1 ? 0.5f : 0.45f) * square);
   try_size(SMALL, 0.17f * turns(dense_tiles<Small>(a, SWIGLU)));
   if (!XT) try_size(LEAST, 0.155f * turns(dense_tiles<Least>(a, SWIGLU)));
   return best;
@@ -101,6 +103,40 @@ inline void launch_tiles(const Dense& a, hipStream_t stream) {
     }
   }
   launch_plan<XT, WT, END, LORA>(whole.size, a, stream);
+}
+
+// A set of products in one launch. The size of tile, one for all of them, by the same costs of a stage: its share of all tiles'
+// stages, or the longest tile's, and half of the shortest's for the end.
+template <class C>
+inline void launch_set(DenseSet set, hipStream_t stream) {
+  int all = 0;
+  for (int i = 0; i < set.count; i++) all += set.tiles[i] = (dense_tiles<C>(set.product[i], false) + 7) / 8 * 8;
+  dense_set_kernel<C><<<dim3(1, all), C::THREADS, 0, stream>>>(set);
+}
+template <class C>
+inline float set_cost(const DenseSet& set, float stage) {
+  float all = 0.0f, most = 0.0f, least = 1e30f;
+  for (int i = 0; i < set.count; i++) {
+    const float stages = (float)((set.product[i].K + 63) / 64);
+    all += dense_tiles<C>(set.product[i], false) * stages;
+    most = std::max(most, stages), least = std::min(least, stages);
+  }
+  return stage * std::max(all / 256.0f + 0.5f * least, most);
+}
+inline void launch_dense_set(DenseSet set, hipStream_t stream) {
+  // the longest first
+  for (int i = 1; i < set.count; i++)
+    for (int j = i; j > 0 && set.product[j].K > set.product[j - 1].K; j--) {
+      std::swap(set.product[j], set.product[j - 1]);
+      if (set.rows == j) set.rows = j - 1;
+      else if (set.rows == j - 1) set.rows = j;
+    }
+  const float wide = set_cost<Wide>(set, 1.5f), tall = set_cost<Long>(set, LONG_COST), square = set_cost<Square>(set, 0.45f);
+  const float small = set_cost<Small>(set, 0.17f);
+  if (wide <= std::min({tall, square, small})) launch_set<Wide>(set, stream);
+  else if (tall <= std::min(square, small)) launch_set<Long>(set, stream);
+  else if (square <= small) launch_set<Square>(set, stream);
+  else launch_set<Small>(set, stream);
 }
 
 // Products of rows with rows (both operands with their k side by side): up to 16 rows by streaming the weights, where a CU has

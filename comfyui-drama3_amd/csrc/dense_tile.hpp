@@ -155,7 +155,7 @@ D3_INLINE void place(int at, int nm, int nn, int& tm, int& tn) {
 template <int WM_, int WN_, int MT_, int NT_, int BUFS_, int DEPTH_ = 1>
 struct Tile {
   static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, BUFS = BUFS_, DEPTH = DEPTH_, WAVES = WM * WN, THREADS = 64 * WAVES;
-  static constexpr int TM = 16 * WM * MT, TN = 16 * WN * NT;
+  static constexpr int TM = 16 * WM * MT, TN = 16 * WN * NT, LDS = BUFS * (TM + TN) * 128;
 };
 
 // The adapters of a wave's rows: the products of p and b, by steps of 32 ranks and one adapter that the rows name. DEPTH steps'
@@ -256,18 +256,17 @@ struct RowAdapters {
 // 6144 x 2048 transposed twice 90, 114). A stage's one barrier stands after group BAR of its second half, when the reads of its own
 // operands are long done.
 template <class C, bool XT, bool WT, int END, bool LORA>
-__global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense a) {
+D3_INLINE void dense_tile(const Dense& a, int tile, uint8_t* smem) {
   constexpr int TM = C::TM, TN = C::TN, W = C::WAVES, BUFS = C::BUFS;
   using SX = Side<TM, XT, W>;
   using SW = Side<TN, WT, W>;
   constexpr int STAGE = SX::BYTES + SW::BYTES;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[BUFS * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, c = lane & 15, wn = w % C::WN, wm = w / C::WN;
   constexpr int UN = END == END_SWIGLU ? TN / 2 : TN;  // columns of out to a tile
   const int columns = END == END_SWIGLU ? a.half : a.N, nm = (a.M + TM - 1) / TM, nn = (columns + UN - 1) / UN;
   int tm, tn;
-  place((int)blockIdx.y, nm, nn, tm, tn);  // (along y: a grid's x has room for 2^32 threads)
+  place(tile, nm, nn, tm, tn);
   const int m0 = tm * TM, n0 = tn * UN, stages = (a.K + 63) / 64;
   const uint32_t lds = lds_address(smem);
 
@@ -483,6 +482,31 @@ __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense a) {
       }
     }
   }
+}
+
+// (tiles along y: a grid's x has room for 2^32 threads)
+template <class C, bool XT, bool WT, int END, bool LORA>
+__global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
+  dense_tile<C, XT, WT, END, LORA>(a, blockIdx.y, smem);
+}
+
+// Up to three products that do not need each other in one launch, the longest first: rows with a transposed w (the gradient of
+// rows), or both transposed (of weights). Their tiles fill the CUs together where each alone would leave some idle at its end.
+struct DenseSet {
+  Dense product[3];
+  int tiles[3];  // rounded up to a multiple of 8, one for each XCD
+  int count, rows;  // rows: which of them is a gradient of rows
+};
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 2) dense_set_kernel(DenseSet set) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
+  int at = blockIdx.y, i = 0;
+  while (i < set.count - 1 && at >= set.tiles[i]) at -= set.tiles[i++];
+  const Dense& a = set.product[i];
+  if (at >= (a.M + C::TM - 1) / C::TM * ((a.N + C::TN - 1) / C::TN)) return;
+  if (i == set.rows) dense_tile<C, false, true, END_ROWS, false>(a, at, smem);
+  else dense_tile<C, true, true, END_ROWS, false>(a, at, smem);
 }
 
 }  // namespace d3

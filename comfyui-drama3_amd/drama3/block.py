@@ -39,6 +39,7 @@ def _at(t):
 
 # ---------------------------------------------------------------------------------------------------------- products
 MAX_ROW_STRIDE = 2 ** 23  # of a product's rows, in elements
+MAX_ROWS = 2 ** 30
 
 
 def _rows(x, what, index, cols=None, rows=None):
@@ -49,8 +50,8 @@ def _rows(x, what, index, cols=None, rows=None):
     T, K = x.shape
     if cols is not None and (K != cols or T != rows):
         raise ValueError(f"{what} [{rows}, {cols}] expected, not {[T, K]}")
-    if K < 8 or K % 8 or K > MAX_ROW_STRIDE or T > _INT_MAX:
-        raise ValueError(f"{what} has a positive multiple of 8 columns up to {MAX_ROW_STRIDE}, not {K}")
+    if K < 8 or K % 8 or K > MAX_ROW_STRIDE or T > MAX_ROWS:
+        raise ValueError(f"{what} has up to {MAX_ROWS} rows of a positive multiple of 8 columns up to {MAX_ROW_STRIDE}, not {[T, K]}")
     if x.get_device() != index:
         raise ValueError(f"{what} on the rows' device expected")
     at = x.data_ptr()

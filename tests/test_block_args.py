@@ -117,6 +117,7 @@ def test_norm_refusals():
 
 @pytest.mark.parametrize("error, match, call", [
     (RuntimeError, "no backward", lambda: block.linear(z(2, 16).requires_grad_(), z(8, 16))),
+    (ValueError, "rows", lambda: block.linear(z(1, 16).expand(2 ** 30 + 1, 16), z(8, 16))),
     (ValueError, "weight", lambda: block.linear(z(2, 16), z(12, 16))),
     (TypeError, "shared_gate", lambda: block.gate_weight(z(16, dtype=F32))),
     (ValueError, "go with shared", lambda: block.sparse_block(z(2, 16), z(2, 16), z(8, 16), z(8, 16), z(8, 16), 2, shared_gate=z(8, 16))),
@@ -153,7 +154,8 @@ P = 1 << 20  # an address that passes the checks of alignment; nothing is launch
     (b"multiples of 8", {"K": 12}),
     (b"multiples of 8", {"N": 20}),
     (b"multiples of 8 each", {"N": 24, "swiglu": 1}),
-    (b"negative", {"T": -1}),
+    (b"2^30 rows", {"T": -1}),
+    (b"2^30 rows", {"T": 2 ** 30 + 1}),
     (b"2\\^31", {"N": 1 << 20, "K": 1 << 12}),
     (b"null pointer", {"x": None}),
     (b"null pointer", {"w": P + 8}),

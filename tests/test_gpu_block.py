@@ -231,6 +231,24 @@ def test_gated_ffn_unaligned_and_strided():
     assert torch.equal(block.gated_ffn(same, gate_up, down), block.gated_ffn(same.contiguous(), gate_up, down))
 
 
+def test_more_rows_than_65536_tiles():
+    """Grids whose tiles or rows pass 2^16, and rows past 4 GiB: each row is its own product, checked where they start, end and pass
+    the borders."""
+    gen = gen_of(11)
+    T = 64 * 65536 + 70
+    x, w = randn(gen, T, 8), randn(gen, 16, 8)
+    out = block.linear(x, w)
+    some = torch.cat([torch.arange(a, a + 70, device=DEV) for a in (0, 64 * 65535, 64 * 65536, T - 70)])
+    v, e = dot(x[some].to(F64), w.to(F64).T)
+    within(out[some], v, rounded(v, e))
+    wide = torch.zeros((70000, 32768), device=DEV, dtype=BF)  # 4.6 GB
+    at = [0, 65535, 65536, 69999]
+    wide[at] = randn(gen, 4, 32768)
+    w = randn(gen, 8, 32768, scale=0.01)
+    v, e = dot(wide[at].to(F64), w.to(F64).T)
+    within(block.linear(wide, w)[at], v, rounded(v, e))
+
+
 # ---------------------------------------------------------------------------------------------------------- adapters
 def lora_inputs(T, K, N, rank, count, seed=0):
     gen = gen_of(seed)
@@ -424,6 +442,20 @@ def test_add_norm_forms(gate, post, of, stream, weights):
 def test_add_norm_rows(T):
     norm_check(T, 512, BF, BF, "channel", True, seed=T)
     norm_check(T, 72, F32, F32, "row", False, seed=T)
+
+
+def test_add_norm_more_rows_than_a_dimension_has_threads():
+    """2^24 + 3 rows (of whole workgroups: 2^33 threads), checked at their ends."""
+    T, H = 2 ** 24 + 3, 520
+    gen = gen_of(12)
+    residual = torch.ones((T, H), device=DEV, dtype=BF)
+    some = torch.tensor([0, 1, 2 ** 23, 2 ** 24 - 1, 2 ** 24, T - 1], device=DEV)
+    residual[some] = randn(gen, 6, H)
+    weight = randn(gen, H)
+    out = block.norm(residual, weight)
+    want = residual[some].to(F64)
+    want = want / (want ** 2).mean(1, keepdim=True).add(1e-6).sqrt() * weight.to(F64)
+    within(out[some], want, rounded(want, want.abs() * 100 * 2.0 ** -24))
 
 
 def test_add_norm_without_rows():
