@@ -10,10 +10,10 @@ int fail(const std::string& msg);
 int hip_fail(hipError_t err, const char* what);
 
 using Wide = Tile<2, 4, 8, 4, 2>;        // 256 x 256, 8 waves, one workgroup a CU
-using Long = Tile<2, 4, 4, 4, 3, 2>;     // 128 x 256, the same
-using Square = Tile<2, 4, 4, 2, 4, 2>;   // 128 x 128, the same
-using Small = Tile<2, 2, 2, 2, 4, 8>;    // 64 x 64, 4 waves, two workgroups a CU
-using Thin = Tile<4, 1, 1, 2, 6, 8>;     // 64 x 32, 4 waves, two workgroups a CU
+using Long = Tile<2, 4, 4, 4, 3, 1>;     // 128 x 256, the same
+using Square = Tile<2, 4, 4, 2, 4, 1>;   // 128 x 128, the same
+using Small = Tile<2, 2, 2, 2, 4, 4>;    // 64 x 64, 4 waves, two workgroups a CU
+using Thin = Tile<4, 1, 1, 2, 6, 4>;     // 64 x 32, 4 waves, two workgroups a CU
 using Flat = Tile<2, 2, 1, 2, 6>;        // 32 x 64, the same for a transposed w, of which LDS holds 64 columns at least
 
 constexpr int64_t MAX_LD = 1 << 23;  // (a tile's rows within 32-bit byte offsets)

@@ -158,18 +158,22 @@ struct Tile {
   static constexpr int TM = 16 * WM * MT, TN = 16 * WN * NT, LDS = BUFS * (TM + TN) * 128;
 };
 
-// The adapters of a wave's rows: the products of p and b, by steps of 32 ranks and one adapter that the rows name. DEPTH steps'
-// operands are on their way at once (decode lines name about as many adapters as rows); the first of them from before the
-// last stage on, the ids from before the first.
+// The adapters of a wave's rows: the products of p and b, by steps of one adapter that the rows name and up to 64 ranks, DEPTH
+// steps' operands on their way at once (decode lines name about as many adapters as rows); the first of them from before the
+// last stage on, the ids from before the first. Past the last adapter a step reads adapter 0 again, whose sums no row takes: a
+// branch a step costs more (500 rows of 24 adapters by turns, rank 32, 2048 x 2048: 15.4 us, 14.6 without). 61 rows of 24 adapters
+// of rank 64 by turns, 4096 x 2048: 7 us without adapters, 16.5 with them (8 steps at a time: 18.3).
 template <class C>
 struct RowAdapters {
-  static constexpr int DEPTH = C::DEPTH;
+  static constexpr int DEPTH = C::DEPTH, NONE = -2;
   int id[C::MT];         // of row c of tile t; -1: none
   uint32_t open[C::MT];  // rows whose adapter is still to come in this run of ranks
-  int now, r0;           // the next step's
-  int who[DEPTH];        // the steps' adapters; -1: none
+  int r0;                // the run's first rank
+  bool two;              // the run has more than 32 ranks
+  bool there[2];         // this lane's ranks of either half are ranks
+  int who[DEPTH];        // the steps' adapters, or NONE
   uint32_t at[C::NT];    // this lane's rows of an adapter's b, in bytes
-  i32x4 bv[DEPTH][C::NT], pv[C::MT];
+  i32x4 bv[DEPTH][2][C::NT], pv[2][C::MT];
 
   D3_INLINE void begin(const Dense& a, int m0, int lane) {
 #pragma unroll
@@ -180,43 +184,46 @@ struct RowAdapters {
     }
   }
   // the next adapter that a row names
-  D3_INLINE void next() {
-    now = -1;
+  D3_INLINE int next() {
+    int now = NONE;
 #pragma unroll
-    for (int t = C::MT - 1; t >= 0; t--)
-      if (open[t]) now = __builtin_amdgcn_readlane(id[t], __ffs((int)open[t]) - 1);
+    for (int t = C::MT - 1; t >= 0; t--) {
+      const int first = __builtin_amdgcn_readlane(id[t], (__ffs((int)open[t]) - 1) & 15);
+      now = open[t] ? first : now;
+    }
 #pragma unroll
     for (int t = 0; t < C::MT; t++) open[t] &= ~(uint32_t)__ballot(id[t] == now);
+    return now;
   }
-  // sends the next step's loads
-  D3_INLINE void load(const Dense& a, int i, int lane) {
-    who[i] = now;
-    if (now < 0) return;
-    const uint8_t* b = (const uint8_t*)(a.b + (size_t)now * a.N * a.rank + r0);
+  // sends the next step's loads (a lane without ranks: the adapter's first ones)
+  D3_INLINE void load(const Dense& a, int i) {
+    who[i] = next();
+    const uint8_t* b = (const uint8_t*)(a.b + (size_t)max(who[i], 0) * a.N * a.rank + r0);
 #pragma unroll
-    for (int u = 0; u < C::NT; u++) {
-      if (r0 + 32 <= a.rank) {
-        bv[i][u] = *(const i32x4*)(b + at[u]);
-      } else {
-        bv[i][u] = i32x4{0, 0, 0, 0};
-        if (r0 + 8 * (lane >> 4) < a.rank) bv[i][u] = *(const i32x4*)(b + at[u]);
-      }
+    for (int u = 0; u < C::NT; u++) bv[i][0][u] = *(const i32x4*)(b + (there[0] ? at[u] : 0u));
+    if (two) {
+#pragma unroll
+      for (int u = 0; u < C::NT; u++) bv[i][1][u] = *(const i32x4*)(b + (there[1] ? at[u] + 64 : 0u));
     }
-    next();
   }
-  // the rows' inner products of ranks r0 .. r0 + 31 (where a row has an adapter: what the others hold is not used), and the first
+  // the rows' inner products of ranks r0 .. r0 + 63 (where a row has an adapter: what the others hold is not used), and the first
   // steps with them
   D3_INLINE void ranks(const Dense& a, int m0, int lane) {
-    const int r = r0 + 8 * (lane >> 4);
+    two = r0 + 32 < a.rank;
 #pragma unroll
-    for (int t = 0; t < C::MT; t++) {
-      pv[t] = i32x4{0, 0, 0, 0};
-      if (id[t] >= 0 && r < a.rank) pv[t] = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + (lane & 15)) * a.rank + r);
-      open[t] = (uint32_t)__ballot(id[t] >= 0) & 0xFFFFu;
+    for (int t = 0; t < C::MT; t++) open[t] = (uint32_t)__ballot(id[t] >= 0) & 0xFFFFu;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int r = r0 + 32 * h + 8 * (lane >> 4);
+      there[h] = r < a.rank;
+#pragma unroll
+      for (int t = 0; t < C::MT; t++) {
+        pv[h][t] = i32x4{0, 0, 0, 0};
+        if (id[t] >= 0 && there[h]) pv[h][t] = *(const i32x4*)(a.p + (size_t)(m0 + 16 * t + (lane & 15)) * a.rank + r);
+      }
     }
-    next();
 #pragma unroll
-    for (int i = 0; i < DEPTH; i++) load(a, i, lane);
+    for (int i = 0; i < DEPTH; i++) load(a, i);
   }
   // n: this lane's rows of b
   D3_INLINE void first(const Dense& a, int m0, const int (&n)[C::NT], int lane) {
@@ -225,25 +232,32 @@ struct RowAdapters {
     r0 = 0;
     ranks(a, m0, lane);
   }
+  D3_INLINE void multiply(f32x4 (&acc)[C::NT][C::MT], int i, int h) {
+#pragma unroll
+    for (int u = 0; u < C::NT; u++) {
+      i32x4 b = bv[i][h][u];
+#pragma unroll
+      for (int j = 0; j < 4; j++) b[j] = there[h] ? b[j] : 0;
+#pragma unroll
+      for (int t = 0; t < C::MT; t++) {
+        // (the other rows keep their sums, also where this adapter holds infinities or NaN)
+        const f32x4 with = mfma_bf16(b, pv[h][t], acc[u][t]);
+        acc[u][t] = id[t] == who[i] ? with : acc[u][t];
+      }
+    }
+  }
   D3_INLINE void add(const Dense& a, f32x4 (&acc)[C::NT][C::MT], int m0, int lane) {
     while (true) {
-      while (who[0] >= 0) {
+      while (who[0] != NONE) {
 #pragma unroll
         for (int i = 0; i < DEPTH; i++) {
-          if (who[i] >= 0) {
-#pragma unroll
-            for (int t = 0; t < C::MT; t++)
-#pragma unroll
-              for (int u = 0; u < C::NT; u++) {
-                // (the other rows keep their sums, also where this adapter holds infinities or NaN)
-                const f32x4 with = mfma_bf16(bv[i][u], pv[t], acc[u][t]);
-                acc[u][t] = id[t] == who[i] ? with : acc[u][t];
-              }
-            load(a, i, lane);
-          }
+          multiply(acc, i, 0);
+          if (two) multiply(acc, i, 1);
+          load(a, i);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if ((r0 += 32) >= a.rank) return;
+      if ((r0 += 64) >= a.rank) return;
       ranks(a, m0, lane);
     }
   }
