@@ -211,19 +211,21 @@ __global__ void __launch_bounds__(MOST) add_norm_kernel(Desc d) {
   }
 }
 
-// SIDE: there is a post norm or a gate; without them dy = scale dresidual, and y is not read. The next row's loads are on
+// SIDE: there is a post norm or a gate; without them dy = scale dresidual. AGAIN: h is made again from y and residual, in float32 as
+// the forward pass made it, and not read as it is stored: its rounding to bf16 would add to dweight as much error as that's
+// own (4096 x 2048 without post and gate 18.5 us so, 22 with one row more to read; with them y is read anyway). The next row's loads are on
 // their way during a row's sums. What all rows share (weight, post, a gate per channel) stays in registers: loads come back in
 // order, so one that a row waits for would wait for the next row's as well.
-template <class TY, class TS, bool SIDE, bool WAVE, int CH, int MOST>
+template <class TY, class TS, bool SIDE, bool AGAIN, bool WAVE, int CH, int MOST>
 __global__ void __launch_bounds__(MOST) add_norm_backward_kernel(Desc d, int groups) {
   __shared__ float slots[2][3][16];
   const int lane = lane_of<WAVE>(), lanes = lanes_of<WAVE>(), group = WAVE ? (int)(blockIdx.x * 4 + threadIdx.x / 64) : (int)blockIdx.x;
   if (group >= groups) return;  // (whole waves, and then without barriers)
-  constexpr int SC = SIDE ? CH : 1;
+  constexpr int SC = SIDE ? CH : 1, YC = SIDE || AGAIN ? CH : 1;
   float sum_w[CH][8] = {}, sum_p[SC][8] = {}, sum_g[SC][8] = {}, w[CH][8] = {}, p[SC][8], g[SC][8];
   float next_g[SC][8], next_rstd = 0.0f, next_rstd_y = 1.0f;
   Eight<TS> next_dh[CH], next_h[CH];
-  Eight<TY> next_dn[CH], next_y[SC];
+  Eight<TY> next_dn[CH], next_y[YC];
 #pragma unroll
   for (int j = 0; j < CH; j++) {
     const int col = 8 * (lane + lanes * j);
@@ -244,10 +246,10 @@ __global__ void __launch_bounds__(MOST) add_norm_backward_kernel(Desc d, int gro
       if (d.dh) next_dh[j].get((const TS*)d.dh + row * d.H, col, d.H);
       if (d.dn) {
         next_dn[j].get((const TY*)d.dn + row * d.H, col, d.H);
-        next_h[j].get((const TS*)d.h + row * d.residual_stride, col, d.H);
+        next_h[j].get((const TS*)(AGAIN ? d.residual : d.h) + row * d.residual_stride, col, d.H);
       }
+      if constexpr (SIDE || AGAIN) next_y[j].get((const TY*)d.y + row * d.y_stride, col, d.H);
       if constexpr (SIDE) {
-        next_y[j].get((const TY*)d.y + row * d.y_stride, col, d.H);
         if (d.gate_kind == GATE_ROW || d.gate_kind == GATE_FULL) gate8(d, (int)row, col, next_g[j]);
       }
     }
@@ -262,10 +264,17 @@ __global__ void __launch_bounds__(MOST) add_norm_backward_kernel(Desc d, int gro
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         dr[j][i] = d.dh ? next_dh[j][i] : 0.0f;
-        if (d.dn) a[j][i] = next_dn[j][i], hat[j][i] = next_h[j][i] * rstd;
+        float side = 0.0f;
         if constexpr (SIDE) {
-          v[j][i] = next_y[j][i];
           if (d.gate_kind != GATE_CHANNEL) g[j][i] = next_g[j][i];
+          v[j][i] = next_y[j][i] * rstd_y;  // y^
+          side = g[j][i] * (v[j][i] * p[j][i]);
+        } else if constexpr (AGAIN) {
+          side = next_y[j][i];
+        }
+        if (d.dn) {
+          a[j][i] = next_dn[j][i];
+          hat[j][i] = (AGAIN ? next_h[j][i] + d.scale * side : next_h[j][i]) * rstd;
         }
       }
     if (row + groups < d.T) get(row + groups);
@@ -307,7 +316,6 @@ __global__ void __launch_bounds__(MOST) add_norm_backward_kernel(Desc d, int gro
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           const float dv = d.scale * dr[j][i];
-          v[j][i] *= rstd_y;  // y^
           full[i] = dv * (v[j][i] * p[j][i]);
           sum_g[j][i] += full[i];
           sum_row += full[i];
@@ -466,7 +474,7 @@ extern "C" int d3_add_norm_backward(const d3_add_norm_desc* desc, void* stream) 
   const int parts = !!d.dweight + !!d.dpost + (d.dgate && d.gate_kind == GATE_CHANNEL);
   const int groups = groups_of(d.T, d.H);
   if (d.T > 0) {
-    if (!(d.dh || d.dn) || (d.dn && (!d.h || !d.rstd)) || (d.post && !d.rstd)) return fail("d3_add_norm_backward: null pointer");
+    if (!(d.dh || d.dn) || (d.dn && (!d.rstd || !(d.stream_type && d.y ? d.residual : d.h))) || (d.post && !d.rstd)) return fail("d3_add_norm_backward: null pointer");
     if (parts && (!d.partials || d.partials_floats < (int64_t)parts * groups * d.H))
       return fail("d3_add_norm_backward: partials too small (d3_add_norm_partials)");
     by_types(d, [&](auto y, auto s) {
@@ -474,10 +482,20 @@ extern "C" int d3_add_norm_backward(const d3_add_norm_desc* desc, void* stream) 
         constexpr bool W = decltype(wave)::value;
         constexpr int CH = decltype(chunks)::value, MOST = decltype(most)::value;
         const int grid = W ? (groups + 3) / 4 : groups;
-        if (d.y && (d.post || d.gate_kind))
-          add_norm_backward_kernel<decltype(y), decltype(s), true, W, CH, MOST><<<grid, lanes, 0, (hipStream_t)stream>>>(d, groups);
-        else
-          add_norm_backward_kernel<decltype(y), decltype(s), false, W, CH, MOST><<<grid, lanes, 0, (hipStream_t)stream>>>(d, groups);
+        // (a float32 stream holds h as it was)
+        constexpr bool STORED_SHORT = std::is_same_v<decltype(s), bf16_t>;
+        const bool again = STORED_SHORT && d.y && d.dn;
+        auto launch = [&](auto side, auto again) {
+          add_norm_backward_kernel<decltype(y), decltype(s), decltype(side)::value, decltype(again)::value, W, CH, MOST>
+              <<<grid, lanes, 0, (hipStream_t)stream>>>(d, groups);
+        };
+        if (d.y && (d.post || d.gate_kind)) {
+          if (again) launch(std::true_type{}, std::bool_constant<STORED_SHORT>{});
+          else launch(std::true_type{}, std::false_type{});
+        } else {
+          if (again) launch(std::false_type{}, std::bool_constant<STORED_SHORT>{});
+          else launch(std::false_type{}, std::false_type{});
+        }
       });
     });
   }

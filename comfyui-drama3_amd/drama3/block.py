@@ -302,26 +302,34 @@ def _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, stats):
 
 
 def add_norm_forward(y, residual, weight, *, post=None, gate=None, scale=1.0, eps=1e-6, unit_offset=False):
-    """add_norm's (h, n) and rstd [2, T] float32, which add_norm_backward takes; autograd does not see it."""
+    """add_norm's (h, n) and what add_norm_backward needs beside them: (rstd [2, T] float32, residual); autograd does not see it."""
     with torch.no_grad():
-        return _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, True)
+        h, n, rstd = _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, True)
+        return h, n, (rstd, residual)
 
 
-def add_norm_backward(dh, dn, y, h, rstd, weight, *, post=None, gate=None, scale=1.0, unit_offset=False,
+def add_norm_backward(dh, dn, y, h, saved, weight, *, post=None, gate=None, scale=1.0, unit_offset=False,
                       needs=(True, True, True, True, True)):
     """(dy, dresidual, dweight, dpost, dgate) of add_norm for the gradients dh and dn of its outputs (either may be None: zero),
-    with y, weight, post, gate, scale and unit_offset as they went in and h and rstd as add_norm_forward returned them. Each
-    gradient has its input's type and shape; None where the input is absent or `needs` says so. Float32 inside, from h as it is
-    stored; sums over the rows (dweight, dpost, a gate per channel) are the same bits from call to call."""
+    with y, weight, post, gate, scale and unit_offset as they went in and h and `saved` as add_norm_forward returned them. Each
+    gradient has its input's type and shape; None where the input is absent or `needs` says so. Float32 inside; of a bfloat16
+    stream h is made again from y and residual, since its rounding would show in the gradients. Sums over the rows (dweight,
+    dpost, a gate per channel) are the same bits from call to call."""
     with torch.no_grad():
         if y is None:
             raise TypeError("y [T, H] float32 or bfloat16 expected")
-        return _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, scale, unit_offset, needs, None)
+        rstd, residual = saved
+        return _add_norm_backward(dh, dn, y, h, rstd, residual, weight, post, gate, scale, unit_offset, needs, None)
 
 
-def _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, scale, unit_offset, needs, out_dtype):
+def _add_norm_backward(dh, dn, y, h, rstd, residual, weight, post, gate, scale, unit_offset, needs, out_dtype):
     index = h.get_device()
-    r = _float_rows(h, "h", index)
+    if y is not None and h.dtype is torch.bfloat16:
+        if residual.dtype is not h.dtype or residual.shape != h.shape:
+            raise ValueError("saved (rstd, residual) of add_norm_forward expected")
+        r = _float_rows(residual, "residual", index)
+    else:
+        r = _float_rows(h, "h", index)
     T, H = _norm_shape(h)
     b = (None, 0, _TYPES[out_dtype]) if y is None else _float_rows(y, "y", index, h.shape)
     out_dtype = out_dtype if y is None else y.dtype
@@ -361,7 +369,8 @@ class _AddNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, residual, weight, post, gate, scale, eps, unit_offset):
         h, n, rstd = _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, True)
-        ctx.save_for_backward(y, h, rstd, weight, post, gate)
+        # (a float32 stream needs h, a bfloat16 one residual: the other is not kept alive)
+        ctx.save_for_backward(y, residual if residual.dtype is torch.bfloat16 else h, rstd, weight, post, gate)
         ctx.options = scale, unit_offset
         ctx.set_materialize_grads(False)
         return h, n
@@ -373,7 +382,7 @@ class _AddNorm(torch.autograd.Function):
         if dh is None and dn is None:
             return (None,) * 8
         y, h, rstd, weight, post, gate = ctx.saved_tensors
-        grads = _add_norm_backward(dh, dn, y, h, rstd, weight, post, gate, *ctx.options, ctx.needs_input_grad[:5], None)
+        grads = _add_norm_backward(dh, dn, y, h, rstd, h, weight, post, gate, *ctx.options, ctx.needs_input_grad[:5], None)
         return grads + (None,) * 3
 
 
@@ -403,7 +412,7 @@ class _Norm(torch.autograd.Function):
         x, rstd, weight = ctx.saved_tensors
         needs = ctx.needs_input_grad
         unit_offset, dtype = ctx.options
-        _, dx, dweight, _, _ = _add_norm_backward(None, dn, None, x, rstd, weight, None, None, 1.0, unit_offset,
+        _, dx, dweight, _, _ = _add_norm_backward(None, dn, None, x, rstd, None, weight, None, None, 1.0, unit_offset,
                                                   (False, needs[0], needs[1], False, False), dtype)
         return dx, dweight, None, None, None
 

@@ -450,8 +450,9 @@ int d3_bf16_grouped(const void* x, int32_t rows, const int64_t* order, int32_t k
  * residual are their strides apart (elements), all others H. Float32 inside; n comes from h before h is rounded.
  *   d3_add_norm: h (with y; without, h is residual and is not written) and n (with weight). rstd [2, T] may be NULL:
  *     rstd(h), and rstd(y) with post.
- *   d3_add_norm_backward: from dh and dn (either may be NULL: zero), y, h (rows residual_stride apart) and rstd as the
- *     forward call left them: dy, dresidual, dweight, dpost, dgate, each where it is not NULL, of its input's type and
+ *   d3_add_norm_backward: from dh and dn (either may be NULL: zero), y, rstd as the forward call left it, and h (rows
+ *     residual_stride apart) as it left that, or residual in its place where the stream is bf16 and y is there (h is then
+ *     made again, unrounded): dy, dresidual, dweight, dpost, dgate, each where it is not NULL, of its input's type and
  *     shape. partials: d3_add_norm_partials(T, H) floats for each of dweight, dpost and a dgate per channel, need no clearing.
  *     Sums over the rows are made in a fixed order.
  *     T = 0 gives zeros. */

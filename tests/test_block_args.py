@@ -98,11 +98,13 @@ def test_add_norm_refusals(error, match, changed):
     ("dh of", {"dh": z(3, 10)}),
     ("dn of", {"dn": z(3, 10, dtype=F32)}),
     ("dn goes with weight", {"weight": None}),
-    ("rstd", {"rstd": z(3, dtype=F32)}),
-    ("rstd", {"rstd": None}),
+    ("rstd", {"saved": (z(3, dtype=F32), None)}),
+    ("rstd", {"saved": (None, None)}),
+    ("saved", {"h": z(3, 10), "dh": z(3, 10), "saved": (z(2, 3, dtype=F32), z(3, 12))}),
+    ("saved", {"h": z(3, 10), "dh": z(3, 10), "saved": (z(2, 3, dtype=F32), z(3, 10, dtype=F32))}),
 ])
 def test_add_norm_backward_refusals(match, changed):
-    args = {"dh": z(3, 10, dtype=F32), "dn": z(3, 10), "y": z(3, 10), "h": z(3, 10, dtype=F32), "rstd": z(2, 3, dtype=F32),
+    args = {"dh": z(3, 10, dtype=F32), "dn": z(3, 10), "y": z(3, 10), "h": z(3, 10, dtype=F32), "saved": (z(2, 3, dtype=F32), None),
             "weight": z(10)}
     with pytest.raises(ValueError, match=match):
         block.add_norm_backward(**{**args, **changed})
@@ -190,7 +192,8 @@ def test_add_norm_entry_refuses(changed):
 
 
 @pytest.mark.parametrize("changed", [{"dh": None, "dn": None}, {"weight": None}, {"rstd": None}, {"h": None}, {"partials_floats": 31},
-                                     {"partials": None}, {"dpost": P}, {"dgate": P}, {"y": None}])
+                                     {"partials": None}, {"dpost": P}, {"dgate": P}, {"y": None},
+                                     {"stream_type": 1}])
 def test_add_norm_backward_entry_refuses(changed):
     args = dict(y=P, h=P, weight=P, dh=P, dn=P, rstd=P, dy=P, dresidual=P, dweight=P, partials=P, partials_floats=32, T=2, H=16,
                 y_stride=16, residual_stride=16, scale=1.0)

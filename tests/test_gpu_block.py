@@ -408,12 +408,12 @@ def norm_check(T, H, of, stream, gate="none", post=False, weights=None, scale=1.
         assert got.dtype == inp.dtype and got.shape == inp.shape, name
         assert torch.equal(got, twice), name
         w, size = want[name], sizes[name]
-        # h as it is stored: half a step of the stream's type in every h^; then float32 sums over H columns and T rows. A gradient is
-        # a sum of products of a few factors of which each may be off by that much: taken on the whole, against the norm of the
-        # terms' magnitudes. (Not against the gradient's own: of one column y^ is 1 - eps / (2 y^2), and dy = rstd b (1 - y^2 rstd^2) is
-        # 1e-6 of the two terms that it is the difference of, each of which float32 holds to 6e-8.)
+        # Half a step of the result's type, and float32 sums over H columns and T rows. A gradient is a sum of products of a few
+        # factors of which each may be off by that much: taken on the whole, against the norm of the terms' magnitudes. (Not
+        # against the gradient's own: of one column y^ is 1 - eps / (2 y^2), and dy = rstd b (1 - y^2 rstd^2) is 1e-6 of the two
+        # terms that it is the difference of, each of which float32 holds to 6e-8.)
         rel = ((got.to(F64) - w).norm() / size.norm().clamp_min(1e-30)).item()
-        limit = HALF[inp.dtype] + 4 * HALF[stream] + 2.0 ** -17
+        limit = HALF[inp.dtype] + 2.0 ** -17
         if w.numel() * T >= 16:
             assert rel < limit, (name, rel, limit)
         assert got.isfinite().all()
