@@ -27,44 +27,60 @@ int check_lora(const std::string& what, const Dense& a, const void* A, const flo
 }
 
 // p[m, r] = alpha[a] sum_k x[m, k] A[a, r, k] for the adapter a of each row m, rounded to bf16 (the operand of the second product:
-// a relative 2^-9 of what the adapter adds). A workgroup takes 32 ranks and 16 rows, one adapter that they name after the
-// other (blockIdx.z of them at the start, gridDim.z apart), so that prompts' rows are read once up to rank 32; its 8 waves
-// each take an eighth of K. Rows without an adapter are not written, nor read later.
-__global__ void __launch_bounds__(ST_THREADS) lora_inner_kernel(const uint16_t* x, int64_t ldx, const uint16_t* A, const float* alpha,
-                                                                const int64_t* ids, int M, int K, int rank, int adapters, uint16_t* p) {
-  __shared__ f32x4 part[ST_WAVES][2][64];
+// a relative 2^-9 of what the adapter adds). Rows without an adapter are not written, nor read later. Two kernels:
+
+// Up to 16 rows: a workgroup takes 16 ranks and an adapter that the rows name (blockIdx.y of them), its 8 waves an eighth of K each.
+__global__ void __launch_bounds__(ST_THREADS) lora_inner_stream_kernel(Dense a, const uint16_t* A, const float* alpha) {
+  __shared__ f32x4 part[ST_WAVES][1][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c = lane & 15;
-  const int m0 = blockIdx.y * 16, r0 = blockIdx.x * 32;
-  const int64_t id = lane < 16 && m0 + lane < M ? ids[m0 + lane] : -1;
-  uint64_t open = __ballot(id >= 0 && id < adapters);
-  const uint16_t* row = x + min(m0 + c, M - 1) * ldx;
+  const int r0 = blockIdx.x * 16;
+  const int64_t id = lane < a.M ? a.ids[lane] : -1;
+  uint64_t open = __ballot(id >= 0 && id < a.adapters), rows = 0;
+  int64_t now = 0;
+  for (int i = 0; i <= (int)blockIdx.y; i++) {
+    if (!open) return;
+    now = __shfl(id, __ffsll((unsigned long long)open) - 1);
+    rows = __ballot(id == now);
+    open &= ~rows;
+  }
+  const uint16_t* x[1] = {a.x + min(c, a.M - 1) * a.ldx};
+  const float scale = alpha[now];
+  f32x4 acc[1];
+  stream_sums<1, 4>(A + ((size_t)now * a.rank + min(r0 + c, a.rank - 1)) * a.K, x, a.K, wave, acc);
+  const f32x4 v = join_waves<1>(part, acc, wave) * scale;
+  if (wave == 0 && (rows >> c & 1) && r0 + 4 * q < a.rank) *(i32x2*)(a.out + (size_t)c * a.rank + r0 + 4 * q) = round4(v);
+}
+
+// More: tiles of 64 rows and 32 ranks, one adapter that the rows name after the other (blockIdx.z of them at the start, gridDim.z
+// apart). A CU reads three times as fast into LDS as straight into operands: 5000 rows of rank 32, K 2048, 20 us that way, 11 so.
+__global__ void __launch_bounds__(Thin::THREADS, 2) lora_inner_tile_kernel(Dense a, const uint16_t* A, const float* alpha) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[Thin::LDS];
+  static_assert(Thin::TM == 64);
+  const int lane = threadIdx.x & 63, m = blockIdx.y * 64 + lane;
+  const int64_t id = m < a.M ? a.ids[m] : -1;
+  uint64_t open = __ballot(id >= 0 && id < a.adapters);
   for (int i = 0; open; i++) {
     const int64_t now = __shfl(id, __ffsll((unsigned long long)open) - 1);
-    const uint64_t rows = __ballot(id == now);
-    open &= ~rows;
+    a.rows = __ballot(id == now);
+    open &= ~a.rows;
     if (i % (int)gridDim.z != (int)blockIdx.z) continue;
-    // (here the adapter's two tiles of ranks are the operand that differs from tile to tile, and the rows the one that all share)
-    const uint16_t* ranks[2];
-#pragma unroll
-    for (int t = 0; t < 2; t++) ranks[t] = A + ((size_t)now * rank + min(r0 + 16 * t + c, rank - 1)) * K;
-    f32x4 acc[2];
-    stream_sums<2>(row, ranks, K, wave, acc);
-    // lane (q, c): rows 4 q .. 4 q + 3, rank c
-    const f32x4 v = join_waves<2>(part, acc, wave) * alpha[now];
-    const int r = r0 + 16 * wave + c;
-    if (wave < 2 && r < rank) {
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (rows >> (4 * q + j) & 1) p[(size_t)(m0 + 4 * q + j) * rank + r] = (uint16_t)f32_to_bf16(v[j]);
-    }
-    __syncthreads();  // (the sums are read: the next adapter's may take their place)
+    a.w = A + (size_t)now * a.rank * a.K;
+    a.alpha = alpha[now];
+    __syncthreads();  // (the last adapter's stages are read)
+    dense_tile<Thin, false, false, END_INNER, false>(a, blockIdx.y, blockIdx.x, smem);
   }
 }
 
-// few rows: a workgroup for every adapter that 16 rows can name; many: two, which is enough where requests' rows follow each other
-void launch_inner(const Dense& a, const void* A, const float* alpha, hipStream_t stream) {
-  lora_inner_kernel<<<dim3((a.rank + 31) / 32, (a.M + 15) / 16, a.M <= 256 ? 16 : 2), ST_THREADS, 0, stream>>>(
-      a.x, a.ldx, (const uint16_t*)A, alpha, a.ids, a.M, a.K, a.rank, a.adapters, (uint16_t*)a.p);
+void launch_inner(const Dense& of, const void* A, const float* alpha, hipStream_t stream) {
+  Dense a = of;
+  a.out = (uint16_t*)of.p, a.ldo = a.N = a.rank, a.ldw = a.K;
+  if (a.M <= 16) {
+    lora_inner_stream_kernel<<<dim3((a.rank + 15) / 16, a.M), ST_THREADS, 0, stream>>>(a, (const uint16_t*)A, alpha);
+  } else {
+    // few rows: a workgroup for each of 32 adapters; many, where requests' rows follow each other: two
+    lora_inner_tile_kernel<<<dim3((a.rank + 31) / 32, (a.M + 63) / 64, a.M <= 256 ? 32 : 2), Thin::THREADS, 0, stream>>>(
+        a, (const uint16_t*)A, alpha);
+  }
 }
 
 }  // namespace

@@ -7,27 +7,28 @@
 
 namespace d3 {
 
-constexpr int ST_WAVES = 8, ST_THREADS = 64 * ST_WAVES, ST_AT_ONCE = 4;  // stages of 64 k whose loads a wave sends together
+constexpr int ST_WAVES = 8, ST_THREADS = 64 * ST_WAVES;
 
-// this wave's part of the sums of 16 rows (lane's own at w) with RT times 16 others (lane's own at x[t])
-template <int RT>
+// this wave's part of the sums of 16 rows (lane's own at w) with RT times 16 others (lane's own at x[t]), AT_ONCE stages of 64 k whose
+// loads it sends together
+template <int RT, int AT_ONCE>
 D3_INLINE void stream_sums(const uint16_t* w, const uint16_t* const (&x)[RT], int K, int wave, f32x4 (&acc)[RT]) {
   const int q = (threadIdx.x & 63) >> 4, stages = (K + 63) / 64;
   const int first = stages * wave / ST_WAVES, last = stages * (wave + 1) / ST_WAVES;
 #pragma unroll
   for (int t = 0; t < RT; t++) acc[t] = f32x4{0, 0, 0, 0};
   int s = first;
-  for (; s + ST_AT_ONCE <= last && (s + ST_AT_ONCE) * 64 <= K; s += ST_AT_ONCE) {
-    i32x4 wv[2 * ST_AT_ONCE], xv[RT][2 * ST_AT_ONCE];
+  for (; s + AT_ONCE <= last && (s + AT_ONCE) * 64 <= K; s += AT_ONCE) {
+    i32x4 wv[2 * AT_ONCE], xv[RT][2 * AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < 2 * ST_AT_ONCE; i++) wv[i] = *(const i32x4*)(w + s * 64 + i * 32 + 8 * q);
+    for (int i = 0; i < 2 * AT_ONCE; i++) wv[i] = *(const i32x4*)(w + s * 64 + i * 32 + 8 * q);
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
-      for (int i = 0; i < 2 * ST_AT_ONCE; i++) xv[t][i] = *(const i32x4*)(x[t] + s * 64 + i * 32 + 8 * q);
+      for (int i = 0; i < 2 * AT_ONCE; i++) xv[t][i] = *(const i32x4*)(x[t] + s * 64 + i * 32 + 8 * q);
     __builtin_amdgcn_sched_barrier(0);  // (all loads on their way before the first product)
 #pragma unroll
-    for (int i = 0; i < 2 * ST_AT_ONCE; i++)
+    for (int i = 0; i < 2 * AT_ONCE; i++)
 #pragma unroll
       for (int t = 0; t < RT; t++) acc[t] = mfma_bf16(wv[i], xv[t][i], acc[t]);
   }
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(ST_THREADS) dense_stream_kernel(Dense a) {
   const int n0 = blockIdx.x * (END == END_SWIGLU ? 8 : 16), n = END == END_SWIGLU ? n0 + (c >> 1) + (c & 1) * a.half : min(n0 + c, a.N - 1);
   const uint16_t* x[1] = {a.x + min(c, a.M - 1) * a.ldx};
   f32x4 acc[1];
-  stream_sums<1>(a.w + n * a.ldw, x, a.K, wave, acc);
+  stream_sums<1, 4>(a.w + n * a.ldw, x, a.K, wave, acc);
   if constexpr (LORA) {
     // the rows' adapters, an eighth of them to each wave: lane l has row l's
     const int64_t id = lane < a.M ? a.ids[lane] : -1;

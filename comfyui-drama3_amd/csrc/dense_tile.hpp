@@ -26,6 +26,7 @@ enum DenseEnd {
   END_ROWS,     // out bf16
   END_SWIGLU,   // w holds `half` gate rows, then as many up rows: out [M, half] = SiLU(gate) * up, and pre where it is given
   END_DSWIGLU,  // the sums are the gradient of SiLU(gate) * up: out [M, 2 half] = the gradients of gate and up (from pre)
+  END_INNER,    // out bf16 = alpha times the sums, of the tile's rows (up to 64) whose bit is set in `rows`
 };
 
 struct Dense {
@@ -40,6 +41,8 @@ struct Dense {
   const uint16_t* b;  // [adapters, N, rank]
   const int64_t* ids;
   int rank, adapters;
+  uint64_t rows;
+  float alpha;
 };
 
 // dma16 as an instruction that the compiler may move other memory accesses past: its place among the barriers (which
@@ -270,7 +273,7 @@ struct RowAdapters {
 // 6144 x 2048 transposed twice 90, 114). A stage's one barrier stands after group BAR of its second half, when the reads of its own
 // operands are long done.
 template <class C, bool XT, bool WT, int END, bool LORA>
-D3_INLINE void dense_tile(const Dense& a, int tile, uint8_t* smem) {
+D3_INLINE void dense_tile(const Dense& a, int tm, int tn, uint8_t* smem) {
   constexpr int TM = C::TM, TN = C::TN, W = C::WAVES, BUFS = C::BUFS;
   using SX = Side<TM, XT, W>;
   using SW = Side<TN, WT, W>;
@@ -278,9 +281,6 @@ D3_INLINE void dense_tile(const Dense& a, int tile, uint8_t* smem) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, c = lane & 15, wn = w % C::WN, wm = w / C::WN;
   constexpr int UN = END == END_SWIGLU ? TN / 2 : TN;  // columns of out to a tile
-  const int columns = END == END_SWIGLU ? a.half : a.N, nm = (a.M + TM - 1) / TM, nn = (columns + UN - 1) / UN;
-  int tm, tn;
-  place(tile, nm, nn, tm, tn);
   const int m0 = tm * TM, n0 = tn * UN, stages = (a.K + 63) / 64;
   const uint32_t lds = lds_address(smem);
 
@@ -471,6 +471,9 @@ D3_INLINE void dense_tile(const Dense& a, int tile, uint8_t* smem) {
         const int n = n0 + (wn * C::NT + u) * 16;
         if constexpr (END == END_ROWS) {
           store_two(a.out + m * a.ldo + n, round4(acc[u][t]), round4(acc[u + 1][t]), row ? a.N - n : 0);
+        } else if constexpr (END == END_INNER) {
+          const bool mine = row && (a.rows >> (m - m0) & 1);
+          store_two(a.out + m * a.ldo + n, round4(acc[u][t] * a.alpha), round4(acc[u + 1][t] * a.alpha), mine ? a.N - n : 0);
         } else {
           i32x2 dg[2], du[2];
 #pragma unroll
@@ -498,11 +501,22 @@ D3_INLINE void dense_tile(const Dense& a, int tile, uint8_t* smem) {
   }
 }
 
+// the tiles of a's out, tile `at` of them (END_SWIGLU: half as many columns)
+template <class C, int END>
+D3_INLINE bool tile_at(const Dense& a, int at, int& tm, int& tn) {
+  constexpr int UN = END == END_SWIGLU ? C::TN / 2 : C::TN;
+  const int nm = (a.M + C::TM - 1) / C::TM, nn = ((END == END_SWIGLU ? a.half : a.N) + UN - 1) / UN;
+  if (at >= nm * nn) return false;
+  place(at, nm, nn, tm, tn);
+  return true;
+}
+
 // (tiles along y: a grid's x has room for 2^32 threads)
 template <class C, bool XT, bool WT, int END, bool LORA>
 __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
-  dense_tile<C, XT, WT, END, LORA>(a, blockIdx.y, smem);
+  int tm, tn;
+  if (tile_at<C, END>(a, blockIdx.y, tm, tn)) dense_tile<C, XT, WT, END, LORA>(a, tm, tn, smem);
 }
 
 // Up to three products that do not need each other in one launch, the longest first: rows with a transposed w (the gradient of
@@ -515,12 +529,12 @@ struct DenseSet {
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, 2) dense_set_kernel(DenseSet set) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
-  int at = blockIdx.y, i = 0;
+  int at = blockIdx.y, i = 0, tm, tn;
   while (i < set.count - 1 && at >= set.tiles[i]) at -= set.tiles[i++];
   const Dense& a = set.product[i];
-  if (at >= (a.M + C::TM - 1) / C::TM * ((a.N + C::TN - 1) / C::TN)) return;
-  if (i == set.rows) dense_tile<C, false, true, END_ROWS, false>(a, at, smem);
-  else dense_tile<C, true, true, END_ROWS, false>(a, at, smem);
+  if (!tile_at<C, END_ROWS>(a, at, tm, tn)) return;
+  if (i == set.rows) dense_tile<C, false, true, END_ROWS, false>(a, tm, tn, smem);
+  else dense_tile<C, true, true, END_ROWS, false>(a, tm, tn, smem);
 }
 
 }  // namespace d3
