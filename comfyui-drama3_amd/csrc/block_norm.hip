@@ -6,8 +6,9 @@
 // with post and weight read as 1 + w where they are kept as offsets. Sums, h inside the pass and all products are float32; h and
 // n are each rounded once, to the stream's and the block's type (n comes from h before its rounding).
 //
-// HBM-bound: a row is read once, held in registers through its sums, and written once. A lane takes 8 columns at a time;
-// 64, 256 or 1024 lanes a row, so that a lane holds at most 32 columns.
+// HBM-bound: a row is read once, held in registers through its sums, and written once: 8192 rows of 2048, a float32 stream
+// and a bfloat16 block output, 41 us (4.9 TB/s); 4096 bfloat16 rows 14.2 us forward (4.7 TB/s), 20.8 backward (4.9 TB/s). A lane
+// takes 8 columns at a time, 8 to 32 in all: a wave a row up to 1024 columns (four rows a workgroup), a workgroup a row above.
 //
 // Backward, for dh and dn (gradients of h and n), with z^ = z rstd(z) and m(z) the mean over a row:
 //   a = dn weight        dresidual = dh + rstd(h) (a - h^ m(a h^))        dv = scale dresidual
@@ -42,7 +43,7 @@ struct Eight;
 template <>
 struct Eight<bf16_t> {
   u32x4_at2 w;
-    D3_INLINE void get(const bf16_t* row, int col, int H) {
+  D3_INLINE void get(const bf16_t* row, int col, int H) {
     if (col + 8 <= H) {
       w = *(const u32x4_at2*)(row + col);
     } else {
@@ -58,7 +59,7 @@ struct Eight<bf16_t> {
 template <>
 struct Eight<float> {
   f32x4_at4 a, b;
-    D3_INLINE void get(const float* row, int col, int H) {
+  D3_INLINE void get(const float* row, int col, int H) {
     if (col + 8 <= H) {
       a = *(const f32x4_at4*)(row + col), b = *(const f32x4_at4*)(row + col + 4);
     } else {
@@ -213,9 +214,9 @@ __global__ void __launch_bounds__(MOST) add_norm_kernel(Desc d) {
 
 // SIDE: there is a post norm or a gate; without them dy = scale dresidual. AGAIN: h is made again from y and residual, in float32 as
 // the forward pass made it, and not read as it is stored: its rounding to bf16 would add to dweight as much error as that's
-// own (4096 x 2048 without post and gate 18.5 us so, 22 with one row more to read; with them y is read anyway). The next row's loads are on
-// their way during a row's sums. What all rows share (weight, post, a gate per channel) stays in registers: loads come back in
-// order, so one that a row waits for would wait for the next row's as well.
+// own (4096 x 2048 without post and gate 20.8 us so, 18.5 from the stored h: one row less to read; with them y is read
+// anyway). The next row's loads are on their way during a row's sums. What all rows share (weight, post, a gate per channel)
+// stays in registers: loads come back in order, so one that a row waits for would wait for the next row's as well.
 template <class TY, class TS, bool SIDE, bool AGAIN, bool WAVE, int CH, int MOST>
 __global__ void __launch_bounds__(MOST) add_norm_backward_kernel(Desc d, int groups) {
   __shared__ float slots[2][3][16];

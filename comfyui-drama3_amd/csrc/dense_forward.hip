@@ -27,7 +27,7 @@ int check_lora(const std::string& what, const Dense& a, const void* A, const flo
 }
 
 // p[m, r] = alpha[a] sum_k x[m, k] A[a, r, k] for the adapter a of each row m, rounded to bf16 (the operand of the second product:
-// a relative 2^-9 of what the adapter adds). Rows without an adapter are not written, nor read later. Two kernels:
+// within 2^-8 of each value's size). Rows without an adapter are not written, nor read later. Two kernels:
 
 // Up to 16 rows: a workgroup takes 16 ranks and an adapter that the rows name (blockIdx.y of them), its 8 waves an eighth of K each.
 __global__ void __launch_bounds__(ST_THREADS) lora_inner_stream_kernel(Dense a, const uint16_t* A, const float* alpha) {
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(ST_THREADS) lora_inner_stream_kernel(Dense a, 
 }
 
 // More: tiles of 64 rows and 32 ranks, one adapter that the rows name after the other (blockIdx.z of them at the start, gridDim.z
-// apart). A CU reads three times as fast into LDS as straight into operands: 5000 rows of rank 32, K 2048, 20 us that way, 11 so.
+// apart). 5000 rows of 12 requests, rank 32, K 2048: 12.4 us, 20.3 with the rows and adapters read straight into operands.
 __global__ void __launch_bounds__(Thin::THREADS, 2) lora_inner_tile_kernel(Dense a, const uint16_t* A, const float* alpha) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[Thin::LDS];
   static_assert(Thin::TM == 64);
