@@ -475,7 +475,8 @@ extern "C" int d3_add_norm_backward(const d3_add_norm_desc* desc, void* stream) 
   const int parts = !!d.dweight + !!d.dpost + (d.dgate && d.gate_kind == GATE_CHANNEL);
   const int groups = groups_of(d.T, d.H);
   if (d.T > 0) {
-    if (!(d.dh || d.dn) || (d.dn && (!d.rstd || !(d.stream_type && d.y ? d.residual : d.h))) || (d.post && !d.rstd)) return fail("d3_add_norm_backward: null pointer");
+    if (!(d.dh || d.dn) || (d.dn && (!d.rstd || !(d.stream_type && d.y ? d.residual : d.h))) || (d.post && !d.rstd))
+      return fail("d3_add_norm_backward: null pointer");
     if (parts && (!d.partials || d.partials_floats < (int64_t)parts * groups * d.H))
       return fail("d3_add_norm_backward: partials too small (d3_add_norm_partials)");
     by_types(d, [&](auto y, auto s) {
