@@ -12,10 +12,7 @@ generic. Weights are N(0, 0.02) (norms' around 1), activations N(0, 1) with a fe
 rows follow each other, as prompts packed into one pass do; in decode lines every row is a request of its own. Some requests
 have no adapter (id -1).
 """
-import functools
 import math
-import pathlib
-import sys
 
 import torch
 
@@ -234,8 +231,9 @@ def run(state):
     return (h, n) + tuple(g for g in grads if g is not None)
 
 
-@functools.cache
 def _block():
+    import pathlib
+    import sys
     package = str(pathlib.Path(__file__).resolve().parents[1] / "comfyui-drama3_amd")
     if package not in sys.path:
         sys.path.insert(0, package)
