@@ -59,12 +59,14 @@ class AddNormDesc(ctypes.Structure):
 
 
 class Layout:
-    """A descriptor struct of include/drama3_moe.h as its fields' names and format codes in order: pack(...) gives its bytes (a
-    ctypes.Structure of as many fields takes four times as long to fill)."""
+    """A descriptor struct of include/drama3_moe.h as its fields' names and format codes in order: pack(...) gives its bytes, those that
+    pad its end among them, since the C entries copy the whole struct (a ctypes.Structure of as many fields takes four times as
+    long to fill)."""
 
     def __init__(self, **runs):
         self.fields = [(name, code) for code, names in runs.values() for name in names.split()]
-        self.struct = struct.Struct("".join(code for _, code in self.fields))  # native sizes and alignment
+        # native sizes and alignment; the end aligned as the widest fields are (8 bytes)
+        self.struct = struct.Struct("".join(code for _, code in self.fields) + "0Q")
         self.pack = self.struct.pack
 
 

@@ -219,3 +219,15 @@ def test_descriptor_layout_matches_header(layout, cname, tmp_path):
     for i, (name, code) in enumerate(layout.fields):
         assert got[name] == (struct.calcsize(codes[:i + 1]) - struct.calcsize(code), struct.calcsize(code)), name
     assert len(got) == len(layout.fields)
+
+
+@pytest.mark.parametrize("layout, cname", [(_lib.ADD_NORM, "d3_add_norm_desc"), (_lib.DENSE, "d3_dense_desc"),
+                                           (_lib.GATED_FFN_BACKWARD, "d3_gated_ffn_backward_desc")])
+def test_descriptors_are_whole(layout, cname, tmp_path):
+    """A packed descriptor has as many bytes as the header's struct, of which the C entries read every one."""
+    prog = tmp_path / "size.c"
+    prog.write_text(f'#include <stdio.h>\n#include "{HEADER}"\nint main(void) {{ printf("%zu\\n", sizeof({cname})); return 0; }}\n')
+    exe = tmp_path / "size"
+    subprocess.run(["gcc", "-std=c11", "-o", str(exe), str(prog)], check=True, capture_output=True)
+    size = int(subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout)
+    assert layout.struct.size == size == len(layout.pack(*(0.0 if code == "f" else 0 for _, code in layout.fields)))
