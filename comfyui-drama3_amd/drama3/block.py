@@ -301,24 +301,40 @@ def _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, stats):
     return h, n, rstd
 
 
+class _Saved(tuple):
+    """add_norm_forward's (rstd, residual) with what residual's version was (None: its type keeps none)."""
+    version = None
+
+
+def _version(t):
+    return None if t.is_inference() else t._version
+
+
 def add_norm_forward(y, residual, weight, *, post=None, gate=None, scale=1.0, eps=1e-6, unit_offset=False):
-    """add_norm's (h, n) and what add_norm_backward needs beside them: (rstd [2, T] float32, residual); autograd does not see it."""
+    """add_norm's (h, n) and what add_norm_backward needs beside them: (rstd [2, T] float32, residual); autograd does not see it.
+    The residual stream is kept, not copied: a bfloat16 one has to stay as it is until add_norm_backward has read it (one that torch
+    knows to have changed is refused there); a float32 one is not read again."""
     with torch.no_grad():
         h, n, rstd = _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, True)
-        return h, n, (rstd, residual)
+        saved = _Saved((rstd, residual))
+        saved.version = _version(residual)
+        return h, n, saved
 
 
 def add_norm_backward(dh, dn, y, h, saved, weight, *, post=None, gate=None, scale=1.0, unit_offset=False,
                       needs=(True, True, True, True, True)):
     """(dy, dresidual, dweight, dpost, dgate) of add_norm for the gradients dh and dn of its outputs (either may be None: zero),
-    with y, weight, post, gate, scale and unit_offset as they went in and h and `saved` as add_norm_forward returned them. Each
-    gradient has its input's type and shape; None where the input is absent or `needs` says so. Float32 inside; of a bfloat16
-    stream h is made again from y and residual, since its rounding would show in the gradients. Sums over the rows (dweight,
-    dpost, a gate per channel) are the same bits from call to call."""
+    with y, residual (a bfloat16 one), weight, post, gate, scale and unit_offset as they went in and h and `saved` as
+    add_norm_forward returned them. Each gradient has its input's type and shape; None where the input is absent or `needs` says
+    so. Float32 inside; of a bfloat16 stream h is not read but made again from y and `saved`'s residual, since its rounding would
+    show in the gradients. Sums over the rows (dweight, dpost, a gate per channel) are the same bits from call to call."""
     with torch.no_grad():
         if y is None:
             raise TypeError("y [T, H] float32 or bfloat16 expected")
         rstd, residual = saved
+        if h.dtype is torch.bfloat16 and isinstance(saved, _Saved) and saved.version != _version(residual):
+            raise RuntimeError("add_norm_backward: residual was changed in place after add_norm_forward, which a bfloat16 stream's "
+                               "gradients read again")
         return _add_norm_backward(dh, dn, y, h, rstd, residual, weight, post, gate, scale, unit_offset, needs, None)
 
 

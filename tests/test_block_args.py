@@ -231,3 +231,25 @@ def test_descriptors_are_whole(layout, cname, tmp_path):
     subprocess.run(["gcc", "-std=c11", "-o", str(exe), str(prog)], check=True, capture_output=True)
     size = int(subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout)
     assert layout.struct.size == size == len(layout.pack(*(0.0 if code == "f" else 0 for _, code in layout.fields)))
+
+
+@pytest.mark.parametrize("stream", [BF, F32])
+def test_add_norm_backward_refuses_a_changed_residual(stream, monkeypatch):
+    """A bfloat16 stream's gradients read the residual again: one written to between the explicit pair's calls is refused."""
+    launched = []
+    monkeypatch.setattr(block.kernels, "launch", lambda name, *args: launched.append(name))
+    residual, y, weight = z(3, 16, dtype=stream), z(3, 16), z(16)
+    h, n, saved = block.add_norm_forward(y, residual, weight)
+    assert len(saved) == 2 and saved[1] is residual
+    block.add_norm_backward(h, n, y, h, saved, weight)
+    residual.add_(1)
+    if stream is F32:
+        block.add_norm_backward(h, n, y, h, saved, weight)
+    else:
+        with pytest.raises(RuntimeError, match="residual was changed"):
+            block.add_norm_backward(h, n, y, h, saved, weight)
+    with torch.inference_mode():  # (keeps no versions)
+        residual = z(3, 16, dtype=stream)
+        h, n, saved = block.add_norm_forward(y, residual, weight)
+        block.add_norm_backward(h, n, y, h, saved, weight)
+    assert launched.count("d3_add_norm") == 2
