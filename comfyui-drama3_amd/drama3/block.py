@@ -8,11 +8,13 @@
 The reference has no kernels for these. Nothing waits on the host; outputs and workspaces are allocated per call, so calls on
 different streams are independent and each can be captured in a graph. The C entries are in include/drama3_moe.h.
 
-Gradients: gated_ffn (without adapters), add_norm and norm are differentiable (torch.autograd, first order). Under graph capture
+Gradients: gated_ffn (without adapters), add_norm and norm are differentiable (torch.autograd, reverse mode, first order); inputs
+with a forward-mode tangent are refused, here and in what has no backward pass. Under graph capture
 their autograd backward is refused, since torch may then touch a stream outside the capture; a captured training step calls
 gated_ffn_forward and gated_ffn_backward, add_norm_forward and add_norm_backward, which the autograd forms are made of.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, kernels
 
@@ -31,6 +33,16 @@ def _any_grad(*tensors):
         if t is not None and t.requires_grad:
             return True
     return False
+
+
+def _no_tangent(name, *tensors):
+    """Refuses forward-mode AD's dual tensors, whose requires_grad is False: their tangents would be dropped, as if zero. (Outside a
+    dual level there are none; asking each of five tensors would cost 4 us a call.)"""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _at(t):
@@ -120,6 +132,7 @@ def _dense(x, T, K, stride, w, N, index, swiglu=False, pre=None, lora=None, ids=
 def linear(x, weight):
     """x weight^T of rows x [T, K] and a weight [N, K] (bfloat16): [T, N] bfloat16, float32 sums rounded once. A router's logits,
     say; widths are multiples of 8. No backward pass."""
+    _no_tangent("linear", x, weight)
     if torch.is_grad_enabled() and _any_grad(x, weight):
         raise RuntimeError("linear has no backward pass: call it under torch.no_grad()")
     index = x.get_device()
@@ -134,6 +147,7 @@ def lora_linear(x, weight, a, b, alpha, ids):
     int64; a row whose id is outside 0 .. A - 1 (-1, say) has none. [T, N] bfloat16, rounded once; sums in float32, the inner
     product x a^T alpha rounded to bfloat16 between its two products. Widths and rank are multiples of 8 (pad adapters of smaller
     rank with zeros). For decode lines and for prompts packed into one pass."""
+    _no_tangent("lora_linear", x, weight, a, b, alpha)
     if torch.is_grad_enabled() and _any_grad(x, weight, a, b, alpha):
         raise RuntimeError("lora_linear has no backward pass: call it under torch.no_grad()")
     index = x.get_device()
@@ -208,6 +222,7 @@ def gated_ffn(x, gate_up, down, *, gate_up_lora=None, down_lora=None, ids=None):
     decoded together, a prompt, a training batch. Differentiable.
     gate_up_lora, down_lora = (a, b, alpha) with `ids` [T]: the rows' adapters beside either projection, as lora_linear's (then not
     differentiable)."""
+    _no_tangent("gated_ffn", x, gate_up, down, *(gate_up_lora or ()), *(down_lora or ()))
     if gate_up_lora is None and down_lora is None:
         if ids is not None:
             raise ValueError("ids go with gate_up_lora or down_lora")
@@ -408,6 +423,7 @@ def add_norm(y, residual, weight, *, post=None, gate=None, scale=1.0, eps=1e-6, 
     block as well). y and residual [T, H], float32 or bfloat16 each; weight and post [H]; gate a value per row [T, 1], per
     channel [H] or per element [T, H]. rms(z) = sqrt(mean(z^2) + eps); with unit_offset weight and post are read as 1 + w.
     weight None: n is None. Float32 inside, h and n each rounded once (n comes from h before its rounding). Differentiable."""
+    _no_tangent("add_norm", y, residual, weight, post, gate)
     if torch.is_grad_enabled() and _any_grad(y, residual, weight, post, gate):
         return _AddNorm.apply(y, residual, weight, post, gate, scale, eps, unit_offset)
     return _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, False)[:2]
@@ -452,6 +468,7 @@ def norm(x, weight, *, eps=1e-6, unit_offset=False, dtype=None):
     dtype = x.dtype if dtype is None else dtype
     if dtype not in _TYPES or x.dtype not in _TYPES:
         raise TypeError("float32 or bfloat16 expected")
+    _no_tangent("norm", x, weight)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)):
         return _Norm.apply(x, weight, eps, unit_offset, dtype)
     return _norm(x, weight, eps, unit_offset, dtype, False)[0]
@@ -475,7 +492,9 @@ def sparse_block(n, h, router, gate_up, down, topk, *, shared=None, shared_gate=
     shared = (gate_up, down): the shared expert, gated_ffn with `shared_lora` = (gate_up_lora, down_lora) of the rows' adapters
     `ids`; it enters times sigmoid(n . gate) where shared_gate (gate_weight's) is given. The routed and the shared output are each
     added to the stream, times `scale`, and rounded to its type. Any number of rows; nothing waits on the host. No backward pass."""
-    tensors = (n, h, router, gate_up, down, shared_gate, next_weight, *(shared or ()))
+    loras = [t for lora in shared_lora for t in lora or ()]
+    tensors = (n, h, router, gate_up, down, shared_gate, next_weight, *(shared or ()), *loras)
+    _no_tangent("sparse_block", *tensors)
     if torch.is_grad_enabled() and _any_grad(*tensors):
         raise RuntimeError("sparse_block has no backward pass: call it under torch.no_grad()")
     if shared is None and (shared_gate is not None or ids is not None or tuple(shared_lora) != (None, None)):

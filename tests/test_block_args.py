@@ -253,3 +253,32 @@ def test_add_norm_backward_refuses_a_changed_residual(stream, monkeypatch):
         h, n, saved = block.add_norm_forward(y, residual, weight)
         block.add_norm_backward(h, n, y, h, saved, weight)
     assert launched.count("d3_add_norm") == 2
+
+
+DUAL_CALLS = {
+    "linear": (lambda *t: block.linear(*t), [(2, 16), (8, 16)]),
+    "lora_linear": (lambda *t: block.lora_linear(*t, torch.zeros(2, dtype=torch.int64)),
+                    [(2, 16), (24, 16), (3, 8, 16), (3, 24, 8), (3,)]),
+    "gated_ffn": (lambda *t: block.gated_ffn(*t), [(2, 16), (32, 16), (16, 16)]),
+    "gated_ffn with adapters": (lambda x, g, d, *t: block.gated_ffn(x, g, d, down_lora=t, ids=torch.zeros(2, dtype=torch.int64)),
+                                [(2, 16), (32, 16), (16, 16), (1, 8, 16), (1, 16, 8), (1,)]),
+    "add_norm": (lambda y, r, w, p, g: block.add_norm(y, r, w, post=p, gate=g), [(2, 16), (2, 16), (16,), (16,), (2, 1)]),
+    "norm": (lambda *t: block.norm(*t), [(2, 16), (16,)]),
+    "sparse_block": (lambda n, h, r, gu, d, sgu, sd, sg, w, a, b, al: block.sparse_block(
+        n, h, r, gu, d, 2, shared=(sgu, sd), shared_gate=sg, next_weight=w, shared_lora=(None, (a, b, al)),
+        ids=torch.zeros(2, dtype=torch.int64)),
+        [(2, 16), (2, 16), (8, 16), (256, 16), (128, 16), (32, 16), (16, 16), (8, 16), (16,), (1, 8, 16), (1, 16, 8), (1,)]),
+}
+
+
+@pytest.mark.parametrize("name, which", [(name, i) for name, (_, shapes) in DUAL_CALLS.items() for i in range(len(shapes))])
+def test_forward_mode_is_refused(name, which, monkeypatch):
+    """A tangent is never dropped: a dual tensor (whose requires_grad is False) in any place is refused before any launch."""
+    monkeypatch.setattr(block.kernels, "launch", lambda *args: pytest.fail("launched"))
+    call, shapes = DUAL_CALLS[name]
+    tensors = [z(*s, dtype=F32 if s in ((1,), (3,)) else BF) for s in shapes]
+    with torch.autograd.forward_ad.dual_level():
+        tensors[which] = torch.autograd.forward_ad.make_dual(tensors[which], torch.ones_like(tensors[which]))
+        assert not tensors[which].requires_grad
+        with pytest.raises(RuntimeError, match=f"{name.split()[0]} has no forward-mode"):
+            call(*tensors)
