@@ -11,7 +11,8 @@ different streams are independent and each can be captured in a graph. The C ent
 Gradients: gated_ffn (without adapters), add_norm and norm are differentiable (torch.autograd, reverse mode, first order); inputs
 with a forward-mode tangent are refused, here and in what has no backward pass. Under graph capture
 their autograd backward is refused, since torch may then touch a stream outside the capture; a captured training step calls
-gated_ffn_forward and gated_ffn_backward, add_norm_forward and add_norm_backward, which the autograd forms are made of.
+gated_ffn_forward and gated_ffn_backward, add_norm_forward and add_norm_backward, norm_forward and norm_backward, which the
+autograd forms are made of.
 """
 import torch
 from torch.autograd import forward_ad
@@ -25,7 +26,9 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 def _no_capture(name):
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{name}: autograd's backward pass is not captured; call {name}_backward in the captured step")
+        raise RuntimeError(f"{name}: autograd's backward pass is not captured; call the explicit pairs in the captured step "
+                           "(gated_ffn_forward and gated_ffn_backward, add_norm_forward and add_norm_backward, norm_forward and "
+                           "norm_backward)")
 
 
 def _any_grad(*tensors):
@@ -440,13 +443,10 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dn):
-        _no_capture("add_norm")
+        _no_capture("norm")
         x, rstd, weight = ctx.saved_tensors
-        needs = ctx.needs_input_grad
         unit_offset, dtype = ctx.options
-        _, dx, dweight, _, _ = _add_norm_backward(None, dn, None, x, rstd, None, weight, None, None, 1.0, unit_offset,
-                                                  (False, needs[0], needs[1], False, False), dtype)
-        return dx, dweight, None, None, None
+        return _norm_backward(dn, x, rstd, weight, unit_offset, dtype, ctx.needs_input_grad[:2]) + (None,) * 3
 
 
 def _norm(x, weight, eps, unit_offset, dtype, stats):
@@ -462,12 +462,38 @@ def _norm(x, weight, eps, unit_offset, dtype, stats):
     return n, rstd
 
 
-def norm(x, weight, *, eps=1e-6, unit_offset=False, dtype=None):
-    """x / rms(x) * weight of rows x [T, H] (float32 or bfloat16), in `dtype` (x's without it): the norm before a model's first
-    block; add_norm makes the others. Differentiable."""
+def _norm_backward(dn, x, rstd, weight, unit_offset, dtype, needs):
+    _, dx, dweight, _, _ = _add_norm_backward(None, dn, None, x, rstd, None, weight, None, None, 1.0, unit_offset,
+                                              (False, *needs, False, False), dtype)
+    return dx, dweight
+
+
+def _norm_type(x, dtype):
     dtype = x.dtype if dtype is None else dtype
     if dtype not in _TYPES or x.dtype not in _TYPES:
         raise TypeError("float32 or bfloat16 expected")
+    return dtype
+
+
+def norm_forward(x, weight, *, eps=1e-6, unit_offset=False, dtype=None):
+    """norm's n and what norm_backward needs beside x: rstd [2, T] float32 (its second row is add_norm's); autograd does not see it."""
+    with torch.no_grad():
+        return _norm(x, weight, eps, unit_offset, _norm_type(x, dtype), True)
+
+
+def norm_backward(dn, x, saved, weight, *, unit_offset=False, needs=(True, True)):
+    """(dx, dweight) of norm for the gradient dn of its output, with x, weight and unit_offset as they went in and `saved` as
+    norm_forward returned it, each of its input's type; None where `needs` says so. dweight is the same bits from call to call."""
+    with torch.no_grad():
+        if dn is None or weight is None or dn.dtype not in _TYPES:
+            raise ValueError("dn [T, H] float32 or bfloat16, and weight, expected")
+        return _norm_backward(dn, x, saved, weight, unit_offset, dn.dtype, needs)
+
+
+def norm(x, weight, *, eps=1e-6, unit_offset=False, dtype=None):
+    """x / rms(x) * weight of rows x [T, H] (float32 or bfloat16), in `dtype` (x's without it): the norm before a model's first
+    block; add_norm makes the others. Differentiable."""
+    dtype = _norm_type(x, dtype)
     _no_tangent("norm", x, weight)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)):
         return _Norm.apply(x, weight, eps, unit_offset, dtype)

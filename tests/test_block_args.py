@@ -282,3 +282,31 @@ def test_forward_mode_is_refused(name, which, monkeypatch):
         assert not tensors[which].requires_grad
         with pytest.raises(RuntimeError, match=f"{name.split()[0]} has no forward-mode"):
             call(*tensors)
+
+
+def test_norm_backward_under_capture_names_its_own_pair(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="^norm: .*norm_forward and norm_backward"):
+        block._Norm.backward(None, z(2, 8))
+
+
+@pytest.mark.parametrize("match, changed", [
+    ("dn", {"dn": None}),
+    ("dn", {"dn": z(3, 10, dtype=torch.float16)}),
+    ("dn of", {"dn": z(2, 10)}),
+    ("weight", {"weight": None}),
+    ("weight", {"weight": z(12)}),
+    ("rstd", {"saved": None}),
+    ("rstd", {"saved": z(1, 3, dtype=F32)}),
+    ("on a GPU", {}),
+])
+def test_norm_backward_refusals(match, changed):
+    with pytest.raises(ValueError, match=match):
+        block.norm_backward(**{**{"dn": z(3, 10), "x": z(3, 10, dtype=F32), "saved": z(2, 3, dtype=F32), "weight": z(10)}, **changed})
+
+
+def test_norm_forward_refusals():
+    with pytest.raises(TypeError):
+        block.norm_forward(z(2, 8), z(8), dtype=torch.float16)
+    with pytest.raises(ValueError, match="weight"):
+        block.norm_forward(z(2, 8), None)

@@ -690,3 +690,35 @@ def test_training_step_by_autograd():
     # some ten roundings to bf16 on the longest way, each at most 2^-8 / sqrt(3) of the norm on the average: 2^-8 sqrt(10 / 3)
     for a, b in zip(got, want):
         assert ((a.to(F64) - b).norm() / b.norm()).item() < 2.0 ** -8 * (10 / 3) ** 0.5
+
+
+@pytest.mark.parametrize("stream, dtype", [(BF, BF), (F32, BF), (BF, F32), (F32, F32)])
+def test_norm_pair_captured(stream, dtype):
+    """The explicit pair of a model's first norm: autograd's numbers, eager and in a graph that is replayed on new rows."""
+    gen = gen_of(2)
+    x, weight, dn = randn(gen, 37, 264, dtype=stream), randn(gen, 264, dtype=stream), randn(gen, 37, 264, dtype=dtype)
+
+    def step():
+        n, saved = block.norm_forward(x, weight, unit_offset=True, dtype=dtype)
+        return (n, *block.norm_backward(dn, x, saved, weight, unit_offset=True))
+
+    leaves = [t.clone().requires_grad_() for t in (x, weight)]
+    out = block.norm(*leaves, unit_offset=True, dtype=dtype)
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip((out, *torch.autograd.grad(out, leaves, dn)), want))
+    n, saved = block.norm_forward(x, weight, unit_offset=True, dtype=dtype)
+    for i in range(2):
+        one = block.norm_backward(dn, x, saved, weight, unit_offset=True, needs=(i == 0, i == 1))
+        assert torch.equal(one[i], want[1 + i]) and one[1 - i] is None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        x.copy_(torch.randn(x.shape, device=DEV))
+        dn.copy_(torch.randn(dn.shape, device=DEV))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
