@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(ST_THREADS) lora_inner_stream_kernel(Dense a, 
 }
 
 // More: tiles of 64 rows and 32 ranks, one adapter that the rows name after the other (blockIdx.z of them at the start, gridDim.z
-// apart). 5000 rows of 12 requests, rank 32, K 2048: 12.4 us, 20.3 with the rows and adapters read straight into operands.
+// apart), all 64 rows multiplied and those of the adapter kept: rows of as many adapters by turns take as many times the work. 5000 rows of 12 requests, rank 32, K 2048: 12.4 us, 20.3 with the rows and adapters read straight into operands.
 __global__ void __launch_bounds__(Thin::THREADS, 2) lora_inner_tile_kernel(Dense a, const uint16_t* A, const float* alpha) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[Thin::LDS];
   static_assert(Thin::TM == 64);
@@ -77,9 +77,13 @@ void launch_inner(const Dense& of, const void* A, const float* alpha, hipStream_
   if (a.M <= 16) {
     lora_inner_stream_kernel<<<dim3((a.rank + 15) / 16, a.M), ST_THREADS, 0, stream>>>(a, (const uint16_t*)A, alpha);
   } else {
-    // few rows: a workgroup for each of 32 adapters; many, where requests' rows follow each other: two
-    lora_inner_tile_kernel<<<dim3((a.rank + 31) / 32, (a.M + 63) / 64, a.M <= 256 ? 32 : 2), Thin::THREADS, 0, stream>>>(
-        a, (const uint16_t*)A, alpha);
+    // Which adapters a tile of rows names only the device knows: as many workgroups a tile as it may name (64 rows, `adapters`), while
+    // they fit the CUs at once (two each), at least two; those without an adapter end at once. A whole call, N 1024, rank 32, 32
+    // adapters, by turns and in runs, us: 256 rows 19.7 and 16.2, 300 19.9 and 16.3, 1000 29.4 and 17.5, 5000 148 and 37; two
+    // workgroups a tile: 300 rows 98 and 32, 1000 104 and 23, 5000 159 and 37.
+    const int ranks = (a.rank + 31) / 32, tiles = (a.M + 63) / 64;
+    const int z = std::clamp(512 / std::max<int64_t>((int64_t)ranks * tiles, 1), (int64_t)2, (int64_t)std::max(2, std::min(a.adapters, 64)));
+    lora_inner_tile_kernel<<<dim3(ranks, tiles, z), Thin::THREADS, 0, stream>>>(a, (const uint16_t*)A, alpha);
   }
 }
 

@@ -722,3 +722,36 @@ def test_norm_pair_captured(stream, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_adapters_by_turns_have_no_cliff():
+    """Rows that name 32 adapters by turns: one row more than 256 takes about as long (it took five times as long where the rule of
+    the workgroups an adapter tile gets went by the rows alone)."""
+    times = {}
+    for T in (256, 257, 500):
+        x, w, a, b, alpha = lora_inputs(T, 2048, 1024, 32, 32)
+        ids = ids_of("each", T, 32)
+        for _ in range(3):
+            block.lora_linear(x, w, a, b, alpha, ids)
+        best = float("inf")
+        for _ in range(8):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            for _ in range(20):
+                block.lora_linear(x, w, a, b, alpha, ids)
+            end.record()
+            end.synchronize()
+            best = min(best, start.elapsed_time(end))
+        times[T] = best
+    assert times[257] < 2.5 * times[256] and times[500] < 3 * times[256], times
+
+
+@pytest.mark.parametrize("kind", ["each", "runs", "mixed", "outside"])
+@pytest.mark.parametrize("T, K, N, rank, count", [(300, 136, 72, 40, 70), (517, 264, 136, 8, 33), (1100, 72, 264, 160, 3), (2100, 64, 64, 96, 90)])
+def test_lora_linear_many_rows(T, K, N, rank, count, kind):
+    """More rows than 256 and adapters by turns: tiles of rows that name more adapters than they have workgroups, or fewer."""
+    x, w, a, b, alpha = lora_inputs(T, K, N, rank, count, seed=T)
+    ids = ids_of(kind, T, count)
+    base, e_base = dot(x.to(F64), w.to(F64).T)
+    more, e_more = adapter(x.to(F64), a, b, alpha, ids)
+    within(block.lora_linear(x, w, a, b, alpha, ids), base + more, rounded(base + more, e_base + e_more), kind)
