@@ -6,7 +6,7 @@ entry. A float32 sum of n products is taken to be off by at most n 2^-23 of the 
 import pytest
 import torch
 
-from drama3 import block, kernels
+from drama3 import _lib, block, kernels
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -755,3 +755,68 @@ def test_lora_linear_many_rows(T, K, N, rank, count, kind):
     base, e_base = dot(x.to(F64), w.to(F64).T)
     more, e_more = adapter(x.to(F64), a, b, alpha, ids)
     within(block.lora_linear(x, w, a, b, alpha, ids), base + more, rounded(base + more, e_base + e_more), kind)
+
+
+# --------------------------------------------------------------------- many rows: sums over them, and every size of tile
+def norm_bounds(doubles, dh, dn, scale, offset, eps, additions):
+    """(gradients, bounds) in float64 of dresidual and of what is summed over the rows, for float32 work on a stream that is not
+    rounded on the way: a row's sums and their roots off by 100 steps u = 2^-24 (as in norm_check), each product by one; a
+    sum over the rows by `additions` steps of its terms' magnitudes."""
+    u = 2.0 ** -24
+    y, residual, weight, post, gate = doubles
+    rms = lambda t: (t * t).mean(1, keepdim=True).add(eps).sqrt()  # noqa: E731
+    yhat = y if post is None else y / rms(y)
+    v = yhat if post is None else yhat * (post + offset)
+    g = 1.0 if gate is None else gate
+    h = residual + scale * g * v
+    e_h = 100 * u * ((h - residual).abs() + residual.abs())
+    r = 1 / rms(h)
+    e_r = 100 * u + (e_h * h.abs()).mean(1, keepdim=True) * r ** 2  # relative
+    hat = h * r
+    e_hat = e_h * r + hat.abs() * e_r
+    a = dn * (weight + offset)
+    m = (a * hat).mean(1, keepdim=True)
+    e_m = 100 * u * (a * hat).abs().mean(1, keepdim=True) + (a.abs() * e_hat).mean(1, keepdim=True)
+    dr = dh + r * (a - hat * m)
+    e_dr = (8 * u + e_r) * (dh.abs() + r * (a.abs() + (hat * m).abs())) + r * (e_hat * m.abs() + hat.abs() * e_m)
+
+    def summed(terms, err):
+        return terms.sum(0), err.sum(0) + additions * u * terms.abs().sum(0)
+
+    def product(factor):  # of dv = scale dr and a factor that is off by 100 steps and a few
+        return scale * dr * factor, abs(scale) * factor.abs() * (e_dr + 110 * u * dr.abs())
+
+    found = {"residual": (dr, e_dr), "weight": summed(dn * hat, dn.abs() * (e_hat + 2 * u * hat.abs()))}
+    if post is not None:
+        found["post"] = summed(*product(g * yhat))
+    if gate is not None and gate.dim() == 1:
+        found["gate"] = summed(*product(v))
+    elif gate is not None and gate.shape[1] == 1:
+        terms, err = product(v)  # a row's sum over its columns
+        found["gate"] = terms.sum(1, keepdim=True), (err + 100 * u * terms.abs()).sum(1, keepdim=True)
+    elif gate is not None:
+        found["gate"] = product(v)
+    return found
+
+
+@pytest.mark.parametrize("of, stream, weights", [(BF, BF, BF), (BF, F32, F32), (F32, F32, F32), (F32, BF, F32)])
+@pytest.mark.parametrize("gate, post", [("none", False), ("channel", True), ("row", True), ("full", True), ("channel", False)])
+@pytest.mark.parametrize("T, H", [(8192, 512), (4099, 72), (5000, 1000), (1600, 2048), (1391, 5120), (601, 8200), (600, 16384)])
+def test_add_norm_sums_over_many_rows(T, H, gate, post, of, stream, weights):
+    """More rows than a backward pass has groups, so that each walks several, at widths of every form of the kernel. Every sum over
+    the rows is held to half a step of itself and to float32's steps, which a row left out, or h read back as it was rounded to a
+    bfloat16 stream, exceeds by far."""
+    scale, offset = 0.7, not post
+    y, residual, weight, post_w, g, dh, dn = norm_inputs(T, H, of, stream, gate, post, weights, seed=T + H)
+    opt = {"post": post_w, "gate": g, "scale": scale, "unit_offset": offset}
+    h, _, saved = block.add_norm_forward(y, residual, weight, **opt)
+    grads = dict(zip(("y", "residual", "weight", "post", "gate"), block.add_norm_backward(dh, dn, y, h, saved, weight, **opt)))
+    groups = _lib.lib().d3_add_norm_partials(T, H) // H
+    assert T > groups
+    # a group's rows one after the other, every 128th group, 4 of those and 32 of these
+    additions = -(-T // groups) + -(-groups // 128) + 4 + 32
+    found = norm_bounds([None if t is None else t.to(F64) for t in (y, residual, weight, post_w, g)], dh.to(F64), dn.to(F64), scale,
+                        float(offset), 1e-6, additions)
+    for name, (want, err) in found.items():
+        within(grads[name], want, rounded(want, err, grads[name].dtype), name)
+    norm_check(T, H, of, stream, gate, post, weights, scale=scale, offset=offset, seed=T + H)
