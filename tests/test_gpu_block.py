@@ -820,3 +820,57 @@ def test_add_norm_sums_over_many_rows(T, H, gate, post, of, stream, weights):
     for name, (want, err) in found.items():
         within(grads[name], want, rounded(want, err, grads[name].dtype), name)
     norm_check(T, H, of, stream, gate, post, weights, scale=scale, offset=offset, seed=T + H)
+
+
+@pytest.mark.parametrize("T, H, I, O", [
+    (900, 72, 520, 264),       # gate and up by 64 x 64
+    (4001, 1032, 6152, 4040),  # the second product, gate's and up's gradients and the set of gradients by 256 x 256
+    (2500, 264, 4072, 72),     # gate's and up's gradients: 128 x 256 for whole turns, then 64 x 64
+    (3300, 72, 3080, 520),     # then 128 x 128
+    (5000, 136, 3080, 264),    # then 32 x 64
+])
+def test_gated_ffn_by_other_tiles(T, H, I, O):
+    test_gated_ffn(T, H, I, O)
+
+
+@pytest.mark.parametrize("kind", ["runs", "each", "outside"])
+@pytest.mark.parametrize("T, K, N, rank, count", [
+    (700, 72, 1032, 40, 9),      # 64 x 64
+    (700, 200, 3080, 72, 5),     # 128 x 128
+    (1900, 136, 3080, 136, 7),   # 128 x 256
+    (2500, 72, 4072, 16, 12),    # 128 x 256 for whole turns, then 64 x 64
+    (3300, 264, 3080, 64, 6),    # then 128 x 128
+    (5000, 64, 3080, 96, 4),     # then 64 x 32
+])
+def test_lora_linear_by_other_tiles(T, K, N, rank, count, kind):
+    test_lora_linear(T, K, N, rank, count, kind)
+
+
+@pytest.mark.parametrize("kind", ["runs", "each"])
+@pytest.mark.parametrize("T, H, I, O", [
+    (700, 72, 520, 1032),     # gate and up by 64 x 64, down too
+    (1100, 136, 1032, 2056),  # 128 x 128
+    (3300, 72, 776, 3080),    # 128 x 256, down 128 x 256 for whole turns, then 128 x 128
+    (2500, 72, 2056, 264),    # 128 x 256 for whole turns, then 128 x 128
+    (5000, 64, 776, 136),     # then 64 x 64
+    (5000, 72, 1544, 72),     # then 64 x 32
+])
+def test_gated_ffn_with_adapters_by_other_tiles(T, H, I, O, kind):
+    x, gate_up, down, _ = ffn_inputs(T, H, I, O, seed=T)
+    lora = lora_inputs(T, H, 2 * I, 40, 6, seed=1)[2:], lora_inputs(T, I, O, 72, 6, seed=2)[2:]
+    ids = ids_of(kind, T, 6)
+    ref = Ffn(x, gate_up, down, lora, ids)
+    within(block.gated_ffn(x, gate_up, down, gate_up_lora=lora[0], down_lora=lora[1], ids=ids), ref.out, ref.e_out)
+
+
+@pytest.mark.parametrize("T, K, N", [(300, 72, 2056), (700, 72, 3080), (1900, 72, 3080), (5000, 72, 3080)])
+def test_lora_linear_bad_adapters_stay_in_their_rows_of_other_tiles(T, K, N):
+    """As above, at 64 x 64, 128 x 128, 128 x 256 and the latter followed by 64 x 32."""
+    x, w, a, b, alpha = lora_inputs(T, K, N, 72, 4, seed=T)
+    ids = torch.arange(T, device=DEV) % 4 - 1
+    want = block.lora_linear(x, w, a, b, alpha, ids)
+    a2, b2 = a.clone(), b.clone()
+    a2[1], b2[1, ::2], b2[3], a2[3] = float("inf"), float("nan"), float("nan"), float("nan")
+    got = block.lora_linear(x, w, a2, b2, alpha, ids)
+    assert torch.equal(got[ids != 1], want[ids != 1])
+    assert not got[ids == 1].isfinite().all(1).any()
