@@ -45,19 +45,6 @@ class MoeA8PrefillDesc(ctypes.Structure):
     ]
 
 
-class AddNormDesc(ctypes.Structure):
-    """d3_add_norm_desc (include/drama3_moe.h)."""
-    _fields_ = [
-        ("y", c_void_p), ("residual", c_void_p), ("weight", c_void_p), ("post", c_void_p), ("gate", c_void_p),
-        ("dh", c_void_p), ("dn", c_void_p), ("h", c_void_p), ("n", c_void_p), ("rstd", c_void_p), ("dy", c_void_p),
-        ("dresidual", c_void_p), ("dweight", c_void_p), ("dpost", c_void_p), ("dgate", c_void_p), ("partials", c_void_p),
-        ("partials_floats", c_int64), ("y_stride", c_int64), ("residual_stride", c_int64), ("gate_stride", c_int64),
-        ("y_type", c_int32), ("stream_type", c_int32), ("weight_type", c_int32), ("post_type", c_int32),
-        ("gate_type", c_int32), ("gate_kind", c_int32), ("T", c_int32), ("H", c_int32), ("scale", ctypes.c_float),
-        ("eps", ctypes.c_float), ("unit_offset", c_int32),
-    ]
-
-
 class Layout:
     """A descriptor struct of include/drama3_moe.h as its fields' names and format codes in order: pack(...) gives its bytes, those that
     pad its end among them, since the C entries copy the whole struct (a ctypes.Structure of as many fields takes four times as
