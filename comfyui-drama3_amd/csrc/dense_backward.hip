@@ -26,7 +26,7 @@ extern "C" int d3_gated_ffn_backward(const d3_gated_ffn_backward_desc* d, void* 
     Dense a{};
     a.x = (const uint16_t*)d->dout, a.ldx = O, a.w = (const uint16_t*)d->down, a.ldw = I, a.M = T, a.N = I, a.K = O, a.half = I;
     a.out = (uint16_t*)d->dgate_up_rows, a.ldo = 2 * (int64_t)I, a.pre = (float*)d->pre;
-    launch_tiles<false, true, END_DSWIGLU>(a, s);
+    launch_tiles<true, END_DSWIGLU>(a, s);
   }
   DenseSet set{};
   set.rows = -1;

@@ -27,10 +27,10 @@ inline int dense_tiles(const Dense& a, bool swiglu) {
   return ((a.M + C::TM - 1) / C::TM) * (((swiglu ? a.half : a.N) + un - 1) / un);
 }
 
-template <class C, bool XT, bool WT, int END, bool LORA = false>
+template <class C, bool WT, int END, bool LORA>
 inline void launch_tile(const Dense& a, hipStream_t stream) {
   const int tiles = dense_tiles<C>(a, END == END_SWIGLU);
-  dense_tile_kernel<C, XT, WT, END, LORA><<<dim3(1, tiles), C::THREADS, 0, stream>>>(a);
+  dense_tile_kernel<C, WT, END, LORA><<<dim3(1, tiles), C::THREADS, 0, stream>>>(a);
 }
 
 enum TileSize { WIDE, LONG, SQUARE, SMALL, LEAST };
@@ -42,12 +42,12 @@ constexpr float LONG_COST = 0.82f;
 
 // The tile's size by what a stage of each takes, us, times the turns in which the 256 CUs take the tiles: 1.5 (256 x 256),
 // 0.82 (128 x 256), 0.45 (128 x 128; 0.5 in several turns), 0.17 (64 x 64), 0.155 (64 x 32), measured with the CUs at work.
-// So the large ones, which read least, where they come out even, and small ones for few rows. Measured, us, in this order (t:
-// transposed operands):
+// So the large ones, which read least, where they come out even, and small ones for few rows. Measured, us, in this order (t: a
+// transposed operand; tt: both, as in launch_dense_set):
 //   4096 x 4096 x 11008    266 276 317   -   -     4096 x 2048 x 6144    115  80  91   -   -     4096 x 12288 x 2048  154 170 200  -  -
 //   12288 x 2048 x 4096 tt 177 177 211   -   -     2048 x 6144 x 4096 tt  86 107 106   -   -     1391 x 1536 x 2048    -   -  16  19  -
 //    509 x 1024 x 2048       -   -   - 8.1 7.4       61 x 4096 x 2048      -   -   - 7.9 7.1     1391 x 2048 x 1536 t   -   -  13  16  -
-template <bool XT, bool WT, int END, bool LORA>
+template <bool WT, int END, bool LORA>
 inline TilePlan plan_tiles(const Dense& a) {
   constexpr bool SWIGLU = END == END_SWIGLU;
   using Least = std::conditional_t<WT, Flat, Thin>;
@@ -60,27 +60,24 @@ inline TilePlan plan_tiles(const Dense& a) {
   const float square = turns(dense_tiles<Square>(a, SWIGLU));
   try_size(SQUARE, (square > 1 ? 0.5f : 0.45f) * square);
   try_size(SMALL, 0.17f * turns(dense_tiles<Small>(a, SWIGLU)));
-  if (!XT) try_size(LEAST, 0.155f * turns(dense_tiles<Least>(a, SWIGLU)));
+  try_size(LEAST, 0.155f * turns(dense_tiles<Least>(a, SWIGLU)));
   return best;
 }
 
-template <bool XT, bool WT, int END, bool LORA>
+template <bool WT, int END, bool LORA>
 inline void launch_plan(TileSize size, const Dense& a, hipStream_t stream) {
   if constexpr (!LORA) {
-    if (size == WIDE) return launch_tile<Wide, XT, WT, END, LORA>(a, stream);
+    if (size == WIDE) return launch_tile<Wide, WT, END, LORA>(a, stream);
   }
-  if (size == LONG) launch_tile<Long, XT, WT, END, LORA>(a, stream);
-  else if (size == SQUARE) launch_tile<Square, XT, WT, END, LORA>(a, stream);
-  else if (size == SMALL) launch_tile<Small, XT, WT, END, LORA>(a, stream);
-  if constexpr (!XT) {
-    if (size == LEAST) launch_tile<std::conditional_t<WT, Flat, Thin>, XT, WT, END, LORA>(a, stream);
-  }
+  if (size == LONG) launch_tile<Long, WT, END, LORA>(a, stream);
+  else if (size == SQUARE) launch_tile<Square, WT, END, LORA>(a, stream);
+  else if (size == SMALL) launch_tile<Small, WT, END, LORA>(a, stream);
+  else launch_tile<std::conditional_t<WT, Flat, Thin>, WT, END, LORA>(a, stream);
 }
 
 // a's rows from m on
-template <bool XT>
 inline Dense rows_from(Dense a, int m, int rows) {
-  a.x += XT ? m : m * a.ldx;
+  a.x += m * a.ldx;
   a.out += m * a.ldo;
   if (a.pre) a.pre += (int64_t)m * 2 * a.half;
   if (a.ids) a.ids += m, a.p += (int64_t)m * a.rank;
@@ -90,20 +87,20 @@ inline Dense rows_from(Dense a, int m, int rows) {
 
 // The whole product by one size of tile, or the rows that fill whole turns of 128 x 256 tiles by those and the rest by
 // what suits it, where that is 8% less (the second launch takes 3 us): 5000 x 4096 x 2048 is 2.5 turns.
-template <bool XT, bool WT, int END, bool LORA = false>
+template <bool WT, int END, bool LORA = false>
 inline void launch_tiles(const Dense& a, hipStream_t stream) {
-  const TilePlan whole = plan_tiles<XT, WT, END, LORA>(a);
+  const TilePlan whole = plan_tiles<WT, END, LORA>(a);
   const int columns = dense_tiles<Long>(Dense{.M = 1, .N = a.N, .K = a.K, .half = a.half}, END == END_SWIGLU);
   const int full = dense_tiles<Long>(a, END == END_SWIGLU) / 256, rows = 256 * full / columns * Long::TM;
   if (full >= 1 && rows > 0 && rows < a.M) {
-    const Dense rest = rows_from<XT>(a, rows, a.M - rows);
-    const TilePlan left = plan_tiles<XT, WT, END, LORA>(rest);
+    const Dense rest = rows_from(a, rows, a.M - rows);
+    const TilePlan left = plan_tiles<WT, END, LORA>(rest);
     if (LONG_COST * full + left.cost < 0.92f * whole.cost) {
-      launch_tile<Long, XT, WT, END, LORA>(rows_from<XT>(a, 0, rows), stream);
-      return launch_plan<XT, WT, END, LORA>(left.size, rest, stream);
+      launch_tile<Long, WT, END, LORA>(rows_from(a, 0, rows), stream);
+      return launch_plan<WT, END, LORA>(left.size, rest, stream);
     }
   }
-  launch_plan<XT, WT, END, LORA>(whole.size, a, stream);
+  launch_plan<WT, END, LORA>(whole.size, a, stream);
 }
 
 // A set of products in one launch. The size of tile, one for all of them, by the same costs of a stage: its share of all tiles'
@@ -147,7 +144,7 @@ template <int END, bool LORA>
 inline void launch_dense(const Dense& a, hipStream_t stream) {
   const int columns = END == END_SWIGLU ? (a.half + 7) / 8 : (a.N + 15) / 16;
   if (a.M <= 16 && columns <= 256) dense_stream_kernel<END, LORA><<<columns, ST_THREADS, 0, stream>>>(a);
-  else launch_tiles<false, false, END, LORA>(a, stream);
+  else launch_tiles<false, END, LORA>(a, stream);
 }
 
 inline int launched(const char* what) {

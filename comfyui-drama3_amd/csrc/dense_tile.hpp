@@ -512,11 +512,11 @@ D3_INLINE bool tile_at(const Dense& a, int at, int& tm, int& tn) {
 }
 
 // (tiles along y: a grid's x has room for 2^32 threads)
-template <class C, bool XT, bool WT, int END, bool LORA>
+template <class C, bool WT, int END, bool LORA>
 __global__ void __launch_bounds__(C::THREADS, 2) dense_tile_kernel(Dense a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDS];
   int tm, tn;
-  if (tile_at<C, END>(a, blockIdx.y, tm, tn)) dense_tile<C, XT, WT, END, LORA>(a, tm, tn, smem);
+  if (tile_at<C, END>(a, blockIdx.y, tm, tn)) dense_tile<C, false, WT, END, LORA>(a, tm, tn, smem);
 }
 
 // Up to three products that do not need each other in one launch, the longest first: rows with a transposed w (the gradient of
