@@ -436,6 +436,9 @@ int check(const char* what, const Desc* d) {
   if ((d->y_type | d->stream_type | d->weight_type | d->post_type | d->gate_type) & ~1) return fail(at + ": types are 0 (float32) or 1 (bf16)");
   if (d->gate_kind < 0 || d->gate_kind > 3 || (d->gate_kind && !d->gate)) return fail(at + ": gate_kind is 0 to 3, with a gate from 1 on");
   if (d->T > 0 && (d->post || d->gate_kind) && !d->y) return fail(at + ": post and gate go with y");
+  if (d->T > 1 && ((d->y && d->y_stride < d->H) || d->residual_stride < d->H || (d->gate_kind == GATE_FULL && d->gate_stride < d->H) ||
+                   (d->gate_kind == GATE_ROW && d->gate_stride < 1)))
+    return fail(at + ": rows that lie less than their columns apart");
   return 0;
 }
 

@@ -447,7 +447,7 @@ int d3_bf16_grouped(const void* x, int32_t rows, const int64_t* order, int32_t k
  *   rstd(z) = 1 / sqrt(mean(z^2) + eps); post and weight read as 1 + w with unit_offset.
  * Types are 0 (float32) or 1 (bf16): h, residual and their gradients have stream_type, y, n and theirs y_type. gate_kind: 0
  * none, 1 a value per row (gate[t * gate_stride]), 2 per channel, 3 per element (rows gate_stride apart). Rows of y and
- * residual are their strides apart (elements), all others H. Float32 inside; n comes from h before h is rounded.
+ * residual are their strides apart (elements, H at least), all others H. Float32 inside; n comes from h before h is rounded.
  *   d3_add_norm: h (with y; without, h is residual and is not written) and n (with weight). rstd [2, T] may be NULL:
  *     rstd(h), and rstd(y) with post.
  *   d3_add_norm_backward: from dh and dn (either may be NULL: zero), y, rstd as the forward call left it, and h (rows

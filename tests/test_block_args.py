@@ -310,3 +310,13 @@ def test_norm_forward_refusals():
         block.norm_forward(z(2, 8), z(8), dtype=torch.float16)
     with pytest.raises(ValueError, match="weight"):
         block.norm_forward(z(2, 8), None)
+
+
+@pytest.mark.parametrize("changed", [{"y_stride": 0}, {"y_stride": 15}, {"residual_stride": -16}, {"residual_stride": 8}, {"gate_kind": 3, "gate": P},
+                                     {"gate_kind": 3, "gate": P, "gate_stride": -16}, {"gate_kind": 1, "gate": P}])
+@pytest.mark.parametrize("entry", ["d3_add_norm", "d3_add_norm_backward"])
+def test_add_norm_entries_refuse_strides(entry, changed):
+    """A descriptor whose strides were left out, or run backwards, is refused and not read."""
+    args = dict(y=P, residual=P, weight=P, dh=P, dn=P, h=P, n=P, rstd=P, dy=P, T=2, H=16, y_stride=16, residual_stride=16, scale=1.0, eps=1e-6)
+    assert call(entry, _lib.ADD_NORM, **{**args, **changed}) == -1
+    assert b"apart" in _lib.lib().d3_last_error()
