@@ -56,7 +56,7 @@ def route(logits, k):
     logits = logits.contiguous()
     ids = torch.empty((rows, k), dtype=torch.int64, device=logits.device)
     weights = torch.empty((rows, k), dtype=torch.float32, device=logits.device)
-    _call("d3_route", _p(logits), rows, n, k, _p(ids), _p(weights), _stream(logits))
+    launch("d3_route", logits.get_device(), _p(logits), rows, n, k, _p(ids), _p(weights))
     return ids, weights
 
 

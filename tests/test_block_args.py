@@ -320,3 +320,31 @@ def test_add_norm_entries_refuse_strides(entry, changed):
     args = dict(y=P, residual=P, weight=P, dh=P, dn=P, h=P, n=P, rstd=P, dy=P, T=2, H=16, y_stride=16, residual_stride=16, scale=1.0, eps=1e-6)
     assert call(entry, _lib.ADD_NORM, **{**args, **changed}) == -1
     assert b"apart" in _lib.lib().d3_last_error()
+
+
+def test_route_goes_to_its_logits_device(monkeypatch):
+    """sparse_block's routing, as its products, runs with the rows' device as the current one, whichever that is."""
+    seen = []
+
+    class Device:
+        def __init__(self, index):
+            seen.append(index)
+
+        def __enter__(self):
+            seen.append("in")
+
+        def __exit__(self, *_):
+            seen.append("out")
+
+    class Lib:
+        def d3_route(self, *args):
+            seen.append(args[-1])
+            return 0
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: ("stream of", index), raising=False)
+    monkeypatch.setattr(block.kernels._lib, "lib", Lib)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 1)
+    block.kernels.route(z(2, 16), 4)
+    assert seen == [1, "in", ("stream of", 1), "out"]
