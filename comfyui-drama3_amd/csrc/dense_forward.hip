@@ -13,6 +13,7 @@ int check_dense(const std::string& what, const Dense& a) {
   if (a.M == 0) return 0;
   if (bad_rows(a.x, a.ldx, a.K) || bad_rows(a.w, a.ldw, a.K) || bad_rows(a.out, a.ldo, a.half ? a.half : a.N))
     return fail(what + ": null pointer, or rows that are not 16-byte aligned or more than 2^23 apart");
+  if (a.pre && a.half && ((uintptr_t)a.pre & 15u)) return fail(what + ": pre must be 16-byte aligned");
   if ((int64_t)(a.N / 8) * ((a.M + 15) / 16) > INT32_MAX) return fail(what + ": too many rows for one launch");
   return 0;
 }

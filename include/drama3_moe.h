@@ -495,7 +495,7 @@ int d3_add_norm_backward(const d3_add_norm_desc* desc, void* stream);
 
 /* Dense products of bf16 rows x [T, K] (x_stride elements apart) with bf16 weights w [N, K], float32 sums: out [T, N] bf16; with
  * swiglu (N / 2 gate rows, then as many up rows) out [T, N / 2] = SiLU(gate) * up, and pre [T, N] float32 = gate and up where
- * it is not NULL. K, N (swiglu: N / 2) and x_stride (up to 2^23) multiples of 8, rows 16-byte aligned, up to 2^30 of them.
+ * it is not NULL. K, N (swiglu: N / 2) and x_stride (up to 2^23) multiples of 8, rows (pre's too) 16-byte aligned, up to 2^30 of them.
  * With adapters > 0 every row has its adapter's low-rank product added before anything else: alpha[i] (x[t] a[i]^T) b[i]^T,
  * i = ids[t] (int64; a row with an id outside [0, adapters) has none), a [adapters, rank, K] and b [adapters, N, rank]
  * bf16, alpha [adapters] float32, rank a multiple of 8; inner [T, rank] bf16 is workspace that needs no clearing. */

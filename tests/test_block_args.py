@@ -348,3 +348,9 @@ def test_route_goes_to_its_logits_device(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 1)
     block.kernels.route(z(2, 16), 4)
     assert seen == [1, "in", ("stream of", 1), "out"]
+
+
+def test_dense_entry_refuses_an_unaligned_pre():
+    """Gate and up are stored 16 bytes at a time, as the backward entry reads them."""
+    assert call("d3_dense", _lib.DENSE, x=P, w=P, out=P, pre=P + 4, x_stride=16, T=2, N=16, K=16, swiglu=1) == -1
+    assert b"pre must be" in _lib.lib().d3_last_error()
