@@ -7,7 +7,7 @@
 // n are each rounded once, to the stream's and the block's type (n comes from h before its rounding).
 //
 // HBM-bound: a row is read once, held in registers through its sums, and written once: 8192 rows of 2048, a float32 stream
-// and a bfloat16 block output, 41 us (4.9 TB/s); 4096 bfloat16 rows 14.2 us forward (4.7 TB/s), 20.8 backward (4.9 TB/s). A lane
+// and a bfloat16 block output, 42 us (4.8 TB/s); 4096 bfloat16 rows 14.2 us forward (4.7 TB/s), 21.0 backward (4.8 TB/s). A lane
 // takes 8 columns at a time, 8 to 32 in all: a wave a row up to 1024 columns (four rows a workgroup), a workgroup a row above.
 //
 // Backward, for dh and dn (gradients of h and n), with z^ = z rstd(z) and m(z) the mean over a row:

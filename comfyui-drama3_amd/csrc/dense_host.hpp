@@ -42,8 +42,8 @@ constexpr float LONG_COST = 0.82f;
 
 // The tile's size by what a stage of each takes, us, times the turns in which the 256 CUs take the tiles: 1.5 (256 x 256),
 // 0.82 (128 x 256), 0.45 (128 x 128; 0.5 in several turns), 0.17 (64 x 64), 0.155 (64 x 32), measured with the CUs at work.
-// So the large ones, which read least, where they come out even, and small ones for few rows. Measured, us, in this order (t: a
-// transposed operand; tt: both, as in launch_dense_set):
+// So the large ones, which read least, where they come out even, and small ones for few rows. Measured, us, each product alone, in this
+// order (t: a transposed operand; tt: both, as in launch_dense_set):
 //   4096 x 4096 x 11008    266 276 317   -   -     4096 x 2048 x 6144    115  80  91   -   -     4096 x 12288 x 2048  154 170 200  -  -
 //   12288 x 2048 x 4096 tt 177 177 211   -   -     2048 x 6144 x 4096 tt  86 107 106   -   -     1391 x 1536 x 2048    -   -  16  19  -
 //    509 x 1024 x 2048       -   -   - 8.1 7.4       61 x 4096 x 2048      -   -   - 7.9 7.1     1391 x 2048 x 1536 t   -   -  13  16  -

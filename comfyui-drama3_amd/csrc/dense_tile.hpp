@@ -164,8 +164,8 @@ struct Tile {
 // The adapters of a wave's rows: the products of p and b, by steps of one adapter that the rows name and up to 64 ranks, DEPTH
 // steps' operands on their way at once (decode lines name about as many adapters as rows); the first of them from before the
 // last stage on, the ids from before the first. Past the last adapter a step reads adapter 0 again, whose sums no row takes: a
-// branch a step costs more (500 rows of 24 adapters by turns, rank 32, 2048 x 2048: 15.4 us, 14.6 without). 61 rows of 24 adapters
-// of rank 64 by turns, 4096 x 2048: 7.1 us without adapters, 16.5 with them.
+// branch a step costs more (500 rows of 24 adapters by turns, rank 32, 2048 x 2048, this product alone: 15.4 us, 14.6 without). 61 rows
+// of 24 adapters of rank 64, 4096 x 2048, alone: 7.4 us without adapters, 16.7 with them by turns, 13.2 in runs.
 template <class C>
 struct RowAdapters {
   static constexpr int DEPTH = C::DEPTH, NONE = -2;
@@ -269,9 +269,9 @@ struct RowAdapters {
 // The loop over the stages is one stream of MFMA groups (NT products of one row tile each). Beside each group go the LDS reads of
 // the operands that the half stage after needs, into the registers that the group has just read, and, in a stage's second
 // half, its share of the copies of the stage BUFS later: with all copies at the start of a stage the waves stood in line
-// to send them, and copies and products took turns (256 x 256 on 4096 x 4096 x 11008: 285 us, 321 so before; 2048 x
-// 6144 x 4096 transposed twice 90, 114). A stage's one barrier stands after group BAR of its second half, when the reads of its own
-// operands are long done.
+// to send them, and copies and products took turns (256 x 256 on 4096 x 4096 x 11008, alone: 321 us so, 285 after that step, and
+// 266 once its addresses no longer spilled; 2048 x 6144 x 4096 transposed twice 114, 90, 86). A stage's one barrier stands after
+// group BAR of its second half, when the reads of its own operands are long done.
 template <class C, bool XT, bool WT, int END, bool LORA>
 D3_INLINE void dense_tile(const Dense& a, int tm, int tn, uint8_t* smem) {
   constexpr int TM = C::TM, TN = C::TN, W = C::WAVES, BUFS = C::BUFS;
