@@ -320,12 +320,13 @@ def _add_norm(y, residual, weight, post, gate, scale, eps, unit_offset, stats):
 
 
 class _Saved(tuple):
-    """add_norm_forward's (rstd, residual) with what residual's version was (None: its type keeps none)."""
+    """add_norm_forward's (rstd, residual) with what residual's version was (None: not known)."""
     version = None
 
 
 def _version(t):
-    return None if t.is_inference() else t._version
+    """(A view's version counts writes to its whole base: those to other layers' rows of one buffer, say.)"""
+    return None if t.is_inference() or t._is_view() else t._version
 
 
 def add_norm_forward(y, residual, weight, *, post=None, gate=None, scale=1.0, eps=1e-6, unit_offset=False):
@@ -350,7 +351,7 @@ def add_norm_backward(dh, dn, y, h, saved, weight, *, post=None, gate=None, scal
         if y is None:
             raise TypeError("y [T, H] float32 or bfloat16 expected")
         rstd, residual = saved
-        if h.dtype is torch.bfloat16 and isinstance(saved, _Saved) and saved.version != _version(residual):
+        if dn is not None and h.dtype is torch.bfloat16 and isinstance(saved, _Saved) and saved.version != _version(residual):
             raise RuntimeError("add_norm_backward: residual was changed in place after add_norm_forward, which a bfloat16 stream's "
                                "gradients read again")
         return _add_norm_backward(dh, dn, y, h, rstd, residual, weight, post, gate, scale, unit_offset, needs, None)

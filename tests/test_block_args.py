@@ -354,3 +354,16 @@ def test_dense_entry_refuses_an_unaligned_pre():
     """Gate and up are stored 16 bytes at a time, as the backward entry reads them."""
     assert call("d3_dense", _lib.DENSE, x=P, w=P, out=P, pre=P + 4, x_stride=16, T=2, N=16, K=16, swiglu=1) == -1
     assert b"pre must be" in _lib.lib().d3_last_error()
+
+
+def test_add_norm_backward_takes_a_residual_that_it_does_not_read_or_that_stayed(monkeypatch):
+    """Neither a write to other rows of the buffer that residual is a part of, nor one to a residual that dh alone needs not, is refused."""
+    monkeypatch.setattr(block.kernels, "launch", lambda *args: None)
+    buffer, y, weight = z(2, 3, 16), z(3, 16), z(16)
+    h, n, saved = block.add_norm_forward(y, buffer[0], weight)
+    buffer[1].add_(1)
+    block.add_norm_backward(h, n, y, h, saved, weight)
+    residual = z(3, 16)
+    h, n, saved = block.add_norm_forward(y, residual, weight)
+    residual.add_(1)
+    block.add_norm_backward(h, None, y, h, saved, weight)
